@@ -1,0 +1,395 @@
+// Rows into an 8-bit paged cache and pages out of it (layout: pages8.cuh).
+#include "pages8.cuh"
+
+namespace {
+
+struct Append8Args {
+    const float* qkv;        // [rows][ldq]: q heads | k heads | ..., value heads from column v_off on
+    int ldq, rows, n_heads, dim, vdim;
+    const float* q_norm;     // see PagedAppendArgs
+    const float* k_norm;
+    float eps;
+    const double* freqs;     // [n_rot / 2]
+    int n_rot;
+    const int* positions;    // [rows], one row a sequence; or null:
+    const int* slots;
+    const int4* segs;        // [n_segs] portions (first row, rows, slot, position of the first row), of slots of their own
+    int n_segs, per;         // per: most pages that a portion touches
+    PageTable t;
+    float* q_out;            // [rows][H][hd]
+    Pages8 c;
+    int head_norm, v_off;
+    float mscale;
+    int maps, no_append;
+};
+
+constexpr int WARPS = 8, THREADS = 32 * WARPS;
+constexpr int COLS = 4;                      // columns of a head row that a lane holds
+
+// Column i of a lane: with VEC four neighbours, so that a head row is one 16-byte load a lane, else every 32nd.
+template <bool VEC>
+__device__ __forceinline__ int col(int lane, int i) { return VEC ? 4 * lane + i : lane + 32 * i; }
+
+template <bool VEC>
+__device__ __forceinline__ void load_head(const float* p, int n, int lane, float (&x)[COLS]) {
+    if (VEC) {
+        const float4 v = 4 * lane < n ? __ldcg((const float4*)p + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < COLS; i++) x[i] = lane + 32 * i < n ? p[lane + 32 * i] : 0.f;
+    }
+}
+
+__device__ __forceinline__ float square_sum(const float (&x)[COLS]) { return x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3]; }
+
+// Rotation of a head row in the half-split order (of both maps' halves of a row that has two).  cs / sn: cosines and sines of the row's pairs.
+template <bool VEC>
+__device__ __forceinline__ void rotate(float (&x)[COLS], int lane, int n, int dim, int n_rot, const float* cs, const float* sn) {
+    const int half = n_rot >> 1;
+    if (half == 0) return;
+    float y[COLS];
+    if (VEC) {          // half and dim are multiples of four: a lane's four columns turn with the same lane's
+        const int d = 4 * lane, in = d >= dim ? d - dim : d;
+        const bool first = in < half, turns = in < n_rot && d < n;
+        const int other = first ? lane + (half >> 2) : lane - (half >> 2);
+#pragma unroll
+        for (int i = 0; i < COLS; i++) y[i] = __shfl_sync(0xffffffffu, x[i], other & 31);
+        if (turns) {
+            const float4 c = *(const float4*)(cs + (first ? in : in - half)), s = *(const float4*)(sn + (first ? in : in - half));
+            const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+            for (int i = 0; i < COLS; i++) x[i] = first ? x[i] * cc[i] - y[i] * ss[i] : x[i] * cc[i] + y[i] * ss[i];
+        }
+    } else {
+        float z[COLS];
+#pragma unroll
+        for (int i = 0; i < COLS; i++) {
+            const int d = lane + 32 * i, in = d >= dim ? d - dim : d;
+            const bool first = in < half, turns = in < n_rot && d < n;
+            const int o = turns ? (first ? d + half : d - half) : d;
+#pragma unroll
+            for (int j = 0; j < COLS; j++) {
+                const float v = __shfl_sync(0xffffffffu, x[j], o & 31);
+                if (o >> 5 == j) y[i] = v;
+            }
+            z[i] = x[i];
+            if (turns) {
+                const int p = first ? in : in - half;
+                z[i] = first ? x[i] * cs[p] - y[i] * sn[p] : x[i] * cs[p] + y[i] * sn[p];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < COLS; i++) x[i] = z[i];
+    }
+}
+
+// A lane's codes of a head row.
+template <bool VEC>
+__device__ __forceinline__ void store_codes(uint8_t* row, int lane, int hd, const float (&x)[COLS], float inv) {
+    const uint32_t lo = to_e4m3x2(x[0] * inv, x[1] * inv), hi = to_e4m3x2(x[2] * inv, x[3] * inv);
+    if (VEC) {
+        if (4 * lane < hd) ((uint32_t*)row)[lane] = lo | hi << 16;
+    } else {
+        const uint32_t w = lo | hi << 16;
+#pragma unroll
+        for (int i = 0; i < COLS; i++)
+            if (lane + 32 * i < hd) row[lane + 32 * i] = (uint8_t)(w >> 8 * i);
+    }
+}
+
+__device__ __forceinline__ uint32_t rescaled(uint32_t two, float f) {
+    const float2 v = e4m3x2_to_f2(two);
+    return to_e4m3x2(v.x * f, v.y * f);
+}
+
+// The codes of a page's head but those of rows [lo, hi), in a unit that is 1 / f of theirs.
+__device__ void rescale_page(uint8_t* page, int hd, int lo, int hi, float f) {
+    for (int c = threadIdx.x; c < PAGE * hd / 16; c += THREADS) {
+        const int r = c / (hd / 16);
+        if (r >= lo && r < hi) continue;
+        uint4 w = ((const uint4*)page)[c];
+        uint32_t* x = &w.x;
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = rescaled(x[i], f) | rescaled(x[i] >> 16, f) << 16;
+        ((uint4*)page)[c] = w;
+    }
+}
+
+__device__ __forceinline__ float block_max(float v, float* red) {
+    v = warp_max(v);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    float m = red[0];
+#pragma unroll
+    for (int i = 1; i < WARPS; i++) m = fmaxf(m, red[i]);
+    return m;
+}
+
+// Rows [row, row + n) at positions [pos, pos + n), all in one page, of KV head g.
+template <bool VEC>
+__device__ void append_to_page(const Append8Args& a, int row, int n, int slot, int pos, int g, float* cs, float* red) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int page = page_at(a.t, a.c.n_pages, slot, pos >> PAGE_SHIFT);
+    if (page < 0) return;
+    const int half = a.n_rot >> 1, pitch = (half + 3) & ~3, kdim = a.maps * a.dim, G = a.c.kv_heads, hd = a.c.hd;
+    const int nq = a.n_heads * a.dim, nk = G * kdim, off = pos & (PAGE - 1);
+    float* sn = cs + (a.positions ? 1 : PAGE) * pitch;      // as many rows as the launch has shared memory for
+    const size_t head = (size_t)page * G + g;
+    const float old_k = a.c.ku[head], old_v = a.c.vu[head];
+    float k[PAGE / WARPS][COLS], v[PAGE / WARPS][COLS];
+#pragma unroll
+    for (int i = 0; i < PAGE / WARPS; i++) {
+        const int r = warp + WARPS * i;
+        if (r < n) {
+            const float* p = a.qkv + (size_t)(row + r) * a.ldq;
+            load_head<VEC>(p + nq + g * kdim, kdim, lane, k[i]);
+            load_head<VEC>(p + a.v_off + g * a.vdim, a.vdim, lane, v[i]);
+        }
+    }
+    __syncthreads();      // the tables may still be read for the rows before
+    for (int i = tid; i < n * half; i += THREADS) {
+        float s, c;
+        sincosf(rot_angle(pos + i / half, a.freqs[i % half]), &s, &c);
+        cs[i / half * pitch + i % half] = c * a.mscale;
+        sn[i / half * pitch + i % half] = s * a.mscale;
+    }
+    __syncthreads();
+    float top_k = 0.f, top_v = 0.f;
+#pragma unroll
+    for (int i = 0; i < PAGE / WARPS; i++) {
+        const int r = warp + WARPS * i;
+        if (r < n) {
+            if (a.k_norm) {
+                float s;
+                if (a.head_norm) {
+                    s = square_sum(k[i]);
+                } else {
+                    const float* p = a.qkv + (size_t)(row + r) * a.ldq + nq;
+                    s = 0.f;
+                    for (int c = 0; c < nk; c += 128) {
+                        float x[COLS];
+                        load_head<VEC>(p + c, nk - c, lane, x);
+                        s += square_sum(x);
+                    }
+                }
+                const float inv = 1.f / sqrtf(warp_sum(s) / (float)(a.head_norm ? a.dim : nk) + a.eps);
+                const float* w = a.k_norm + (a.head_norm ? 0 : g * kdim);
+#pragma unroll
+                for (int j = 0; j < COLS; j++) {
+                    const int d = col<VEC>(lane, j);
+                    if (d < kdim) k[i][j] *= inv * __ldg(w + d);
+                }
+            }
+            rotate<VEC>(k[i], lane, kdim, a.dim, a.n_rot, cs + r * pitch, sn + r * pitch);
+#pragma unroll
+            for (int j = 0; j < COLS; j++) {
+                top_k = fmaxf(top_k, fabsf(k[i][j]));
+                top_v = fmaxf(top_v, fabsf(v[i][j]));
+            }
+        }
+    }
+    float unit_k = unit_for(block_max(top_k, red)), unit_v = unit_for(block_max(top_v, red));
+    uint8_t *kp = a.c.k + head * PAGE * hd, *vp = a.c.v + head * PAGE * hd;
+    if (off > 0) {        // positions before these stay: the page's unit does not shrink
+        unit_k = fmaxf(unit_k, old_k);
+        unit_v = fmaxf(unit_v, old_v);
+        if (unit_k > old_k) rescale_page(kp, hd, off, off + n, old_k / unit_k);
+        if (unit_v > old_v) rescale_page(vp, hd, off, off + n, old_v / unit_v);
+    }
+    if (tid == 0) {
+        a.c.ku[head] = unit_k;
+        a.c.vu[head] = unit_v;
+    }
+    const float ik = 1.f / unit_k, iv = 1.f / unit_v;
+#pragma unroll
+    for (int i = 0; i < PAGE / WARPS; i++) {
+        const int r = warp + WARPS * i;
+        if (r < n) {
+            store_codes<VEC>(kp + (off + r) * hd, lane, hd, k[i], ik);
+            store_codes<VEC>(vp + (off + r) * hd, lane, hd, v[i], iv);
+        }
+    }
+}
+
+// Queries of one row, a warp a head.
+template <bool VEC>
+__device__ void query_row(const Append8Args& a, int row, int pos, float* cs, float* red) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, half = a.n_rot >> 1, pitch = (half + 3) & ~3, nq = a.n_heads * a.dim, hd = a.c.hd;
+    float* sn = cs + pitch;
+    const float* p = a.qkv + (size_t)row * a.ldq;
+    for (int i = tid; i < half; i += THREADS) {
+        float s, c;
+        sincosf(rot_angle(pos, a.freqs[i]), &s, &c);
+        cs[i] = c * a.mscale;
+        sn[i] = s * a.mscale;
+    }
+    float inv = 1.f;
+    if (a.q_norm && !a.head_norm) {
+        float s = 0.f;
+        for (int c = 128 * warp; c < nq; c += 128 * WARPS) {
+            float x[COLS];
+            load_head<VEC>(p + c, nq - c, lane, x);
+            s += square_sum(x);
+        }
+        s = warp_sum(s);
+        if (lane == 0) red[warp] = s;
+        __syncthreads();
+        s = 0.f;
+#pragma unroll
+        for (int i = 0; i < WARPS; i++) s += red[i];
+        inv = 1.f / sqrtf(s / (float)nq + a.eps);
+    } else {
+        __syncthreads();
+    }
+    for (int h = warp; h < a.n_heads; h += WARPS) {
+        float x[COLS];
+        load_head<VEC>(p + h * a.dim, a.dim, lane, x);
+        if (a.q_norm) {
+            if (a.head_norm) inv = 1.f / sqrtf(warp_sum(square_sum(x)) / (float)a.dim + a.eps);
+            const float* w = a.q_norm + (a.head_norm ? 0 : h * a.dim);
+#pragma unroll
+            for (int j = 0; j < COLS; j++) {
+                const int d = col<VEC>(lane, j);
+                if (d < a.dim) x[j] *= inv * __ldg(w + d);
+            }
+        }
+        rotate<VEC>(x, lane, a.dim, a.dim, a.n_rot, cs, sn);
+        // a map's query stands in the map's columns of an otherwise empty row
+        float* q = a.q_out + ((size_t)row * a.n_heads + h) * hd;
+        const int at = h % a.maps * a.dim;
+        if (VEC && a.maps == 1) {
+            if (4 * lane < hd) ((float4*)q)[lane] = make_float4(x[0], x[1], x[2], x[3]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < COLS; j++) {
+                const int d = col<VEC>(lane, j);
+                if (d < a.dim) q[at + d] = x[j];
+            }
+            for (int d = lane; d < hd; d += 32)
+                if (d < at || d >= at + a.dim) q[d] = 0.f;
+        }
+    }
+}
+
+// Norm of q and k, rotation, q to padded fp32 rows; k and v become codes of the pages they go to, whose units grow so that the largest magnitude fits.  A page whose first
+// position is among the rows begins anew.  CTAs: a KV head and a page of a portion each (its rows stay in registers between the largest magnitude and the codes, eight a
+// warp), then one a query row.
+template <bool VEC>
+__global__ void __launch_bounds__(THREADS) append8_kernel(const __grid_constant__ Append8Args a) {
+    extern __shared__ __align__(16) float cs[];
+    __shared__ float red[WARPS];
+    pdl_launch();
+    pdl_wait();
+    const int G = a.c.kv_heads, units = a.positions ? a.rows : a.n_segs, kv_ctas = a.no_append ? 0 : units * a.per * G;
+    int b = blockIdx.x;
+    if (b < kv_ctas) {
+        const int g = b % G, j = b / G % a.per, u = b / G / a.per;
+        if (a.segs) {
+            const int4 s = a.segs[u];
+            const int first = (s.w >> PAGE_SHIFT) + j, lo = max(s.w, first * PAGE), hi = min(s.w + s.y, (first + 1) * PAGE);
+            if (s.w < 0 || s.x < 0 || s.x + s.y > a.rows || lo >= hi) return;
+            append_to_page<VEC>(a, s.x + lo - s.w, hi - lo, s.z, lo, g, cs, red);
+            return;
+        }
+        // rows of one slot take their turns in one CTA: the first of them appends them all, in order
+        const int slot = a.slots[u];
+        int before = 0, behind = 0;
+        for (int i = threadIdx.x; i < a.rows; i += THREADS)
+            if (a.slots[i] == slot) {
+                before |= i < u;
+                behind |= i > u;
+            }
+        if (__syncthreads_or(before)) return;
+        behind = __syncthreads_or(behind);
+        for (int i = u; i < (behind ? a.rows : u + 1); i++) {
+            if (a.slots[i] != slot || a.positions[i] < 0) continue;
+            append_to_page<VEC>(a, i, 1, slot, a.positions[i], g, cs, red);
+            __syncthreads();      // what it wrote is read by the next one's rescaling
+        }
+        return;
+    }
+    const int row = b - kv_ctas;
+    int pos = -1;
+    if (a.positions) {
+        pos = a.positions[row];
+    } else {
+        for (int i = 0; i < a.n_segs; i++) {
+            const int4 s = a.segs[i];
+            if (row >= s.x && row < s.x + s.y) pos = s.w + row - s.x;
+        }
+    }
+    if (pos >= 0) query_row<VEC>(a, row, pos, cs, red);
+}
+
+// Pages as f16 values.  list: (slot, page of the slot, rows that are wanted); the rows behind them, and pages that are not there, become zeros.
+// A CTA a page and KV head: 8 + 8 KB in, 16 + 16 KB out for heads of 128.
+__global__ void __launch_bounds__(256) read8_kernel(const Pages8 c, const PageTable t, const int4* list, __half* k_out, __half* v_out) {
+    pdl_launch();
+    pdl_wait();
+    const int4 e = list[blockIdx.x];
+    const int g = blockIdx.y, page = page_at(t, c.n_pages, e.x, e.y), chunks = c.hd / 16;
+    const size_t head = (size_t)max(page, 0) * c.kv_heads + g, out = ((size_t)blockIdx.x * c.kv_heads + g) * PAGE * c.hd;
+    const __half2 ku = __float2half2_rn(c.ku[head]), vu = __float2half2_rn(c.vu[head]);
+    const int rows = page < 0 ? 0 : e.z;
+    for (int i = threadIdx.x; i < PAGE * chunks; i += 256) {
+        const bool in = i / chunks < rows;
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+            const uint4 w = in ? ldg16((m ? c.v : c.k) + head * PAGE * c.hd + 16 * (size_t)i) : make_uint4(0, 0, 0, 0);
+            const uint32_t* x = &w.x;
+            uint32_t y[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const uint32_t h = e4m3x2_to_h2(x[j >> 1] >> (j & 1) * 16);
+                const __half2 f = in ? __hmul2(*reinterpret_cast<const __half2*>(&h), m ? vu : ku) : __half2half2(__ushort_as_half(0));
+                y[j] = *reinterpret_cast<const uint32_t*>(&f);
+            }
+            uint4* o = (uint4*)((m ? v_out : k_out) + out + 16 * (size_t)i);
+            o[0] = make_uint4(y[0], y[1], y[2], y[3]);
+            o[1] = make_uint4(y[4], y[5], y[6], y[7]);
+        }
+    }
+}
+
+bool bad_cache(const Pages8& c, const PageTable& t) {
+    return !c.k || !c.v || !c.ku || !c.vu || c.n_pages < 1 || c.kv_heads < 1 || c.kv_heads > 65535 || (c.hd != 64 && c.hd != 128) || !t.table || t.n_slots < 1 || t.max_pages < 1 ||
+           (((uintptr_t)c.k | (uintptr_t)c.v) & 15);
+}
+
+}  // namespace
+
+// Returns a cudaError_t value, as does the entry point below.
+B2_API int b2_append8(const Append8Args* a, int pdl, cudaStream_t st) {
+    if (!a || bad_cache(a->c, a->t) || !a->qkv || !a->q_out || a->rows < 1 || a->n_heads < 1 || a->dim < 1 || a->vdim < 1 || a->maps < 1 || a->maps > 2 || a->n_heads % a->maps ||
+        a->maps * a->dim > a->c.hd || a->vdim > a->c.hd || a->n_rot < 0 || a->n_rot > a->dim || (a->n_rot & 1) || (a->n_rot && !a->freqs) || (!a->q_norm != !a->k_norm) ||
+        ((a->maps > 1 || a->no_append) && a->q_norm) || (!a->positions == !a->segs) || (a->positions && !a->slots) || (a->segs && a->n_segs < 1) || a->per < 1 || a->v_off < 0 ||
+        a->ldq < a->n_heads * a->dim || ((uintptr_t)a->q_out & 15))
+        return (int)cudaErrorInvalidValue;
+    const int kdim = a->maps * a->dim, nq = a->n_heads * a->dim;
+    if (!a->no_append && (a->ldq < nq + a->c.kv_heads * kdim || a->v_off + a->c.kv_heads * a->vdim > a->ldq)) return (int)cudaErrorInvalidValue;
+    const long long ctas = (a->no_append ? 0ll : (a->positions ? (long long)a->rows : (long long)a->n_segs * a->per) * a->c.kv_heads) + a->rows;
+    if (ctas > 0x7fffffffll) return (int)cudaErrorInvalidValue;
+    const bool vec = !((a->dim | a->vdim | a->ldq | a->v_off | (a->n_rot >> 1)) & 3) && !((uintptr_t)a->qkv & 15);
+    const int pitch = ((a->n_rot >> 1) + 3) & ~3, rows = a->positions ? 1 : PAGE;
+    const size_t smem = 2 * sizeof(float) * rows * (pitch ? pitch : 4);
+    Append8Args copy = *a;
+    if (a->positions) copy.per = 1;
+    void* args[] = {&copy};
+    const void* fn = vec ? (const void*)append8_kernel<true> : (const void*)append8_kernel<false>;
+    static PerDeviceOnce once;
+    if (once.first()) {
+        cudaFuncSetAttribute(append8_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024);
+        cudaFuncSetAttribute(append8_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024);
+    }
+    return launch_rows(fn, dim3((unsigned)ctas), dim3(THREADS), smem, args, st, pdl);
+}
+
+B2_API int b2_read8(const Pages8* c, const PageTable* t, const int4* list, int n, __half* k_out, __half* v_out, int pdl, cudaStream_t st) {
+    if (!c || !t || bad_cache(*c, *t) || !list || !k_out || !v_out || n < 1 || ((uintptr_t)list & 15) || (((uintptr_t)k_out | (uintptr_t)v_out) & 15)) return (int)cudaErrorInvalidValue;
+    Pages8 cc = *c;
+    PageTable tt = *t;
+    void* args[] = {&cc, &tt, &list, &k_out, &v_out};
+    return launch_rows((const void*)read8_kernel, dim3(n, c->kv_heads), dim3(256), 0, args, st, pdl);
+}

@@ -1,0 +1,54 @@
+"""The 8-bit paged cache's host side: which portions and tensors are refused."""
+import pytest
+import torch
+
+import pages8_oracle as O
+from ollama_b200.ops import pages8 as P
+
+TABLE = torch.zeros(3, 4, dtype=torch.int32)
+
+
+def test_portions():
+    p = P.portions8([(0, 5, 2, 62), (5, 130, 0, 0), (135, 1, 1, 255)], TABLE)
+    assert p.rows == 136 and p.per == 3 and p.segs.tolist() == [[0, 5, 2, 62], [5, 130, 0, 0], [135, 1, 1, 255]]
+
+
+@pytest.mark.parametrize("parts", [[], [(0, 0, 0, 0)], [(1, 3, 0, 0)], [(0, 3, 0, 0), (2, 3, 1, 0)], [(0, 3, 0, 0), (4, 3, 1, 0)], [(0, 3, 3, 0)], [(0, 3, -1, 0)], [(0, 3, 0, -1)],
+                                   [(0, 3, 0, 254)], [(0, 1, 0, 256)], [(0, 3, 0, 0), (3, 3, 0, 3)]])
+def test_portions_that_are_refused(parts):
+    with pytest.raises(ValueError):
+        P.portions8(parts, TABLE)
+
+
+def test_pages_that_are_refused():
+    ok = torch.zeros(2, 3, 64, 64, dtype=torch.uint8)
+    P.Pages8(ok, torch.ones(2, 3))
+    for codes, unit in ((ok.float(), torch.ones(2, 3)), (ok[:, :, :32], torch.ones(2, 3)), (ok.transpose(0, 1), torch.ones(3, 2)), (ok, torch.ones(2, 4)), (ok, torch.ones(2, 3).half()),
+                        (torch.zeros(2, 3, 64, 96, dtype=torch.uint8), torch.ones(2, 3)), (ok[0], torch.ones(2, 3))):
+        with pytest.raises(ValueError):
+            P.Pages8(codes, unit)
+    for dim in (0, 129):
+        with pytest.raises(ValueError):
+            P.Pages8.empty(2, 3, dim, device="cpu")
+
+
+def test_calls_on_the_cpu_are_refused():
+    k, v = P.Pages8.empty(2, 1, 64, device="cpu"), P.Pages8.empty(2, 1, 64, device="cpu")
+    x, q, i = torch.zeros(1, 192), torch.zeros(1, 1, 64), torch.zeros(1, dtype=torch.int32)
+    prep = dict(heads=1, dim=64, vdim=64, q_norm=None, k_norm=None, eps=1e-5, freqs=None, n_rot=0)
+    with pytest.raises(ValueError, match="cpu"):
+        P.append8(x, k, v, TABLE, q, positions=i, slots=i, **prep)
+    with pytest.raises(ValueError, match="cpu"):
+        P.attn_decode8(x, k, v, i, i, TABLE, torch.zeros(1, 64), n_ctx=64, scale=1.0, **prep)
+    with pytest.raises(ValueError, match="cpu"):
+        P.attn_prompt8(q, k, v, P.portions8([(0, 1, 0, 0)], TABLE), TABLE, torch.zeros(1, 64), vdim=64, scale=1.0)
+    with pytest.raises(ValueError, match="cpu"):
+        P.read8(k, v, torch.zeros(1, 4, dtype=torch.int32), TABLE, torch.zeros(1, 1, 64, 64), torch.zeros(1, 1, 64, 64))
+
+
+def test_the_definition():
+    """The oracle's rounding is the type's, and its units hold the largest magnitude."""
+    x = torch.cat([torch.arange(-448, 449).double() / 3, torch.randn(4000, generator=torch.Generator().manual_seed(1)).double() * 0.01])
+    assert torch.equal(O.e4m3(x), x.float().to(torch.float8_e4m3fn).double())
+    top = torch.tensor([0.0, 448.0, 448.1, 1.0, 3.5, 3.6, 57344.0, 1e9, 2.0 ** -20], dtype=torch.float64)
+    assert O.unit_for(top).tolist() == [2.0 ** -15, 1.0, 2.0, 2.0 ** -8, 2.0 ** -7, 2.0 ** -6, 128.0, 128.0, 2.0 ** -15]
