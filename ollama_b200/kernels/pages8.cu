@@ -3,26 +3,6 @@
 
 namespace {
 
-struct Append8Args {
-    const float* qkv;        // [rows][ldq]: q heads | k heads | ..., value heads from column v_off on
-    int ldq, rows, n_heads, dim, vdim;
-    const float* q_norm;     // see PagedAppendArgs
-    const float* k_norm;
-    float eps;
-    const double* freqs;     // [n_rot / 2]
-    int n_rot;
-    const int* positions;    // [rows], one row a sequence; or null:
-    const int* slots;
-    const int4* segs;        // [n_segs] portions (first row, rows, slot, position of the first row), of slots of their own
-    int n_segs, per;         // per: most pages that a portion touches
-    PageTable t;
-    float* q_out;            // [rows][H][hd]
-    Pages8 c;
-    int head_norm, v_off;
-    float mscale;
-    int maps, no_append;
-};
-
 constexpr int WARPS = 8, THREADS = 32 * WARPS;
 constexpr int COLS = 4;                      // columns of a head row that a lane holds
 
@@ -195,9 +175,9 @@ __device__ void append_to_page(const Append8Args& a, int row, int n, int slot, i
     if (off > 0) {        // positions before these stay: the page's unit does not shrink
         unit_k = fmaxf(unit_k, old_k);
         unit_v = fmaxf(unit_v, old_v);
-        if (unit_k > old_k) rescale_page(kp, hd, off, off + n, old_k / unit_k);
-        if (unit_v > old_v) rescale_page(vp, hd, off, off + n, old_v / unit_v);
     }
+    if (unit_k > old_k && n < PAGE) rescale_page(kp, hd, off, off + n, old_k / unit_k);
+    if (unit_v > old_v && n < PAGE) rescale_page(vp, hd, off, off + n, old_v / unit_v);
     if (tid == 0) {
         a.c.ku[head] = unit_k;
         a.c.vu[head] = unit_v;
@@ -280,8 +260,8 @@ template <bool VEC>
 __global__ void __launch_bounds__(THREADS) append8_kernel(const __grid_constant__ Append8Args a) {
     extern __shared__ __align__(16) float cs[];
     __shared__ float red[WARPS];
-    pdl_launch();
     pdl_wait();
+    pdl_launch();         // behind the wait: a kernel that starts now may read whatever was written before this one
     const int G = a.c.kv_heads, units = a.positions ? a.rows : a.n_segs, kv_ctas = a.no_append ? 0 : units * a.per * G;
     int b = blockIdx.x;
     if (b < kv_ctas) {
@@ -360,9 +340,9 @@ bool bad_cache(const Pages8& c, const PageTable& t) {
 
 }  // namespace
 
-// Returns a cudaError_t value, as does the entry point below.
-B2_API int b2_append8(const Append8Args* a, int pdl, cudaStream_t st) {
-    if (!a || bad_cache(a->c, a->t) || !a->qkv || !a->q_out || a->rows < 1 || a->n_heads < 1 || a->dim < 1 || a->vdim < 1 || a->maps < 1 || a->maps > 2 || a->n_heads % a->maps ||
+int append8_launch(const Append8Args& in, int pdl, cudaStream_t st) {
+    const Append8Args* a = &in;
+    if (bad_cache(a->c, a->t) || !a->qkv || !a->q_out || a->rows < 1 || a->n_heads < 1 || a->dim < 1 || a->vdim < 1 || a->maps < 1 || a->maps > 2 || a->n_heads % a->maps ||
         a->maps * a->dim > a->c.hd || a->vdim > a->c.hd || a->n_rot < 0 || a->n_rot > a->dim || (a->n_rot & 1) || (a->n_rot && !a->freqs) || (!a->q_norm != !a->k_norm) ||
         ((a->maps > 1 || a->no_append) && a->q_norm) || (!a->positions == !a->segs) || (a->positions && !a->slots) || (a->segs && a->n_segs < 1) || a->per < 1 || a->v_off < 0 ||
         a->ldq < a->n_heads * a->dim || ((uintptr_t)a->q_out & 15))
@@ -385,6 +365,9 @@ B2_API int b2_append8(const Append8Args* a, int pdl, cudaStream_t st) {
     }
     return launch_rows(fn, dim3((unsigned)ctas), dim3(THREADS), smem, args, st, pdl);
 }
+
+// Returns a cudaError_t value, as does the entry point below.
+B2_API int b2_append8(const Append8Args* a, int pdl, cudaStream_t st) { return a ? append8_launch(*a, pdl, st) : (int)cudaErrorInvalidValue; }
 
 B2_API int b2_read8(const Pages8* c, const PageTable* t, const int4* list, int n, __half* k_out, __half* v_out, int pdl, cudaStream_t st) {
     if (!c || !t || bad_cache(*c, *t) || !list || !k_out || !v_out || n < 1 || ((uintptr_t)list & 15) || (((uintptr_t)k_out | (uintptr_t)v_out) & 15)) return (int)cudaErrorInvalidValue;

@@ -21,6 +21,50 @@ struct PageTable {
     int n_slots, max_pages;
 };
 
+// What rows are appended, b2_append8.
+struct Append8Args {
+    const float* qkv;        // [rows][ldq]: q heads | k heads | ..., value heads from column v_off on
+    int ldq, rows, n_heads, dim, vdim;
+    const float* q_norm;     // see PagedAppendArgs
+    const float* k_norm;
+    float eps;
+    const double* freqs;     // [n_rot / 2]
+    int n_rot;
+    const int* positions;    // [rows], one row a sequence; or null:
+    const int* slots;
+    const int4* segs;        // [n_segs] portions (first row, rows, slot, position of the first row), of slots of their own
+    int n_segs, per;         // per: most pages that a portion touches
+    PageTable t;
+    float* q_out;            // [rows][H][hd]
+    Pages8 c;
+    int head_norm, v_off;
+    float mscale;
+    int maps, no_append;
+};
+
+// Attention of rows, b2_attn8 (attn_pages8.cu).
+struct Attn8Args {
+    const float* q;          // [rows][H][hd], rotated
+    int rows, n_heads, vdim;
+    Pages8 c;
+    PageTable t;
+    const int* positions;    // [rows], or null:
+    const int* slots;
+    const int4* segs;        // [n_segs] portions (first row, rows, slot, position of the first row)
+    int n_segs;
+    int chunk, window, keep;
+    float scale, softcap;
+    int tiles;               // most row tiles of a sequence
+    int ctas;                // that the keys are dealt out to
+    float* part_acc;         // [items + ctas][16][hd]
+    float2* part_ml;         // [items + ctas][16] (largest score, sum)
+    void* out;               // [rows][ldo], head h at column h * vdim
+    int ldo, out16;
+    HeadGate gate;
+    DiffHeads diff;
+    int behind;              // the launch follows the one that appends the rows, which writes neither positions, slots nor tables
+};
+
 // Codes of two values (the first in the low byte), rounded to nearest even; magnitudes beyond 448 become 448, what is no number stays none.
 __device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {
     uint16_t r;
@@ -52,3 +96,6 @@ __device__ __forceinline__ int page_at(const PageTable& t, int n_pages, int slot
     const int p = __ldg(t.table + (size_t)slot * t.max_pages + i);
     return (unsigned)p < (unsigned)n_pages ? p : -1;
 }
+
+// A cudaError_t value.
+int append8_launch(const Append8Args& a, int pdl, cudaStream_t st);

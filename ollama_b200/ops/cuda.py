@@ -702,7 +702,7 @@ def attn_prefill_tc_status(clear: bool = False) -> int:
 
 def gemm_status() -> int:
     """0 = ok; 1 = a bounded wait inside a tensor-core kernel (the GEMMs, the tcgen05 attention) expired."""
-    return int(lib().b2_moe_fp4_status()) | int(lib().b2_gemm_status()) | int(lib().b2_gemm_q_status()) | int(lib().b2_attn_prefill_tc_status()) | int(lib().b2_gemm_q_grouped_status())
+    return int(lib().b2_moe_fp4_status()) | int(lib().b2_gemm_status()) | int(lib().b2_gemm_q_status()) | int(lib().b2_attn_prefill_tc_status()) | int(lib().b2_gemm_q_grouped_status()) | int(lib().b2_attn8_status())
 
 
 GEMM_Q_TYPES = {WT_Q4_K, WT_Q6_K, WT_Q8_0, WT_BF16, WT_F16}

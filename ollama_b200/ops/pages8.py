@@ -17,10 +17,12 @@ from dataclasses import dataclass
 
 import torch
 
-from .cuda import _check, lib, ptr
+from .cuda import _check, lib
 from .rows import NO_DIFF, NO_GATE, DiffHeads, F, HeadGate, I, P, _st
 
 PAGE = 64
+MAX_UNITS = 256                  # sequences of one launch of the attention kernel
+f32, bf16, i32 = torch.float32, torch.bfloat16, torch.int32
 
 _Pages8 = _st("_Pages8", [("k", P), ("ku", P), ("v", P), ("vu", P), ("n_pages", I), ("kv_heads", I), ("hd", I)])
 _PageTable = _st("_PageTable", [("table", P), ("n_slots", I), ("max_pages", I)])
@@ -28,11 +30,11 @@ Append8Args = _st("Append8Args", [("qkv", P), ("ldq", I), ("rows", I), ("n_heads
                                   ("n_rot", I), ("positions", P), ("slots", P), ("segs", P), ("n_segs", I), ("per", I), ("t", _PageTable), ("q_out", P), ("c", _Pages8),
                                   ("head_norm", I), ("v_off", I), ("mscale", F), ("maps", I), ("no_append", I)])
 Attn8Args = _st("Attn8Args", [("q", P), ("rows", I), ("n_heads", I), ("vdim", I), ("c", _Pages8), ("t", _PageTable), ("positions", P), ("slots", P), ("segs", P), ("n_segs", I),
-                              ("chunk", I), ("window", I), ("keep", I), ("scale", F), ("softcap", F), ("n_splits", I), ("part_acc", P), ("part_ml", P), ("out", P), ("ldo", I),
-                              ("out16", I), ("gate", HeadGate), ("diff", DiffHeads)])
+                              ("chunk", I), ("window", I), ("keep", I), ("scale", F), ("softcap", F), ("tiles", I), ("ctas", I), ("part_acc", P), ("part_ml", P), ("out", P),
+                              ("ldo", I), ("out16", I), ("gate", HeadGate), ("diff", DiffHeads), ("behind", I)])
 
 
-@dataclass
+@dataclass(frozen=True)
 class Pages8:
     """Keys or values of a layer: ``codes`` [pages, KV heads, 64, 64 or 128] uint8, ``unit`` [pages, KV heads] fp32."""
 
@@ -41,10 +43,12 @@ class Pages8:
 
     def __post_init__(self):
         c, u = self.codes, self.unit
-        if c.dim() != 4 or c.shape[2] != PAGE or c.shape[3] not in (64, 128) or c.dtype != torch.uint8 or not c.is_contiguous():
+        if c.dim() != 4 or c.shape[2] != PAGE or c.shape[3] not in (64, 128) or c.dtype != torch.uint8 or not c.is_contiguous() or not c.shape[0] or not c.shape[1]:
             raise ValueError(f"Pages8: codes {tuple(c.shape)} {c.dtype}")
-        if u.shape != c.shape[:2] or u.dtype != torch.float32 or not u.is_contiguous() or u.device != c.device:
+        if u.shape != c.shape[:2] or u.dtype != f32 or not u.is_contiguous() or u.device != c.device:
             raise ValueError(f"Pages8: units {tuple(u.shape)} {u.dtype} on {u.device}")
+        # device and sizes, in the order in which calls need them
+        object.__setattr__(self, "_sizes", (c.get_device(), c.shape[0], c.shape[1], c.shape[3]))
 
     @classmethod
     def empty(cls, n_pages: int, kv_heads: int, dim: int, device="cuda") -> "Pages8":
@@ -59,13 +63,14 @@ class Pages8:
         return self.codes.view(torch.float8_e4m3fn)
 
 
-@dataclass
+@dataclass(frozen=True)
 class Portions8:
     """Portions of prompts in a step, of different slots: what :func:`append8` and :func:`attn_prompt8` have to know of them."""
 
     segs: torch.Tensor               # [n, 4]: first row, rows, slot, position of the first row
     rows: int                        # of all portions
     per: int                         # most pages that a portion's rows go to
+    longest: int                     # most rows of one
 
 
 def portions8(parts, table: torch.Tensor, *, window: int = 0, keep: int = 0, chunk: int = 0) -> Portions8:
@@ -82,39 +87,98 @@ def portions8(parts, table: torch.Tensor, *, window: int = 0, keep: int = 0, chu
     if not at:
         raise ValueError("portions8: no rows")
     segs = torch.tensor(parts, dtype=torch.int32).to(table.device)
-    return Portions8(segs, at, max((p + n - 1) // PAGE - p // PAGE + 1 for _, n, _, p in parts))
+    return Portions8(segs, at, max((p + n - 1) // PAGE - p // PAGE + 1 for _, n, _, p in parts), max(n for _, n, _, _ in parts))
 
 
 def _on_device(f):
     """Run ``f`` with its first tensor's device current."""
     @functools.wraps(f)
     def call(x, *a, **kw):
-        if x.device.type != "cuda":
+        dev = x.get_device()
+        if dev < 0:
             raise ValueError(f"{f.__name__}: tensors on {x.device}")
-        if x.device.index == torch.cuda.current_device():
+        if dev == torch.cuda.current_device():
             return f(x, *a, **kw)
-        with torch.cuda.device(x.device):
+        with torch.cuda.device(dev):
             return f(x, *a, **kw)
     return call
 
 
-def _stream(x: torch.Tensor) -> C.c_void_p:
-    return C.c_void_p(torch.cuda.current_stream(x.device).cuda_stream)
+@functools.lru_cache(maxsize=None)
+def _entry(name: str):
+    f = getattr(lib(), name)
+    f.restype, f.argtypes = I, {"b2_append8": [P, I, P], "b2_attn8": [P, I, P], "b2_decode8": [P, P, I, P], "b2_read8": [P, P, P, I, P, P, I, P], "b2_attn8_status": []}[name]
+    return f
 
 
-def _need(what: str, name: str, t: torch.Tensor | None, dtype, device, *shape, contiguous: bool = True) -> None:
-    """A tensor of the type, on the device, of the shape (None: any size) with rows that are one piece."""
-    if t is None or t.dtype not in (dtype if isinstance(dtype, tuple) else (dtype,)) or t.device != device or t.dim() != len(shape) or \
-            any(s is not None and s != n for s, n in zip(shape, t.shape)) or (not t.is_contiguous() if contiguous else t.numel() and t.stride(-1) != 1):
-        raise ValueError(f"{what}: {name} " + ("is missing" if t is None else f"{tuple(t.shape)} {t.dtype} on {t.device}, strides {t.stride()}"))
+def _stream(dev: int) -> int:
+    return torch.cuda.current_stream(dev).cuda_stream
 
 
-def _cache(what: str, k: Pages8, v: Pages8, table: torch.Tensor, device) -> tuple:
-    if k.codes.shape != v.codes.shape or k.codes.device != device or v.codes.device != device:
+@functools.lru_cache(maxsize=64)
+def _sms(dev: int) -> int:
+    return torch.cuda.get_device_properties(dev).multi_processor_count
+
+
+def _refuse(what: str, name: str, t: torch.Tensor | None):
+    raise ValueError(f"{what}: {name} " + ("is missing" if t is None else f"{tuple(t.shape)} {t.dtype} on {t.device}, strides {t.stride()}"))
+
+
+def _flat(what: str, name: str, t: torch.Tensor | None, dtype, dev: int, shape) -> int:
+    """Address of a tensor that is one piece, of that type, device and shape."""
+    if t is None or t.dtype is not dtype or t.get_device() != dev or t.shape != shape or not t.is_contiguous():
+        _refuse(what, name, t)
+    return t.data_ptr()
+
+
+def _vector(what: str, name: str, t: torch.Tensor | None, dtype, dev: int, least: int) -> int:
+    """Address of a vector of at least so many elements."""
+    if t is None or t.dtype is not dtype or t.get_device() != dev or t.dim() != 1 or t.numel() < least or not t.is_contiguous():
+        _refuse(what, name, t)
+    return t.data_ptr()
+
+
+def _cache(what: str, k: Pages8, v: Pages8, table: torch.Tensor, dev: int) -> tuple:
+    if k._sizes != v._sizes or k._sizes[0] != dev:
         raise ValueError(f"{what}: keys {tuple(k.codes.shape)} on {k.codes.device}, values {tuple(v.codes.shape)} on {v.codes.device}")
-    _need(what, "table", table, torch.int32, device, None, None)
-    n, g, _, hd = k.codes.shape
-    return _Pages8(ptr(k.codes), ptr(k.unit), ptr(v.codes), ptr(v.unit), n, g, hd), _PageTable(ptr(table), table.shape[0], table.shape[1])
+    if table.dtype is not i32 or table.get_device() != dev or table.dim() != 2 or not table.is_contiguous():
+        _refuse(what, "table", table)
+    return _Pages8(k.codes.data_ptr(), k.unit.data_ptr(), v.codes.data_ptr(), v.unit.data_ptr(), *k._sizes[1:]), _PageTable(table.data_ptr(), *table.shape)
+
+
+def _append_args(w, dev, c, t, qkv, q_out, n, heads, dim, vdim, q_norm, k_norm, eps, freqs, n_rot, head_norm, v_off, mscale, maps, append, where) -> Append8Args:
+    G, hd = c.kv_heads, c.hd
+    if qkv.dtype is not f32 or qkv.stride(1) != 1 and qkv.shape[1] != 1:
+        _refuse(w, "qkv", qkv)
+    cols, v_off = qkv.shape[1], (heads + maps * G) * dim if v_off is None else v_off
+    if heads < 1 or heads % G or dim < 1 or vdim < 1 or maps not in (1, 2) or heads % maps or maps * dim > hd or vdim > hd or v_off < 0 or \
+            heads * dim > cols or (append and max((heads + maps * G) * dim, v_off + G * vdim) > cols):
+        raise ValueError(f"{w}: {heads} heads of {dim}, {G} of {vdim} from column {v_off} on, {maps} maps, in {cols} columns and cache rows of {hd}")
+    if n_rot < 0 or n_rot > dim or n_rot % 2:
+        raise ValueError(f"{w}: {n_rot} rotated dimensions of {dim}")
+    if (q_norm is None) != (k_norm is None) or (q_norm is not None and (maps > 1 or not append)):
+        raise ValueError(f"{w}: norms")
+    qn = kn = None
+    if q_norm is not None:
+        qn, kn = _vector(w, "q_norm", q_norm, f32, dev, dim if head_norm else heads * dim), _vector(w, "k_norm", k_norm, f32, dev, dim if head_norm else G * dim)
+    return Append8Args(qkv.data_ptr(), qkv.stride(0), n, heads, dim, vdim, qn, kn, eps, _vector(w, "freqs", freqs, torch.float64, dev, n_rot // 2) if n_rot else None, n_rot, *where, t,
+                       q_out, c, head_norm, v_off, mscale, maps, not append)
+
+
+def _attn_args(w, dev, c, t, q, n, heads, where, units, longest, acc, ml, ctas, out, vdim, scale, softcap, chunk, window, keep, gate, diff) -> Attn8Args:
+    if out.dtype is not bf16 and out.dtype is not f32 or out.get_device() != dev or out.dim() != 2 or out.shape[0] != n or out.stride(1) != 1:
+        _refuse(w, "out", out)
+    if heads < 1 or heads % c.kv_heads or not 1 <= vdim <= c.hd or (diff.on and heads // c.kv_heads % 2) or out.shape[1] < (heads // 2 if diff.on else heads) * vdim:
+        raise ValueError(f"{w}: {heads} heads on {c.kv_heads} of {vdim} columns into rows of {out.shape[1]}")
+    if chunk < 0 or window < 0 or keep < 0 or (chunk and window) or softcap < 0:
+        raise ValueError(f"{w}: chunk {chunk}, window {window}, keep {keep}, softcap {softcap}")
+    return Attn8Args(q, n, heads, vdim, c, t, *where, chunk, window, keep, scale, softcap, -(-longest * (heads // c.kv_heads) // 16), ctas, acc, ml, out.data_ptr(), out.stride(0),
+                     out.dtype is bf16, gate, diff, 0)
+
+
+def _pieces(c, heads: int, units: int, longest: int, ctas: int) -> int:
+    """Rows of partial results: an item's 16 for each sequence's row tiles and KV heads, and for each CTA whose run ends inside one."""
+    return (min(units, MAX_UNITS) * -(-longest * (heads // c.kv_heads) // 16) * c.kv_heads + ctas) * 16
 
 
 @_on_device
@@ -122,44 +186,23 @@ def append8(qkv, k: Pages8, v: Pages8, table, q_out, *, heads, dim, vdim, q_norm
             head_norm=False, v_off=None, mscale=1.0, maps=1, append=True, pdl=False) -> None:
     """Norm of q and k, rotation, q to padded fp32 rows [rows, H, 64 or 128], k and v into the cache; arguments as of :func:`rows.paged_append`.  Rows are one token a
     sequence at ``positions`` of ``slots`` (of rows of one slot the later ones are appended after the earlier ones), or those of ``portions``."""
-    dev, w = qkv.device, "append8"
+    w, dev = "append8", qkv.get_device()
     c, t = _cache(w, k, v, table, dev)
-    n, G = qkv.shape[0], c.kv_heads
-    _need(w, "qkv", qkv, torch.float32, dev, None, None, contiguous=False)
-    _need(w, "q_out", q_out, torch.float32, dev, n, heads, c.hd)
-    kv = G if append else 0
-    v_off = (heads + maps * G) * dim if v_off is None else v_off
-    if heads < 1 or heads % G or dim < 1 or vdim < 1 or maps not in (1, 2) or heads % maps or maps * dim > c.hd or vdim > c.hd or v_off < 0 or \
-            max((heads + maps * kv) * dim, v_off + G * vdim if append else 0) > qkv.shape[1]:
-        raise ValueError(f"{w}: {heads} heads of {dim}, {G} of {vdim} from column {v_off} on, {maps} maps, in {qkv.shape[1]} columns and cache rows of {c.hd}")
-    if n_rot < 0 or n_rot > dim or n_rot % 2:
-        raise ValueError(f"{w}: {n_rot} rotated dimensions of {dim}")
-    if n_rot:
-        _need(w, "freqs", freqs, torch.float64, dev, None)
-        if len(freqs) < n_rot // 2:
-            raise ValueError(f"{w}: {len(freqs)} frequencies for {n_rot} dimensions")
-    if (q_norm is None) != (k_norm is None) or (q_norm is not None and (maps > 1 or not append)):
-        raise ValueError(f"{w}: norms")
-    for name, x, h in (("q_norm", q_norm, heads), ("k_norm", k_norm, G)):
-        if x is not None:
-            _need(w, name, x, torch.float32, dev, None)
-            if len(x) < dim * (1 if head_norm else h):
-                raise ValueError(f"{w}: {name} of {len(x)}")
+    if qkv.dim() != 2:
+        _refuse(w, "qkv", qkv)
+    n = qkv.shape[0]
     if (portions is None) == (positions is None):
         raise ValueError(f"{w}: either positions and slots or portions")
     if portions is None:
-        _need(w, "positions", positions, torch.int32, dev, n)
-        _need(w, "slots", slots, torch.int32, dev, n)
-        where = (ptr(positions), ptr(slots), None, 0, 1)
+        where = (_flat(w, "positions", positions, i32, dev, (n,)), _flat(w, "slots", slots, i32, dev, (n,)), None, 0, 1)
     else:
-        if portions.rows > n or portions.segs.device != dev:
+        if portions.rows > n or portions.segs.get_device() != dev:
             raise ValueError(f"{w}: portions of {portions.rows} rows on {portions.segs.device}")
-        where = (None, None, ptr(portions.segs), portions.segs.shape[0], portions.per)
-    if not n:
-        return
-    a = Append8Args(ptr(qkv), qkv.stride(0), n, heads, dim, vdim, ptr(q_norm), ptr(k_norm), eps, ptr(freqs) if n_rot else None, n_rot, *where, t, ptr(q_out), c, int(head_norm),
-                    v_off, mscale, maps, int(not append))
-    _check(lib().b2_append8(C.byref(a), int(pdl), _stream(qkv)), w)
+        where = (None, None, portions.segs.data_ptr(), portions.segs.shape[0], portions.per)
+    a = _append_args(w, dev, c, t, qkv, _flat(w, "q_out", q_out, f32, dev, (n, heads, c.hd)), n, heads, dim, vdim, q_norm, k_norm, eps, freqs, n_rot, head_norm, v_off, mscale, maps,
+                     append, where)
+    if n:
+        _check(_entry("b2_append8")(C.byref(a), pdl, _stream(dev)), w)
 
 
 def read8(k: Pages8, v: Pages8, pages, table, k_out, v_out, pdl=False) -> None:
@@ -170,31 +213,14 @@ def read8(k: Pages8, v: Pages8, pages, table, k_out, v_out, pdl=False) -> None:
 
 @_on_device
 def _read8(pages, k, v, table, k_out, v_out, pdl) -> None:
-    dev, w = pages.device, "read8"
+    w, dev = "read8", pages.get_device()
     c, t = _cache(w, k, v, table, dev)
-    _need(w, "pages", pages, torch.int32, dev, None, 4)
     n = pages.shape[0]
-    for name, o in (("k_out", k_out), ("v_out", v_out)):
-        _need(w, name, o, torch.float16, dev, n, c.kv_heads, PAGE, c.hd)
+    at = _flat(w, "pages", pages, i32, dev, (n, 4))
+    shape = (n, c.kv_heads, PAGE, c.hd)
+    out = _flat(w, "k_out", k_out, torch.float16, dev, shape), _flat(w, "v_out", v_out, torch.float16, dev, shape)
     if n:
-        _check(lib().b2_read8(C.byref(c), C.byref(t), C.c_void_p(ptr(pages)), n, C.c_void_p(ptr(k_out)), C.c_void_p(ptr(v_out)), int(pdl), _stream(pages)), w)
-
-
-def _attend(w, q, k, v, table, out, where, vdim, scale, softcap, chunk, window, keep, gate, diff, pdl) -> None:
-    dev = q.device
-    c, t = _cache(w, k, v, table, dev)
-    n, heads = q.shape[:2]
-    _need(w, "q", q, torch.float32, dev, None, None, c.hd)
-    _need(w, "out", out, (torch.float32, torch.bfloat16), dev, n, None, contiguous=False)
-    if heads < 1 or heads % c.kv_heads or not 1 <= vdim <= c.hd or (diff.on and heads // c.kv_heads % 2) or out.shape[1] < (heads // 2 if diff.on else heads) * vdim:
-        raise ValueError(f"{w}: {heads} heads on {c.kv_heads} of {vdim} columns into rows of {out.shape[1]}")
-    if chunk < 0 or window < 0 or keep < 0 or (chunk and window) or softcap < 0:
-        raise ValueError(f"{w}: chunk {chunk}, window {window}, keep {keep}, softcap {softcap}")
-    splits = 1
-    acc, ml = torch.empty(n, heads, splits, c.hd, device=dev), torch.empty(n, heads, splits, 2, device=dev)
-    a = Attn8Args(ptr(q), n, heads, vdim, c, t, *where, chunk, window, keep, scale, softcap, splits, ptr(acc), ptr(ml), ptr(out), out.stride(0),
-                  int(out.dtype == torch.bfloat16), gate, diff)
-    _check(lib().b2_attn8(C.byref(a), int(pdl), _stream(q)), w)
+        _check(_entry("b2_read8")(C.byref(c), C.byref(t), at, n, *out, pdl, _stream(dev)), w)
 
 
 @_on_device
@@ -202,18 +228,44 @@ def attn_decode8(qkv, k: Pages8, v: Pages8, positions, slots, table, out, *, hea
                  keep=0, head_norm=False, v_off=None, mscale=1.0, gate=NO_GATE, maps=1, append=True, diff=NO_DIFF, pdl=False) -> None:
     """Decode attention on raw projections, one token a sequence: what :func:`append8` does, then attention of the rows' positions over the cache, difference of maps and
     gate into rows of ``out``.  ``n_ctx``: most keys that a sequence holds."""
-    n = qkv.shape[0]
-    q = torch.empty(n, heads, k.codes.shape[3], device=qkv.device)
-    append8(qkv, k, v, table, q, heads=heads, dim=dim, vdim=vdim, q_norm=q_norm, k_norm=k_norm, eps=eps, freqs=freqs, n_rot=n_rot, positions=positions, slots=slots,
-            head_norm=head_norm, v_off=v_off, mscale=mscale, maps=maps, append=append, pdl=pdl)
+    w, dev = "attn_decode8", qkv.get_device()
+    c, t = _cache(w, k, v, table, dev)
+    if qkv.dim() != 2:
+        _refuse(w, "qkv", qkv)
+    n, ctas = qkv.shape[0], _sms(dev)
+    at, sl = _flat(w, "positions", positions, i32, dev, (n,)), _flat(w, "slots", slots, i32, dev, (n,))
+    # rotated queries, partial results, their statistics
+    nq, pieces = n * heads * c.hd, _pieces(c, heads, n, 1, ctas)
+    ws = torch.empty(nq + pieces * (c.hd + 2), device=qkv.device)
+    q = ws.data_ptr()
+    p = _append_args(w, dev, c, t, qkv, q, n, heads, dim, vdim, q_norm, k_norm, eps, freqs, n_rot, head_norm, v_off, mscale, maps, append, (at, sl, None, 0, 1))
+    a = _attn_args(w, dev, c, t, q, n, heads, (at, sl, None, 0), n, 1, q + 4 * nq, q + 4 * (nq + pieces * c.hd), ctas, out, vdim, scale, softcap, chunk, window, keep, gate, diff)
     if n:
-        _attend("attn_decode8", q, k, v, table, out, (ptr(positions), ptr(slots), None, 0), vdim, scale, softcap, chunk, window, keep, gate, diff, pdl)
+        _check(_entry("b2_decode8")(C.byref(p), C.byref(a), pdl, _stream(dev)), w)
 
 
 @_on_device
 def attn_prompt8(q, k: Pages8, v: Pages8, portions: Portions8, table, out, *, vdim, scale, softcap=0.0, chunk=0, window=0, keep=0, gate=NO_GATE, diff=NO_DIFF, pdl=False) -> None:
     """Attention of the rows of ``portions``, whose queries ``q`` [rows, H, 64 or 128] and whose keys and values in the cache :func:`append8` has prepared.  ``portions``
     have to be made with this call's masks."""
-    if portions.rows > q.shape[0] or portions.segs.device != q.device:
-        raise ValueError(f"attn_prompt8: portions of {portions.rows} rows on {portions.segs.device} for {q.shape[0]} on {q.device}")
-    _attend("attn_prompt8", q, k, v, table, out, (None, None, ptr(portions.segs), portions.segs.shape[0]), vdim, scale, softcap, chunk, window, keep, gate, diff, pdl)
+    w, dev = "attn_prompt8", q.get_device()
+    c, t = _cache(w, k, v, table, dev)
+    if q.dim() != 3:
+        _refuse(w, "q", q)
+    n, heads, _ = q.shape
+    at = _flat(w, "q", q, f32, dev, (n, heads, c.hd))
+    segs = portions.segs
+    if portions.rows > n or segs.get_device() != dev:
+        raise ValueError(f"{w}: portions of {portions.rows} rows on {segs.device} for {n} on {q.device}")
+    ctas, units = _sms(dev), segs.shape[0]
+    pieces = _pieces(c, heads, units, portions.longest, ctas)
+    ws = torch.empty(pieces * (c.hd + 2), device=q.device)
+    acc = ws.data_ptr()
+    a = _attn_args(w, dev, c, t, at, n, heads, (None, None, segs.data_ptr(), units), units, portions.longest, acc, acc + 4 * pieces * c.hd, ctas, out, vdim, scale, softcap, chunk,
+                   window, keep, gate, diff)
+    _check(_entry("b2_attn8")(C.byref(a), pdl, _stream(dev)), w)
+
+
+def status() -> int:
+    """0, or 1 once a wait of an attention kernel has run out since the last call; synchronises."""
+    return _entry("b2_attn8_status")()

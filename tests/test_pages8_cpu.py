@@ -10,7 +10,7 @@ TABLE = torch.zeros(3, 4, dtype=torch.int32)
 
 def test_portions():
     p = P.portions8([(0, 5, 2, 62), (5, 130, 0, 0), (135, 1, 1, 255)], TABLE)
-    assert p.rows == 136 and p.per == 3 and p.segs.tolist() == [[0, 5, 2, 62], [5, 130, 0, 0], [135, 1, 1, 255]]
+    assert p.rows == 136 and p.per == 3 and p.longest == 130 and p.segs.tolist() == [[0, 5, 2, 62], [5, 130, 0, 0], [135, 1, 1, 255]]
 
 
 @pytest.mark.parametrize("parts", [[], [(0, 0, 0, 0)], [(1, 3, 0, 0)], [(0, 3, 0, 0), (2, 3, 1, 0)], [(0, 3, 0, 0), (4, 3, 1, 0)], [(0, 3, 3, 0)], [(0, 3, -1, 0)], [(0, 3, 0, -1)],

@@ -15,6 +15,8 @@ NAN8 = 0x7f
 def library():
     from ollama_b200.ops import cuda as K
     K.need("stack")
+    yield
+    assert K.gemm_status() == 0
 
 
 def i32(v):
