@@ -54,10 +54,10 @@ struct Attn8Args {
     int n_segs;
     int chunk, window, keep;
     float scale, softcap;
-    int tiles;               // most row tiles of a sequence
-    int ctas;                // that the keys are dealt out to
-    float* part_acc;         // [items + ctas][16][hd]
-    float2* part_ml;         // [items + ctas][16] (largest score, sum)
+    int row_tile, tiles;     // query rows (of a sequence, for the heads of a KV head) that are taken together, 8 or 16; most such tiles of a sequence
+    int ctas;                // that fit the GPU at once
+    float* part_acc;         // [items + ctas][row_tile][hd]
+    float2* part_ml;         // [items + ctas][row_tile] (largest score, sum)
     void* out;               // [rows][ldo], head h at column h * vdim
     int ldo, out16;
     HeadGate gate;

@@ -30,7 +30,7 @@ Append8Args = _st("Append8Args", [("qkv", P), ("ldq", I), ("rows", I), ("n_heads
                                   ("n_rot", I), ("positions", P), ("slots", P), ("segs", P), ("n_segs", I), ("per", I), ("t", _PageTable), ("q_out", P), ("c", _Pages8),
                                   ("head_norm", I), ("v_off", I), ("mscale", F), ("maps", I), ("no_append", I)])
 Attn8Args = _st("Attn8Args", [("q", P), ("rows", I), ("n_heads", I), ("vdim", I), ("c", _Pages8), ("t", _PageTable), ("positions", P), ("slots", P), ("segs", P), ("n_segs", I),
-                              ("chunk", I), ("window", I), ("keep", I), ("scale", F), ("softcap", F), ("tiles", I), ("ctas", I), ("part_acc", P), ("part_ml", P), ("out", P),
+                              ("chunk", I), ("window", I), ("keep", I), ("scale", F), ("softcap", F), ("row_tile", I), ("tiles", I), ("ctas", I), ("part_acc", P), ("part_ml", P), ("out", P),
                               ("ldo", I), ("out16", I), ("gate", HeadGate), ("diff", DiffHeads), ("behind", I)])
 
 
@@ -165,20 +165,27 @@ def _append_args(w, dev, c, t, qkv, q_out, n, heads, dim, vdim, q_norm, k_norm, 
                        q_out, c, head_norm, v_off, mscale, maps, not append)
 
 
-def _attn_args(w, dev, c, t, q, n, heads, where, units, longest, acc, ml, ctas, out, vdim, scale, softcap, chunk, window, keep, gate, diff) -> Attn8Args:
+def _attn_args(w, dev, c, t, q, n, heads, where, tiles, acc, ml, ctas, out, vdim, scale, softcap, chunk, window, keep, gate, diff) -> Attn8Args:
     if out.dtype is not bf16 and out.dtype is not f32 or out.get_device() != dev or out.dim() != 2 or out.shape[0] != n or out.stride(1) != 1:
         _refuse(w, "out", out)
     if heads < 1 or heads % c.kv_heads or not 1 <= vdim <= c.hd or (diff.on and heads // c.kv_heads % 2) or out.shape[1] < (heads // 2 if diff.on else heads) * vdim:
         raise ValueError(f"{w}: {heads} heads on {c.kv_heads} of {vdim} columns into rows of {out.shape[1]}")
     if chunk < 0 or window < 0 or keep < 0 or (chunk and window) or softcap < 0:
         raise ValueError(f"{w}: chunk {chunk}, window {window}, keep {keep}, softcap {softcap}")
-    return Attn8Args(q, n, heads, vdim, c, t, *where, chunk, window, keep, scale, softcap, -(-longest * (heads // c.kv_heads) // 16), ctas, acc, ml, out.data_ptr(), out.stride(0),
+    return Attn8Args(q, n, heads, vdim, c, t, *where, chunk, window, keep, scale, softcap, *tiles, ctas, acc, ml, out.data_ptr(), out.stride(0),
                      out.dtype is bf16, gate, diff, 0)
 
 
-def _pieces(c, heads: int, units: int, longest: int, ctas: int) -> int:
-    """Rows of partial results: an item's 16 for each sequence's row tiles and KV heads, and for each CTA whose run ends inside one."""
-    return (min(units, MAX_UNITS) * -(-longest * (heads // c.kv_heads) // 16) * c.kv_heads + ctas) * 16
+def _row_tiles(rows: int) -> tuple[int, int]:
+    """(query rows that are taken together, tiles of them) where a sequence has so many rows for the heads of a KV head."""
+    tile = 8 if rows <= 8 else 16
+    return tile, -(-rows // tile)
+
+
+def _pieces(c, tiles, units: int, dev: int) -> tuple[int, int]:
+    """(CTAs that fit the GPU at once, rows of partial results: those of as many CTAs, and of one more for each item)."""
+    ctas = _sms(dev) * (2 if tiles[0] == 8 else 1)
+    return ctas, (min(units, MAX_UNITS) * tiles[1] * c.kv_heads + ctas) * tiles[0]
 
 
 @_on_device
@@ -232,14 +239,15 @@ def attn_decode8(qkv, k: Pages8, v: Pages8, positions, slots, table, out, *, hea
     c, t = _cache(w, k, v, table, dev)
     if qkv.dim() != 2:
         _refuse(w, "qkv", qkv)
-    n, ctas = qkv.shape[0], _sms(dev)
+    n = qkv.shape[0]
     at, sl = _flat(w, "positions", positions, i32, dev, (n,)), _flat(w, "slots", slots, i32, dev, (n,))
     # rotated queries, partial results, their statistics
-    nq, pieces = n * heads * c.hd, _pieces(c, heads, n, 1, ctas)
+    tiles = _row_tiles(heads // c.kv_heads)
+    nq, (ctas, pieces) = n * heads * c.hd, _pieces(c, tiles, n, dev)
     ws = torch.empty(nq + pieces * (c.hd + 2), device=qkv.device)
     q = ws.data_ptr()
     p = _append_args(w, dev, c, t, qkv, q, n, heads, dim, vdim, q_norm, k_norm, eps, freqs, n_rot, head_norm, v_off, mscale, maps, append, (at, sl, None, 0, 1))
-    a = _attn_args(w, dev, c, t, q, n, heads, (at, sl, None, 0), n, 1, q + 4 * nq, q + 4 * (nq + pieces * c.hd), ctas, out, vdim, scale, softcap, chunk, window, keep, gate, diff)
+    a = _attn_args(w, dev, c, t, q, n, heads, (at, sl, None, 0), tiles, q + 4 * nq, q + 4 * (nq + pieces * c.hd), ctas, out, vdim, scale, softcap, chunk, window, keep, gate, diff)
     if n:
         _check(_entry("b2_decode8")(C.byref(p), C.byref(a), pdl, _stream(dev)), w)
 
@@ -257,11 +265,12 @@ def attn_prompt8(q, k: Pages8, v: Pages8, portions: Portions8, table, out, *, vd
     segs = portions.segs
     if portions.rows > n or segs.get_device() != dev:
         raise ValueError(f"{w}: portions of {portions.rows} rows on {segs.device} for {n} on {q.device}")
-    ctas, units = _sms(dev), segs.shape[0]
-    pieces = _pieces(c, heads, units, portions.longest, ctas)
+    units = segs.shape[0]
+    tiles = _row_tiles(portions.longest * (heads // c.kv_heads))
+    ctas, pieces = _pieces(c, tiles, units, dev)
     ws = torch.empty(pieces * (c.hd + 2), device=q.device)
     acc = ws.data_ptr()
-    a = _attn_args(w, dev, c, t, at, n, heads, (None, None, segs.data_ptr(), units), units, portions.longest, acc, acc + 4 * pieces * c.hd, ctas, out, vdim, scale, softcap, chunk,
+    a = _attn_args(w, dev, c, t, at, n, heads, (None, None, segs.data_ptr(), units), tiles, acc, acc + 4 * pieces * c.hd, ctas, out, vdim, scale, softcap, chunk,
                    window, keep, gate, diff)
     _check(_entry("b2_attn8")(C.byref(a), pdl, _stream(dev)), w)
 
