@@ -314,11 +314,7 @@ __global__ void __launch_bounds__(Lay<D, NB>::THREADS, Lay<D, NB>::PER_SM)
                     uint4* row = reinterpret_cast<uint4*>(ring + slot * L::BOX + lane * D);
                     bool none = false;
 #pragma unroll
-                    for (int c = 0; c < CHUNKS; c++) {
-                        const uint4 w = row[c];
-                        none |= ((((w.x & 0x7f7f7f7fu) + 0x01010101u) | ((w.y & 0x7f7f7f7fu) + 0x01010101u) | ((w.z & 0x7f7f7f7fu) + 0x01010101u) |
-                                  ((w.w & 0x7f7f7f7fu) + 0x01010101u)) & 0x80808080u) != 0;
-                    }
+                    for (int c = 0; c < CHUNKS; c++) none |= holds_nan(row[c]);
                     bad = __ballot_sync(0xffffffffu, none);
                     if (none) {
 #pragma unroll

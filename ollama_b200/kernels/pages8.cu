@@ -303,27 +303,38 @@ __global__ void __launch_bounds__(THREADS) append8_kernel(const __grid_constant_
     if (pos >= 0) query_row<VEC>(a, row, pos, cs, red);
 }
 
-// Pages as f16 values.  list: (slot, page of the slot, rows that are wanted); the rows behind them, and pages that are not there, become zeros.
+// Pages as f16 values.  list: (slot, page of the slot, rows that are wanted); the rows behind them, and pages that are not there, become zeros.  clean: for attention whose products
+// take weights of zero times every value: a row of values that holds what is no number becomes zeros and its key none, so that only queries that see it have no result.
 // A CTA a page and KV head: 8 + 8 KB in, 16 + 16 KB out for heads of 128.
-__global__ void __launch_bounds__(256) read8_kernel(const Pages8 c, const PageTable t, const int4* list, __half* k_out, __half* v_out) {
+__global__ void __launch_bounds__(256) read8_kernel(const Pages8 c, const PageTable t, const int4* list, __half* k_out, __half* v_out, int clean) {
     pdl_launch();
     pdl_wait();
     const int4 e = list[blockIdx.x];
     const int g = blockIdx.y, page = page_at(t, c.n_pages, e.x, e.y), chunks = c.hd / 16;
     const size_t head = (size_t)max(page, 0) * c.kv_heads + g, out = ((size_t)blockIdx.x * c.kv_heads + g) * PAGE * c.hd;
-    const __half2 ku = __float2half2_rn(c.ku[head]), vu = __float2half2_rn(c.vu[head]);
+    const __half2 unit[2] = {__float2half2_rn(c.ku[head]), __float2half2_rn(c.vu[head])};
     const int rows = page < 0 ? 0 : e.z;
     for (int i = threadIdx.x; i < PAGE * chunks; i += 256) {
         const bool in = i / chunks < rows;
+        uint4 w[2];
+#pragma unroll
+        for (int m = 0; m < 2; m++) w[m] = in ? ldg16((m ? c.v : c.k) + head * PAGE * c.hd + 16 * (size_t)i) : make_uint4(0, 0, 0, 0);
+        if (clean) {
+            bool none = holds_nan(w[1]);
+            for (int o = 1; o < chunks; o <<= 1) none |= __shfl_xor_sync(0xffffffffu, (int)none, o);
+            if (none) {
+                w[0] = make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu);
+                w[1] = make_uint4(0, 0, 0, 0);
+            }
+        }
 #pragma unroll
         for (int m = 0; m < 2; m++) {
-            const uint4 w = in ? ldg16((m ? c.v : c.k) + head * PAGE * c.hd + 16 * (size_t)i) : make_uint4(0, 0, 0, 0);
-            const uint32_t* x = &w.x;
+            const uint32_t* x = &w[m].x;
             uint32_t y[8];
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const uint32_t h = e4m3x2_to_h2(x[j >> 1] >> (j & 1) * 16);
-                const __half2 f = in ? __hmul2(*reinterpret_cast<const __half2*>(&h), m ? vu : ku) : __half2half2(__ushort_as_half(0));
+                const __half2 f = in ? __hmul2(*reinterpret_cast<const __half2*>(&h), unit[m]) : __half2half2(__ushort_as_half(0));
                 y[j] = *reinterpret_cast<const uint32_t*>(&f);
             }
             uint4* o = (uint4*)((m ? v_out : k_out) + out + 16 * (size_t)i);
@@ -369,10 +380,10 @@ int append8_launch(const Append8Args& in, int pdl, cudaStream_t st) {
 // Returns a cudaError_t value, as does the entry point below.
 B2_API int b2_append8(const Append8Args* a, int pdl, cudaStream_t st) { return a ? append8_launch(*a, pdl, st) : (int)cudaErrorInvalidValue; }
 
-B2_API int b2_read8(const Pages8* c, const PageTable* t, const int4* list, int n, __half* k_out, __half* v_out, int pdl, cudaStream_t st) {
+B2_API int b2_read8(const Pages8* c, const PageTable* t, const int4* list, int n, __half* k_out, __half* v_out, int clean, int pdl, cudaStream_t st) {
     if (!c || !t || bad_cache(*c, *t) || !list || !k_out || !v_out || n < 1 || ((uintptr_t)list & 15) || (((uintptr_t)k_out | (uintptr_t)v_out) & 15)) return (int)cudaErrorInvalidValue;
     Pages8 cc = *c;
     PageTable tt = *t;
-    void* args[] = {&cc, &tt, &list, &k_out, &v_out};
+    void* args[] = {&cc, &tt, &list, &k_out, &v_out, &clean};
     return launch_rows((const void*)read8_kernel, dim3(n, c->kv_heads), dim3(256), 0, args, st, pdl);
 }

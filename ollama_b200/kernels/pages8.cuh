@@ -82,6 +82,11 @@ __device__ __forceinline__ float2 e4m3x2_to_f2(uint32_t two) {
     return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
+// Whether one of 16 codes is no number.
+__device__ __forceinline__ bool holds_nan(const uint4& w) {
+    return ((((w.x & 0x7f7f7f7fu) + 0x01010101u) | ((w.y & 0x7f7f7f7fu) + 0x01010101u) | ((w.z & 0x7f7f7f7fu) + 0x01010101u) | ((w.w & 0x7f7f7f7fu) + 0x01010101u)) & 0x80808080u) != 0;
+}
+
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 // The unit in which a magnitude is at most 448 = 1.75 * 2^8: the least such power of two, within the limits.
 __device__ __forceinline__ float unit_for(float top) {

@@ -15,10 +15,11 @@ import ctypes as C
 import functools
 from dataclasses import dataclass
 
+import numpy as np
 import torch
 
-from .cuda import _check, lib
-from .rows import NO_DIFF, NO_GATE, DiffHeads, F, HeadGate, I, P, _st
+from .cuda import AttnPrefillArgs, _check, lib
+from .rows import NO_DIFF, NO_GATE, AttnPagedArgs, DiffHeads, F, HeadGate, I, P, _st
 
 PAGE = 64
 MAX_UNITS = 256                  # sequences of one launch of the attention kernel
@@ -65,29 +66,48 @@ class Pages8:
 
 @dataclass(frozen=True)
 class Portions8:
-    """Portions of prompts in a step, of different slots: what :func:`append8` and :func:`attn_prompt8` have to know of them."""
+    """Portions of prompts in a step, of different slots: what :func:`append8` and :func:`attn_prompt8` have to know of them.  Int32 tensors on the table's device."""
 
     segs: torch.Tensor               # [n, 4]: first row, rows, slot, position of the first row
     rows: int                        # of all portions
     per: int                         # most pages that a portion's rows go to
     longest: int                     # most rows of one
+    masks: tuple[int, int, int]      # window, keep, chunk
+    # for attention on values that are read out first: tiles of 128 (of 64) rows, the pages that they may see, and where each portion's pages are among those
+    tiles: torch.Tensor              # [tiles, 4]: first row, rows, portion, position
+    half_tiles: torch.Tensor
+    pages: torch.Tensor              # [pages, 4]: see read8
+    table: torch.Tensor              # [n, pages of a slot]
 
 
 def portions8(parts, table: torch.Tensor, *, window: int = 0, keep: int = 0, chunk: int = 0) -> Portions8:
     """``parts``: (first row, rows, slot, position of the first row) of each portion, rows one after the other; the masks are those of the attention."""
     n_slots, max_pages = table.shape
+    if window < 0 or keep < 0 or chunk < 0 or (chunk and window):
+        raise ValueError(f"portions8: chunk {chunk}, window {window}, keep {keep}")
     at, slots = 0, set()
-    for row, n, slot, pos in parts:
+    tiles, halves, pages = [], [], []
+    where = np.zeros((len(parts), max_pages), np.int32)
+    for i, (row, n, slot, pos) in enumerate(parts):
         if n < 1 or row != at or not 0 <= slot < n_slots or pos < 0 or pos + n > max_pages * PAGE:
             raise ValueError(f"portions8: {n} rows from {row} on at position {pos} of slot {slot}, in a table {tuple(table.shape)}")
         if slot in slots:
             raise ValueError(f"portions8: two portions of slot {slot}")
         at += n
         slots.add(slot)
+        tiles += [(row + r, min(128, n - r), i, pos + r) for r in range(0, n, 128)]
+        halves += [(row + r, min(64, n - r), i, pos + r) for r in range(0, n, 64)]
+        last = (pos + n - 1) // PAGE
+        first = (pos - pos % chunk if chunk else max(0, pos - window + 1) if window else 0) // 128 * 2          # tiles of 128 keys
+        seen = [*range(0, min(first, -(-keep // 128) * 2) if window else 0), *range(first, last + 1)]
+        where[i, seen] = np.arange(len(pages), len(pages) + len(seen))
+        pages += [(slot, b, min(PAGE, pos + n - b * PAGE), 0) for b in seen]
     if not at:
         raise ValueError("portions8: no rows")
-    segs = torch.tensor(parts, dtype=torch.int32).to(table.device)
-    return Portions8(segs, at, max((p + n - 1) // PAGE - p // PAGE + 1 for _, n, _, p in parts), max(n for _, n, _, _ in parts))
+    lists = [np.asarray(x, np.int32) for x in (parts, tiles, halves, pages, where)]
+    flat = torch.from_numpy(np.concatenate([x.reshape(-1) for x in lists])).to(table.device)
+    segs, tiles, halves, pages, where = (t.view(x.shape) for t, x in zip(flat.split([x.size for x in lists]), lists))
+    return Portions8(segs, at, max((p + n - 1) // PAGE - p // PAGE + 1 for _, n, _, p in parts), max(n for _, n, _, _ in parts), (window, keep, chunk), tiles, halves, pages, where)
 
 
 def _on_device(f):
@@ -107,7 +127,7 @@ def _on_device(f):
 @functools.lru_cache(maxsize=None)
 def _entry(name: str):
     f = getattr(lib(), name)
-    f.restype, f.argtypes = I, {"b2_append8": [P, I, P], "b2_attn8": [P, I, P], "b2_decode8": [P, P, I, P], "b2_read8": [P, P, P, I, P, P, I, P], "b2_attn8_status": []}[name]
+    f.restype, f.argtypes = I, {"b2_append8": [P, I, P], "b2_attn8": [P, I, P], "b2_decode8": [P, P, I, P], "b2_read8": [P, P, P, I, P, P, I, I, P], "b2_attn_prefill_paged": [P, P, I, I, I, P], "b2_attn8_status": []}[name]
     return f
 
 
@@ -227,7 +247,7 @@ def _read8(pages, k, v, table, k_out, v_out, pdl) -> None:
     shape = (n, c.kv_heads, PAGE, c.hd)
     out = _flat(w, "k_out", k_out, torch.float16, dev, shape), _flat(w, "v_out", v_out, torch.float16, dev, shape)
     if n:
-        _check(_entry("b2_read8")(C.byref(c), C.byref(t), at, n, *out, pdl, _stream(dev)), w)
+        _check(_entry("b2_read8")(C.byref(c), C.byref(t), at, n, *out, False, pdl, _stream(dev)), w)
 
 
 @_on_device
@@ -263,16 +283,37 @@ def attn_prompt8(q, k: Pages8, v: Pages8, portions: Portions8, table, out, *, vd
     n, heads, _ = q.shape
     at = _flat(w, "q", q, f32, dev, (n, heads, c.hd))
     segs = portions.segs
-    if portions.rows > n or segs.get_device() != dev:
-        raise ValueError(f"{w}: portions of {portions.rows} rows on {segs.device} for {n} on {q.device}")
+    if portions.rows > n or segs.get_device() != dev or portions.masks != (window, keep, chunk) or portions.table.shape[1] != table.shape[1]:
+        raise ValueError(f"{w}: portions of {portions.rows} rows on {segs.device} with window, keep, chunk {portions.masks} for {n} on {q.device} with {(window, keep, chunk)}")
     units = segs.shape[0]
     tiles = _row_tiles(portions.longest * (heads // c.kv_heads))
     ctas, pieces = _pieces(c, tiles, units, dev)
+    a = _attn_args(w, dev, c, t, at, n, heads, (None, None, segs.data_ptr(), units), tiles, 0, 0, ctas, out, vdim, scale, softcap, chunk, window, keep, gate, diff)
+    if _reads_out(portions, heads, c.kv_heads) and _attn_read(w, dev, a, portions, q, out, pdl):
+        return
     ws = torch.empty(pieces * (c.hd + 2), device=q.device)
-    acc = ws.data_ptr()
-    a = _attn_args(w, dev, c, t, at, n, heads, (None, None, segs.data_ptr(), units), tiles, acc, acc + 4 * pieces * c.hd, ctas, out, vdim, scale, softcap, chunk,
-                   window, keep, gate, diff)
+    a.part_acc, a.part_ml = ws.data_ptr(), ws.data_ptr() + 4 * pieces * c.hd
     _check(_entry("b2_attn8")(C.byref(a), pdl, _stream(dev)), w)
+
+
+def _reads_out(portions: Portions8, heads: int, kv_heads: int) -> bool:
+    """Whether the pages are read out to f16 first."""
+    return portions.longest * (heads // kv_heads) > 256
+
+
+def _attn_read(w, dev, a: Attn8Args, portions: Portions8, q, out, pdl) -> bool:
+    """Attention on tcgen05 over the portions' pages as f16 values; False: not taken, nothing launched."""
+    c, diff = a.c, a.diff.on
+    if not a.out16 or a.out % 16 or (diff and a.gate.kind):
+        return False
+    pages, tiles = portions.pages, portions.half_tiles if diff else portions.tiles
+    n = pages.shape[0]
+    k, v = torch.empty(2, n, c.kv_heads, PAGE, c.hd, device=q.device, dtype=torch.float16)
+    _check(_entry("b2_read8")(C.byref(c), C.byref(a.t), pages.data_ptr(), n, k.data_ptr(), v.data_ptr(), True, pdl, _stream(dev)), w)
+    p = AttnPrefillArgs(a.q, k.data_ptr(), v.data_ptr(), a.out, None, a.rows, a.n_heads, c.kv_heads, 0, 0, 0, 0, 1, 0, a.scale, a.softcap, None, None)
+    pg = AttnPagedArgs(tiles.data_ptr(), portions.table.data_ptr(), portions.table.shape[1], a.chunk, a.vdim, a.ldo, a.window, a.keep, a.gate, a.diff)
+    _check(_entry("b2_attn_prefill_paged")(C.byref(p), C.byref(pg), c.hd, tiles.shape[0], n, _stream(dev)), w)
+    return True
 
 
 def status() -> int:

@@ -13,6 +13,19 @@ def test_portions():
     assert p.rows == 136 and p.per == 3 and p.longest == 130 and p.segs.tolist() == [[0, 5, 2, 62], [5, 130, 0, 0], [135, 1, 1, 255]]
 
 
+def test_pages_that_portions_see():
+    table = torch.zeros(2, 20, dtype=torch.int32)
+    p = P.portions8([(0, 130, 1, 700), (130, 3, 0, 0)], table, window=200, keep=70)
+    # keys from 501 on, in tiles of 128 from 384 (page 6) on, to 829 (page 12), and the kept ones in the first tile
+    assert p.pages.tolist() == [[1, b, 64, 0] for b in (0, 1, 6, 7, 8, 9, 10, 11)] + [[1, 12, 62, 0], [0, 0, 3, 0]]
+    assert p.table[0, [0, 1, 6, 12]].tolist() == [0, 1, 2, 8] and p.table[1, 0] == 9
+    assert p.tiles.tolist() == [[0, 128, 0, 700], [128, 2, 0, 828], [130, 3, 1, 0]] and p.half_tiles.tolist()[2] == [128, 2, 0, 828]
+    assert P.portions8([(0, 2, 0, 300)], table, chunk=150).pages.tolist() == [[0, 4, 46, 0]]
+    for mask in (dict(window=-1), dict(keep=-1), dict(chunk=-3), dict(chunk=3, window=5)):
+        with pytest.raises(ValueError):
+            P.portions8([(0, 2, 0, 300)], table, **mask)
+
+
 @pytest.mark.parametrize("parts", [[], [(0, 0, 0, 0)], [(1, 3, 0, 0)], [(0, 3, 0, 0), (2, 3, 1, 0)], [(0, 3, 0, 0), (4, 3, 1, 0)], [(0, 3, 3, 0)], [(0, 3, -1, 0)], [(0, 3, 0, -1)],
                                    [(0, 3, 0, 254)], [(0, 1, 0, 256)], [(0, 3, 0, 0), (3, 3, 0, 3)]])
 def test_portions_that_are_refused(parts):

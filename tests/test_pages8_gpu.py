@@ -197,20 +197,20 @@ def test_append_of_what_is_no_number():
 
 def test_attention_over_what_is_no_number():
     """A key or a value that is no number leaves queries without a result that see it, and no others."""
-    for what in ("k", "v"):
+    for what, dtype in (("k", torch.float32), ("v", torch.float32), ("k", torch.bfloat16), ("v", torch.bfloat16)):
         s = Setup(H=4, G=2, dim=64, norm="", n_rot=0, slots=1, n_ctx=300, seed=3)
         x = s.rnd(200, s.ld)
         x[150, (s.nq if what == "k" else s.v_off) + 64 + 5] = math.nan           # KV head 1
         q, plan = torch.empty(200, 4, 64, device="cuda"), s.P.portions8([(0, 200, 0, 0)], s.table)
         s.P.append8(x.cuda(), s.k, s.v, s.table, q, portions=plan, **s.prep())
         for mask in (dict(), dict(window=20), dict(window=30, keep=4), dict(chunk=64)):
-            out = torch.zeros(200, 256, device="cuda")
-            s.P.attn_prompt8(q, s.k, s.v, plan, s.table, out, vdim=64, scale=0.1, **mask)
+            out = torch.zeros(200, 256, device="cuda", dtype=dtype)
+            s.P.attn_prompt8(q, s.k, s.v, s.P.portions8([(0, 200, 0, 0)], s.table, **mask), s.table, out, vdim=64, scale=0.1, **mask)
             sees = O.visible(torch.arange(200), 200, **mask)[:, 150].cuda()
             o = out.view(200, 4, 64)
             assert torch.isfinite(o[:, :2]).all() and torch.isfinite(o[~sees]).all() and o[sees][:, 2:].isnan().any(-1).all()
             for p in (150, 169, 170, 180, 199):                                    # a row appended again: its own key is none only at 150
-                y, out1 = x[p:p + 1].cuda(), torch.zeros(1, 256, device="cuda")
+                y, out1 = x[p:p + 1].cuda(), torch.zeros(1, 256, device="cuda", dtype=dtype)
                 s.P.attn_decode8(y, s.k, s.v, i32([p]), i32([0]), s.table, out1, n_ctx=300, scale=0.1, **s.prep(), **mask)
                 o1 = out1.view(4, 64)
                 assert torch.isfinite(o1[:2]).all() and (o1[2:].isnan().any(-1).all() if sees[p] else torch.isfinite(o1[2:]).all())
