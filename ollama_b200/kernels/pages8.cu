@@ -107,8 +107,18 @@ __device__ __forceinline__ float block_max(float v, float* red) {
     return m;
 }
 
-// Rows [row, row + n) at positions [pos, pos + n), all in one page, of KV head g.
-template <bool VEC>
+__device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory"); }
+__device__ __forceinline__ float peer_value(const float* p, int rank) {
+    uint32_t at;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at));
+    return v;
+}
+
+// Rows [row, row + n) at positions [pos, pos + n), all in one page, of KV head g.  PEERS: the CTAs of the cluster have a page's KV heads, and a norm over the whole row takes each
+// head's sum from its CTA.
+template <bool VEC, bool PEERS>
 __device__ void append_to_page(const Append8Args& a, int row, int n, int slot, int pos, int g, float* cs, float* red) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int page = page_at(a.t, a.c.n_pages, slot, pos >> PAGE_SHIFT);
@@ -126,6 +136,9 @@ __device__ void append_to_page(const Append8Args& a, int row, int n, int slot, i
             const float* p = a.qkv + (size_t)(row + r) * a.ldq;
             load_head<VEC>(p + nq + g * kdim, kdim, lane, k[i]);
             load_head<VEC>(p + a.v_off + g * a.vdim, a.vdim, lane, v[i]);
+        } else if (PEERS) {
+#pragma unroll
+            for (int j = 0; j < COLS; j++) k[i][j] = 0.f;
         }
     }
     __syncthreads();      // the tables may still be read for the rows before
@@ -136,6 +149,16 @@ __device__ void append_to_page(const Append8Args& a, int row, int n, int slot, i
         sn[i / half * pitch + i % half] = s * a.mscale;
     }
     __syncthreads();
+    __shared__ float own[PAGE];              // PEERS: sums of the head's rows
+    const bool whole = PEERS && a.k_norm && !a.head_norm;
+    if (whole) {
+#pragma unroll
+        for (int i = 0; i < PAGE / WARPS; i++) {
+            const float sum = warp_sum(square_sum(k[i]));      // rows behind the last one hold nothing that is used
+            if (lane == 0) own[warp + WARPS * i] = sum;
+        }
+        cluster_sync();
+    }
     float top_k = 0.f, top_v = 0.f;
 #pragma unroll
     for (int i = 0; i < PAGE / WARPS; i++) {
@@ -145,6 +168,8 @@ __device__ void append_to_page(const Append8Args& a, int row, int n, int slot, i
                 float s;
                 if (a.head_norm) {
                     s = square_sum(k[i]);
+                } else if (PEERS) {
+                    s = lane < G ? peer_value(own + r, lane) : 0.f;
                 } else {
                     const float* p = a.qkv + (size_t)(row + r) * a.ldq + nq;
                     s = 0.f;
@@ -191,14 +216,48 @@ __device__ void append_to_page(const Append8Args& a, int row, int n, int slot, i
             store_codes<VEC>(vp + (off + r) * hd, lane, hd, v[i], iv);
         }
     }
+    if (whole) cluster_sync();               // a peer may still read this CTA's sums
 }
 
-// Queries of one row, a warp a head.
+// Queries of one row, a warp a head; of the first HELD heads of a warp the values stay in registers between a norm over the row and the rotation.
+constexpr int HELD = 4;
+template <bool VEC>
+__device__ __forceinline__ void query_head(const Append8Args& a, int row, int h, float (&x)[COLS], float inv, const float* cs, const float* sn) {
+    const int lane = threadIdx.x & 31, hd = a.c.hd;
+    if (a.q_norm) {
+        if (a.head_norm) inv = 1.f / sqrtf(warp_sum(square_sum(x)) / (float)a.dim + a.eps);
+        const float* w = a.q_norm + (a.head_norm ? 0 : h * a.dim);
+#pragma unroll
+        for (int j = 0; j < COLS; j++) {
+            const int d = col<VEC>(lane, j);
+            if (d < a.dim) x[j] *= inv * __ldg(w + d);
+        }
+    }
+    rotate<VEC>(x, lane, a.dim, a.dim, a.n_rot, cs, sn);
+    // a map's query stands in the map's columns of an otherwise empty row
+    float* q = a.q_out + ((size_t)row * a.n_heads + h) * hd;
+    const int at = h % a.maps * a.dim;
+    if (VEC && a.maps == 1) {
+        if (4 * lane < hd) ((float4*)q)[lane] = make_float4(x[0], x[1], x[2], x[3]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < COLS; j++) {
+            const int d = col<VEC>(lane, j);
+            if (d < a.dim) q[at + d] = x[j];
+        }
+        for (int d = lane; d < hd; d += 32)
+            if (d < at || d >= at + a.dim) q[d] = 0.f;
+    }
+}
 template <bool VEC>
 __device__ void query_row(const Append8Args& a, int row, int pos, float* cs, float* red) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, half = a.n_rot >> 1, pitch = (half + 3) & ~3, nq = a.n_heads * a.dim, hd = a.c.hd;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, half = a.n_rot >> 1, pitch = (half + 3) & ~3, nq = a.n_heads * a.dim;
     float* sn = cs + pitch;
     const float* p = a.qkv + (size_t)row * a.ldq;
+    float x[HELD][COLS];
+#pragma unroll
+    for (int i = 0; i < HELD; i++)
+        if (warp + WARPS * i < a.n_heads) load_head<VEC>(p + (warp + WARPS * i) * a.dim, a.dim, lane, x[i]);
     for (int i = tid; i < half; i += THREADS) {
         float s, c;
         sincosf(rot_angle(pos, a.freqs[i]), &s, &c);
@@ -208,10 +267,13 @@ __device__ void query_row(const Append8Args& a, int row, int pos, float* cs, flo
     float inv = 1.f;
     if (a.q_norm && !a.head_norm) {
         float s = 0.f;
-        for (int c = 128 * warp; c < nq; c += 128 * WARPS) {
-            float x[COLS];
-            load_head<VEC>(p + c, nq - c, lane, x);
-            s += square_sum(x);
+#pragma unroll
+        for (int i = 0; i < HELD; i++)
+            if (warp + WARPS * i < a.n_heads) s += square_sum(x[i]);
+        for (int h = warp + WARPS * HELD; h < a.n_heads; h += WARPS) {
+            float y[COLS];
+            load_head<VEC>(p + h * a.dim, a.dim, lane, y);
+            s += square_sum(y);
         }
         s = warp_sum(s);
         if (lane == 0) red[warp] = s;
@@ -223,84 +285,75 @@ __device__ void query_row(const Append8Args& a, int row, int pos, float* cs, flo
     } else {
         __syncthreads();
     }
-    for (int h = warp; h < a.n_heads; h += WARPS) {
-        float x[COLS];
-        load_head<VEC>(p + h * a.dim, a.dim, lane, x);
-        if (a.q_norm) {
-            if (a.head_norm) inv = 1.f / sqrtf(warp_sum(square_sum(x)) / (float)a.dim + a.eps);
-            const float* w = a.q_norm + (a.head_norm ? 0 : h * a.dim);
 #pragma unroll
-            for (int j = 0; j < COLS; j++) {
-                const int d = col<VEC>(lane, j);
-                if (d < a.dim) x[j] *= inv * __ldg(w + d);
-            }
-        }
-        rotate<VEC>(x, lane, a.dim, a.dim, a.n_rot, cs, sn);
-        // a map's query stands in the map's columns of an otherwise empty row
-        float* q = a.q_out + ((size_t)row * a.n_heads + h) * hd;
-        const int at = h % a.maps * a.dim;
-        if (VEC && a.maps == 1) {
-            if (4 * lane < hd) ((float4*)q)[lane] = make_float4(x[0], x[1], x[2], x[3]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < COLS; j++) {
-                const int d = col<VEC>(lane, j);
-                if (d < a.dim) q[at + d] = x[j];
-            }
-            for (int d = lane; d < hd; d += 32)
-                if (d < at || d >= at + a.dim) q[d] = 0.f;
-        }
+    for (int i = 0; i < HELD; i++)
+        if (warp + WARPS * i < a.n_heads) query_head<VEC>(a, row, warp + WARPS * i, x[i], inv, cs, sn);
+    for (int h = warp + WARPS * HELD; h < a.n_heads; h += WARPS) {
+        load_head<VEC>(p + h * a.dim, a.dim, lane, x[0]);
+        query_head<VEC>(a, row, h, x[0], inv, cs, sn);
     }
 }
 
 // Norm of q and k, rotation, q to padded fp32 rows; k and v become codes of the pages they go to, whose units grow so that the largest magnitude fits.  A page whose first
-// position is among the rows begins anew.  CTAs: a KV head and a page of a portion each (its rows stay in registers between the largest magnitude and the codes, eight a
-// warp), then one a query row.
+// position is among the rows begins anew.  Of single rows a CTA has a KV head of a row, and then one the queries of a row.
 template <bool VEC>
 __global__ void __launch_bounds__(THREADS) append8_kernel(const __grid_constant__ Append8Args a) {
     extern __shared__ __align__(16) float cs[];
     __shared__ float red[WARPS];
     pdl_wait();
     pdl_launch();         // behind the wait: a kernel that starts now may read whatever was written before this one
-    const int G = a.c.kv_heads, units = a.positions ? a.rows : a.n_segs, kv_ctas = a.no_append ? 0 : units * a.per * G;
-    int b = blockIdx.x;
-    if (b < kv_ctas) {
-        const int g = b % G, j = b / G % a.per, u = b / G / a.per;
-        if (a.segs) {
-            const int4 s = a.segs[u];
-            const int first = (s.w >> PAGE_SHIFT) + j, lo = max(s.w, first * PAGE), hi = min(s.w + s.y, (first + 1) * PAGE);
-            if (s.w < 0 || s.x < 0 || s.x + s.y > a.rows || lo >= hi) return;
-            append_to_page<VEC>(a, s.x + lo - s.w, hi - lo, s.z, lo, g, cs, red);
-            return;
-        }
-        // rows of one slot take their turns in one CTA: the first of them appends them all, in order
-        const int slot = a.slots[u];
-        int before = 0, behind = 0;
-        for (int i = threadIdx.x; i < a.rows; i += THREADS)
-            if (a.slots[i] == slot) {
-                before |= i < u;
-                behind |= i > u;
-            }
-        if (__syncthreads_or(before)) return;
-        behind = __syncthreads_or(behind);
-        for (int i = u; i < (behind ? a.rows : u + 1); i++) {
-            if (a.slots[i] != slot || a.positions[i] < 0) continue;
-            append_to_page<VEC>(a, i, 1, slot, a.positions[i], g, cs, red);
-            __syncthreads();      // what it wrote is read by the next one's rescaling
-        }
+    const int G = a.c.kv_heads, kv_ctas = a.no_append ? 0 : a.rows * G, b = blockIdx.x;
+    if (b >= kv_ctas) {
+        const int pos = a.positions[b - kv_ctas];
+        if (pos >= 0) query_row<VEC>(a, b - kv_ctas, pos, cs, red);
         return;
     }
-    const int row = b - kv_ctas;
-    int pos = -1;
-    if (a.positions) {
-        pos = a.positions[row];
-    } else {
-        for (int i = 0; i < a.n_segs; i++) {
-            const int4 s = a.segs[i];
-            if (row >= s.x && row < s.x + s.y) pos = s.w + row - s.x;
+    // rows of one slot take their turns in one CTA: the first of them appends them all, in order
+    const int g = b % G, u = b / G, slot = a.slots[u];
+    int before = 0, behind = 0;
+    for (int i = threadIdx.x; i < a.rows; i += THREADS)
+        if (a.slots[i] == slot) {
+            before |= i < u;
+            behind |= i > u;
         }
+    if (__syncthreads_or(before)) return;
+    behind = __syncthreads_or(behind);
+    for (int i = u; i < (behind ? a.rows : u + 1); i++) {
+        if (a.slots[i] != slot || a.positions[i] < 0) continue;
+        append_to_page<VEC, false>(a, i, 1, slot, a.positions[i], g, cs, red);
+        __syncthreads();      // what it wrote is read by the next one's rescaling
     }
-    if (pos >= 0) query_row<VEC>(a, row, pos, cs, red);
+}
+
+// The same for portions of prompts, in two launches, since a page's rows stay in registers between the largest magnitude and the codes, eight a warp, and would leave the queries
+// two CTAs an SM (2048 rows of 32 heads on 8: 49 us in one).  Keys and values: a KV head and a page of a portion each.
+template <bool VEC, bool PEERS>
+__global__ void __launch_bounds__(THREADS, 2) append8_pages_kernel(const __grid_constant__ Append8Args a) {
+    extern __shared__ __align__(16) float cs[];
+    __shared__ float red[WARPS];
+    pdl_wait();
+    pdl_launch();
+    const int G = a.c.kv_heads, g = blockIdx.x % G, j = blockIdx.x / G % a.per;
+    const int4 s = a.segs[blockIdx.x / G / a.per];
+    const int first = (s.w >> PAGE_SHIFT) + j, lo = max(s.w, first * PAGE), hi = min(s.w + s.y, (first + 1) * PAGE);
+    if (s.w < 0 || s.x < 0 || s.x + s.y > a.rows || lo >= hi) return;
+    append_to_page<VEC, PEERS>(a, s.x + lo - s.w, hi - lo, s.z, lo, g, cs, red);
+}
+
+// Queries: a row each.  `behind`: launched behind the keys and values, which it does not read, while they are under way.
+template <bool VEC>
+__global__ void __launch_bounds__(THREADS, 4) append8_queries_kernel(const __grid_constant__ Append8Args a, int behind) {
+    extern __shared__ __align__(16) float cs[];
+    __shared__ float red[WARPS];
+    pdl_launch();
+    if (!behind) pdl_wait();
+    int pos = -1;
+    for (int i = 0; i < a.n_segs; i++) {
+        const int4 s = a.segs[i];
+        if ((int)blockIdx.x >= s.x && (int)blockIdx.x < s.x + s.y) pos = s.w + blockIdx.x - s.x;
+    }
+    if (pos >= 0) query_row<VEC>(a, blockIdx.x, pos, cs, red);
+    if (behind) pdl_wait();      // the launch does not end before the one it follows
 }
 
 // Pages as f16 values.  list: (slot, page of the slot, rows that are wanted); the rows behind them, and pages that are not there, become zeros.  clean: for attention whose products
@@ -360,21 +413,41 @@ int append8_launch(const Append8Args& in, int pdl, cudaStream_t st) {
         return (int)cudaErrorInvalidValue;
     const int kdim = a->maps * a->dim, nq = a->n_heads * a->dim;
     if (!a->no_append && (a->ldq < nq + a->c.kv_heads * kdim || a->v_off + a->c.kv_heads * a->vdim > a->ldq)) return (int)cudaErrorInvalidValue;
-    const long long ctas = (a->no_append ? 0ll : (a->positions ? (long long)a->rows : (long long)a->n_segs * a->per) * a->c.kv_heads) + a->rows;
-    if (ctas > 0x7fffffffll) return (int)cudaErrorInvalidValue;
+    const long long ctas = a->no_append ? 0 : a->positions ? (long long)a->rows * a->c.kv_heads : (long long)a->n_segs * a->per * a->c.kv_heads;
+    if (ctas + a->rows > 0x7fffffffll) return (int)cudaErrorInvalidValue;
     const bool vec = !((a->dim | a->vdim | a->ldq | a->v_off | (a->n_rot >> 1)) & 3) && !((uintptr_t)a->qkv & 15);
-    const int pitch = ((a->n_rot >> 1) + 3) & ~3, rows = a->positions ? 1 : PAGE;
-    const size_t smem = 2 * sizeof(float) * rows * (pitch ? pitch : 4);
+    const int pitch = ((a->n_rot >> 1) + 3) & ~3;
+    const size_t one = 2 * sizeof(float) * (pitch ? pitch : 4);      // cosines and sines of a row
     Append8Args copy = *a;
-    if (a->positions) copy.per = 1;
-    void* args[] = {&copy};
-    const void* fn = vec ? (const void*)append8_kernel<true> : (const void*)append8_kernel<false>;
-    static PerDeviceOnce once;
-    if (once.first()) {
-        cudaFuncSetAttribute(append8_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024);
-        cudaFuncSetAttribute(append8_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024);
+    if (a->positions) {
+        void* args[] = {&copy};
+        return launch_rows(vec ? (const void*)append8_kernel<true> : (const void*)append8_kernel<false>, dim3((unsigned)(ctas + a->rows)), dim3(THREADS), one, args, st, pdl);
     }
-    return launch_rows(fn, dim3((unsigned)ctas), dim3(THREADS), smem, args, st, pdl);
+    int behind = 0;
+    if (ctas) {
+        const bool peers = a->k_norm && !a->head_norm && a->c.kv_heads <= 8;      // clusters of as many CTAs
+        const void* fn = peers ? (vec ? (const void*)append8_pages_kernel<true, true> : (const void*)append8_pages_kernel<false, true>)
+                               : (vec ? (const void*)append8_pages_kernel<true, false> : (const void*)append8_pages_kernel<false, false>);
+        void* args[] = {&copy};
+        cudaLaunchAttribute at[2];
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)ctas);
+        cfg.blockDim = dim3(THREADS);
+        cfg.dynamicSmemBytes = PAGE * one;
+        cfg.stream = st;
+        at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[0].val.programmaticStreamSerializationAllowed = pdl ? 1 : 0;
+        at[1].id = cudaLaunchAttributeClusterDimension;
+        at[1].val.clusterDim.x = peers ? a->c.kv_heads : 1;
+        at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 2;
+        const int rc = (int)cudaLaunchKernelExC(&cfg, fn, args);
+        if (rc) return rc;
+        behind = 1;
+    }
+    void* args[] = {&copy, &behind};
+    return launch_rows(vec ? (const void*)append8_queries_kernel<true> : (const void*)append8_queries_kernel<false>, dim3(a->rows), dim3(THREADS), one, args, st, pdl || behind);
 }
 
 // Returns a cudaError_t value, as does the entry point below.
