@@ -21,48 +21,76 @@ __device__ __forceinline__ void load_head(const float* p, int n, int lane, float
     }
 }
 
-__device__ __forceinline__ float square_sum(const float (&x)[COLS]) { return x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3]; }
-
-// Rotation of a head row in the half-split order (of both maps' halves of a row that has two).  cs / sn: cosines and sines of the row's pairs.
+// x *= inv * w
 template <bool VEC>
-__device__ __forceinline__ void rotate(float (&x)[COLS], int lane, int n, int dim, int n_rot, const float* cs, const float* sn) {
-    const int half = n_rot >> 1;
-    if (half == 0) return;
-    float y[COLS];
-    if (VEC) {          // half and dim are multiples of four: a lane's four columns turn with the same lane's
-        const int d = 4 * lane, in = d >= dim ? d - dim : d;
-        const bool first = in < half, turns = in < n_rot && d < n;
-        const int other = first ? lane + (half >> 2) : lane - (half >> 2);
-#pragma unroll
-        for (int i = 0; i < COLS; i++) y[i] = __shfl_sync(0xffffffffu, x[i], other & 31);
-        if (turns) {
-            const float4 c = *(const float4*)(cs + (first ? in : in - half)), s = *(const float4*)(sn + (first ? in : in - half));
-            const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-            for (int i = 0; i < COLS; i++) x[i] = first ? x[i] * cc[i] - y[i] * ss[i] : x[i] * cc[i] + y[i] * ss[i];
+__device__ __forceinline__ void weigh(float (&x)[COLS], float inv, const float* w, int n, int lane) {
+    if (VEC) {
+        if (4 * lane < n) {
+            const float4 v = __ldg((const float4*)w + lane);
+            x[0] *= inv * v.x; x[1] *= inv * v.y; x[2] *= inv * v.z; x[3] *= inv * v.w;
         }
     } else {
-        float z[COLS];
 #pragma unroll
-        for (int i = 0; i < COLS; i++) {
-            const int d = lane + 32 * i, in = d >= dim ? d - dim : d;
-            const bool first = in < half, turns = in < n_rot && d < n;
-            const int o = turns ? (first ? d + half : d - half) : d;
-#pragma unroll
-            for (int j = 0; j < COLS; j++) {
-                const float v = __shfl_sync(0xffffffffu, x[j], o & 31);
-                if (o >> 5 == j) y[i] = v;
-            }
-            z[i] = x[i];
-            if (turns) {
-                const int p = first ? in : in - half;
-                z[i] = first ? x[i] * cs[p] - y[i] * sn[p] : x[i] * cs[p] + y[i] * sn[p];
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < COLS; i++) x[i] = z[i];
+        for (int i = 0; i < COLS; i++)
+            if (lane + 32 * i < n) x[i] *= inv * __ldg(w + lane + 32 * i);
     }
 }
+
+__device__ __forceinline__ float square_sum(const float (&x)[COLS]) { return x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3]; }
+
+// Rotation of head rows in the half-split order (of both maps' halves of a row that has two): x = c x + s y, y the other one of a column's pair.
+template <bool VEC>
+struct Turn {
+    float c[COLS], s[COLS];
+    int other[VEC ? 1 : COLS];               // where y is: a lane (whose columns turn with this lane's), or columns
+
+    // cs / sn: cosines and sines of the row's pairs; n: columns of the head row, of maps of dim columns
+    __device__ __forceinline__ Turn(int lane, int n, int dim, int n_rot, const float* cs, const float* sn) {
+        const int half = n_rot >> 1;
+        if (VEC) {          // half and dim are multiples of four
+            const int d = 4 * lane, in = d >= dim ? d - dim : d;
+            const bool first = in < half;
+            float4 co = make_float4(1.f, 1.f, 1.f, 1.f), si = make_float4(0.f, 0.f, 0.f, 0.f);
+            other[0] = lane;
+            if (in < n_rot && d < n) {
+                co = *(const float4*)(cs + (first ? in : in - half));
+                si = *(const float4*)(sn + (first ? in : in - half));
+                other[0] = first ? lane + (half >> 2) : lane - (half >> 2);
+            }
+            const float sign = first ? -1.f : 1.f;
+            c[0] = co.x; c[1] = co.y; c[2] = co.z; c[3] = co.w;
+            s[0] = sign * si.x; s[1] = sign * si.y; s[2] = sign * si.z; s[3] = sign * si.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < COLS; i++) {
+                const int d = lane + 32 * i, in = d >= dim ? d - dim : d;
+                const bool first = in < half, turns = in < n_rot && d < n;
+                c[i] = turns ? cs[first ? in : in - half] : 1.f;
+                s[i] = turns ? (first ? -sn[in] : sn[in - half]) : 0.f;
+                other[VEC ? 0 : i] = turns ? (first ? d + half : d - half) : d;
+            }
+        }
+    }
+    __device__ __forceinline__ void operator()(float (&x)[COLS]) const {
+        float y[COLS];
+#pragma unroll
+        for (int i = 0; i < COLS; i++) {
+            if (VEC) {
+                y[i] = __shfl_sync(0xffffffffu, x[i], other[0]);
+            } else {
+                const int o = other[VEC ? 0 : i];
+#pragma unroll
+                for (int j = 0; j < COLS; j++) {
+                    const float v = __shfl_sync(0xffffffffu, x[j], o & 31);
+                    if (o >> 5 == j) y[i] = v;
+                }
+            }
+        }
+        // a column that does not turn is not multiplied with another one, which may be infinite
+#pragma unroll
+        for (int i = 0; i < COLS; i++) x[i] = s[i] == 0.f ? x[i] * c[i] : fmaf(x[i], c[i], y[i] * s[i]);
+    }
+};
 
 // A lane's codes of a head row.
 template <bool VEC>
@@ -142,11 +170,36 @@ __device__ void append_to_page(const Append8Args& a, int row, int n, int slot, i
         }
     }
     __syncthreads();      // the tables may still be read for the rows before
-    for (int i = tid; i < n * half; i += THREADS) {
-        float s, c;
-        sincosf(rot_angle(pos + i / half, a.freqs[i % half]), &s, &c);
-        cs[i / half * pitch + i % half] = c * a.mscale;
-        sn[i / half * pitch + i % half] = s * a.mscale;
+    if (n == 1) {
+        for (int p = tid; p < half; p += THREADS) {
+            float si, co;
+            sincosf(rot_angle(pos, a.freqs[p]), &si, &co);
+            cs[p] = co * a.mscale;
+            sn[p] = si * a.mscale;
+        }
+    } else if (half > 0) {
+        // Row 8 i + j turns by the angle of row j and that of 8 i positions more: 16 angles a pair instead of 64 (half <= 64: four threads a pair).  The products of their cosines
+        // and sines are off by some 2^-23, the codes by up to 2^-4.
+        const int p = tid & 63, part = tid >> 6;
+        float* step = sn + PAGE * pitch;      // [16][2][pitch]: rows 0 .. 7, then 0, 8 .. 56 positions
+        if (p < half) {
+            const double f = a.freqs[p];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int e = 4 * part + i;
+                float si, co;
+                sincosf(rot_angle(e < 8 ? pos + e : 8 * (e - 8), f), &si, &co);
+                step[2 * e * pitch + p] = e < 8 ? co * a.mscale : co;
+                step[(2 * e + 1) * pitch + p] = e < 8 ? si * a.mscale : si;
+            }
+        }
+        __syncthreads();
+        if (p < half)
+            for (int r = part; r < n; r += 4) {
+                const float c0 = step[2 * (r & 7) * pitch + p], s0 = step[(2 * (r & 7) + 1) * pitch + p], c1 = step[2 * (8 + (r >> 3)) * pitch + p], s1 = step[(2 * (8 + (r >> 3)) + 1) * pitch + p];
+                cs[r * pitch + p] = c0 * c1 - s0 * s1;
+                sn[r * pitch + p] = s0 * c1 + c0 * s1;
+            }
     }
     __syncthreads();
     __shared__ float own[PAGE];              // PEERS: sums of the head's rows
@@ -159,6 +212,7 @@ __device__ void append_to_page(const Append8Args& a, int row, int n, int slot, i
         }
         cluster_sync();
     }
+    const float per_column = 1.f / (float)(a.head_norm ? a.dim : nk);
     float top_k = 0.f, top_v = 0.f;
 #pragma unroll
     for (int i = 0; i < PAGE / WARPS; i++) {
@@ -179,15 +233,9 @@ __device__ void append_to_page(const Append8Args& a, int row, int n, int slot, i
                         s += square_sum(x);
                     }
                 }
-                const float inv = 1.f / sqrtf(warp_sum(s) / (float)(a.head_norm ? a.dim : nk) + a.eps);
-                const float* w = a.k_norm + (a.head_norm ? 0 : g * kdim);
-#pragma unroll
-                for (int j = 0; j < COLS; j++) {
-                    const int d = col<VEC>(lane, j);
-                    if (d < kdim) k[i][j] *= inv * __ldg(w + d);
-                }
+                weigh<VEC>(k[i], rsqrtf(warp_sum(s) * per_column + a.eps), a.k_norm + (a.head_norm ? 0 : g * kdim), kdim, lane);
             }
-            rotate<VEC>(k[i], lane, kdim, a.dim, a.n_rot, cs + r * pitch, sn + r * pitch);
+            if (half > 0) Turn<VEC>(lane, kdim, a.dim, a.n_rot, cs + r * pitch, sn + r * pitch)(k[i]);
 #pragma unroll
             for (int j = 0; j < COLS; j++) {
                 top_k = fmaxf(top_k, fabsf(k[i][j]));
@@ -222,24 +270,19 @@ __device__ void append_to_page(const Append8Args& a, int row, int n, int slot, i
 // Queries of one row, a warp a head; of the first HELD heads of a warp the values stay in registers between a norm over the row and the rotation.
 constexpr int HELD = 4;
 template <bool VEC>
-__device__ __forceinline__ void query_head(const Append8Args& a, int row, int h, float (&x)[COLS], float inv, const float* cs, const float* sn) {
+__device__ __forceinline__ void query_head(const Append8Args& a, int row, int h, float (&x)[COLS], float inv, float per_column, const Turn<VEC>& turn) {
     const int lane = threadIdx.x & 31, hd = a.c.hd;
     if (a.q_norm) {
-        if (a.head_norm) inv = 1.f / sqrtf(warp_sum(square_sum(x)) / (float)a.dim + a.eps);
-        const float* w = a.q_norm + (a.head_norm ? 0 : h * a.dim);
-#pragma unroll
-        for (int j = 0; j < COLS; j++) {
-            const int d = col<VEC>(lane, j);
-            if (d < a.dim) x[j] *= inv * __ldg(w + d);
-        }
+        if (a.head_norm) inv = rsqrtf(warp_sum(square_sum(x)) * per_column + a.eps);
+        weigh<VEC>(x, inv, a.q_norm + (a.head_norm ? 0 : h * a.dim), a.dim, lane);
     }
-    rotate<VEC>(x, lane, a.dim, a.dim, a.n_rot, cs, sn);
+    if (a.n_rot > 0) turn(x);
     // a map's query stands in the map's columns of an otherwise empty row
     float* q = a.q_out + ((size_t)row * a.n_heads + h) * hd;
-    const int at = h % a.maps * a.dim;
     if (VEC && a.maps == 1) {
         if (4 * lane < hd) ((float4*)q)[lane] = make_float4(x[0], x[1], x[2], x[3]);
     } else {
+        const int at = a.maps > 1 && h & 1 ? a.dim : 0;
 #pragma unroll
         for (int j = 0; j < COLS; j++) {
             const int d = col<VEC>(lane, j);
@@ -250,14 +293,19 @@ __device__ __forceinline__ void query_head(const Append8Args& a, int row, int h,
     }
 }
 template <bool VEC>
-__device__ void query_row(const Append8Args& a, int row, int pos, float* cs, float* red) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, half = a.n_rot >> 1, pitch = (half + 3) & ~3, nq = a.n_heads * a.dim;
-    float* sn = cs + pitch;
+__device__ __forceinline__ void load_heads(const Append8Args& a, int row, float (&x)[HELD][COLS]) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const float* p = a.qkv + (size_t)row * a.ldq;
-    float x[HELD][COLS];
 #pragma unroll
     for (int i = 0; i < HELD; i++)
         if (warp + WARPS * i < a.n_heads) load_head<VEC>(p + (warp + WARPS * i) * a.dim, a.dim, lane, x[i]);
+}
+// x: load_heads of the row
+template <bool VEC>
+__device__ __forceinline__ void query_row(const Append8Args& a, int row, int pos, float (&x)[HELD][COLS], float* cs, float* red) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, half = a.n_rot >> 1, pitch = (half + 3) & ~3, nq = a.n_heads * a.dim;
+    float* sn = cs + pitch;
+    const float* p = a.qkv + (size_t)row * a.ldq;
     for (int i = tid; i < half; i += THREADS) {
         float s, c;
         sincosf(rot_angle(pos, a.freqs[i]), &s, &c);
@@ -281,16 +329,18 @@ __device__ void query_row(const Append8Args& a, int row, int pos, float* cs, flo
         s = 0.f;
 #pragma unroll
         for (int i = 0; i < WARPS; i++) s += red[i];
-        inv = 1.f / sqrtf(s / (float)nq + a.eps);
+        inv = rsqrtf(s / (float)nq + a.eps);
     } else {
         __syncthreads();
     }
+    const float per_column = 1.f / (float)a.dim;
+    const Turn<VEC> turn(lane, a.dim, a.dim, a.n_rot, cs, sn);
 #pragma unroll
     for (int i = 0; i < HELD; i++)
-        if (warp + WARPS * i < a.n_heads) query_head<VEC>(a, row, warp + WARPS * i, x[i], inv, cs, sn);
+        if (warp + WARPS * i < a.n_heads) query_head<VEC>(a, row, warp + WARPS * i, x[i], inv, per_column, turn);
     for (int h = warp + WARPS * HELD; h < a.n_heads; h += WARPS) {
         load_head<VEC>(p + h * a.dim, a.dim, lane, x[0]);
-        query_head<VEC>(a, row, h, x[0], inv, cs, sn);
+        query_head<VEC>(a, row, h, x[0], inv, per_column, turn);
     }
 }
 
@@ -305,7 +355,10 @@ __global__ void __launch_bounds__(THREADS) append8_kernel(const __grid_constant_
     const int G = a.c.kv_heads, kv_ctas = a.no_append ? 0 : a.rows * G, b = blockIdx.x;
     if (b >= kv_ctas) {
         const int pos = a.positions[b - kv_ctas];
-        if (pos >= 0) query_row<VEC>(a, b - kv_ctas, pos, cs, red);
+        if (pos < 0) return;
+        float x[HELD][COLS];
+        load_heads<VEC>(a, b - kv_ctas, x);
+        query_row<VEC>(a, b - kv_ctas, pos, x, cs, red);
         return;
     }
     // rows of one slot take their turns in one CTA: the first of them appends them all, in order
@@ -340,19 +393,22 @@ __global__ void __launch_bounds__(THREADS, 2) append8_pages_kernel(const __grid_
     append_to_page<VEC, PEERS>(a, s.x + lo - s.w, hi - lo, s.z, lo, g, cs, red);
 }
 
-// Queries: a row each.  `behind`: launched behind the keys and values, which it does not read, while they are under way.
+// Queries: a row each.  `behind`: launched behind the keys and values, which it does not read, while they are under way.  (CTAs that take several rows and have the next one's
+// values on their way: 32.8 us instead of 31.1 for 2048 rows of 32 heads on 8.)
 template <bool VEC>
 __global__ void __launch_bounds__(THREADS, 4) append8_queries_kernel(const __grid_constant__ Append8Args a, int behind) {
     extern __shared__ __align__(16) float cs[];
     __shared__ float red[WARPS];
     pdl_launch();
     if (!behind) pdl_wait();
+    float x[HELD][COLS];
+    load_heads<VEC>(a, blockIdx.x, x);
     int pos = -1;
     for (int i = 0; i < a.n_segs; i++) {
         const int4 s = a.segs[i];
         if ((int)blockIdx.x >= s.x && (int)blockIdx.x < s.x + s.y) pos = s.w + blockIdx.x - s.x;
     }
-    if (pos >= 0) query_row<VEC>(a, blockIdx.x, pos, cs, red);
+    if (pos >= 0) query_row<VEC>(a, blockIdx.x, pos, x, cs, red);
     if (behind) pdl_wait();      // the launch does not end before the one it follows
 }
 
@@ -415,7 +471,7 @@ int append8_launch(const Append8Args& in, int pdl, cudaStream_t st) {
     if (!a->no_append && (a->ldq < nq + a->c.kv_heads * kdim || a->v_off + a->c.kv_heads * a->vdim > a->ldq)) return (int)cudaErrorInvalidValue;
     const long long ctas = a->no_append ? 0 : a->positions ? (long long)a->rows * a->c.kv_heads : (long long)a->n_segs * a->per * a->c.kv_heads;
     if (ctas + a->rows > 0x7fffffffll) return (int)cudaErrorInvalidValue;
-    const bool vec = !((a->dim | a->vdim | a->ldq | a->v_off | (a->n_rot >> 1)) & 3) && !((uintptr_t)a->qkv & 15);
+    const bool vec = !((a->dim | a->vdim | a->ldq | a->v_off | (a->n_rot >> 1)) & 3) && !(((uintptr_t)a->qkv | (uintptr_t)a->q_norm | (uintptr_t)a->k_norm) & 15);
     const int pitch = ((a->n_rot >> 1) + 3) & ~3;
     const size_t one = 2 * sizeof(float) * (pitch ? pitch : 4);      // cosines and sines of a row
     Append8Args copy = *a;
@@ -433,7 +489,7 @@ int append8_launch(const Append8Args& in, int pdl, cudaStream_t st) {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)ctas);
         cfg.blockDim = dim3(THREADS);
-        cfg.dynamicSmemBytes = PAGE * one;
+        cfg.dynamicSmemBytes = (PAGE + 16) * one;
         cfg.stream = st;
         at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         at[0].val.programmaticStreamSerializationAllowed = pdl ? 1 : 0;
