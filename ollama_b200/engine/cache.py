@@ -2,12 +2,15 @@
 
 Keys and values live in pages of 64 positions taken from one pool: a slot owns the pages that cover its tokens and a table row says
 where each block of 64 positions is.  The pool is shared by all layer runs (a page has a place in every run's storage), so that its
-size is counted in tokens, not in sequences.  Recurrent layers keep a fixed-size state per slot.
+size is counted in tokens, not in sequences.  Recurrent layers keep a fixed-size state per slot.  Keys and values of attention heads may be held in 8 bits
+(``fp8``, see ops/pages8.py): E4M3 codes and a unit for each page and KV head.
 """
 from __future__ import annotations
 
 import numpy as np
 import torch
+
+from ..ops.pages8 import Pages8
 
 PAGE = 64
 
@@ -17,9 +20,9 @@ class CacheFull(RuntimeError):
 
 
 class PagedCache:
-    def __init__(self, n_slots: int, n_ctx: int, pool_tokens: int | None = None, device="cuda"):
+    def __init__(self, n_slots: int, n_ctx: int, pool_tokens: int | None = None, device="cuda", fp8: bool = False):
         """``n_ctx``: most tokens of one sequence; ``pool_tokens``: tokens the pool holds in all (default: every slot full)."""
-        self.n_slots, self.n_ctx, self.device = n_slots, n_ctx, device
+        self.n_slots, self.n_ctx, self.device, self.fp8 = n_slots, n_ctx, device, fp8
         self.max_pages = max(1, -(-n_ctx // PAGE))
         self.n_pages = max(1, -(-pool_tokens // PAGE) if pool_tokens is not None else n_slots * self.max_pages)
         self.free = list(range(self.n_pages - 1, -1, -1))
@@ -36,6 +39,14 @@ class PagedCache:
         t = torch.zeros(self.n_pages, kv_heads, PAGE, dim, device=self.device, dtype=dtype)
         self.paged.append(t)
         return t
+
+    def add_heads(self, kv_heads: int, dim: int, dtype) -> torch.Tensor | Pages8:
+        """Storage of one layer run's keys or values of attention heads, in 8 bits where the cache has them so and rows are 64 or 128 16-bit values."""
+        if not (self.fp8 and dtype == torch.float16 and dim in (64, 128)):
+            return self.add_pages(kv_heads, dim, dtype)
+        p = Pages8.empty(self.n_pages, kv_heads, dim, self.device)
+        self.paged += [p.codes, p.unit]
+        return p
 
     def add_state(self, *shape: int) -> torch.Tensor:
         t = torch.zeros(self.n_slots, *shape, device=self.device, dtype=torch.float32)

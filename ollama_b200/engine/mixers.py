@@ -6,12 +6,26 @@ import torch
 
 from .. import envconfig
 from ..models.stack import AttentionMixer, Mamba2Mixer
+from ..ops import pages8 as P8
 from ..ops import rows as O
 from ..ops import ssd as D
 from .blocks import Mat, Norm, Step, WeightSource, up
 
 
 MIN_SPLIT = 128                  # keys
+
+
+def attend8(be, m, decode: bool, qkv, kc: P8.Pages8, vc: P8.Pages8, out, hd: int, buf, diff, prep: dict, mask: dict) -> int:
+    """Attention of a step's rows over an 8-bit cache; ``buf(name, columns, type)``: row buffers.  Returns the launches."""
+    table, heads = be.cache.table, prep["heads"]
+    if decode:
+        P8.attn_decode8(qkv, kc, vc, m.positions, m.slots, table, out, n_ctx=be.n_ctx, diff=diff, **prep, **mask)
+        return 3
+    q = buf("q", heads * hd, torch.float32).view(qkv.shape[0], heads, hd)
+    portions = m.portions(table, **{k: mask[k] for k in ("window", "keep", "chunk") if k in mask})
+    P8.append8(qkv, kc, vc, table, q, portions=portions, **prep)
+    P8.attn_prompt8(q, kc, vc, portions, table, out, vdim=prep["vdim"], diff=diff, **mask)
+    return 4
 
 
 class HeadAttention:
@@ -70,7 +84,8 @@ class HeadAttention:
     def make_cache(self, cache, kv: tuple[torch.Tensor, ...] | None = None) -> tuple[torch.Tensor, ...]:
         """``kv``: the memory of the layer run whose keys and values are used."""
         ty = torch.float32 if self.f32 else torch.float16
-        mem = (cache.add_pages(self.m.kv_heads, self.dk, ty), cache.add_pages(self.m.kv_heads, self.dv, ty)) if kv is None else kv[:2]
+        add = cache.add_heads if self.hd else cache.add_pages
+        mem = (add(self.m.kv_heads, self.dk, ty), add(self.m.kv_heads, self.dv, ty)) if kv is None else kv[:2]
         return mem if self.conv_w is None else (*mem, cache.add_state(max(self.m.conv - 1, 1), self.n8))
 
     def splits(self, nb: int, n_ctx: int, sms: int) -> tuple[int, int]:
@@ -113,6 +128,9 @@ class HeadAttention:
         prep = dict(heads=heads, maps=m.maps, append=m.kv_from is None, dim=m.dim, vdim=m.vdim, q_norm=self.q_norm, k_norm=self.k_norm, eps=be.stack.eps, freqs=self.freqs, n_rot=self.n_rot,
                     head_norm=m.qk_norm == "head", v_off=self.v_off, mscale=self.magnitude, pdl=s.pdl)
         mask = dict(scale=m.scale, softcap=m.softcap, chunk=m.chunk, window=m.window, keep=m.keep, gate=gate)
+        if isinstance(kc, P8.Pages8):
+            s.launched(attend8(be, s.m, s.decode, qkv, kc, vc, out, self.hd, s.buf, diff, prep, mask))
+            return
         s.launched(2)
         if s.decode and self.hd:
             n, keys = self.splits(nb, be.n_ctx, be.sms)

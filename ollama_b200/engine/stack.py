@@ -30,11 +30,12 @@ from ..models.config import ModelConfig, config_from_gguf
 from ..models.stack import AttentionMixer, DenseMLP, ExpertMLP, LatentMixer, LayerRun, Mamba2Mixer, MambaMixer
 from ..models.weights import QWeight, load_tensor
 from ..ops import cuda as K
+from ..ops import pages8 as P8
 from ..ops import reference as R
 from ..ops import rows as O
 from .blocks import LONG_PORTION, ExpertFFN, GatedFFN, LatentAttention, LongPortions, Mat, Norm, SideInput, Step, WeightSource, make_norm, up
 from .cache import CacheFull, PagedCache
-from .mixers import HeadAttention, StateSpaceHeads
+from .mixers import HeadAttention, StateSpaceHeads, attend8
 from .shared import DepthAverage, SharedNormLayer
 from .steps import StepEngine
 
@@ -68,9 +69,17 @@ class _Meta:
     """Device arrays that describe the rows of a step."""
 
     def __init__(self, tokens, positions, slots, offs=None, segs=None, tiles=None, half_tiles=None, long: dict[int, LongPortions] | None = None,
-                 longest: int = 1):
+                 longest: int = 1, parts: Sequence[tuple[int, int, int, int]] = ()):
+        self.parts, self._portions = parts, {}       # (first row, rows, slot, position of the first row) of each portion
         self.tokens, self.positions, self.slots, self.offs, self.segs, self.tiles, self.half_tiles = tokens, positions, slots, offs, segs, tiles, half_tiles
         self.long, self.longest = long, longest      # by window (0: none); rows of the longest portion
+
+    def portions(self, table: torch.Tensor, **mask: int) -> P8.Portions8:
+        """The portions as attention over 8-bit caches takes them, made once for each mask."""
+        key = tuple(sorted(mask.items()))
+        if key not in self._portions:
+            self._portions[key] = P8.portions8(self.parts, table, **mask)
+        return self._portions[key]
 
 
 class StackBackend(StepEngine):
@@ -90,8 +99,9 @@ class StackBackend(StepEngine):
         self.f32 = dtype == "float32"
         self.act_dtype = torch.float32 if self.f32 else torch.bfloat16
         kv_type = (getattr(opts, "kv_cache_type", None) or "f16").lower()
-        if kv_type != "f16":
-            logging.getLogger("ollama_b200.engine").warning("K/V cache type %s is stored as f16 (stack models have no quantised cache)", kv_type)
+        self.fp8 = kv_type == "fp8" and not self.f32       # heads of up to 128 columns; other layers and 32-bit models keep theirs
+        if kv_type != "f16" and not self.fp8:
+            logging.getLogger("ollama_b200.engine").warning("K/V cache type %s is stored as %s (the 8-bit cache of 16-bit stack models is fp8)", kv_type, "f32" if self.f32 else "f16")
         self._init_steps()
         self.supports_verify = not self.cfg.recurrent
         self.max_batch = MAX_DECODE_ROWS
@@ -267,9 +277,9 @@ class StackBackend(StepEngine):
         """``pool_tokens``: positions the page pool holds for all slots together (default: every slot can fill its context)."""
         dev = self.device
         self.n_slots, self.n_ctx = n_slots, n_ctx
-        self.cache = PagedCache(n_slots, n_ctx, pool_tokens, dev)
+        self.cache = PagedCache(n_slots, n_ctx, pool_tokens, dev, self.fp8)
         kv_dt = torch.float32 if self.f32 else torch.float16
-        self.mem: list[tuple[torch.Tensor, torch.Tensor]] = []        # per layer run: (keys, values) or (state, convolution inputs)
+        self.mem: list[tuple] = []        # per layer run: (keys, values) or (state, convolution inputs)
         for r in self.runs:
             L = self.layers[r.layer]
             if not self.stack.design.paired:
@@ -277,7 +287,8 @@ class StackBackend(StepEngine):
                 kv = {} if j is None else {"kv": next(self.mem[k] for k in reversed(range(len(self.mem))) if self.runs[k].layer == j)}
                 self.mem.append(L.mix.make_cache(self.cache, **kv))
             elif isinstance(L.mixer, AttentionMixer):
-                self.mem.append((self.cache.add_pages(L.mixer.kv_heads, L.dk, kv_dt), self.cache.add_pages(L.mixer.kv_heads, L.dv, kv_dt)))
+                add = self.cache.add_heads if L.hd else self.cache.add_pages
+                self.mem.append((add(L.mixer.kv_heads, L.dk, kv_dt), add(L.mixer.kv_heads, L.dv, kv_dt)))
             else:
                 self.mem.append((self.cache.add_state(L.inner, L.mixer.state), self.cache.add_state(max(L.mixer.conv - 1, 1), L.inner)))
         MB, i32 = self.max_batch, torch.int32
@@ -385,6 +396,11 @@ class StackBackend(StepEngine):
     def _attention(self, L, mem, qkv, out, B, m, decode, pdl) -> None:
         mx, (kc, vc), b, nb = L.mixer, mem, self.buf, qkv.shape[0]
         table = self.cache.table
+        if isinstance(kc, P8.Pages8):
+            prep = dict(heads=mx.heads, dim=mx.dim, vdim=mx.vdim, q_norm=L.q_norm, k_norm=L.k_norm, eps=self.stack.eps, freqs=L.freqs, n_rot=L.n_rot, pdl=pdl)
+            self._n += attend8(self, m, decode, qkv, kc, vc, out, L.hd, lambda name, cols, ty: B.get(name, cols, ty, nb), O.NO_DIFF, prep,
+                               dict(scale=mx.scale, softcap=mx.softcap, chunk=mx.chunk))
+            return
         if decode and L.hd and O.attn_decode_paged(
                 qkv, kc, vc, m.positions, m.slots, table, out, nb, heads=mx.heads, dim=mx.dim, vdim=mx.vdim, q_norm=L.q_norm, k_norm=L.k_norm,
                 eps=self.stack.eps, freqs=L.freqs, n_rot=L.n_rot, scale=mx.scale, softcap=mx.softcap, chunk=mx.chunk, n_splits=L.n_splits, n_ctx=L.keys,
@@ -531,6 +547,8 @@ class StackBackend(StepEngine):
     def _forward_rows(self, segs: Sequence[tuple[int, Sequence[int], int]], x=None, embeds=None, spans=(), tap=None) -> torch.Tensor:
         """Rows of several sequences, each portion ``(slot, tokens, position of the first)``; returns the hidden rows in order."""
         dev = self.device
+        if self.fp8 and len({s for s, _, _ in segs}) < len(segs):
+            raise ValueError("two portions of one slot in a step on an 8-bit cache")      # a page's unit follows from all its new rows
         self._reserve([s for s, _, _ in segs], [p0 + len(t) for _, t, p0 in segs])
         total = sum(len(t) for _, t, _ in segs)
         cols = np.empty((4, total), np.int32)           # tokens | positions | slots | offset in the portion
@@ -570,7 +588,7 @@ class StackBackend(StepEngine):
             rows = torch.tensor(rest, dtype=torch.int32).to(dev) if rest else None
             self.h2d_bytes += 4 * len(rest)
             long = {w: LongPortions(parts[3 + 2 * i], parts[4 + 2 * i], sum(count), max(count), rows) for i, (w, (_, _, count)) in enumerate(longs.items())}
-        m = _Meta(meta[0], meta[1], meta[2], meta[3], *parts[:2], parts[2] if halves else None, long, max(len(t) for _, t, _ in segs))
+        m = _Meta(meta[0], meta[1], meta[2], meta[3], *parts[:2], parts[2] if halves else None, long, max(len(t) for _, t, _ in segs), seg_rows)
         self._n = 0
         out = self._run_rows(_Rows(at, dev), m, at, decode=False, tap=tap)
         self.kernel_launches += self._n

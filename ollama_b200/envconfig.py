@@ -311,7 +311,7 @@ def as_map() -> dict[str, tuple[object, str]]:
     return {
         "OLLAMA_DEBUG": (log_level(), "Show additional debug information (e.g. OLLAMA_DEBUG=1)"),
         "OLLAMA_FLASH_ATTENTION": (flash_attention(), "Enabled flash attention"),
-        "OLLAMA_KV_CACHE_TYPE": (kv_cache_type(), "Quantization type for the K/V cache (default: f16)"),
+        "OLLAMA_KV_CACHE_TYPE": (kv_cache_type(), "Quantization type for the K/V cache: f16, q8_0, or for stack models fp8 (default: f16)"),
         "OLLAMA_GPU_OVERHEAD": (gpu_overhead(), "Reserve a portion of VRAM per GPU (bytes)"),
         "OLLAMA_HOST": (str(host()), "IP Address for the ollama server (default 127.0.0.1:11434)"),
         "OLLAMA_KEEP_ALIVE": (keep_alive(), "The duration that models stay loaded in memory (default \"5m\")"),

@@ -181,6 +181,13 @@ class Mamba2Mixer:
         return self.inner + 2 * self.groups * self.state
 
 
+def row8(m) -> int:
+    """Columns of a row in an 8-bit cache of the mixer's heads; 0: they have none."""
+    if not isinstance(m, AttentionMixer) or (big := max(m.maps * m.dim, m.vdim)) > 128:
+        return 0
+    return 64 if big <= 64 else 128
+
+
 Mixer = AttentionMixer | LatentMixer | GruMixer | MambaMixer | Mamba2Mixer
 
 
@@ -262,11 +269,20 @@ class Stack:
         return ([LayerRun(i, False) for i in range(lo)] + [LayerRun(i, i == lo, t) for t in range(times) for i in range(lo, hi)]
                 + [LayerRun(i, False) for i in range(hi, len(self.layers))])
 
-    def kv_bytes_per_token(self, elem_bytes: int = 2) -> int:
-        """Cache bytes of one position over all layer runs."""
+    def kv_bytes_per_token(self, elem_bytes: int = 2, fp8: bool = False) -> int:
+        """Cache bytes of one position over all layer runs.  ``fp8``: heads of up to 128 columns in codes of a byte (rows of 64 or 128), with a unit for 64 positions."""
         ms = [self.layers[r.layer].mixer for r in self.runs()]
+        if fp8:
+            eight = [m for m in ms if row8(m) and m.kv_from is None]
+            return sum(2 * m.kv_heads * row8(m) + -(-2 * 4 * m.kv_heads // 64) for m in eight) + \
+                sum(m.kv_heads * (m.maps * m.dim + m.vdim) for m in ms if isinstance(m, AttentionMixer) and not row8(m) and m.kv_from is None) * elem_bytes + \
+                sum(m.kv_rank + m.rot_dim for m in ms if isinstance(m, LatentMixer)) * elem_bytes
         return (sum(m.kv_heads * (m.maps * m.dim + m.vdim) for m in ms if isinstance(m, AttentionMixer) and m.kv_from is None)
                 + sum(m.kv_rank + m.rot_dim for m in ms if isinstance(m, LatentMixer))) * elem_bytes
+
+    def read_out_bytes(self) -> int:
+        """Bytes a position that a prompt reads out of an fp8 cache into 16 bits, of the layer with most."""
+        return max((4 * L.mixer.kv_heads * row8(L.mixer) for L in self.layers if row8(L.mixer)), default=0)
 
     def state_bytes(self) -> int:
         """Recurrent state of one sequence over all layer runs (fp32)."""

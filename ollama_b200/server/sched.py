@@ -127,15 +127,17 @@ def predict_memory(model: Any, num_ctx: int, num_parallel: int, free: int | None
     if isinstance(kv.get(f"{arch}.stack"), str):     # layers of different kinds: their own count of cache and state
         from ..models.stack import parse_stack
         st = parse_stack(kv[f"{arch}.stack"])
-        return size + num_parallel * (st.kv_bytes_per_token() * num_ctx + st.state_bytes())
+        fp8 = (envconfig.kv_cache_type() or "f16").lower() == "fp8" and (envconfig.compute_dtype() or "bfloat16") != "float32"
+        read_out = st.read_out_bytes() * num_ctx if fp8 else 0           # a prompt's attention reads a layer's rows of one sequence as f16
+        return size + num_parallel * (st.kv_bytes_per_token(fp8=fp8) * num_ctx + st.state_bytes()) + read_out
     layers = _first_int(kv.get(f"{arch}.block_count"))
     heads = _first_int(kv.get(f"{arch}.attention.head_count"), 1) or 1
     kvh = _first_int(kv.get(f"{arch}.attention.head_count_kv"), heads) or heads
     d = _first_int(kv.get(f"{arch}.embedding_length"))
     hd = _first_int(kv.get(f"{arch}.attention.key_length"), d // heads if heads else 0)
     per_elem, expanded = 2.0, 0                      # f16 cache
-    if (envconfig.kv_cache_type() or "f16").lower() in ("q8_0", "q4_0") and hd % 32 == 0:
-        per_elem = 1.0 + 2.0 / 32                    # int8 + one f16 scale per 32 dims (q4_0 requests are served as q8_0)
+    if (envconfig.kv_cache_type() or "f16").lower() in ("q8_0", "q4_0", "fp8") and hd % 32 == 0:
+        per_elem = 1.0 + 2.0 / 32                    # int8 + one f16 scale per 32 dims (q4_0 and fp8 requests are served as q8_0)
         if hd in (64, 128):
             expanded = 2 * kvh * hd * num_ctx * 2    # a prompt's attention reads a layer's rows of one sequence as f16
     extra = sum(os.path.getsize(p) for p in list(getattr(model, "draft_paths", None) or []) if os.path.exists(p))

@@ -65,3 +65,40 @@ def test_the_definition():
     assert torch.equal(O.e4m3(x), x.float().to(torch.float8_e4m3fn).double())
     top = torch.tensor([0.0, 448.0, 448.1, 1.0, 3.5, 3.6, 57344.0, 1e9, 2.0 ** -20], dtype=torch.float64)
     assert O.unit_for(top).tolist() == [2.0 ** -15, 1.0, 2.0, 2.0 ** -8, 2.0 ** -7, 2.0 ** -6, 128.0, 128.0, 2.0 ** -15]
+
+
+def test_bytes_that_the_scheduler_counts(monkeypatch):
+    """Heads in codes of a byte with rows of 64 or 128, eight bytes of units for 64 positions and KV head, and a layer's rows as f16 for prompts."""
+    import json
+
+    from ollama_b200.models.stack import parse_stack
+    from ollama_b200.models.synth import STACK_SPECS
+    from ollama_b200.server.sched import predict_memory
+    st = parse_stack(STACK_SPECS["vazatar-1b"])
+    layers = sum(type(st.layers[r.layer].mixer).__name__ == "AttentionMixer" for r in st.runs())
+    assert st.kv_bytes_per_token() == layers * 2 * 4 * 128 * 2 and st.kv_bytes_per_token(fp8=True) == layers * (2 * 4 * 128 + 1) and st.read_out_bytes() == 4 * 4 * 128
+    latents = parse_stack(STACK_SPECS["kavenex-1b"])
+    assert latents.kv_bytes_per_token(fp8=True) == latents.kv_bytes_per_token() and latents.read_out_bytes() == 0
+
+    class Model:
+        size = 1 << 30
+
+        def kv(self):
+            return {"general.architecture": "vazatar", "vazatar.stack": json.dumps(STACK_SPECS["vazatar-1b"])}
+    for kind, dtype, each, more in (("f16", "", 2 * 4 * 128 * 2, 0), ("fp8", "", 2 * 4 * 128 + 1, 4 * 4 * 128), ("q8_0", "", 2 * 4 * 128 * 2, 0), ("fp8", "float32", 2 * 4 * 128 * 2, 0)):
+        monkeypatch.setenv("OLLAMA_KV_CACHE_TYPE", kind)
+        monkeypatch.setenv("B200_DTYPE", dtype)
+        assert predict_memory(Model(), 4096, 3) == (1 << 30) + 3 * (layers * each * 4096 + st.state_bytes()) + more * 4096
+
+
+def test_storage_of_the_paged_cache():
+    from ollama_b200.engine.cache import PagedCache
+    c = PagedCache(2, 100, device="cpu", fp8=True)
+    a, b, d = c.add_heads(3, 64, torch.float16), c.add_heads(3, 64, torch.float32), c.add_pages(1, 96, torch.float16)
+    assert isinstance(a, P.Pages8) and a.codes.shape == (4, 3, 64, 64) and b.dtype == torch.float32 and d.dtype == torch.float16
+    assert isinstance(PagedCache(2, 100, device="cpu").add_heads(3, 64, torch.float16), torch.Tensor)
+    c.reserve(0, 70)
+    a.codes[c.owned[0][1], 1, 5] = 9
+    a.unit[c.owned[0][1], 1] = 4.0
+    c.copy(0, 1, 70)
+    assert (a.codes[c.owned[1][1], 1, 5] == 9).all() and a.unit[c.owned[1][1], 1] == 4.0 and len(c.paged) == 4
