@@ -8,7 +8,7 @@
 // keys, in turns of 32, are shared by as many CTAs as its part of all turns is of the CTAs that fit the GPU, so that a CTA has one item (CTAs with an equal share of all turns each
 // took 80 to 86 us where one item ended inside it and 60 to 72 elsewhere); its warps take the turns in rotation, each through a ring of its own that TMA fills, so that nothing in
 // the loop waits for another warp.  A CTA leaves (largest score, sum, unnormalised result), which the merge kernel adds up.
-#include "pages8.cuh"
+#include "attn_pages8.cuh"
 #include "tc_common.cuh"
 
 __device__ int g_attn8_status = 0;
@@ -18,106 +18,8 @@ namespace {
 using namespace tc;
 
 constexpr int TURN = 32;                     // keys
-constexpr int MAX_UNITS = 256;               // sequences of a launch
 constexpr int BATCH = 128;                   // turns whose places are looked up at a time
-constexpr int LEAST = 8;                     // turns of a CTA, where there are as many
 constexpr int MERGE_THREADS = 256;
-constexpr float LOG2E = 1.4426950408889634f;
-constexpr float NONE = -1e30f;               // largest score of no keys
-
-// The rows of one sequence in the launch.
-struct Unit {
-    int row, rows, slot, pos;                // first row, rows (0: no token), slot, position of the first row
-    int open;                                // first page of the slot that rows of the step go to
-    int parts;                               // CTAs of each of its items
-};
-
-__device__ __forceinline__ Unit unit_at(const Attn8Args& a, int u) {
-    Unit s;
-    if (a.positions) {
-        s = Unit{u, 1, a.slots[u], a.positions[u], 0, 0};
-    } else {
-        const int4 g = a.segs[u];
-        s = Unit{g.x, g.y, g.z, g.w, 0, 0};
-    }
-    if ((unsigned)s.slot >= (unsigned)a.t.n_slots || s.pos < 0 || s.row < 0 || s.row + s.rows > a.rows || s.pos + s.rows > a.t.max_pages * PAGE) s.rows = 0;
-    s.open = s.pos >> PAGE_SHIFT;
-    return s;
-}
-
-// Turns of a unit's items: those with kept keys first, then the ones from the first row's first key on.
-struct Keys {
-    int base, front, turns;
-};
-__device__ __forceinline__ Keys keys_of(const Attn8Args& a, const Unit& s) {
-    Keys k;
-    k.base = first_key(s.pos, a.chunk, a.window) & ~(TURN - 1);
-    k.front = a.window > 0 ? kept_tiles(a.keep, k.base, TURN) : 0;
-    k.turns = s.rows > 0 ? k.front + (s.pos + s.rows - k.base + TURN - 1) / TURN : 0;
-    return k;
-}
-__device__ __forceinline__ int first_of(const Keys& k, int turn) { return turn < k.front ? turn * TURN : k.base + (turn - k.front) * TURN; }
-
-// Items of a unit: row_tile rows of (row, head of the KV head) each, of every KV head.
-__device__ __forceinline__ int row_tiles(const Attn8Args& a, const Unit& s) { return (s.rows * (a.n_heads / a.c.kv_heads) + a.row_tile - 1) / a.row_tile; }
-
-// Sum of the threads' numbers up to each and over all; at least MAX_UNITS threads, `sums` has one place a warp.
-__device__ __forceinline__ uint32_t scan(uint32_t x, uint32_t* sums, uint32_t& all) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-    }
-    __syncthreads();
-    if (lane == 31) sums[warp] = x;
-    __syncthreads();
-    all = 0;
-    for (int w = 0; w < MAX_UNITS / 32; w++) {
-        if (w == warp) x += all;
-        all += sums[w];
-    }
-    return x;
-}
-
-// All units, and the CTAs before each one's (prefix[u]) and in all (prefix[units]).
-__device__ __forceinline__ void deal_out(const Attn8Args& a, int units, Unit* list, uint32_t* prefix, uint32_t* sums) {
-    const int tid = threadIdx.x;
-    Unit s;
-    uint32_t turns = 0, items = 0, total, ctas;
-    if (tid < units) {
-        s = unit_at(a, tid);
-        list[tid] = s;
-        turns = keys_of(a, s).turns;
-        items = row_tiles(a, s) * a.c.kv_heads;
-    }
-    scan(turns * items, sums, total);
-    const uint32_t parts = turns ? max(1u, min((uint32_t)((unsigned long long)turns * a.ctas / total), (turns + LEAST - 1) / LEAST)) : 0;
-    const uint32_t x = scan(parts * items, sums, ctas);
-    if (tid < units) {
-        prefix[tid] = x - parts * items;
-        if (a.behind)        // other rows of the slot may go to earlier pages
-            for (int i = 0; i < units; i++)
-                if (list[i].slot == s.slot && list[i].pos >= 0) s.open = min(s.open, list[i].pos >> PAGE_SHIFT);
-    }
-    if (tid == 0) prefix[units] = ctas;
-    __syncthreads();
-    if (tid < units) {
-        s.parts = parts;
-        list[tid] = s;
-    }
-    __syncthreads();
-}
-
-__device__ __forceinline__ int unit_of(const uint32_t* prefix, int units, uint32_t x) {
-    int lo = 0, hi = units - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (prefix[mid] <= x) lo = mid;
-        else hi = mid - 1;
-    }
-    return lo;               // of units without turns, the one behind them
-}
 
 __device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -169,7 +71,7 @@ struct Place {
 
 __device__ __forceinline__ Place place_of(const Attn8Args& a, const Unit& s, const Keys& k, int g, int turn) {
     Place p;
-    const int n0 = first_of(k, turn), page = max(page_at(a.t, a.c.n_pages, s.slot, n0 >> PAGE_SHIFT), 0);
+    const int n0 = first_of(k, TURN, turn), page = max(page_at(a.t, a.c.n_pages, s.slot, n0 >> PAGE_SHIFT), 0);
     const size_t head = (size_t)page * a.c.kv_heads + g;
     p.y = (int)(head * PAGE) + (n0 & (PAGE - 1));
     p.ku = __ldcg(a.c.ku + head);
@@ -539,7 +441,7 @@ bool bad_args(const Attn8Args& a) {
     return !a.q || !a.c.k || !a.c.v || !a.c.ku || !a.c.vu || a.c.n_pages < 1 || (a.c.hd != 64 && a.c.hd != 128) || a.c.kv_heads < 1 || a.n_heads < 1 || a.n_heads % a.c.kv_heads ||
            a.n_heads > 65535 || a.rows < 1 || a.rows > 65535 || a.vdim < 1 || a.vdim > a.c.hd || !a.t.table || a.t.n_slots < 1 || a.t.max_pages < 1 || a.t.max_pages > (1 << 24) ||
            (!a.positions == !a.segs) || (a.positions && !a.slots) || (a.segs && a.n_segs < 1) || a.chunk < 0 || a.window < 0 || a.keep < 0 || (a.chunk && a.window) || a.softcap < 0.f ||
-           (a.row_tile != 8 && a.row_tile != 16) || a.tiles < 1 || a.ctas < 1 || !a.part_acc || !a.part_ml || !a.out || a.gate.kind < 0 || a.gate.kind > 2 || (a.gate.kind && !a.gate.g) ||
+           !((a.row_tile == 128 && a.turn == 128) || ((a.row_tile == 8 || a.row_tile == 16) && a.turn == TURN)) || a.tiles < 1 || a.ctas < 1 || !a.part_acc || !a.part_ml || !a.out || a.gate.kind < 0 || a.gate.kind > 2 || (a.gate.kind && !a.gate.g) ||
            (a.diff.on && (a.n_heads / a.c.kv_heads & 1)) || a.ldo < (a.diff.on ? a.n_heads / 2 : a.n_heads) * a.vdim ||
            (((uintptr_t)a.c.k | (uintptr_t)a.c.v | (uintptr_t)a.q | (uintptr_t)a.part_acc) & 15) || ((uintptr_t)a.part_ml & 7) || (size_t)a.c.n_pages * a.c.kv_heads * PAGE >= ((size_t)1 << 31);
 }
@@ -571,6 +473,7 @@ int launch(Attn8Args& a, int pdl, cudaStream_t st) {
     return launch_rows((const void*)attn8_kernel<D, NB>, dim3(a.ctas + units * a.tiles * a.c.kv_heads), dim3(L::THREADS), L::TOTAL, args, st, pdl);
 }
 int launch(Attn8Args& a, int pdl, cudaStream_t st) {
+    if (a.row_tile == 128) return attn8_tc_launch(a, a.ctas + (a.positions ? a.rows : a.n_segs) * a.tiles * a.c.kv_heads, pdl, st);
     if (a.c.hd == 128) return a.row_tile == 8 ? launch<128, 1>(a, pdl, st) : launch<128, 2>(a, pdl, st);
     return a.row_tile == 8 ? launch<64, 1>(a, pdl, st) : launch<64, 2>(a, pdl, st);
 }
@@ -628,5 +531,5 @@ B2_API int b2_attn8_status() {
     int v = 0, none = 0;
     if (cudaMemcpyFromSymbol(&v, g_attn8_status, sizeof(int)) != cudaSuccess) return -1;
     if (v) cudaMemcpyToSymbol(g_attn8_status, &none, sizeof(int));
-    return v;
+    return v | attn8_tc_status();
 }

@@ -1,0 +1,112 @@
+// How attention over an 8-bit paged cache is dealt out to CTAs; shared by its kernels (attn_pages8.cu, attn_pages8_tc.cu) and their merge.
+#pragma once
+#include "pages8.cuh"
+
+namespace {
+
+constexpr int MAX_UNITS = 256;               // sequences of a launch
+constexpr int LEAST = 256;                   // keys of a CTA, where there are as many
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float NONE = -1e30f;               // largest score of no keys
+
+// The rows of one sequence in the launch.
+struct Unit {
+    int row, rows, slot, pos;                // first row, rows (0: no token), slot, position of the first row
+    int open;                                // first page of the slot that rows of the step go to
+    int parts;                               // CTAs of each of its items
+};
+
+__device__ __forceinline__ Unit unit_at(const Attn8Args& a, int u) {
+    Unit s;
+    if (a.positions) {
+        s = Unit{u, 1, a.slots[u], a.positions[u], 0, 0};
+    } else {
+        const int4 g = a.segs[u];
+        s = Unit{g.x, g.y, g.z, g.w, 0, 0};
+    }
+    if ((unsigned)s.slot >= (unsigned)a.t.n_slots || s.pos < 0 || s.row < 0 || s.row + s.rows > a.rows || s.pos + s.rows > a.t.max_pages * PAGE) s.rows = 0;
+    s.open = s.pos >> PAGE_SHIFT;
+    return s;
+}
+
+// Turns of a unit's items: those with kept keys first, then the ones from the first row's first key on.
+struct Keys {
+    int base, front, turns;
+};
+__device__ __forceinline__ Keys keys_of(const Attn8Args& a, const Unit& s) {
+    const int turn = a.turn;
+    Keys k;
+    k.base = first_key(s.pos, a.chunk, a.window) & ~(turn - 1);
+    k.front = a.window > 0 ? kept_tiles(a.keep, k.base, turn) : 0;
+    k.turns = s.rows > 0 ? k.front + (s.pos + s.rows - k.base + turn - 1) / turn : 0;
+    return k;
+}
+__device__ __forceinline__ int first_of(const Keys& k, int turn, int i) { return i < k.front ? i * turn : k.base + (i - k.front) * turn; }
+
+// Items of a unit: row_tile rows of (row, head of the KV head) each, of every KV head.
+__device__ __forceinline__ int row_tiles(const Attn8Args& a, const Unit& s) { return (s.rows * (a.n_heads / a.c.kv_heads) + a.row_tile - 1) / a.row_tile; }
+
+// Sum of the threads' numbers up to each and over all; at least MAX_UNITS threads, `sums` has one place a warp.
+__device__ __forceinline__ uint32_t scan(uint32_t x, uint32_t* sums, uint32_t& all) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 31) sums[warp] = x;
+    __syncthreads();
+    all = 0;
+    for (int w = 0; w < MAX_UNITS / 32; w++) {
+        if (w == warp) x += all;
+        all += sums[w];
+    }
+    return x;
+}
+
+// All units, and the CTAs before each one's (prefix[u]) and in all (prefix[units]).
+__device__ __forceinline__ void deal_out(const Attn8Args& a, int units, Unit* list, uint32_t* prefix, uint32_t* sums) {
+    const int tid = threadIdx.x;
+    Unit s;
+    uint32_t turns = 0, items = 0, total, ctas;
+    if (tid < units) {
+        s = unit_at(a, tid);
+        list[tid] = s;
+        turns = keys_of(a, s).turns;
+        items = row_tiles(a, s) * a.c.kv_heads;
+    }
+    scan(turns * items, sums, total);
+    const uint32_t parts = turns ? max(1u, min((uint32_t)((unsigned long long)turns * a.ctas / total), (turns * a.turn + LEAST - 1) / LEAST)) : 0;
+    const uint32_t x = scan(parts * items, sums, ctas);
+    if (tid < units) {
+        prefix[tid] = x - parts * items;
+        if (a.behind)        // other rows of the slot may go to earlier pages
+            for (int i = 0; i < units; i++)
+                if (list[i].slot == s.slot && list[i].pos >= 0) s.open = min(s.open, list[i].pos >> PAGE_SHIFT);
+    }
+    if (tid == 0) prefix[units] = ctas;
+    __syncthreads();
+    if (tid < units) {
+        s.parts = parts;
+        list[tid] = s;
+    }
+    __syncthreads();
+}
+
+__device__ __forceinline__ int unit_of(const uint32_t* prefix, int units, uint32_t x) {
+    int lo = 0, hi = units - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (prefix[mid] <= x) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;               // of units without turns, the one behind them
+}
+
+}  // namespace
+
+// Attention of tiles of 128 query rows, the sums to be merged as those of attn8_kernel; a cudaError_t value (attn_pages8_tc.cu).
+int attn8_tc_launch(const Attn8Args& a, int grid, int pdl, cudaStream_t st);
+// 0, KS_TIMEOUT once a wait of it has run out since the last call, or -1.
+int attn8_tc_status();

@@ -1,0 +1,391 @@
+// Attention of tens to hundreds of query rows over an 8-bit paged cache on tcgen05 (layout: pages8.cuh, how it is dealt out: attn_pages8.cuh).
+//
+// An item is 128 rows of (row of a portion, query head of a KV head), so that a few rows for all heads of a KV head fill a tile, and its keys are shared by several CTAs: 64 rows of
+// four heads behind a long context are 256 rows a KV head, which rows of 16 read (and expand) the cache for 16 times, and a tile a head leaves most SMs idle.
+// Tiles of 128 keys: bulk copies bring the codes into a ring of three boxes, four warps turn them into swizzled f16 tiles, exactly (code times unit is an f16 number), two buffers
+// of keys and of values.  S = Q K^T and P V run as in attn_prefill_tc.cu: two score buffers and two P V tiles in tensor memory, probabilities over the scores they came from, S of
+// tile t + 2 issued behind P V of tile t, P V of tile t - 1 added to the sums under the softmax's next tile.
+// Warps: 0-7 softmax (two share 32 rows, 64 keys each), 8 bulk copies, 9 products and tensor memory, 12-15 codes.  Every wait is bounded; one that runs out sets KS_TIMEOUT, and all
+// roles leave their loops.
+#include "attn_pages8.cuh"
+#include "attn_tc.cuh"
+
+__device__ int g_attn8_tc_status = 0;
+
+namespace {
+
+using namespace tc;
+
+constexpr int BQ = 128, BKV = 128;
+constexpr int ATOM_BYTES = 128 * 128;        // 128 rows x 64 f16
+constexpr int SOFTMAX_WARPS = 8, CODE_WARPS = 4, FIRST_CODE_WARP = 12, THREADS = 32 * (FIRST_CODE_WARP + CODE_WARPS);      // whole groups of four warps, whose registers are split
+constexpr int BOXES = 3;
+constexpr uint32_t TMEM_COLS = 512;
+
+template <int D>
+struct Lay {
+    static constexpr int ATOMS = D / 64, TILE = ATOMS * ATOM_BYTES, BOX = BKV * D;
+    static constexpr int OFF_K = TILE, OFF_V = OFF_K + 2 * TILE, OFF_BOX = OFF_V + 2 * TILE, TOTAL = OFF_BOX + BOXES * BOX + 1024;
+};
+
+__device__ __forceinline__ void bulk_copy(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+
+// 16 codes of row r, columns 16 c .. 16 c + 15, times the unit, into a swizzled tile.  The half that comes first differs between columns below and above 64, whose atoms have the
+// same banks.
+__device__ __forceinline__ void put_codes(uint8_t* tile, int r, int c, const uint4& w, __half2 unit) {
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+    uint32_t y[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const uint32_t h = e4m3x2_to_h2(x[j >> 1] >> (j & 1) * 16);
+        const __half2 f = __hmul2(*reinterpret_cast<const __half2*>(&h), unit);
+        y[j] = *reinterpret_cast<const uint32_t*>(&f);
+    }
+    uint8_t* row = tile + (c >> 2) * ATOM_BYTES + r * 128;
+    const int k = 2 * (c & 3), first = c >> 2 & 1;
+    const uint4 lo = make_uint4(y[0], y[1], y[2], y[3]), hi = make_uint4(y[4], y[5], y[6], y[7]);
+    *reinterpret_cast<uint4*>(row + (((k + first) ^ (r & 7)) << 4)) = first ? hi : lo;
+    *reinterpret_cast<uint4*>(row + (((k + 1 - first) ^ (r & 7)) << 4)) = first ? lo : hi;
+}
+
+template <int D>
+__global__ void __launch_bounds__(THREADS, 1) attn8_tc_kernel(const __grid_constant__ Attn8Args a) {
+    using L = Lay<D>;
+    constexpr int OH = D / 2, CHUNKS = D / 16;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* sm = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    __shared__ uint64_t bars[24];
+    __shared__ Unit list[MAX_UNITS];
+    __shared__ uint32_t prefix[MAX_UNITS + 1], sums[THREADS / 32], tmem_slot;
+    __shared__ int failed;
+    __shared__ float2 units8[BOXES];             // of the two pages in a box
+    __shared__ float x_max[2][2][128], x_sum[2][128];
+    uint64_t *full8 = bars, *empty8 = bars + 3, *k_full = bars + 6, *k_empty = bars + 8, *v_full = bars + 10, *v_empty = bars + 12, *s_full = bars + 14, *p_ready = bars + 16,
+             *o_full = bars + 18, *pair = bars + 20;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int n_units = a.positions ? a.rows : a.n_segs, G = a.c.kv_heads, group = a.n_heads / G;
+    if (tid == 0) {
+        failed = 0;
+        for (int i = 0; i < BOXES; i++) {
+            mbar_init(&full8[i], 1);
+            mbar_init(&empty8[i], CODE_WARPS);
+        }
+        for (int b = 0; b < 2; b++) {
+            mbar_init(&k_full[b], CODE_WARPS);
+            mbar_init(&k_empty[b], 1);
+            mbar_init(&v_full[b], CODE_WARPS);
+            mbar_init(&v_empty[b], 1);
+            mbar_init(&s_full[b], 1);
+            mbar_init(&p_ready[b], SOFTMAX_WARPS);
+            mbar_init(&o_full[b], 1);
+        }
+        for (int q = 0; q < 4; q++) mbar_init(&pair[q], 2);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    pdl_launch();
+    pdl_wait();
+    deal_out(a, n_units, list, prefix, sums);
+    if (blockIdx.x >= prefix[n_units]) return;
+    const int u = unit_of(prefix, n_units, blockIdx.x);
+    const Unit s = list[u];
+    const Keys ks = keys_of(a, s);
+    const int part = (blockIdx.x - prefix[u]) % s.parts, item = (blockIdx.x - prefix[u]) / s.parts, kvh = item % G, m0 = BQ * (item / G), rows_m = min(BQ, s.rows * group - m0);
+    const int x0 = (int)((long long)ks.turns * part / s.parts), n_tiles = (int)((long long)ks.turns * (part + 1) / s.parts) - x0;
+    // positions of the tile's first and last row, the last one's first key
+    const int first_pos = s.pos + m0 / group, last_pos = s.pos + min(s.rows - 1, (m0 + BQ - 1) / group), last_lo = first_key(last_pos, a.chunk, a.window), keep = a.window > 0 ? a.keep : 0;
+    auto n0_of = [&](int t) { return first_of(ks, BKV, x0 + t); };
+    auto masked = [&](int n0) { return n0 + BKV - 1 > first_pos || (n0 < last_lo && n0 + BKV > keep); };      // some row does not see some key
+
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (warp < SOFTMAX_WARPS) {      // queries
+        const int r = 32 * (warp & 3) + lane, c = warp >> 2, m = m0 + r;
+        const bool live = r < rows_m;
+        const float sign = a.scale > 0.f ? 1.f : a.scale < 0.f ? -1.f : 0.f;      // the running maximum is one of plain scores, which takes a scale above zero
+        const float* qp = a.q + ((size_t)(s.row + m / group) * a.n_heads + kvh * group + m % group) * D + OH * c;
+#pragma unroll
+        for (int j = 0; j < OH / 8; j++) {
+            float4 v0 = make_float4(0.f, 0.f, 0.f, 0.f), v1 = v0;
+            if (live) {
+                v0 = *(const float4*)(qp + 8 * j);
+                v1 = *(const float4*)(qp + 8 * j + 4);
+            }
+            const int col = OH * c + 8 * j;
+            *(uint4*)(sm + (col >> 6) * ATOM_BYTES + r * 128 + ((((col & 63) >> 3) ^ (r & 7)) << 4)) = make_uint4(pack_h2(sign * v0.x, sign * v0.y), pack_h2(sign * v0.z, sign * v0.w), pack_h2(sign * v1.x, sign * v1.y), pack_h2(sign * v1.z, sign * v1.w));
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+
+    // 64 K registers: 168 a softmax thread, 88 a thread of the other two groups
+    if (warp >= SOFTMAX_WARPS) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (warp == 8) {
+            // Box 2 t holds the keys of tile t, box 2 t + 1 the values.  The lanes look up the pages of 32 tiles at a time.
+            const int last_page = (s.pos + s.rows - 1) >> PAGE_SHIFT;
+            bool ok = true;
+            int asked = 0;                           // boxes
+            for (int t0 = 0; t0 < n_tiles && ok; t0 += 32) {
+                size_t head[2] = {};
+                float2 ku = make_float2(0.f, 0.f), vu = ku;
+                if (t0 + lane < n_tiles) {
+                    const int p0 = n0_of(t0 + lane) >> PAGE_SHIFT;
+                    for (int i = 0; i < 2; i++) head[i] = (size_t)max(page_at(a.t, a.c.n_pages, s.slot, min(p0 + i, last_page)), 0) * G + kvh;
+                    ku = make_float2(a.c.ku[head[0]], a.c.ku[head[1]]);
+                    vu = make_float2(a.c.vu[head[0]], a.c.vu[head[1]]);
+                }
+                for (int t = t0; t < min(n_tiles, t0 + 32) && ok; t++) {
+                    const size_t h0 = __shfl_sync(0xffffffffu, head[0], t - t0), h1 = __shfl_sync(0xffffffffu, head[1], t - t0);
+                    const float2 uk = make_float2(__shfl_sync(0xffffffffu, ku.x, t - t0), __shfl_sync(0xffffffffu, ku.y, t - t0));
+                    const float2 uv = make_float2(__shfl_sync(0xffffffffu, vu.x, t - t0), __shfl_sync(0xffffffffu, vu.y, t - t0));
+                    for (int v = 0; v < 2; v++) {
+                        const int j = 2 * t + v, slot = j % BOXES;
+                        if (j >= BOXES && !mbar_wait(&empty8[slot], (j / BOXES - 1) & 1)) {
+                            ok = false;
+                            break;
+                        }
+                        if (lane == 0) {
+                            uint8_t* box = sm + L::OFF_BOX + slot * L::BOX;
+                            const uint8_t* from = v ? a.c.v : a.c.k;
+                            units8[slot] = v ? uv : uk;
+                            mbar_expect_tx(&full8[slot], L::BOX);
+                            bulk_copy(box, from + h0 * PAGE * D, PAGE * D, &full8[slot]);
+                            bulk_copy(box + PAGE * D, from + h1 * PAGE * D, PAGE * D, &full8[slot]);
+                        }
+                        asked++;
+                        __syncwarp();
+                    }
+                }
+            }
+            if (!ok && lane == 0) atomicExch(&failed, 1);
+            for (int i = max(0, asked - BOXES); i < asked; i++) mbar_wait(&full8[i % BOXES], (i / BOXES) & 1);      // no copy is under way when the CTA leaves
+        } else if (warp >= FIRST_CODE_WARP) {
+            const int t0 = tid - 32 * FIRST_CODE_WARP;                // 16 codes at a time: chunk t0 + 128 i of a box
+            bool ok = true;
+            for (int t = 0; t < n_tiles && ok; t++) {
+                const int b = t & 1, jk = 2 * t, jv = jk + 1, sk = jk % BOXES, sv = jv % BOXES;
+                const uint8_t *kbox = sm + L::OFF_BOX + sk * L::BOX, *vbox = sm + L::OFF_BOX + sv * L::BOX;
+                uint32_t bad = 0;                    // rows of the thread's chunks whose values hold what is no number: they become zeros and their keys none
+                if (!mbar_wait(&full8[sk], (jk / BOXES) & 1)) { ok = false; break; }
+                if (masked(n0_of(t))) {
+                    if (!mbar_wait(&full8[sv], (jv / BOXES) & 1)) { ok = false; break; }
+#pragma unroll
+                    for (int i = 0; i < CHUNKS; i++) {
+                        uint32_t none = holds_nan(reinterpret_cast<const uint4*>(vbox)[t0 + 128 * i]);
+#pragma unroll
+                        for (int o = 1; o < CHUNKS; o <<= 1) none |= __shfl_xor_sync(0xffffffffu, none, o);
+                        bad |= none << i;
+                    }
+                }
+                if (t >= 2 && !mbar_wait(&k_empty[b], ((t >> 1) - 1) & 1)) { ok = false; break; }
+                {
+                    const float2 un = units8[sk];
+                    const __half2 u0 = __float2half2_rn(un.x), u1 = __float2half2_rn(un.y);
+#pragma unroll
+                    for (int i = 0; i < CHUNKS; i++) {
+                        const int at = t0 + 128 * i, r = at / CHUNKS;
+                        uint4 w = reinterpret_cast<const uint4*>(kbox)[at];
+                        if (bad >> i & 1) w = make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu);
+                        put_codes(sm + L::OFF_K + b * L::TILE, r, at % CHUNKS, w, i < CHUNKS / 2 ? u0 : u1);
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&k_full[b]);
+                    mbar_arrive(&empty8[sk]);
+                }
+                if (!mbar_wait(&full8[sv], (jv / BOXES) & 1)) { ok = false; break; }
+                if (t >= 2 && !mbar_wait(&v_empty[b], ((t >> 1) - 1) & 1)) { ok = false; break; }
+                {
+                    const float2 un = units8[sv];
+                    const __half2 u0 = __float2half2_rn(un.x), u1 = __float2half2_rn(un.y);
+#pragma unroll
+                    for (int i = 0; i < CHUNKS; i++) {
+                        const int at = t0 + 128 * i, r = at / CHUNKS;
+                        uint4 w = reinterpret_cast<const uint4*>(vbox)[at];
+                        if (bad >> i & 1) w = make_uint4(0, 0, 0, 0);
+                        put_codes(sm + L::OFF_V + b * L::TILE, r, at % CHUNKS, w, i < CHUNKS / 2 ? u0 : u1);
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&v_full[b]);
+                    mbar_arrive(&empty8[sv]);
+                }
+            }
+            if (!ok) atomicExch(&failed, 1);
+        } else if (warp == 9 && lane == 0) {
+            {
+                constexpr uint32_t id_s = idesc_f16(BQ, BKV, 0), id_o = idesc_f16(BQ, D, 1);
+                bool ok = true;
+                auto issue_s = [&](int t) {          // S(t) = Q K(t)^T into score buffer t & 1
+                    const int b = t & 1;
+                    if (!mbar_wait(&k_full[b], (t >> 1) & 1)) { ok = false; return; }
+                    tc_fence_after();
+                    const uint8_t* kt = sm + L::OFF_K + b * L::TILE;
+#pragma unroll
+                    for (int at = 0; at < L::ATOMS; at++) {
+                        const uint64_t qd = umma_desc(sm + at * ATOM_BYTES), kd = umma_desc(kt + at * ATOM_BYTES);
+#pragma unroll
+                        for (int k = 0; k < 4; k++) umma_f16(tmem + 128 * b, qd + 2 * k, kd + 2 * k, id_s, (at | k) != 0);
+                    }
+                    umma_commit(&s_full[b]);
+                    umma_commit(&k_empty[b]);
+                };
+                issue_s(0);
+                if (ok && n_tiles > 1) issue_s(1);
+                for (int t = 0; t < n_tiles && ok; t++) {
+                    const int b = t & 1, ph = (t >> 1) & 1;
+                    if (!mbar_wait(&p_ready[b], ph) || !mbar_wait(&v_full[b], ph)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint8_t* vt = sm + L::OFF_V + b * L::TILE;
+#pragma unroll
+                    for (int kk = 0; kk < BKV / 16; kk++)      // O_tile(t) = P(t) V(t); P sits in the first 64 columns of its score buffer
+                        umma_f16_ts(tmem + 256 + 128 * b, tmem + 128 * b + 8 * kk, umma_desc_mn(vt + kk * 16 * 128, ATOM_BYTES), id_o, kk != 0);
+                    umma_commit(&o_full[b]);
+                    umma_commit(&v_empty[b]);
+                    if (t + 2 < n_tiles) issue_s(t + 2);       // runs behind P V(t), which still reads the buffer it overwrites
+                }
+                if (!ok) atomicExch(&failed, 1);
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+        const int q = warp & 3, c = warp >> 2, r = 32 * q + lane;
+        const int qp = s.pos + min((m0 + r) / group, s.rows - 1), row_lo = first_key(qp, a.chunk, a.window);
+        const float size = a.scale == 0.f ? 1.f : fabsf(a.scale), mult = a.softcap > 0.f ? 1.f : size * LOG2E, inv_cap = a.softcap > 0.f ? size / a.softcap : 0.f, cap2 = a.softcap * LOG2E;
+        const uint32_t lane_base = (uint32_t)(32 * q) << 16;
+        float o[OH];
+#pragma unroll
+        for (int j = 0; j < OH; j++) o[j] = 0.f;
+        float m_run = NONE, l_run = 0.f, corr_prev = 1.f;
+        bool ok = true;
+        auto accumulate = [&](int t, float corr) {      // o = o * corr + O_tile(t)
+            const int b = t & 1;
+            if (!mbar_wait(&o_full[b], (t >> 1) & 1)) { ok = false; return; }
+            tc_fence_after();
+#pragma unroll
+            for (int j0 = 0; j0 < OH; j0 += 32) {
+                uint32_t ov[32];
+                tmem_ld32(tmem + lane_base + (uint32_t)(256 + 128 * b + OH * c + j0), ov);
+#pragma unroll
+                for (int j = 0; j < 32; j += 2) {
+                    const float2 y = fma2(make_float2(o[j0 + j], o[j0 + j + 1]), make_float2(corr, corr), make_float2(__uint_as_float(ov[j]), __uint_as_float(ov[j + 1])));
+                    o[j0 + j] = y.x;
+                    o[j0 + j + 1] = y.y;
+                }
+            }
+            tc_fence_before();
+        };
+        for (int t = 0; t < n_tiles && ok; t++) {
+            const int b = t & 1, n0 = n0_of(t);
+            if (!mbar_wait(&s_full[b], (t >> 1) & 1)) { ok = false; break; }
+            tc_fence_after();
+            uint32_t v[2][32];
+            tmem_ld32(tmem + lane_base + (uint32_t)(128 * b + 64 * c), v[0]);
+            tmem_ld32(tmem + lane_base + (uint32_t)(128 * b + 64 * c + 32), v[1]);
+            if (a.softcap > 0.f) {
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int j = 0; j < 32; j++) v[i][j] = __float_as_uint(cap2 * tanh_exp(__uint_as_float(v[i][j]) * inv_cap));
+            }
+            if (masked(n0)) {
+                const int kp0 = n0 + 64 * c;
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int j = 0; j < 32; j++) {
+                        const int kp = kp0 + 32 * i + j;
+                        if (kp > qp || (kp < row_lo && kp >= keep)) v[i][j] = 0xff800000u;
+                    }
+            }
+            float mx = NONE;
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int j = 0; j < 32; j++) mx = fmaxf(mx, __uint_as_float(v[i][j]));
+            // the partner may be a tile ahead when this warp reads: a place each for even and odd tiles
+            x_max[b][c][r] = mx;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&pair[q]);
+            if (!mbar_wait(&pair[q], t & 1)) { ok = false; break; }
+            mx = fmaxf(mx, *(volatile float*)&x_max[b][c ^ 1][r]);
+            const float m_new = fmaxf(m_run, mx), corr = ex2((m_run - m_new) * mult);
+            m_run = m_new;
+            const float2 mult2 = make_float2(mult, mult), less = make_float2(-m_new * mult, -m_new * mult);
+            float2 ls2 = make_float2(0.f, 0.f);
+            uint32_t pw[32];
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int j = 0; j < 32; j += 2) {
+                    const float2 e = fma2(make_float2(__uint_as_float(v[i][j]), __uint_as_float(v[i][j + 1])), mult2, less);
+                    const float2 pr = make_float2(ex2(e.x), ex2(e.y));
+                    ls2 = add2(ls2, pr);
+                    pw[16 * i + (j >> 1)] = pack_h2(pr.x, pr.y);
+                }
+            tmem_st32(tmem + lane_base + (uint32_t)(128 * b + 32 * c), pw);      // both warps of the quarter have read all of S(t) by now
+            l_run = l_run * corr + (ls2.x + ls2.y);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_ready[b]);
+            if (t >= 1) accumulate(t - 1, corr_prev);      // P V(t - 1) finished long ago; P V(t) runs under this
+            corr_prev = corr;
+        }
+        if (ok && n_tiles > 0) accumulate(n_tiles - 1, corr_prev);
+        if (!ok) atomicExch(&failed, 1);
+        x_sum[c][r] = l_run;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&pair[q]);
+        if (ok && !mbar_wait(&pair[q], n_tiles & 1)) {
+            ok = false;
+            atomicExch(&failed, 1);
+        }
+        if (r < rows_m) {
+            const size_t at = (size_t)blockIdx.x * BQ + r;
+            float4* to = reinterpret_cast<float4*>(a.part_acc + at * D + OH * c);
+#pragma unroll
+            for (int j = 0; j < OH; j += 4) to[j / 4] = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+            if (c == 0) a.part_ml[at] = make_float2(m_run * mult, l_run + *(volatile float*)&x_sum[1][r]);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+    }
+    if (tid == 0 && failed) atomicExch(&g_attn8_tc_status, KS_TIMEOUT);
+}
+
+template <int D>
+int launch(Attn8Args& a, int grid, int pdl, cudaStream_t st) {
+    static PerDeviceOnce once;
+    if (once.first()) cudaFuncSetAttribute(attn8_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay<D>::TOTAL);
+    void* args[] = {&a};
+    return launch_rows((const void*)attn8_tc_kernel<D>, dim3(grid), dim3(THREADS), Lay<D>::TOTAL, args, st, pdl);
+}
+
+}  // namespace
+
+int attn8_tc_launch(const Attn8Args& in, int grid, int pdl, cudaStream_t st) {
+    Attn8Args a = in;
+    return a.c.hd == 128 ? launch<128>(a, grid, pdl, st) : launch<64>(a, grid, pdl, st);
+}
+
+int attn8_tc_status() {
+    int v = 0, none = 0;
+    if (cudaMemcpyFromSymbol(&v, g_attn8_tc_status, sizeof(int)) != cudaSuccess) return -1;
+    if (v) cudaMemcpyToSymbol(g_attn8_tc_status, &none, sizeof(int));
+    return v;
+}

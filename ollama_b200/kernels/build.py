@@ -36,7 +36,7 @@ def _stale(target: str, deps: list[str]) -> bool:
 
 
 # sources of a part of the library, for a first start that should compile what one kind of model needs and no more
-GROUPS = {"stack": ("attn_decode_mma.cu", "attn_latent.cu", "attn_paged.cu", "attn_pages8.cu", "attn_prefill_tc.cu", "depth.cu", "elementwise.cu", "gemm_f32.cu", "gemm_tc.cu", "gemv_rows.cu",
+GROUPS = {"stack": ("attn_decode_mma.cu", "attn_latent.cu", "attn_paged.cu", "attn_pages8.cu", "attn_pages8_tc.cu", "attn_prefill_tc.cu", "depth.cu", "elementwise.cu", "gemm_f32.cu", "gemm_tc.cu", "gemv_rows.cu",
                     "gru.cu", "latent.cu", "moe.cu", "moe_rows.cu", "norm_rows.cu", "pages8.cu", "sample.cu", "ssd.cu", "ssd_chunk.cu", "ssm.cu")}
 
 

@@ -54,7 +54,8 @@ struct Attn8Args {
     int n_segs;
     int chunk, window, keep;
     float scale, softcap;
-    int row_tile, tiles;     // query rows (of a sequence, for the heads of a KV head) that are taken together, 8 or 16; most such tiles of a sequence
+    int row_tile, turn;      // query rows (of a sequence, for the heads of a KV head) and keys that are taken together: 8 or 16 and 32, 128 and 128
+    int tiles;               // most row tiles of a sequence
     int ctas;                // that fit the GPU at once
     float* part_acc;         // [items + ctas][row_tile][hd]
     float2* part_ml;         // [items + ctas][row_tile] (largest score, sum)

@@ -31,7 +31,7 @@ Append8Args = _st("Append8Args", [("qkv", P), ("ldq", I), ("rows", I), ("n_heads
                                   ("n_rot", I), ("positions", P), ("slots", P), ("segs", P), ("n_segs", I), ("per", I), ("t", _PageTable), ("q_out", P), ("c", _Pages8),
                                   ("head_norm", I), ("v_off", I), ("mscale", F), ("maps", I), ("no_append", I)])
 Attn8Args = _st("Attn8Args", [("q", P), ("rows", I), ("n_heads", I), ("vdim", I), ("c", _Pages8), ("t", _PageTable), ("positions", P), ("slots", P), ("segs", P), ("n_segs", I),
-                              ("chunk", I), ("window", I), ("keep", I), ("scale", F), ("softcap", F), ("row_tile", I), ("tiles", I), ("ctas", I), ("part_acc", P), ("part_ml", P), ("out", P),
+                              ("chunk", I), ("window", I), ("keep", I), ("scale", F), ("softcap", F), ("row_tile", I), ("turn", I), ("tiles", I), ("ctas", I), ("part_acc", P), ("part_ml", P), ("out", P),
                               ("ldo", I), ("out16", I), ("gate", HeadGate), ("diff", DiffHeads), ("behind", I)])
 
 
@@ -196,16 +196,16 @@ def _attn_args(w, dev, c, t, q, n, heads, where, tiles, acc, ml, ctas, out, vdim
                      out.dtype is bf16, gate, diff, 0)
 
 
-def _row_tiles(rows: int) -> tuple[int, int]:
-    """(query rows that are taken together, tiles of them) where a sequence has so many rows for the heads of a KV head."""
-    tile = 8 if rows <= 8 else 16
-    return tile, -(-rows // tile)
+def _row_tiles(rows: int) -> tuple[int, int, int]:
+    """Where a sequence has so many rows for the heads of a KV head: (query rows and keys that are taken together, tiles of the rows)."""
+    tile = 8 if rows <= 8 else 16 if rows <= 16 else 128
+    return tile, 128 if tile == 128 else 32, -(-rows // tile)
 
 
 def _pieces(c, tiles, units: int, dev: int) -> tuple[int, int]:
     """(CTAs that fit the GPU at once, rows of partial results: those of as many CTAs, and of one more for each item)."""
     ctas = _sms(dev) * (2 if tiles[0] == 8 else 1)
-    return ctas, (min(units, MAX_UNITS) * tiles[1] * c.kv_heads + ctas) * tiles[0]
+    return ctas, (min(units, MAX_UNITS) * tiles[2] * c.kv_heads + ctas) * tiles[0]
 
 
 @_on_device
