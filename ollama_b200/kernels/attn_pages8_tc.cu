@@ -5,7 +5,7 @@
 // Tiles of 128 keys: bulk copies bring the codes into a ring of three boxes, four warps turn them into swizzled f16 tiles, exactly (code times unit is an f16 number), two buffers
 // of keys and of values.  S = Q K^T and P V run as in attn_prefill_tc.cu: two score buffers and two P V tiles in tensor memory, probabilities over the scores they came from, S of
 // tile t + 2 issued behind P V of tile t, P V of tile t - 1 added to the sums under the softmax's next tile.
-// Warps: 0-7 softmax (two share 32 rows, 64 keys each), 8 bulk copies, 9 products and tensor memory, 12-15 codes.  Every wait is bounded; one that runs out sets KS_TIMEOUT, and all
+// Warps: 0-7 softmax (two share 32 rows, 64 keys each), 8 bulk copies, 9 products and tensor memory, 10-15 codes.  Every wait is bounded; one that runs out sets KS_TIMEOUT, and all
 // roles leave their loops.
 #include "attn_pages8.cuh"
 #include "attn_tc.cuh"
@@ -18,7 +18,7 @@ using namespace tc;
 
 constexpr int BQ = 128, BKV = 128;
 constexpr int ATOM_BYTES = 128 * 128;        // 128 rows x 64 f16
-constexpr int SOFTMAX_WARPS = 8, CODE_WARPS = 4, FIRST_CODE_WARP = 12, THREADS = 32 * (FIRST_CODE_WARP + CODE_WARPS);      // whole groups of four warps, whose registers are split
+constexpr int SOFTMAX_WARPS = 8, CODE_WARPS = 6, FIRST_CODE_WARP = 10, THREADS = 32 * (FIRST_CODE_WARP + CODE_WARPS);      // whole groups of four warps, whose registers are split
 constexpr int BOXES = 3;
 constexpr uint32_t TMEM_COLS = 512;
 
@@ -53,7 +53,7 @@ __device__ __forceinline__ void put_codes(uint8_t* tile, int r, int c, const uin
 template <int D>
 __global__ void __launch_bounds__(THREADS, 1) attn8_tc_kernel(const __grid_constant__ Attn8Args a) {
     using L = Lay<D>;
-    constexpr int OH = D / 2, CHUNKS = D / 16;
+    constexpr int OH = D / 2, CHUNKS = D / 16, CODE_THREADS = 32 * CODE_WARPS, EACH = (BKV * CHUNKS + CODE_THREADS - 1) / CODE_THREADS;      // 16 codes at a time of a code thread
     extern __shared__ uint8_t smem_raw[];
     uint8_t* sm = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     __shared__ uint64_t bars[24];
@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn8_tc_kernel(const __grid_const
             if (!ok && lane == 0) atomicExch(&failed, 1);
             for (int i = max(0, asked - BOXES); i < asked; i++) mbar_wait(&full8[i % BOXES], (i / BOXES) & 1);      // no copy is under way when the CTA leaves
         } else if (warp >= FIRST_CODE_WARP) {
-            const int t0 = tid - 32 * FIRST_CODE_WARP;                // 16 codes at a time: chunk t0 + 128 i of a box
+            const int t0 = tid - 32 * FIRST_CODE_WARP;                // its chunks of a box are t0 + CODE_THREADS i
             bool ok = true;
             for (int t = 0; t < n_tiles && ok; t++) {
                 const int b = t & 1, jk = 2 * t, jv = jk + 1, sk = jk % BOXES, sv = jv % BOXES;
@@ -177,8 +177,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn8_tc_kernel(const __grid_const
                 if (masked(n0_of(t))) {
                     if (!mbar_wait(&full8[sv], (jv / BOXES) & 1)) { ok = false; break; }
 #pragma unroll
-                    for (int i = 0; i < CHUNKS; i++) {
-                        uint32_t none = holds_nan(reinterpret_cast<const uint4*>(vbox)[t0 + 128 * i]);
+                    for (int i = 0; i < EACH; i++) {
+                        uint32_t none = t0 + CODE_THREADS * i < BKV * CHUNKS && holds_nan(reinterpret_cast<const uint4*>(vbox)[t0 + CODE_THREADS * i]);
 #pragma unroll
                         for (int o = 1; o < CHUNKS; o <<= 1) none |= __shfl_xor_sync(0xffffffffu, none, o);
                         bad |= none << i;
@@ -188,12 +188,15 @@ __global__ void __launch_bounds__(THREADS, 1) attn8_tc_kernel(const __grid_const
                 {
                     const float2 un = units8[sk];
                     const __half2 u0 = __float2half2_rn(un.x), u1 = __float2half2_rn(un.y);
+                    uint4 w[EACH];             // all of them before anything is stored: the compiler keeps loads behind stores
 #pragma unroll
-                    for (int i = 0; i < CHUNKS; i++) {
-                        const int at = t0 + 128 * i, r = at / CHUNKS;
-                        uint4 w = reinterpret_cast<const uint4*>(kbox)[at];
-                        if (bad >> i & 1) w = make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu);
-                        put_codes(sm + L::OFF_K + b * L::TILE, r, at % CHUNKS, w, i < CHUNKS / 2 ? u0 : u1);
+                    for (int i = 0; i < EACH; i++)
+                        if (t0 + CODE_THREADS * i < BKV * CHUNKS) w[i] = reinterpret_cast<const uint4*>(kbox)[t0 + CODE_THREADS * i];
+#pragma unroll
+                    for (int i = 0; i < EACH; i++) {
+                        const int at = t0 + CODE_THREADS * i;
+                        if (bad >> i & 1) w[i] = make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu);
+                        if (at < BKV * CHUNKS) put_codes(sm + L::OFF_K + b * L::TILE, at / CHUNKS, at % CHUNKS, w[i], at / CHUNKS < PAGE ? u0 : u1);
                     }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -207,12 +210,15 @@ __global__ void __launch_bounds__(THREADS, 1) attn8_tc_kernel(const __grid_const
                 {
                     const float2 un = units8[sv];
                     const __half2 u0 = __float2half2_rn(un.x), u1 = __float2half2_rn(un.y);
+                    uint4 w[EACH];
 #pragma unroll
-                    for (int i = 0; i < CHUNKS; i++) {
-                        const int at = t0 + 128 * i, r = at / CHUNKS;
-                        uint4 w = reinterpret_cast<const uint4*>(vbox)[at];
-                        if (bad >> i & 1) w = make_uint4(0, 0, 0, 0);
-                        put_codes(sm + L::OFF_V + b * L::TILE, r, at % CHUNKS, w, i < CHUNKS / 2 ? u0 : u1);
+                    for (int i = 0; i < EACH; i++)
+                        if (t0 + CODE_THREADS * i < BKV * CHUNKS) w[i] = reinterpret_cast<const uint4*>(vbox)[t0 + CODE_THREADS * i];
+#pragma unroll
+                    for (int i = 0; i < EACH; i++) {
+                        const int at = t0 + CODE_THREADS * i;
+                        if (bad >> i & 1) w[i] = make_uint4(0, 0, 0, 0);
+                        if (at < BKV * CHUNKS) put_codes(sm + L::OFF_V + b * L::TILE, at / CHUNKS, at % CHUNKS, w[i], at / CHUNKS < PAGE ? u0 : u1);
                     }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
