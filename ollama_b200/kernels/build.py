@@ -50,6 +50,7 @@ def build_group(group: str, verbose: bool = False, force: bool = False) -> str:
 def build(verbose: bool = False, force: bool = False) -> str:
     _compile(sorted(f for f in os.listdir(HERE) if f.endswith(".cu")), LIB, verbose, force)
     build_host(verbose, force)
+    build_calls(verbose, force)
     return LIB
 
 
@@ -107,6 +108,27 @@ def build_host(verbose: bool = False, force: bool = False) -> str | None:
             sys.stderr.write(r.stdout + r.stderr)
             raise RuntimeError("device probe build failed")
     return HOSTLIB
+
+
+def build_calls(verbose: bool = False, force: bool = False) -> str:
+    """The Python module of calls whose arguments are checked in C++ (ops/pages8_call.cpp); needs torch's headers, no GPU."""
+    import sysconfig
+
+    from torch.utils.cpp_extension import include_paths, library_paths
+    ops = os.path.join(os.path.dirname(HERE), "ops")
+    src, out = os.path.join(ops, "pages8_call.cpp"), os.path.join(ops, "_pages8.so")
+    if force or _stale(out, [src, os.path.join(HERE, "pages8_args.h")]):
+        cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
+        part = f"{out}.{os.getpid()}"
+        cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", *(f"-I{d}" for d in (*include_paths(), os.path.join(cuda, "include"), sysconfig.get_paths()["include"])),
+               "-o", part, src, *(f"-L{d}" for d in (*library_paths(), os.path.join(cuda, "lib64"))), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-lcudart"]
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if verbose or r.returncode:
+            sys.stderr.write(r.stdout + r.stderr)
+        if r.returncode:
+            raise RuntimeError("g++ failed on pages8_call.cpp")
+        os.replace(part, out)
+    return out
 
 
 if __name__ == "__main__":

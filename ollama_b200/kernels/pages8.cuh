@@ -2,69 +2,11 @@
 // KV head, [page][kv head].  Units are powers of two between 2^-15 and 2^7, so that every value of the cache, code times unit, is an f16 number too
 // (448 * 2^7 = 57344, 2^-9 * 2^-15 the least subnormal), and a unit that grows leaves old codes as they are but for the subnormal ones.
 #pragma once
+#include "pages8_args.h"
 #include "rows.cuh"
 
 constexpr int UNIT_LOW = -15, UNIT_HIGH = 7;
 constexpr float E4M3_MAX = 448.f;
-
-// Keys and values of one layer run.
-struct Pages8 {
-    uint8_t* k;
-    float* ku;
-    uint8_t* v;
-    float* vu;
-    int n_pages, kv_heads, hd;
-};
-// Where the pages of a slot are: table[slot][i] holds positions 64 i .. 64 i + 63.
-struct PageTable {
-    const int* table;
-    int n_slots, max_pages;
-};
-
-// What rows are appended, b2_append8.
-struct Append8Args {
-    const float* qkv;        // [rows][ldq]: q heads | k heads | ..., value heads from column v_off on
-    int ldq, rows, n_heads, dim, vdim;
-    const float* q_norm;     // see PagedAppendArgs
-    const float* k_norm;
-    float eps;
-    const double* freqs;     // [n_rot / 2]
-    int n_rot;
-    const int* positions;    // [rows], one row a sequence; or null:
-    const int* slots;
-    const int4* segs;        // [n_segs] portions (first row, rows, slot, position of the first row), of slots of their own
-    int n_segs, per;         // per: most pages that a portion touches
-    PageTable t;
-    float* q_out;            // [rows][H][hd]
-    Pages8 c;
-    int head_norm, v_off;
-    float mscale;
-    int maps, no_append;
-};
-
-// Attention of rows, b2_attn8 (attn_pages8.cu).
-struct Attn8Args {
-    const float* q;          // [rows][H][hd], rotated
-    int rows, n_heads, vdim;
-    Pages8 c;
-    PageTable t;
-    const int* positions;    // [rows], or null:
-    const int* slots;
-    const int4* segs;        // [n_segs] portions (first row, rows, slot, position of the first row)
-    int n_segs;
-    int chunk, window, keep;
-    float scale, softcap;
-    int row_tile, turn;      // query rows (of a sequence, for the heads of a KV head) and keys that are taken together: 8 or 16 and 32, 128 and 128
-    int tiles;               // most row tiles of a sequence
-    int ctas;                // that fit the GPU at once
-    float* part_acc;         // [items + ctas][row_tile][hd]
-    float2* part_ml;         // [items + ctas][row_tile] (largest score, sum)
-    void* out;               // [rows][ldo], head h at column h * vdim
-    int ldo, out16;
-    HeadGate gate;
-    DiffHeads diff;
-    int behind;              // the launch follows the one that appends the rows, which writes neither positions, slots nor tables
-};
 
 // Codes of two values (the first in the low byte), rounded to nearest even; magnitudes beyond 448 become 448, what is no number stays none.
 __device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {

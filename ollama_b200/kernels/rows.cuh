@@ -1,6 +1,7 @@
 // Element access shared by the kernels that exist in a 16-bit and a 32-bit form.
 #pragma once
 #include "common.cuh"
+#include "pages8_args.h"      // HeadGate, DiffHeads
 
 __device__ __forceinline__ float to_f(float v) { return v; }
 __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -52,16 +53,6 @@ __device__ __forceinline__ int first_key(int pos, int chunk, int window) { retur
 // Tiles of `tile` keys ahead of the one that holds position `first` which contain kept keys.
 __device__ __forceinline__ int kept_tiles(int keep, int first, int tile) { return min((keep + tile - 1) / tile, first / tile); }
 
-// Sigmoid gate of attention results: kind 1 one number per element, 2 one per head; before the sigmoid.
-struct HeadGate {
-    const float* g;          // [rows][ld]
-    int ld, kind;
-};
-// Differential attention: a head's result is a1 - lambda a2 of its two maps, divided by its root mean square, times `scale`.
-struct DiffHeads {
-    float lambda, scale, eps;
-    int on;
-};
 __device__ __forceinline__ float sigmoid_f(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
 __device__ __forceinline__ float sigmoid_exact(float v) { return 1.f / (1.f + expf(-v)); }
 
