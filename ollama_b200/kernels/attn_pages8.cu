@@ -65,20 +65,15 @@ struct Lay {
 
 struct Place {
     int y;                   // row of the tensor maps
-    float ku, vu;
     int n0;                  // first key; all bits flipped where the page is one that rows of this step go to
 };
 
 __device__ __forceinline__ Place place_of(const Attn8Args& a, const Unit& s, const Keys& k, int g, int turn) {
-    Place p;
     const int n0 = first_of(k, TURN, turn), page = max(page_at(a.t, a.c.n_pages, s.slot, n0 >> PAGE_SHIFT), 0);
-    const size_t head = (size_t)page * a.c.kv_heads + g;
-    p.y = (int)(head * PAGE) + (n0 & (PAGE - 1));
-    p.ku = __ldcg(a.c.ku + head);
-    p.vu = __ldcg(a.c.vu + head);
-    p.n0 = n0 >> PAGE_SHIFT >= s.open ? ~n0 : n0;
-    return p;
+    return Place{(int)(((size_t)page * a.c.kv_heads + g) * PAGE) + (n0 & (PAGE - 1)), n0 >> PAGE_SHIFT >= s.open ? ~n0 : n0};
 }
+// Units of the keys and values there.
+__device__ __forceinline__ float2 units_of(const Attn8Args& a, const Place& p) { return make_float2(__ldcg(a.c.ku + p.y / PAGE), __ldcg(a.c.vu + p.y / PAGE)); }
 
 template <int D, int NB>
 __global__ void __launch_bounds__(Lay<D, NB>::THREADS, Lay<D, NB>::PER_SM)
@@ -89,8 +84,8 @@ __global__ void __launch_bounds__(Lay<D, NB>::THREADS, Lay<D, NB>::PER_SM)
     uint8_t* sm = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     __shared__ uint64_t bars[WARPS * SLOTS];
     __shared__ Place places[2 * BATCH];
-    __shared__ Unit list[MAX_UNITS];
-    __shared__ uint32_t prefix[MAX_UNITS + 1], sums[WARPS];
+    __shared__ float2 code_units[2 * BATCH];
+    __shared__ DealRoom room;
     __shared__ float2 s_ml[WARPS][L::ROWS];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tq = lane & 3;
     const int units = a.positions ? a.rows : a.n_segs, G = a.c.kv_heads, group = a.n_heads / G;
@@ -98,17 +93,18 @@ __global__ void __launch_bounds__(Lay<D, NB>::THREADS, Lay<D, NB>::PER_SM)
     if (tid == 0) asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     pdl_launch();
     if (!a.behind) pdl_wait();
-    deal_out(a, units, list, prefix, sums);
-    if (blockIdx.x >= prefix[units]) {
+    Unit s;
+    uint32_t first;
+    if (!find_unit<true>(a, units, blockIdx.x, room, s, first)) {
         if (a.behind) pdl_wait();      // the launch does not end before the one it follows
         return;
     }
-    const int u = unit_of(prefix, units, blockIdx.x);
-    const Unit s = list[u];
     const Keys ks = keys_of(a, s);
-    const int part = (blockIdx.x - prefix[u]) % s.parts, item = (blockIdx.x - prefix[u]) / s.parts, kvh = item % G, m0 = L::ROWS * (item / G), rows_m = min(L::ROWS, s.rows * group - m0);
+    const int part = (blockIdx.x - first) % s.parts, item = (blockIdx.x - first) / s.parts, kvh = item % G, m0 = L::ROWS * (item / G), rows_m = min(L::ROWS, s.rows * group - m0);
     const int x0 = (int)((long long)ks.turns * part / s.parts), turns = (int)((long long)ks.turns * (part + 1) / s.parts) - x0;
-    if (tid < min(turns, 2 * BATCH)) places[tid] = place_of(a, s, ks, kvh, x0 + tid);
+    const bool looks = tid < min(turns, 2 * BATCH);
+    Place here = {};
+    if (looks) here = places[tid] = place_of(a, s, ks, kvh, x0 + tid);
     __syncthreads();
 
     // Box 2 k of the warp's ring is the keys of its turn k, box 2 k + 1 the values.
@@ -126,8 +122,6 @@ __global__ void __launch_bounds__(Lay<D, NB>::THREADS, Lay<D, NB>::PER_SM)
         // The rows are still being appended: pages that none of them goes to can be fetched, and their units are what they were.
         for (; asked < min(boxes, SLOTS) && places[warp + WARPS * (asked >> 1)].n0 >= 0; asked++) issue(asked, asked);
         pdl_wait();
-        if (tid < min(turns, 2 * BATCH) && places[tid].n0 < 0) places[tid] = place_of(a, s, ks, kvh, x0 + tid);
-        __syncwarp();
     }
     for (; asked < SLOTS; asked++) issue(asked, asked);
 
@@ -174,13 +168,20 @@ __global__ void __launch_bounds__(Lay<D, NB>::THREADS, Lay<D, NB>::PER_SM)
             for (int c = 0; c < CHUNKS; c++) o[n][c][0] = o[n][c][1] = o[n][c][2] = o[n][c][3] = 0.f;
         }
 
-        if (a.behind) __syncthreads();      // places that have been looked up again
+        if (looks) code_units[tid] = units_of(a, here);
+        __syncthreads();
         for (int batch = 0; batch * BATCH < turns; batch++) {
             // the places of the batch after the next one, which replace this one's
             const int next = BATCH * (batch + 2) + tid, end = min(turns, BATCH * (batch + 1));
-            const Place ahead = tid < BATCH && next < turns ? place_of(a, s, ks, kvh, x0 + next) : Place{};
+            Place ahead = {};
+            float2 ahead_units = {};
+            if (tid < BATCH && next < turns) {
+                ahead = place_of(a, s, ks, kvh, x0 + next);
+                ahead_units = units_of(a, ahead);
+            }
             while (ok && warp + WARPS * (j >> 1) < end) {
                 Place p = places[(warp + WARPS * (j >> 1)) % (2 * BATCH)];
+                const float2 un = code_units[(warp + WARPS * (j >> 1)) % (2 * BATCH)];
                 p.n0 = max(p.n0, ~p.n0);
                 if (!mbar_wait(&full[slot], phase)) {
                     ok = false;
@@ -225,10 +226,10 @@ __global__ void __launch_bounds__(Lay<D, NB>::THREADS, Lay<D, NB>::PER_SM)
                     }
                     __syncwarp();
                 }
-                const float f = a.scale * p.ku * (a.softcap > 0.f ? 1.f / a.softcap : LOG2E);
-                const float turn_unit = __fdividef(v_unit, p.vu);      // sums count in the unit of the last turn's values
-                bool still = v_unit == p.vu;                           // sums stay as they are
-                v_unit = p.vu;
+                const float f = a.scale * un.x * (a.softcap > 0.f ? 1.f / a.softcap : LOG2E);
+                const float turn_unit = __fdividef(v_unit, un.y);      // sums count in the unit of the last turn's values
+                bool still = v_unit == un.y;                           // sums stay as they are
+                v_unit = un.y;
                 uint32_t pf[NB][2][2];
                 float corr[NB][2];
 #pragma unroll
@@ -300,7 +301,10 @@ __global__ void __launch_bounds__(Lay<D, NB>::THREADS, Lay<D, NB>::PER_SM)
             }
             if (BATCH * (batch + 2) < turns) {
                 __syncthreads();
-                if (tid < BATCH) places[(batch & 1) * BATCH + tid] = ahead;
+                if (tid < BATCH) {
+                    places[(batch & 1) * BATCH + tid] = ahead;
+                    code_units[(batch & 1) * BATCH + tid] = ahead_units;
+                }
                 __syncthreads();
             }
         }
@@ -357,7 +361,7 @@ __global__ void __launch_bounds__(Lay<D, NB>::THREADS, Lay<D, NB>::PER_SM)
 
 // Sums of an item's row m at column d, over the CTAs first .. first + parts - 1 that had the item.
 __device__ __forceinline__ float merged(const Attn8Args& a, int hd, uint32_t first, int parts, int m, int d) {
-    constexpr int BATCH = 8;                // CTAs whose sums are requested together
+    constexpr int BATCH = 16;               // CTAs whose sums are requested together
     float top = NONE, v = 0.f, l = 0.f;
     for (int c = 0; c < parts; c += BATCH) {
         float2 ml[BATCH];
@@ -386,14 +390,12 @@ __device__ __forceinline__ float merged(const Attn8Args& a, int hd, uint32_t fir
 
 // A CTA a row and as many heads (maps) as it has threads for, one a column.
 __global__ void __launch_bounds__(MERGE_THREADS) attn8_merge_kernel(const __grid_constant__ Attn8Args a) {
-    __shared__ Unit list[MAX_UNITS];
-    __shared__ uint32_t prefix[MAX_UNITS + 1], sums[MERGE_THREADS / 32];
+    __shared__ DealRoom room;
     __shared__ float second[MERGE_THREADS], red[MERGE_THREADS / 32];
     const int hd = a.c.hd, tid = threadIdx.x, G = a.c.kv_heads, group = a.n_heads / G, units = a.positions ? a.rows : a.n_segs;
     const int h = blockIdx.x * (MERGE_THREADS / hd) + tid / hd, d = tid % hd, row = blockIdx.y;
     pdl_launch();
     if (!a.behind) pdl_wait();
-    deal_out(a, units, list, prefix, sums);
     int u = -1;
     if (a.positions) {
         u = row;
@@ -403,16 +405,17 @@ __global__ void __launch_bounds__(MERGE_THREADS) attn8_merge_kernel(const __grid
             if (row >= s.x && row < s.x + s.y) u = i;
         }
     }
+    Unit s;
+    uint32_t first;
+    const bool any = u >= 0 && find_unit<false>(a, units, u, room, s, first);
     if (a.behind) pdl_wait();
-    if (u < 0) return;
-    const Unit s = list[u];
-    if (s.parts == 0) return;
+    if (!any) return;
     const bool in = h < a.n_heads;
     float v = 0.f;
     if (in) {
         const int m = (row - s.row) * group + h % group;
         const uint32_t item = m / a.row_tile * G + h / group;
-        v = merged(a, hd, prefix[u] + item * s.parts, s.parts, m % a.row_tile, d);
+        v = merged(a, hd, first + item * s.parts, s.parts, m % a.row_tile, d);
     }
     int ho = h;
     if (a.diff.on) {        // threads of even maps take the odd ones' results

@@ -65,6 +65,11 @@ __device__ __forceinline__ uint32_t scan(uint32_t x, uint32_t* sums, uint32_t& a
     return x;
 }
 
+// CTAs of each item of a unit, of so many turns in all.
+__device__ __forceinline__ uint32_t parts_of(const Attn8Args& a, uint32_t turns, uint32_t total) {
+    return turns ? max(1u, min((uint32_t)((unsigned long long)turns * a.ctas / total), (turns * a.turn + LEAST - 1) / LEAST)) : 0;
+}
+
 // All units, and the CTAs before each one's (prefix[u]) and in all (prefix[units]).
 __device__ __forceinline__ void deal_out(const Attn8Args& a, int units, Unit* list, uint32_t* prefix, uint32_t* sums) {
     const int tid = threadIdx.x;
@@ -77,7 +82,7 @@ __device__ __forceinline__ void deal_out(const Attn8Args& a, int units, Unit* li
         items = row_tiles(a, s) * a.c.kv_heads;
     }
     scan(turns * items, sums, total);
-    const uint32_t parts = turns ? max(1u, min((uint32_t)((unsigned long long)turns * a.ctas / total), (turns * a.turn + LEAST - 1) / LEAST)) : 0;
+    const uint32_t parts = parts_of(a, turns, total);
     const uint32_t x = scan(parts * items, sums, ctas);
     if (tid < units) {
         prefix[tid] = x - parts * items;
@@ -102,6 +107,52 @@ __device__ __forceinline__ int unit_of(const uint32_t* prefix, int units, uint32
         else hi = mid - 1;
     }
     return lo;               // of units without turns, the one behind them
+}
+
+struct DealRoom {
+    Unit list[MAX_UNITS];
+    uint32_t prefix[MAX_UNITS + 1], sums[32];
+};
+// The unit of CTA x (BY_CTA) or unit x, and the first of its CTAs; false: there is none.  Of up to 32 units every warp finds out by itself: with the block's scans a small step took
+// 2 us more.
+template <bool BY_CTA>
+__device__ __forceinline__ bool find_unit(const Attn8Args& a, int units, uint32_t x, DealRoom& room, Unit& s, uint32_t& first) {
+    if (units > 32) {
+        deal_out(a, units, room.list, room.prefix, room.sums);
+        if (BY_CTA && x >= room.prefix[units]) return false;
+        const int u = BY_CTA ? unit_of(room.prefix, units, x) : x;
+        s = room.list[u];
+        first = room.prefix[u];
+        return s.parts > 0;
+    }
+    constexpr uint32_t ALL = 0xffffffffu;
+    const int lane = threadIdx.x & 31;
+    Unit m = {};
+    uint32_t turns = 0, items = 0;
+    if (lane < units) {
+        m = unit_at(a, lane);
+        turns = keys_of(a, m).turns;
+        items = row_tiles(a, m) * a.c.kv_heads;
+    }
+    const uint32_t parts = parts_of(a, turns, __reduce_add_sync(ALL, turns * items)), n = parts * items;
+    uint32_t end = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(ALL, end, o);
+        if (lane >= o) end += y;
+    }
+    const uint32_t mine = __ballot_sync(ALL, BY_CTA ? x >= end - n && x < end : lane == (int)x && n > 0);
+    if (!mine) return false;
+    const int u = __ffs(mine) - 1;
+    s.row = __shfl_sync(ALL, m.row, u);
+    s.rows = __shfl_sync(ALL, m.rows, u);
+    s.slot = __shfl_sync(ALL, m.slot, u);
+    s.pos = __shfl_sync(ALL, m.pos, u);
+    s.parts = __shfl_sync(ALL, (int)parts, u);
+    first = __shfl_sync(ALL, end - n, u);
+    // other rows of the slot may go to earlier pages
+    s.open = __reduce_min_sync(ALL, lane < units && m.slot == s.slot && m.pos >= 0 ? m.pos >> PAGE_SHIFT : 0x7fffffff);
+    return true;
 }
 
 }  // namespace

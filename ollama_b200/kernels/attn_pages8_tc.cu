@@ -57,8 +57,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn8_tc_kernel(const __grid_const
     extern __shared__ uint8_t smem_raw[];
     uint8_t* sm = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     __shared__ uint64_t bars[24];
-    __shared__ Unit list[MAX_UNITS];
-    __shared__ uint32_t prefix[MAX_UNITS + 1], sums[THREADS / 32], tmem_slot;
+    __shared__ DealRoom room;
+    __shared__ uint32_t tmem_slot;
     __shared__ int failed;
     __shared__ float2 units8[BOXES];             // of the two pages in a box
     __shared__ float x_max[2][2][128], x_sum[2][128];
@@ -86,12 +86,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn8_tc_kernel(const __grid_const
     }
     pdl_launch();
     pdl_wait();
-    deal_out(a, n_units, list, prefix, sums);
-    if (blockIdx.x >= prefix[n_units]) return;
-    const int u = unit_of(prefix, n_units, blockIdx.x);
-    const Unit s = list[u];
+    Unit s;
+    uint32_t first;
+    if (!find_unit<true>(a, n_units, blockIdx.x, room, s, first)) return;
     const Keys ks = keys_of(a, s);
-    const int part = (blockIdx.x - prefix[u]) % s.parts, item = (blockIdx.x - prefix[u]) / s.parts, kvh = item % G, m0 = BQ * (item / G), rows_m = min(BQ, s.rows * group - m0);
+    const int part = (blockIdx.x - first) % s.parts, item = (blockIdx.x - first) / s.parts, kvh = item % G, m0 = BQ * (item / G), rows_m = min(BQ, s.rows * group - m0);
     const int x0 = (int)((long long)ks.turns * part / s.parts), n_tiles = (int)((long long)ks.turns * (part + 1) / s.parts) - x0;
     // positions of the tile's first and last row, the last one's first key
     const int first_pos = s.pos + m0 / group, last_pos = s.pos + min(s.rows - 1, (m0 + BQ - 1) / group), last_lo = first_key(last_pos, a.chunk, a.window), keep = a.window > 0 ? a.keep : 0;

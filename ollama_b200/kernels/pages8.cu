@@ -363,14 +363,13 @@ __global__ void __launch_bounds__(THREADS) append8_kernel(const __grid_constant_
     }
     // rows of one slot take their turns in one CTA: the first of them appends them all, in order
     const int g = b % G, u = b / G, slot = a.slots[u];
-    int before = 0, behind = 0;
-    for (int i = threadIdx.x; i < a.rows; i += THREADS)
-        if (a.slots[i] == slot) {
-            before |= i < u;
-            behind |= i > u;
-        }
-    if (__syncthreads_or(before)) return;
-    behind = __syncthreads_or(behind);
+    uint32_t before = 0, behind = 0;      // every warp for itself
+    for (int i = threadIdx.x & 31; i < ((a.rows + 31) & ~31); i += 32) {
+        const bool same = i < a.rows && a.slots[i] == slot;
+        before |= __ballot_sync(0xffffffffu, same && i < u);
+        behind |= __ballot_sync(0xffffffffu, same && i > u);
+    }
+    if (before) return;
     for (int i = u; i < (behind ? a.rows : u + 1); i++) {
         if (a.slots[i] != slot || a.positions[i] < 0) continue;
         append_to_page<VEC, false>(a, i, 1, slot, a.positions[i], g, cs, red);
