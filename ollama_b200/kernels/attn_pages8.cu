@@ -19,7 +19,7 @@ using namespace tc;
 
 constexpr int TURN = 32;                     // keys
 constexpr int BATCH = 128;                   // turns whose places are looked up at a time
-constexpr int MERGE_THREADS = 256;
+constexpr int MERGE_COLUMNS = 256;
 
 __device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -359,18 +359,18 @@ __global__ void __launch_bounds__(Lay<D, NB>::THREADS, Lay<D, NB>::PER_SM)
     }
 }
 
-// Sums of an item's row m at column d, over the CTAs first .. first + parts - 1 that had the item.
-__device__ __forceinline__ float merged(const Attn8Args& a, int hd, uint32_t first, int parts, int m, int d) {
-    constexpr int BATCH = 16;               // CTAs whose sums are requested together
+// Sums of an item's row m at column d, over the CTAs from .. to - 1: unnormalised result, sum, largest score.
+template <int BATCH>        // CTAs whose sums are requested together
+__device__ __forceinline__ float3 merged(const Attn8Args& a, int hd, uint32_t from, uint32_t to, int m, int d) {
     float top = NONE, v = 0.f, l = 0.f;
-    for (int c = 0; c < parts; c += BATCH) {
+    for (uint32_t c = from; c < to; c += BATCH) {
         float2 ml[BATCH];
         float x[BATCH], mn = top;
 #pragma unroll
         for (int i = 0; i < BATCH; i++) {
-            const size_t at = (size_t)(first + c + i) * a.row_tile + m;
-            ml[i] = c + i < parts ? __ldcg(a.part_ml + at) : make_float2(NONE, 0.f);
-            x[i] = c + i < parts ? __ldcg(a.part_acc + at * hd + d) : 0.f;
+            const size_t at = (size_t)(c + i) * a.row_tile + m;
+            ml[i] = c + i < to ? __ldcg(a.part_ml + at) : make_float2(NONE, 0.f);
+            x[i] = c + i < to ? __ldcg(a.part_acc + at * hd + d) : 0.f;
         }
 #pragma unroll
         for (int i = 0; i < BATCH; i++) mn = fmaxf(mn, ml[i].x);
@@ -385,15 +385,19 @@ __device__ __forceinline__ float merged(const Attn8Args& a, int hd, uint32_t fir
             l = fmaf(ml[i].y, f, l);
         }
     }
-    return v / l;
+    return make_float3(v, l, top);
 }
 
-// A CTA a row and as many heads (maps) as it has threads for, one a column.
-__global__ void __launch_bounds__(MERGE_THREADS) attn8_merge_kernel(const __grid_constant__ Attn8Args a) {
+// A CTA a row and MERGE_COLUMNS columns of its heads (maps), a thread a column.  With HALVES two threads share a column, each with half of the CTAs' sums, and ask for
+// more of them together.
+template <int HALVES>
+__global__ void __launch_bounds__(MERGE_COLUMNS * HALVES) attn8_merge_kernel(const __grid_constant__ Attn8Args a) {
+    constexpr int HALF = MERGE_COLUMNS, BATCH = 8 * HALVES;
     __shared__ DealRoom room;
-    __shared__ float second[MERGE_THREADS], red[MERGE_THREADS / 32];
-    const int hd = a.c.hd, tid = threadIdx.x, G = a.c.kv_heads, group = a.n_heads / G, units = a.positions ? a.rows : a.n_segs;
-    const int h = blockIdx.x * (MERGE_THREADS / hd) + tid / hd, d = tid % hd, row = blockIdx.y;
+    __shared__ float3 theirs[HALVES == 2 ? HALF : 1];
+    __shared__ float second[HALF], red[HALF / 32];
+    const int hd = a.c.hd, tid = threadIdx.x % HALF, half = threadIdx.x / HALF, G = a.c.kv_heads, group = a.n_heads / G, units = a.positions ? a.rows : a.n_segs;
+    const int h = blockIdx.x * (HALF / hd) + tid / hd, d = tid % hd, row = blockIdx.y;
     pdl_launch();
     if (!a.behind) pdl_wait();
     int u = -1;
@@ -405,36 +409,45 @@ __global__ void __launch_bounds__(MERGE_THREADS) attn8_merge_kernel(const __grid
             if (row >= s.x && row < s.x + s.y) u = i;
         }
     }
+    const int ho = a.diff.on ? h >> 1 : h;
+    const bool in = h < a.n_heads, out = in && half == 0 && d < a.vdim && !(a.diff.on && h & 1);
+    float gate = 1.f;
+    if (out && a.gate.kind) gate = sigmoid_f(a.gate.g[(size_t)row * a.gate.ld + (a.gate.kind == 1 ? ho * a.vdim + d : ho)]);
     Unit s;
     uint32_t first;
     const bool any = u >= 0 && find_unit<false>(a, units, u, room, s, first);
     if (a.behind) pdl_wait();
     if (!any) return;
-    const bool in = h < a.n_heads;
-    float v = 0.f;
+    float3 x = make_float3(0.f, 1.f, 0.f);
     if (in) {
         const int m = (row - s.row) * group + h % group;
-        const uint32_t item = m / a.row_tile * G + h / group;
-        v = merged(a, hd, first + item * s.parts, s.parts, m % a.row_tile, d);
+        const uint32_t from = first + (m / a.row_tile * G + h / group) * s.parts, to = from + s.parts, middle = HALVES == 2 ? from + (s.parts + 1) / 2 : to;
+        x = merged<BATCH>(a, hd, half ? middle : from, half ? to : middle, m % a.row_tile, d);
     }
-    int ho = h;
+    if (HALVES == 2) {
+        if (half) theirs[tid] = x;
+        __syncthreads();
+        const float3 y = theirs[tid];
+        const float top = fmaxf(x.z, y.z), f = ex2(x.z - top), g = ex2(y.z - top);
+        x.x = x.x * f + y.x * g;
+        x.y = x.y * f + y.y * g;
+    }
+    float v = x.x / x.y;
     if (a.diff.on) {        // threads of even maps take the odd ones' results
         if (d >= a.vdim) v = 0.f;
-        second[tid] = v;
+        if (!half) second[tid] = v;
         __syncthreads();
         const int map = tid / hd & 1;
         if (!map) v -= a.diff.lambda * second[tid + hd];
         const float sq = warp_sum(v * v);
-        if ((tid & 31) == 0) red[tid >> 5] = sq;
+        if (!half && (tid & 31) == 0) red[tid >> 5] = sq;
         __syncthreads();
-        if (map) return;
         float sum = 0.f;
         for (int w = 0; w < hd / 32; w++) sum += red[tid / hd * (hd / 32) + w];
         v *= a.diff.scale / sqrtf(sum / (float)a.vdim + a.diff.eps);
-        ho = h >> 1;
     }
-    if (!in || d >= a.vdim) return;
-    if (a.gate.kind) v *= sigmoid_f(a.gate.g[(size_t)row * a.gate.ld + (a.gate.kind == 1 ? ho * a.vdim + d : ho)]);
+    if (!out) return;
+    v *= gate;
     const size_t oi = (size_t)row * a.ldo + (size_t)ho * a.vdim + d;
     if (a.out16) ((__nv_bfloat16*)a.out)[oi] = __float2bfloat16_rn(v);
     else ((float*)a.out)[oi] = v;
@@ -485,7 +498,15 @@ int launch(Attn8Args& a, int pdl, cudaStream_t st) {
 
 static int attn8_launch(const Attn8Args& in, int pdl, cudaStream_t st) {
     if (bad_args(in)) return (int)cudaErrorInvalidValue;
-    const int units = in.positions ? in.rows : in.n_segs, heads = MERGE_THREADS / in.c.hd;
+    static PerDeviceOnce once;      // an SM that is set for less shared memory takes the attention kernel's CTAs only when it is empty
+    if (once.first()) {
+        cudaFuncSetAttribute(attn8_merge_kernel<1>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+        cudaFuncSetAttribute(attn8_merge_kernel<2>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    }
+    int dev = 0, sms = 0;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    const int units = in.positions ? in.rows : in.n_segs, heads = MERGE_COLUMNS / in.c.hd;
     for (int u = 0; u < units; u += MAX_UNITS) {
         Attn8Args a = in;
         const int n = units - u < MAX_UNITS ? units - u : MAX_UNITS;
@@ -504,7 +525,11 @@ static int attn8_launch(const Attn8Args& in, int pdl, cudaStream_t st) {
         int rc = launch(a, pdl || a.behind, st);
         if (rc) return rc;
         void* args[] = {&a};
-        rc = launch_rows((const void*)attn8_merge_kernel, dim3((a.n_heads + heads - 1) / heads, a.rows), dim3(MERGE_THREADS), 0, args, st, 1);
+        const dim3 grid((a.n_heads + heads - 1) / heads, a.rows);
+        // Two threads a column while there are no more CTAs than SMs (16 heads at 6144: 16.6 -> 13.0 us a step); beyond, other CTAs' loads fill the time, and two cost
+        // (64 rows of 32 heads at 30000: 88 -> 103 us).
+        const bool wide = grid.x * grid.y <= (unsigned)sms;
+        rc = launch_rows(wide ? (const void*)attn8_merge_kernel<2> : (const void*)attn8_merge_kernel<1>, grid, dim3(wide ? 2 * MERGE_COLUMNS : MERGE_COLUMNS), 0, args, st, 1);
         if (rc) return rc;
         pdl = 1;
     }

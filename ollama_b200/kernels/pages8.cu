@@ -149,13 +149,9 @@ __device__ __forceinline__ float peer_value(const float* p, int rank) {
 template <bool VEC, bool PEERS>
 __device__ void append_to_page(const Append8Args& a, int row, int n, int slot, int pos, int g, float* cs, float* red) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int page = page_at(a.t, a.c.n_pages, slot, pos >> PAGE_SHIFT);
-    if (page < 0) return;
     const int half = a.n_rot >> 1, pitch = (half + 3) & ~3, kdim = a.maps * a.dim, G = a.c.kv_heads, hd = a.c.hd;
     const int nq = a.n_heads * a.dim, nk = G * kdim, off = pos & (PAGE - 1);
     float* sn = cs + (a.positions ? 1 : PAGE) * pitch;      // as many rows as the launch has shared memory for
-    const size_t head = (size_t)page * G + g;
-    const float old_k = a.c.ku[head], old_v = a.c.vu[head];
     float k[PAGE / WARPS][COLS], v[PAGE / WARPS][COLS];
 #pragma unroll
     for (int i = 0; i < PAGE / WARPS; i++) {
@@ -169,6 +165,10 @@ __device__ void append_to_page(const Append8Args& a, int row, int n, int slot, i
             for (int j = 0; j < COLS; j++) k[i][j] = 0.f;
         }
     }
+    const int page = page_at(a.t, a.c.n_pages, slot, pos >> PAGE_SHIFT);
+    if (page < 0) return;
+    const size_t head = (size_t)page * G + g;
+    const float old_k = a.c.ku[head], old_v = a.c.vu[head];
     __syncthreads();      // the tables may still be read for the rows before
     if (n == 1) {
         for (int p = tid; p < half; p += THREADS) {
@@ -347,17 +347,17 @@ __device__ __forceinline__ void query_row(const Append8Args& a, int row, int pos
 // Norm of q and k, rotation, q to padded fp32 rows; k and v become codes of the pages they go to, whose units grow so that the largest magnitude fits.  A page whose first
 // position is among the rows begins anew.  Of single rows a CTA has a KV head of a row, and then one the queries of a row.
 template <bool VEC>
-__global__ void __launch_bounds__(THREADS) append8_kernel(const __grid_constant__ Append8Args a) {
+__global__ void __launch_bounds__(THREADS, 4) append8_kernel(const __grid_constant__ Append8Args a) {
     extern __shared__ __align__(16) float cs[];
     __shared__ float red[WARPS];
     pdl_wait();
     pdl_launch();         // behind the wait: a kernel that starts now may read whatever was written before this one
     const int G = a.c.kv_heads, kv_ctas = a.no_append ? 0 : a.rows * G, b = blockIdx.x;
     if (b >= kv_ctas) {
-        const int pos = a.positions[b - kv_ctas];
-        if (pos < 0) return;
         float x[HELD][COLS];
         load_heads<VEC>(a, b - kv_ctas, x);
+        const int pos = a.positions[b - kv_ctas];
+        if (pos < 0) return;
         query_row<VEC>(a, b - kv_ctas, pos, x, cs, red);
         return;
     }
@@ -475,6 +475,11 @@ int append8_launch(const Append8Args& in, int pdl, cudaStream_t st) {
     const size_t one = 2 * sizeof(float) * (pitch ? pitch : 4);      // cosines and sines of a row
     Append8Args copy = *a;
     if (a->positions) {
+        static PerDeviceOnce once;      // an SM that is set for less shared memory takes the CTAs of the attention behind this launch only when it is empty
+        if (once.first()) {
+            cudaFuncSetAttribute(append8_kernel<true>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+            cudaFuncSetAttribute(append8_kernel<false>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+        }
         void* args[] = {&copy};
         return launch_rows(vec ? (const void*)append8_kernel<true> : (const void*)append8_kernel<false>, dim3((unsigned)(ctas + a->rows)), dim3(THREADS), one, args, st, pdl);
     }
