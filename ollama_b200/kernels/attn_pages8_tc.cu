@@ -18,7 +18,7 @@ using namespace tc;
 
 constexpr int BQ = 128, BKV = 128;
 constexpr int ATOM_BYTES = 128 * 128;        // 128 rows x 64 f16
-constexpr int SOFTMAX_WARPS = 8, CODE_WARPS = 6, FIRST_CODE_WARP = 10, THREADS = 32 * (FIRST_CODE_WARP + CODE_WARPS);      // whole groups of four warps, whose registers are split
+constexpr int SOFTMAX_WARPS = 8, CODE_WARPS = 8, FIRST_CODE_WARP = 12, THREADS = 32 * (FIRST_CODE_WARP + CODE_WARPS);      // whole groups of four warps, whose registers are split
 constexpr int BOXES = 3;
 constexpr uint32_t TMEM_COLS = 512;
 
@@ -53,7 +53,7 @@ __device__ __forceinline__ void put_codes(uint8_t* tile, int r, int c, const uin
 template <int D>
 __global__ void __launch_bounds__(THREADS, 1) attn8_tc_kernel(const __grid_constant__ Attn8Args a) {
     using L = Lay<D>;
-    constexpr int OH = D / 2, CHUNKS = D / 16, CODE_THREADS = 32 * CODE_WARPS, EACH = (BKV * CHUNKS + CODE_THREADS - 1) / CODE_THREADS;      // 16 codes at a time of a code thread
+    constexpr int OH = D / 2, CHUNKS = D / 16, CODE_THREADS = 32 * CODE_WARPS, EACH = BKV * CHUNKS / CODE_THREADS;      // 16 codes at a time of a code thread
     extern __shared__ uint8_t smem_raw[];
     uint8_t* sm = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     __shared__ uint64_t bars[24];
@@ -61,6 +61,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn8_tc_kernel(const __grid_const
     __shared__ uint32_t tmem_slot;
     __shared__ int failed;
     __shared__ float2 units8[BOXES];             // of the two pages in a box
+    __shared__ uint8_t no_number[2][BKV];        // of a tile that some row does not see all of: keys whose values hold what is no number
     __shared__ float x_max[2][2][128], x_sum[2][128];
     uint64_t *full8 = bars, *empty8 = bars + 3, *k_full = bars + 6, *k_empty = bars + 8, *v_full = bars + 10, *v_empty = bars + 12, *s_full = bars + 14, *p_ready = bars + 16,
              *o_full = bars + 18, *pair = bars + 20;
@@ -97,6 +98,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn8_tc_kernel(const __grid_const
     auto n0_of = [&](int t) { return first_of(ks, BKV, x0 + t); };
     auto masked = [&](int n0) { return n0 + BKV - 1 > first_pos || (n0 < last_lo && n0 + BKV > keep); };      // some row does not see some key
 
+    // The boxes in the order in which the products take them: K(0), K(1), V(0), K(2), V(1), ... V(n - 1).  x: tile, y: 1 with values
+    auto box_of = [&](int j) { return j == 2 * n_tiles - 1 ? make_int2(n_tiles - 1, 1) : j > 0 && (j & 1) == 0 ? make_int2(j / 2 - 1, 1) : make_int2((j + 1) / 2, 0); };
+
     if (warp == 9) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -123,44 +127,42 @@ __global__ void __launch_bounds__(THREADS, 1) attn8_tc_kernel(const __grid_const
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
 
-    // 64 K registers: 168 a softmax thread, 88 a thread of the other two groups
+    // 60 K registers: 168 a softmax thread, 48 a thread of the other three groups
     if (warp >= SOFTMAX_WARPS) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
         if (warp == 8) {
-            // Box 2 t holds the keys of tile t, box 2 t + 1 the values.  The lanes look up the pages of 32 tiles at a time.
+            // The lanes look up the pages of 32 boxes at a time.
             const int last_page = (s.pos + s.rows - 1) >> PAGE_SHIFT;
             bool ok = true;
             int asked = 0;                           // boxes
-            for (int t0 = 0; t0 < n_tiles && ok; t0 += 32) {
-                size_t head[2] = {};
-                float2 ku = make_float2(0.f, 0.f), vu = ku;
-                if (t0 + lane < n_tiles) {
-                    const int p0 = n0_of(t0 + lane) >> PAGE_SHIFT;
-                    for (int i = 0; i < 2; i++) head[i] = (size_t)max(page_at(a.t, a.c.n_pages, s.slot, min(p0 + i, last_page)), 0) * G + kvh;
-                    ku = make_float2(a.c.ku[head[0]], a.c.ku[head[1]]);
-                    vu = make_float2(a.c.vu[head[0]], a.c.vu[head[1]]);
+            for (int j0 = 0; j0 < 2 * n_tiles && ok; j0 += 32) {
+                int head[2] = {};
+                float2 un = make_float2(0.f, 0.f);
+                if (j0 + lane < 2 * n_tiles) {
+                    const int2 of = box_of(j0 + lane);
+                    const int p0 = n0_of(of.x) >> PAGE_SHIFT;
+                    const float* units = of.y ? a.c.vu : a.c.ku;
+                    for (int i = 0; i < 2; i++) head[i] = max(page_at(a.t, a.c.n_pages, s.slot, min(p0 + i, last_page)), 0) * G + kvh;
+                    un = make_float2(units[head[0]], units[head[1]]);
                 }
-                for (int t = t0; t < min(n_tiles, t0 + 32) && ok; t++) {
-                    const size_t h0 = __shfl_sync(0xffffffffu, head[0], t - t0), h1 = __shfl_sync(0xffffffffu, head[1], t - t0);
-                    const float2 uk = make_float2(__shfl_sync(0xffffffffu, ku.x, t - t0), __shfl_sync(0xffffffffu, ku.y, t - t0));
-                    const float2 uv = make_float2(__shfl_sync(0xffffffffu, vu.x, t - t0), __shfl_sync(0xffffffffu, vu.y, t - t0));
-                    for (int v = 0; v < 2; v++) {
-                        const int j = 2 * t + v, slot = j % BOXES;
-                        if (j >= BOXES && !mbar_wait(&empty8[slot], (j / BOXES - 1) & 1)) {
-                            ok = false;
-                            break;
-                        }
-                        if (lane == 0) {
-                            uint8_t* box = sm + L::OFF_BOX + slot * L::BOX;
-                            const uint8_t* from = v ? a.c.v : a.c.k;
-                            units8[slot] = v ? uv : uk;
-                            mbar_expect_tx(&full8[slot], L::BOX);
-                            bulk_copy(box, from + h0 * PAGE * D, PAGE * D, &full8[slot]);
-                            bulk_copy(box + PAGE * D, from + h1 * PAGE * D, PAGE * D, &full8[slot]);
-                        }
-                        asked++;
-                        __syncwarp();
+                for (int j = j0; j < min(2 * n_tiles, j0 + 32); j++) {
+                    const size_t h0 = __shfl_sync(0xffffffffu, head[0], j - j0), h1 = __shfl_sync(0xffffffffu, head[1], j - j0);
+                    const float2 u = make_float2(__shfl_sync(0xffffffffu, un.x, j - j0), __shfl_sync(0xffffffffu, un.y, j - j0));
+                    const int slot = j % BOXES;
+                    if (j >= BOXES && !mbar_wait(&empty8[slot], (j / BOXES - 1) & 1)) {
+                        ok = false;
+                        break;
                     }
+                    if (lane == 0) {
+                        uint8_t* box = sm + L::OFF_BOX + slot * L::BOX;
+                        const uint8_t* from = box_of(j).y ? a.c.v : a.c.k;
+                        units8[slot] = u;
+                        mbar_expect_tx(&full8[slot], L::BOX);
+                        bulk_copy(box, from + h0 * PAGE * D, PAGE * D, &full8[slot]);
+                        bulk_copy(box + PAGE * D, from + h1 * PAGE * D, PAGE * D, &full8[slot]);
+                    }
+                    asked++;
+                    __syncwarp();
                 }
             }
             if (!ok && lane == 0) atomicExch(&failed, 1);
@@ -168,63 +170,34 @@ __global__ void __launch_bounds__(THREADS, 1) attn8_tc_kernel(const __grid_const
         } else if (warp >= FIRST_CODE_WARP) {
             const int t0 = tid - 32 * FIRST_CODE_WARP;                // its chunks of a box are t0 + CODE_THREADS i
             bool ok = true;
-            for (int t = 0; t < n_tiles && ok; t++) {
-                const int b = t & 1, jk = 2 * t, jv = jk + 1, sk = jk % BOXES, sv = jv % BOXES;
-                const uint8_t *kbox = sm + L::OFF_BOX + sk * L::BOX, *vbox = sm + L::OFF_BOX + sv * L::BOX;
-                uint32_t bad = 0;                    // rows of the thread's chunks whose values hold what is no number: they become zeros and their keys none
-                if (!mbar_wait(&full8[sk], (jk / BOXES) & 1)) { ok = false; break; }
-                if (masked(n0_of(t))) {
-                    if (!mbar_wait(&full8[sv], (jv / BOXES) & 1)) { ok = false; break; }
+            for (int j = 0; j < 2 * n_tiles; j++) {
+                const int slot = j % BOXES, tile = box_of(j).x, is_v = box_of(j).y, b = tile & 1;
+                if (!mbar_wait(&full8[slot], (j / BOXES) & 1)) { ok = false; break; }
+                const uint4* box = reinterpret_cast<const uint4*>(sm + L::OFF_BOX + slot * L::BOX);
+                uint4 w[EACH];             // all of them before anything is stored: the compiler keeps loads behind stores
+#pragma unroll
+                for (int i = 0; i < EACH; i++) w[i] = box[t0 + CODE_THREADS * i];
+                if (tile >= 2 && !mbar_wait(is_v ? &v_empty[b] : &k_empty[b], ((tile >> 1) - 1) & 1)) { ok = false; break; }
+                if (is_v && masked(n0_of(tile))) {       // a weight of zero times what is no number: such values become zeros, and their keys' scores none
 #pragma unroll
                     for (int i = 0; i < EACH; i++) {
-                        uint32_t none = t0 + CODE_THREADS * i < BKV * CHUNKS && holds_nan(reinterpret_cast<const uint4*>(vbox)[t0 + CODE_THREADS * i]);
+                        uint32_t none = holds_nan(w[i]);
 #pragma unroll
                         for (int o = 1; o < CHUNKS; o <<= 1) none |= __shfl_xor_sync(0xffffffffu, none, o);
-                        bad |= none << i;
+                        if (none) w[i] = make_uint4(0, 0, 0, 0);
+                        if ((t0 + CODE_THREADS * i) % CHUNKS == 0) no_number[b][(t0 + CODE_THREADS * i) / CHUNKS] = none != 0;
                     }
                 }
-                if (t >= 2 && !mbar_wait(&k_empty[b], ((t >> 1) - 1) & 1)) { ok = false; break; }
-                {
-                    const float2 un = units8[sk];
-                    const __half2 u0 = __float2half2_rn(un.x), u1 = __float2half2_rn(un.y);
-                    uint4 w[EACH];             // all of them before anything is stored: the compiler keeps loads behind stores
+                const float2 un = units8[slot];
+                const __half2 u0 = __float2half2_rn(un.x), u1 = __float2half2_rn(un.y);
+                uint8_t* to = sm + (is_v ? L::OFF_V : L::OFF_K) + b * L::TILE;
 #pragma unroll
-                    for (int i = 0; i < EACH; i++)
-                        if (t0 + CODE_THREADS * i < BKV * CHUNKS) w[i] = reinterpret_cast<const uint4*>(kbox)[t0 + CODE_THREADS * i];
-#pragma unroll
-                    for (int i = 0; i < EACH; i++) {
-                        const int at = t0 + CODE_THREADS * i;
-                        if (bad >> i & 1) w[i] = make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu);
-                        if (at < BKV * CHUNKS) put_codes(sm + L::OFF_K + b * L::TILE, at / CHUNKS, at % CHUNKS, w[i], at / CHUNKS < PAGE ? u0 : u1);
-                    }
-                }
+                for (int i = 0; i < EACH; i++) put_codes(to, (t0 + CODE_THREADS * i) / CHUNKS, (t0 + CODE_THREADS * i) % CHUNKS, w[i], i < EACH / 2 ? u0 : u1);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) {
-                    mbar_arrive(&k_full[b]);
-                    mbar_arrive(&empty8[sk]);
-                }
-                if (!mbar_wait(&full8[sv], (jv / BOXES) & 1)) { ok = false; break; }
-                if (t >= 2 && !mbar_wait(&v_empty[b], ((t >> 1) - 1) & 1)) { ok = false; break; }
-                {
-                    const float2 un = units8[sv];
-                    const __half2 u0 = __float2half2_rn(un.x), u1 = __float2half2_rn(un.y);
-                    uint4 w[EACH];
-#pragma unroll
-                    for (int i = 0; i < EACH; i++)
-                        if (t0 + CODE_THREADS * i < BKV * CHUNKS) w[i] = reinterpret_cast<const uint4*>(vbox)[t0 + CODE_THREADS * i];
-#pragma unroll
-                    for (int i = 0; i < EACH; i++) {
-                        const int at = t0 + CODE_THREADS * i;
-                        if (bad >> i & 1) w[i] = make_uint4(0, 0, 0, 0);
-                        if (at < BKV * CHUNKS) put_codes(sm + L::OFF_V + b * L::TILE, at / CHUNKS, at % CHUNKS, w[i], at / CHUNKS < PAGE ? u0 : u1);
-                    }
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(&v_full[b]);
-                    mbar_arrive(&empty8[sv]);
+                    mbar_arrive(is_v ? &v_full[b] : &k_full[b]);
+                    mbar_arrive(&empty8[slot]);
                 }
             }
             if (!ok) atomicExch(&failed, 1);
@@ -306,11 +279,14 @@ __global__ void __launch_bounds__(THREADS, 1) attn8_tc_kernel(const __grid_const
             }
             if (masked(n0)) {
                 const int kp0 = n0 + 64 * c;
+                if (!mbar_wait(&v_full[b], (t >> 1) & 1)) { ok = false; break; }
+                const uint32_t none[2] = {__ballot_sync(0xffffffffu, no_number[b][64 * c + lane]), __ballot_sync(0xffffffffu, no_number[b][64 * c + 32 + lane])};
 #pragma unroll
                 for (int i = 0; i < 2; i++)
 #pragma unroll
                     for (int j = 0; j < 32; j++) {
                         const int kp = kp0 + 32 * i + j;
+                        if (none[i] >> j & 1) v[i][j] = 0x7fffffffu;
                         if (kp > qp || (kp < row_lo && kp >= keep)) v[i][j] = 0xff800000u;
                     }
             }
