@@ -18,9 +18,10 @@ using namespace tc;
 
 constexpr int BQ = 128, BKV = 128;
 constexpr int ATOM_BYTES = 128 * 128;        // 128 rows x 64 f16
-constexpr int SOFTMAX_WARPS = 8, CODE_WARPS = 8, FIRST_CODE_WARP = 12, THREADS = 32 * (FIRST_CODE_WARP + CODE_WARPS);      // whole groups of four warps, whose registers are split
+constexpr int SOFTMAX_WARPS = 8, CODE_WARPS = 8, TEAM = CODE_WARPS / 2, FIRST_CODE_WARP = 12, THREADS = 32 * (FIRST_CODE_WARP + CODE_WARPS);      // whole groups of four warps, whose registers are split
 constexpr int BOXES = 3;
 constexpr uint32_t TMEM_COLS = 512;
+constexpr float LAG = 8.f;
 
 template <int D>
 struct Lay {
@@ -32,10 +33,21 @@ __device__ __forceinline__ void bulk_copy(void* dst, const void* src, uint32_t b
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
 
+__device__ __forceinline__ void tmem_ld8(uint32_t at, uint32_t (&v)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(at));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t at, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * SOFTMAX_WARPS) : "memory"); }
+
 // 16 codes of row r, columns 16 c .. 16 c + 15, times the unit, into a swizzled tile.  The half that comes first differs between columns below and above 64, whose atoms have the
 // same banks.
 __device__ __forceinline__ void put_codes(uint8_t* tile, int r, int c, const uint4& w, __half2 unit) {
-    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+    const int k = 2 * (c & 3), first = c >> 2 & 1;
+    const uint32_t x[4] = {first ? w.z : w.x, first ? w.w : w.y, first ? w.x : w.z, first ? w.y : w.w};
     uint32_t y[8];
 #pragma unroll
     for (int j = 0; j < 8; j++) {
@@ -44,45 +56,42 @@ __device__ __forceinline__ void put_codes(uint8_t* tile, int r, int c, const uin
         y[j] = *reinterpret_cast<const uint32_t*>(&f);
     }
     uint8_t* row = tile + (c >> 2) * ATOM_BYTES + r * 128;
-    const int k = 2 * (c & 3), first = c >> 2 & 1;
-    const uint4 lo = make_uint4(y[0], y[1], y[2], y[3]), hi = make_uint4(y[4], y[5], y[6], y[7]);
-    *reinterpret_cast<uint4*>(row + (((k + first) ^ (r & 7)) << 4)) = first ? hi : lo;
-    *reinterpret_cast<uint4*>(row + (((k + 1 - first) ^ (r & 7)) << 4)) = first ? lo : hi;
+    *reinterpret_cast<uint4*>(row + (((k + first) ^ (r & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
+    *reinterpret_cast<uint4*>(row + (((k + 1 - first) ^ (r & 7)) << 4)) = make_uint4(y[4], y[5], y[6], y[7]);
 }
 
 template <int D>
 __global__ void __launch_bounds__(THREADS, 1) attn8_tc_kernel(const __grid_constant__ Attn8Args a) {
     using L = Lay<D>;
-    constexpr int OH = D / 2, CHUNKS = D / 16, CODE_THREADS = 32 * CODE_WARPS, EACH = BKV * CHUNKS / CODE_THREADS;      // 16 codes at a time of a code thread
+    constexpr int OH = D / 2, PITCH = D + 4, CHUNKS = D / 16, CODE_THREADS = 32 * TEAM, EACH = BKV * CHUNKS / CODE_THREADS;      // 16 codes at a time of a code thread
     extern __shared__ uint8_t smem_raw[];
     uint8_t* sm = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    __shared__ uint64_t bars[24];
+    __shared__ uint64_t bars[20];
     __shared__ DealRoom room;
     __shared__ uint32_t tmem_slot;
     __shared__ int failed;
     __shared__ float2 units8[BOXES];             // of the two pages in a box
     __shared__ uint8_t no_number[2][BKV];        // of a tile that some row does not see all of: keys whose values hold what is no number
-    __shared__ float x_max[2][2][128], x_sum[2][128];
+    __shared__ float2 x_ml[2][128];              // of the two groups: reference, sum
     uint64_t *full8 = bars, *empty8 = bars + 3, *k_full = bars + 6, *k_empty = bars + 8, *v_full = bars + 10, *v_empty = bars + 12, *s_full = bars + 14, *p_ready = bars + 16,
-             *o_full = bars + 18, *pair = bars + 20;
+             *o_full = bars + 18;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int n_units = a.positions ? a.rows : a.n_segs, G = a.c.kv_heads, group = a.n_heads / G;
     if (tid == 0) {
         failed = 0;
         for (int i = 0; i < BOXES; i++) {
             mbar_init(&full8[i], 1);
-            mbar_init(&empty8[i], CODE_WARPS);
+            mbar_init(&empty8[i], TEAM);
         }
         for (int b = 0; b < 2; b++) {
-            mbar_init(&k_full[b], CODE_WARPS);
+            mbar_init(&k_full[b], TEAM);
             mbar_init(&k_empty[b], 1);
-            mbar_init(&v_full[b], CODE_WARPS);
+            mbar_init(&v_full[b], TEAM);
             mbar_init(&v_empty[b], 1);
             mbar_init(&s_full[b], 1);
-            mbar_init(&p_ready[b], SOFTMAX_WARPS);
+            mbar_init(&p_ready[b], SOFTMAX_WARPS / 2);
             mbar_init(&o_full[b], 1);
         }
-        for (int q = 0; q < 4; q++) mbar_init(&pair[q], 2);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     pdl_launch();
@@ -168,31 +177,40 @@ __global__ void __launch_bounds__(THREADS, 1) attn8_tc_kernel(const __grid_const
             if (!ok && lane == 0) atomicExch(&failed, 1);
             for (int i = max(0, asked - BOXES); i < asked; i++) mbar_wait(&full8[i % BOXES], (i / BOXES) & 1);      // no copy is under way when the CTA leaves
         } else if (warp >= FIRST_CODE_WARP) {
-            const int t0 = tid - 32 * FIRST_CODE_WARP;                // its chunks of a box are t0 + CODE_THREADS i
+            // Two teams of four warps take every second box each: what one waits for behind its stores is covered by the other
+            const int t0 = tid - 32 * FIRST_CODE_WARP & CODE_THREADS - 1, team = warp - FIRST_CODE_WARP >= TEAM;      // its chunks of a box are t0 + CODE_THREADS i
             bool ok = true;
-            for (int j = 0; j < 2 * n_tiles; j++) {
+            for (int j = team; j < 2 * n_tiles; j += 2) {
                 const int slot = j % BOXES, tile = box_of(j).x, is_v = box_of(j).y, b = tile & 1;
                 if (!mbar_wait(&full8[slot], (j / BOXES) & 1)) { ok = false; break; }
-                const uint4* box = reinterpret_cast<const uint4*>(sm + L::OFF_BOX + slot * L::BOX);
-                uint4 w[EACH];             // all of them before anything is stored: the compiler keeps loads behind stores
-#pragma unroll
-                for (int i = 0; i < EACH; i++) w[i] = box[t0 + CODE_THREADS * i];
                 if (tile >= 2 && !mbar_wait(is_v ? &v_empty[b] : &k_empty[b], ((tile >> 1) - 1) & 1)) { ok = false; break; }
-                if (is_v && masked(n0_of(tile))) {       // a weight of zero times what is no number: such values become zeros, and their keys' scores none
-#pragma unroll
-                    for (int i = 0; i < EACH; i++) {
-                        uint32_t none = holds_nan(w[i]);
-#pragma unroll
-                        for (int o = 1; o < CHUNKS; o <<= 1) none |= __shfl_xor_sync(0xffffffffu, none, o);
-                        if (none) w[i] = make_uint4(0, 0, 0, 0);
-                        if ((t0 + CODE_THREADS * i) % CHUNKS == 0) no_number[b][(t0 + CODE_THREADS * i) / CHUNKS] = none != 0;
-                    }
-                }
+                const bool look = is_v && masked(n0_of(tile));
+                const uint4* box = reinterpret_cast<const uint4*>(sm + L::OFF_BOX + slot * L::BOX);
                 const float2 un = units8[slot];
-                const __half2 u0 = __float2half2_rn(un.x), u1 = __float2half2_rn(un.y);
                 uint8_t* to = sm + (is_v ? L::OFF_V : L::OFF_K) + b * L::TILE;
 #pragma unroll
-                for (int i = 0; i < EACH; i++) put_codes(to, (t0 + CODE_THREADS * i) / CHUNKS, (t0 + CODE_THREADS * i) % CHUNKS, w[i], i < EACH / 2 ? u0 : u1);
+                for (int h = 0; h < 2; h++) {          // a page
+                    const __half2 unit = __float2half2_rn(h ? un.y : un.x);
+                    uint4 w[EACH / 2];             // all of them before anything is stored: the compiler keeps loads behind stores
+#pragma unroll
+                    for (int i = 0; i < EACH / 2; i++) w[i] = box[t0 + CODE_THREADS * (h * EACH / 2 + i)];
+                    if (look) {       // a weight of zero times what is no number: such values become zeros, and their keys' scores none
+#pragma unroll
+                        for (int i = 0; i < EACH / 2; i++) {
+                            const int at = t0 + CODE_THREADS * (h * EACH / 2 + i);
+                            uint32_t none = holds_nan(w[i]);
+#pragma unroll
+                            for (int o = 1; o < CHUNKS; o <<= 1) none |= __shfl_xor_sync(0xffffffffu, none, o);
+                            if (none) w[i] = make_uint4(0, 0, 0, 0);
+                            if (at % CHUNKS == 0) no_number[b][at / CHUNKS] = none != 0;
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < EACH / 2; i++) {
+                        const int at = t0 + CODE_THREADS * (h * EACH / 2 + i);
+                        put_codes(to, at / CHUNKS, at % CHUNKS, w[i], unit);
+                    }
+                }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) {
@@ -227,9 +245,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn8_tc_kernel(const __grid_const
                     tc_fence_after();
                     const uint8_t* vt = sm + L::OFF_V + b * L::TILE;
 #pragma unroll
-                    for (int kk = 0; kk < BKV / 16; kk++)      // O_tile(t) = P(t) V(t); P sits in the first 64 columns of its score buffer
-                        umma_f16_ts(tmem + 256 + 128 * b, tmem + 128 * b + 8 * kk, umma_desc_mn(vt + kk * 16 * 128, ATOM_BYTES), id_o, kk != 0);
-                    umma_commit(&o_full[b]);
+                    for (int kk = 0; kk < BKV / 16; kk++)      // P(t) V(t) onto its group's result; P sits in the first 64 columns of its score buffer
+                        umma_f16_ts(tmem + 256 + 128 * b, tmem + 128 * b + 8 * kk, umma_desc_mn(vt + kk * 16 * 128, ATOM_BYTES), id_o, t >= 2 || kk != 0);
+                    if (t + 2 >= n_tiles) umma_commit(&o_full[b]);
                     umma_commit(&v_empty[b]);
                     if (t + 2 < n_tiles) issue_s(t + 2);       // runs behind P V(t), which still reads the buffer it overwrites
                 }
@@ -238,107 +256,113 @@ __global__ void __launch_bounds__(THREADS, 1) attn8_tc_kernel(const __grid_const
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+        // Warps 0-3 have the even tiles, 4-7 the odd ones: a thread a row, with a reference, a sum and a result (in tensor memory) of its own, so that one group's exponentials run
+        // beside the other's products.  The reference is a score that none passes by more than a factor of 2^LAG; the result is scaled when one does.
         const int q = warp & 3, c = warp >> 2, r = 32 * q + lane;
         const int qp = s.pos + min((m0 + r) / group, s.rows - 1), row_lo = first_key(qp, a.chunk, a.window);
         const float size = a.scale == 0.f ? 1.f : fabsf(a.scale), mult = a.softcap > 0.f ? 1.f : size * LOG2E, inv_cap = a.softcap > 0.f ? size / a.softcap : 0.f, cap2 = a.softcap * LOG2E;
-        const uint32_t lane_base = (uint32_t)(32 * q) << 16;
-        float o[OH];
-#pragma unroll
-        for (int j = 0; j < OH; j++) o[j] = 0.f;
-        float m_run = NONE, l_run = 0.f, corr_prev = 1.f;
+        const uint32_t lane_base = (uint32_t)(32 * q) << 16, scores = tmem + lane_base + 128 * c, result = scores + 256;
+        float m_ref = NONE, l_run = 0.f;
         bool ok = true;
-        auto accumulate = [&](int t, float corr) {      // o = o * corr + O_tile(t)
-            const int b = t & 1;
-            if (!mbar_wait(&o_full[b], (t >> 1) & 1)) { ok = false; return; }
+        for (int t = c; t < n_tiles; t += 2) {
+            const int n0 = n0_of(t);
+            if (!mbar_wait(&s_full[c], (t >> 1) & 1)) { ok = false; break; }
             tc_fence_after();
+            uint32_t v[4][32];
 #pragma unroll
-            for (int j0 = 0; j0 < OH; j0 += 32) {
-                uint32_t ov[32];
-                tmem_ld32(tmem + lane_base + (uint32_t)(256 + 128 * b + OH * c + j0), ov);
-#pragma unroll
-                for (int j = 0; j < 32; j += 2) {
-                    const float2 y = fma2(make_float2(o[j0 + j], o[j0 + j + 1]), make_float2(corr, corr), make_float2(__uint_as_float(ov[j]), __uint_as_float(ov[j + 1])));
-                    o[j0 + j] = y.x;
-                    o[j0 + j + 1] = y.y;
-                }
-            }
-            tc_fence_before();
-        };
-        for (int t = 0; t < n_tiles && ok; t++) {
-            const int b = t & 1, n0 = n0_of(t);
-            if (!mbar_wait(&s_full[b], (t >> 1) & 1)) { ok = false; break; }
-            tc_fence_after();
-            uint32_t v[2][32];
-            tmem_ld32(tmem + lane_base + (uint32_t)(128 * b + 64 * c), v[0]);
-            tmem_ld32(tmem + lane_base + (uint32_t)(128 * b + 64 * c + 32), v[1]);
+            for (int i = 0; i < 4; i++) tmem_ld32(scores + 32 * i, v[i]);
             if (a.softcap > 0.f) {
 #pragma unroll
-                for (int i = 0; i < 2; i++)
+                for (int i = 0; i < 4; i++)
 #pragma unroll
                     for (int j = 0; j < 32; j++) v[i][j] = __float_as_uint(cap2 * tanh_exp(__uint_as_float(v[i][j]) * inv_cap));
             }
             if (masked(n0)) {
-                const int kp0 = n0 + 64 * c;
-                if (!mbar_wait(&v_full[b], (t >> 1) & 1)) { ok = false; break; }
-                const uint32_t none[2] = {__ballot_sync(0xffffffffu, no_number[b][64 * c + lane]), __ballot_sync(0xffffffffu, no_number[b][64 * c + 32 + lane])};
+                if (!mbar_wait(&v_full[c], (t >> 1) & 1)) { ok = false; break; }
 #pragma unroll
-                for (int i = 0; i < 2; i++)
+                for (int i = 0; i < 4; i++) {
+                    const uint32_t none = __ballot_sync(0xffffffffu, no_number[c][32 * i + lane]);
 #pragma unroll
                     for (int j = 0; j < 32; j++) {
-                        const int kp = kp0 + 32 * i + j;
-                        if (none[i] >> j & 1) v[i][j] = 0x7fffffffu;
+                        const int kp = n0 + 32 * i + j;
+                        if (none >> j & 1) v[i][j] = 0x7fffffffu;
                         if (kp > qp || (kp < row_lo && kp >= keep)) v[i][j] = 0xff800000u;
                     }
-            }
-            float mx = NONE;
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int j = 0; j < 32; j++) mx = fmaxf(mx, __uint_as_float(v[i][j]));
-            // the partner may be a tile ahead when this warp reads: a place each for even and odd tiles
-            x_max[b][c][r] = mx;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&pair[q]);
-            if (!mbar_wait(&pair[q], t & 1)) { ok = false; break; }
-            mx = fmaxf(mx, *(volatile float*)&x_max[b][c ^ 1][r]);
-            const float m_new = fmaxf(m_run, mx), corr = ex2((m_run - m_new) * mult);
-            m_run = m_new;
-            const float2 mult2 = make_float2(mult, mult), less = make_float2(-m_new * mult, -m_new * mult);
-            float2 ls2 = make_float2(0.f, 0.f);
-            uint32_t pw[32];
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int j = 0; j < 32; j += 2) {
-                    const float2 e = fma2(make_float2(__uint_as_float(v[i][j]), __uint_as_float(v[i][j + 1])), mult2, less);
-                    const float2 pr = make_float2(ex2(e.x), ex2(e.y));
-                    ls2 = add2(ls2, pr);
-                    pw[16 * i + (j >> 1)] = pack_h2(pr.x, pr.y);
                 }
-            tmem_st32(tmem + lane_base + (uint32_t)(128 * b + 32 * c), pw);      // both warps of the quarter have read all of S(t) by now
-            l_run = l_run * corr + (ls2.x + ls2.y);
+            }
+            float top[4] = {NONE, NONE, NONE, NONE};
+#pragma unroll
+            for (int j = 0; j < 32; j++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) top[i] = fmaxf(top[i], __uint_as_float(v[i][j]));
+            const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            if (__any_sync(0xffffffffu, (mx - m_ref) * mult > LAG)) {
+                const float m_new = fmaxf(m_ref, mx), corr = ex2((m_ref - m_new) * mult);
+                m_ref = m_new;
+                l_run *= corr;
+                if (t >= 2) {        // S(t) is behind P V(t - 2)
+#pragma unroll 1
+                    for (int j = 0; j < D; j += 8) {
+                        uint32_t o[8];
+                        tmem_ld8(result + j, o);
+#pragma unroll
+                        for (int i = 0; i < 8; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+                        tmem_st8(result + j, o);
+                    }
+                }
+            }
+            const float2 mult2 = make_float2(mult, mult), less = make_float2(-m_ref * mult, -m_ref * mult);
+            float2 ls2[2] = {};
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                uint32_t pw[32];
+#pragma unroll
+                for (int j = 0; j < 32; j++) {
+                    const int i = 2 * h + (j >> 4), k = 2 * j & 31;
+                    const float2 e = fma2(make_float2(__uint_as_float(v[i][k]), __uint_as_float(v[i][k + 1])), mult2, less);
+                    const float2 pr = make_float2(ex2(e.x), ex2(e.y));
+                    ls2[j & 1] = add2(ls2[j & 1], pr);
+                    pw[j] = pack_h2(pr.x, pr.y);
+                }
+                tmem_st32(scores + 32 * h, pw);      // over scores that have been read
+            }
+            l_run += ls2[0].x + ls2[0].y + (ls2[1].x + ls2[1].y);
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&p_ready[b]);
-            if (t >= 1) accumulate(t - 1, corr_prev);      // P V(t - 1) finished long ago; P V(t) runs under this
-            corr_prev = corr;
+            if (lane == 0) mbar_arrive(&p_ready[c]);
         }
-        if (ok && n_tiles > 0) accumulate(n_tiles - 1, corr_prev);
+        // The groups' sums become one, in shared memory that the products no longer read, and go out in whole rows
+        if (ok && c < n_tiles && !mbar_wait(&o_full[c], 0)) ok = false;
         if (!ok) atomicExch(&failed, 1);
-        x_sum[c][r] = l_run;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&pair[q]);
-        if (ok && !mbar_wait(&pair[q], n_tiles & 1)) {
-            ok = false;
-            atomicExch(&failed, 1);
-        }
-        if (r < rows_m) {
-            const size_t at = (size_t)blockIdx.x * BQ + r;
-            float4* to = reinterpret_cast<float4*>(a.part_acc + at * D + OH * c);
+        tc_fence_after();
+        x_ml[c][r] = make_float2(m_ref * mult, l_run);
+        softmax_sync();
+        const float2 x0 = x_ml[0][r], x1 = x_ml[1][r];
+        const float top = fmaxf(x0.x, x1.x), w = ex2((c ? x1.x : x0.x) - top);
+        float* row = reinterpret_cast<float*>(sm + L::OFF_K) + r * PITCH;
+        for (int g = 1; g >= 0; g--) {
+            if (c == g && c < n_tiles) {
+#pragma unroll 1
+                for (int j = 0; j < D; j += 32) {
+                    uint32_t o[32];
+                    tmem_ld32(result + j, o);
 #pragma unroll
-            for (int j = 0; j < OH; j += 4) to[j / 4] = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
-            if (c == 0) a.part_ml[at] = make_float2(m_run * mult, l_run + *(volatile float*)&x_sum[1][r]);
+                    for (int i = 0; i < 32; i += 4) {
+                        float4 y = c == 0 && n_tiles > 1 ? *reinterpret_cast<float4*>(row + j + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        y.x = fmaf(__uint_as_float(o[i]), w, y.x);
+                        y.y = fmaf(__uint_as_float(o[i + 1]), w, y.y);
+                        y.z = fmaf(__uint_as_float(o[i + 2]), w, y.z);
+                        y.w = fmaf(__uint_as_float(o[i + 3]), w, y.w);
+                        *reinterpret_cast<float4*>(row + j + i) = y;
+                    }
+                }
+            }
+            softmax_sync();
         }
+        const size_t at = (size_t)blockIdx.x * BQ;
+        float4* to = reinterpret_cast<float4*>(a.part_acc + at * D);
+        for (int i = tid; i < rows_m * (D / 4); i += 32 * SOFTMAX_WARPS) to[i] = *reinterpret_cast<const float4*>(sm + L::OFF_K + ((i / (D / 4)) * PITCH + 4 * (i % (D / 4))) * 4);
+        if (c == 0 && r < rows_m) a.part_ml[at + r] = make_float2(top, x0.y * w + x1.y * ex2(x1.x - top));
     }
     tc_fence_before();
     __syncthreads();
