@@ -91,8 +91,8 @@ __global__ void __launch_bounds__(Lay<D, NB>::THREADS, Lay<D, NB>::PER_SM)
     const int units = a.positions ? a.rows : a.n_segs, G = a.c.kv_heads, group = a.n_heads / G;
     if (tid < WARPS * SLOTS) mbar_init(&bars[tid], 1);
     if (tid == 0) asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    pdl_launch();
     if (!a.behind) pdl_wait();
+    pdl_launch();         // what the merging kernel reads before its own wait has been written
     Unit s;
     uint32_t first;
     if (!find_unit<true>(a, units, blockIdx.x, room, s, first)) {
@@ -399,7 +399,6 @@ __global__ void __launch_bounds__(MERGE_COLUMNS * HALVES) attn8_merge_kernel(con
     const int hd = a.c.hd, tid = threadIdx.x % HALF, half = threadIdx.x / HALF, G = a.c.kv_heads, group = a.n_heads / G, units = a.positions ? a.rows : a.n_segs;
     const int h = blockIdx.x * (HALF / hd) + tid / hd, d = tid % hd, row = blockIdx.y;
     pdl_launch();
-    if (!a.behind) pdl_wait();
     int u = -1;
     if (a.positions) {
         u = row;
@@ -416,7 +415,7 @@ __global__ void __launch_bounds__(MERGE_COLUMNS * HALVES) attn8_merge_kernel(con
     Unit s;
     uint32_t first;
     const bool any = u >= 0 && find_unit<false>(a, units, u, room, s, first);
-    if (a.behind) pdl_wait();
+    pdl_wait();
     if (!any) return;
     float3 x = make_float3(0.f, 1.f, 0.f);
     if (in) {

@@ -41,6 +41,8 @@ __device__ __forceinline__ void tmem_st8(uint32_t at, const uint32_t (&v)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
+// bits 0 .. n - 1
+__device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? 0xffffffffu : n > 0 ? (1u << n) - 1 : 0u; }
 __device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * SOFTMAX_WARPS) : "memory"); }
 
 // 16 codes of row r, columns 16 c .. 16 c + 15, times the unit, into a swizzled tile.  The half that comes first differs between columns below and above 64, whose atoms have the
@@ -77,7 +79,23 @@ __global__ void __launch_bounds__(THREADS, 1) attn8_tc_kernel(const __grid_const
              *o_full = bars + 18;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int n_units = a.positions ? a.rows : a.n_segs, G = a.c.kv_heads, group = a.n_heads / G;
-    if (tid == 0) {
+    pdl_wait();
+    pdl_launch();        // behind the wait, so that what the merging kernel reads before its own has been written
+    Unit s;
+    uint32_t first;
+    if (!find_unit<true>(a, n_units, blockIdx.x, room, s, first)) return;
+    const Keys ks = keys_of(a, s);
+    const int part = (blockIdx.x - first) % s.parts, item = (blockIdx.x - first) / s.parts, kvh = item % G, m0 = BQ * (item / G), rows_m = min(BQ, s.rows * group - m0);
+    const int x0 = (int)((long long)ks.turns * part / s.parts), n_tiles = (int)((long long)ks.turns * (part + 1) / s.parts) - x0;
+    // positions of the tile's first and last row, the last one's first key
+    const int first_pos = s.pos + m0 / group, last_pos = s.pos + min(s.rows - 1, (m0 + BQ - 1) / group), last_lo = first_key(last_pos, a.chunk, a.window), keep = a.window > 0 ? a.keep : 0;
+    auto n0_of = [&](int t) { return first_of(ks, BKV, x0 + t); };
+    auto masked = [&](int n0) { return n0 + BKV - 1 > first_pos || (n0 < last_lo && n0 + BKV > keep); };      // some row does not see some key
+
+    // The boxes in the order in which the products take them: K(0), K(1), V(0), K(2), V(1), ... V(n - 1).  x: tile, y: 1 with values
+    auto box_of = [&](int j) { return j == 2 * n_tiles - 1 ? make_int2(n_tiles - 1, 1) : j > 0 && (j & 1) == 0 ? make_int2(j / 2 - 1, 1) : make_int2((j + 1) / 2, 0); };
+
+    if (warp == 8 && lane == 0) {
         failed = 0;
         for (int i = 0; i < BOXES; i++) {
             mbar_init(&full8[i], 1);
@@ -94,40 +112,57 @@ __global__ void __launch_bounds__(THREADS, 1) attn8_tc_kernel(const __grid_const
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    pdl_launch();
-    pdl_wait();
-    Unit s;
-    uint32_t first;
-    if (!find_unit<true>(a, n_units, blockIdx.x, room, s, first)) return;
-    const Keys ks = keys_of(a, s);
-    const int part = (blockIdx.x - first) % s.parts, item = (blockIdx.x - first) / s.parts, kvh = item % G, m0 = BQ * (item / G), rows_m = min(BQ, s.rows * group - m0);
-    const int x0 = (int)((long long)ks.turns * part / s.parts), n_tiles = (int)((long long)ks.turns * (part + 1) / s.parts) - x0;
-    // positions of the tile's first and last row, the last one's first key
-    const int first_pos = s.pos + m0 / group, last_pos = s.pos + min(s.rows - 1, (m0 + BQ - 1) / group), last_lo = first_key(last_pos, a.chunk, a.window), keep = a.window > 0 ? a.keep : 0;
-    auto n0_of = [&](int t) { return first_of(ks, BKV, x0 + t); };
-    auto masked = [&](int n0) { return n0 + BKV - 1 > first_pos || (n0 < last_lo && n0 + BKV > keep); };      // some row does not see some key
-
-    // The boxes in the order in which the products take them: K(0), K(1), V(0), K(2), V(1), ... V(n - 1).  x: tile, y: 1 with values
-    auto box_of = [&](int j) { return j == 2 * n_tiles - 1 ? make_int2(n_tiles - 1, 1) : j > 0 && (j & 1) == 0 ? make_int2(j / 2 - 1, 1) : make_int2((j + 1) / 2, 0); };
-
+    // Warp 8, the copies: its lanes look up the pages of 32 boxes at a time.
+    const int last_page = (s.pos + s.rows - 1) >> PAGE_SHIFT;
+    int head[2] = {}, asked = 0;                     // boxes
+    float2 un = make_float2(0.f, 0.f);
+    auto look_up = [&](int j0) {
+        if (j0 + lane < 2 * n_tiles) {
+            const int2 of = box_of(j0 + lane);
+            const int p0 = n0_of(of.x) >> PAGE_SHIFT;
+            const float* units = of.y ? a.c.vu : a.c.ku;
+            for (int i = 0; i < 2; i++) head[i] = max(page_at(a.t, a.c.n_pages, s.slot, min(p0 + i, last_page)), 0) * G + kvh;
+            un = make_float2(units[head[0]], units[head[1]]);
+        }
+    };
+    auto ask = [&](int j) {
+        const size_t h0 = __shfl_sync(0xffffffffu, head[0], j & 31), h1 = __shfl_sync(0xffffffffu, head[1], j & 31);
+        const float2 u = make_float2(__shfl_sync(0xffffffffu, un.x, j & 31), __shfl_sync(0xffffffffu, un.y, j & 31));
+        if (lane == 0) {
+            const int slot = j % BOXES;
+            uint8_t* box = sm + L::OFF_BOX + slot * L::BOX;
+            const uint8_t* from = box_of(j).y ? a.c.v : a.c.k;
+            units8[slot] = u;
+            mbar_expect_tx(&full8[slot], L::BOX);
+            bulk_copy(box, from + h0 * PAGE * D, PAGE * D, &full8[slot]);
+            bulk_copy(box + PAGE * D, from + h1 * PAGE * D, PAGE * D, &full8[slot]);
+        }
+        asked++;
+        __syncwarp();
+    };
+    if (warp == 8) {                 // the first of them before anything else
+        look_up(0);
+        for (int j = 0; j < min(2 * n_tiles, BOXES); j++) ask(j);
+    }
     if (warp == 9) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    if (warp < SOFTMAX_WARPS) {      // queries
-        const int r = 32 * (warp & 3) + lane, c = warp >> 2, m = m0 + r;
-        const bool live = r < rows_m;
+    if (warp < SOFTMAX_WARPS || warp >= FIRST_CODE_WARP) {      // queries: whole rows by neighbouring threads
+        constexpr int N = 32 * (SOFTMAX_WARPS + CODE_WARPS), QUADS = D / 4, LOADS = BQ * QUADS / N;
+        const int t0 = tid - (warp < SOFTMAX_WARPS ? 0 : 32 * (FIRST_CODE_WARP - SOFTMAX_WARPS));
         const float sign = a.scale > 0.f ? 1.f : a.scale < 0.f ? -1.f : 0.f;      // the running maximum is one of plain scores, which takes a scale above zero
-        const float* qp = a.q + ((size_t)(s.row + m / group) * a.n_heads + kvh * group + m % group) * D + OH * c;
+        float4 x[LOADS];
 #pragma unroll
-        for (int j = 0; j < OH / 8; j++) {
-            float4 v0 = make_float4(0.f, 0.f, 0.f, 0.f), v1 = v0;
-            if (live) {
-                v0 = *(const float4*)(qp + 8 * j);
-                v1 = *(const float4*)(qp + 8 * j + 4);
-            }
-            const int col = OH * c + 8 * j;
-            *(uint4*)(sm + (col >> 6) * ATOM_BYTES + r * 128 + ((((col & 63) >> 3) ^ (r & 7)) << 4)) = make_uint4(pack_h2(sign * v0.x, sign * v0.y), pack_h2(sign * v0.z, sign * v0.w), pack_h2(sign * v1.x, sign * v1.y), pack_h2(sign * v1.z, sign * v1.w));
+        for (int i = 0; i < LOADS; i++) {
+            const int r = (t0 + N * i) / QUADS, col = (t0 + N * i) % QUADS * 4, m = m0 + r;
+            x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r < rows_m) x[i] = *(const float4*)(a.q + ((size_t)(s.row + m / group) * a.n_heads + kvh * group + m % group) * D + col);
+        }
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+            const int r = (t0 + N * i) / QUADS, col = (t0 + N * i) % QUADS * 4;
+            *(uint2*)(sm + (col >> 6) * ATOM_BYTES + r * 128 + ((((col & 63) >> 3) ^ (r & 7)) << 4) + (col & 4) * 2) = make_uint2(pack_h2(sign * x[i].x, sign * x[i].y), pack_h2(sign * x[i].z, sign * x[i].w));
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -140,39 +175,14 @@ __global__ void __launch_bounds__(THREADS, 1) attn8_tc_kernel(const __grid_const
     if (warp >= SOFTMAX_WARPS) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
         if (warp == 8) {
-            // The lanes look up the pages of 32 boxes at a time.
-            const int last_page = (s.pos + s.rows - 1) >> PAGE_SHIFT;
             bool ok = true;
-            int asked = 0;                           // boxes
-            for (int j0 = 0; j0 < 2 * n_tiles && ok; j0 += 32) {
-                int head[2] = {};
-                float2 un = make_float2(0.f, 0.f);
-                if (j0 + lane < 2 * n_tiles) {
-                    const int2 of = box_of(j0 + lane);
-                    const int p0 = n0_of(of.x) >> PAGE_SHIFT;
-                    const float* units = of.y ? a.c.vu : a.c.ku;
-                    for (int i = 0; i < 2; i++) head[i] = max(page_at(a.t, a.c.n_pages, s.slot, min(p0 + i, last_page)), 0) * G + kvh;
-                    un = make_float2(units[head[0]], units[head[1]]);
+            for (int j = BOXES; j < 2 * n_tiles; j++) {
+                if ((j & 31) == 0) look_up(j);
+                if (!mbar_wait(&empty8[j % BOXES], (j / BOXES - 1) & 1)) {
+                    ok = false;
+                    break;
                 }
-                for (int j = j0; j < min(2 * n_tiles, j0 + 32); j++) {
-                    const size_t h0 = __shfl_sync(0xffffffffu, head[0], j - j0), h1 = __shfl_sync(0xffffffffu, head[1], j - j0);
-                    const float2 u = make_float2(__shfl_sync(0xffffffffu, un.x, j - j0), __shfl_sync(0xffffffffu, un.y, j - j0));
-                    const int slot = j % BOXES;
-                    if (j >= BOXES && !mbar_wait(&empty8[slot], (j / BOXES - 1) & 1)) {
-                        ok = false;
-                        break;
-                    }
-                    if (lane == 0) {
-                        uint8_t* box = sm + L::OFF_BOX + slot * L::BOX;
-                        const uint8_t* from = box_of(j).y ? a.c.v : a.c.k;
-                        units8[slot] = u;
-                        mbar_expect_tx(&full8[slot], L::BOX);
-                        bulk_copy(box, from + h0 * PAGE * D, PAGE * D, &full8[slot]);
-                        bulk_copy(box + PAGE * D, from + h1 * PAGE * D, PAGE * D, &full8[slot]);
-                    }
-                    asked++;
-                    __syncwarp();
-                }
+                ask(j);
             }
             if (!ok && lane == 0) atomicExch(&failed, 1);
             for (int i = max(0, asked - BOXES); i < asked; i++) mbar_wait(&full8[i % BOXES], (i / BOXES) & 1);      // no copy is under way when the CTA leaves
@@ -281,13 +291,16 @@ __global__ void __launch_bounds__(THREADS, 1) attn8_tc_kernel(const __grid_const
                 if (!mbar_wait(&v_full[c], (t >> 1) & 1)) { ok = false; break; }
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const uint32_t none = __ballot_sync(0xffffffffu, no_number[c][32 * i + lane]);
+                    const int k0 = n0 + 32 * i;
+                    const uint32_t none = __ballot_sync(0xffffffffu, no_number[c][32 * i + lane]), seen = below(qp + 1 - k0) & (~below(row_lo - k0) | below(keep - k0));
+                    if (none) {
 #pragma unroll
-                    for (int j = 0; j < 32; j++) {
-                        const int kp = n0 + 32 * i + j;
-                        if (none >> j & 1) v[i][j] = 0x7fffffffu;
-                        if (kp > qp || (kp < row_lo && kp >= keep)) v[i][j] = 0xff800000u;
+                        for (int j = 0; j < 32; j++)
+                            if (none >> j & 1) v[i][j] = 0x7fffffffu;
                     }
+#pragma unroll
+                    for (int j = 0; j < 32; j++)
+                        if (!(seen >> j & 1)) v[i][j] = 0xff800000u;
                 }
             }
             float top[4] = {NONE, NONE, NONE, NONE};
@@ -340,19 +353,22 @@ __global__ void __launch_bounds__(THREADS, 1) attn8_tc_kernel(const __grid_const
         const float2 x0 = x_ml[0][r], x1 = x_ml[1][r];
         const float top = fmaxf(x0.x, x1.x), w = ex2((c ? x1.x : x0.x) - top);
         float* row = reinterpret_cast<float*>(sm + L::OFF_K) + r * PITCH;
-        for (int g = 1; g >= 0; g--) {
-            if (c == g && c < n_tiles) {
+        for (int add = 0; add < 2; add++) {          // a half of the columns: first the other group's, then its own
+            const int j0 = OH * (c ^ 1 ^ add);
+            if (c < n_tiles || add) {
 #pragma unroll 1
-                for (int j = 0; j < D; j += 32) {
+                for (int j = j0; j < j0 + OH; j += 32) {
                     uint32_t o[32];
-                    tmem_ld32(result + j, o);
+                    if (c < n_tiles) tmem_ld32(result + j, o);
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) {
-                        float4 y = c == 0 && n_tiles > 1 ? *reinterpret_cast<float4*>(row + j + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-                        y.x = fmaf(__uint_as_float(o[i]), w, y.x);
-                        y.y = fmaf(__uint_as_float(o[i + 1]), w, y.y);
-                        y.z = fmaf(__uint_as_float(o[i + 2]), w, y.z);
-                        y.w = fmaf(__uint_as_float(o[i + 3]), w, y.w);
+                        float4 y = add && (c ^ 1) < n_tiles ? *reinterpret_cast<float4*>(row + j + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (c < n_tiles) {
+                            y.x = fmaf(__uint_as_float(o[i]), w, y.x);
+                            y.y = fmaf(__uint_as_float(o[i + 1]), w, y.y);
+                            y.z = fmaf(__uint_as_float(o[i + 2]), w, y.z);
+                            y.w = fmaf(__uint_as_float(o[i + 3]), w, y.w);
+                        }
                         *reinterpret_cast<float4*>(row + j + i) = y;
                     }
                 }
