@@ -45,11 +45,8 @@ __device__ __forceinline__ void tmem_st8(uint32_t at, const uint32_t (&v)[8]) {
 __device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? 0xffffffffu : n > 0 ? (1u << n) - 1 : 0u; }
 __device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * SOFTMAX_WARPS) : "memory"); }
 
-// 16 codes of row r, columns 16 c .. 16 c + 15, times the unit, into a swizzled tile.  The half that comes first differs between columns below and above 64, whose atoms have the
-// same banks.
-__device__ __forceinline__ void put_codes(uint8_t* tile, int r, int c, const uint4& w, __half2 unit) {
-    const int k = 2 * (c & 3), first = c >> 2 & 1;
-    const uint32_t x[4] = {first ? w.z : w.x, first ? w.w : w.y, first ? w.x : w.z, first ? w.y : w.w};
+// 16 codes times the unit as f16 at p (the first eight of x) and q
+__device__ __forceinline__ void put_codes(uint8_t* p, uint8_t* q, const uint32_t (&x)[4], __half2 unit) {
     uint32_t y[8];
 #pragma unroll
     for (int j = 0; j < 8; j++) {
@@ -57,9 +54,8 @@ __device__ __forceinline__ void put_codes(uint8_t* tile, int r, int c, const uin
         const __half2 f = __hmul2(*reinterpret_cast<const __half2*>(&h), unit);
         y[j] = *reinterpret_cast<const uint32_t*>(&f);
     }
-    uint8_t* row = tile + (c >> 2) * ATOM_BYTES + r * 128;
-    *reinterpret_cast<uint4*>(row + (((k + first) ^ (r & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
-    *reinterpret_cast<uint4*>(row + (((k + 1 - first) ^ (r & 7)) << 4)) = make_uint4(y[4], y[5], y[6], y[7]);
+    *reinterpret_cast<uint4*>(p) = make_uint4(y[0], y[1], y[2], y[3]);
+    *reinterpret_cast<uint4*>(q) = make_uint4(y[4], y[5], y[6], y[7]);
 }
 
 template <int D>
@@ -189,6 +185,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn8_tc_kernel(const __grid_const
         } else if (warp >= FIRST_CODE_WARP) {
             // Two teams of four warps take every second box each: what one waits for behind its stores is covered by the other
             const int t0 = tid - 32 * FIRST_CODE_WARP & CODE_THREADS - 1, team = warp - FIRST_CODE_WARP >= TEAM;      // its chunks of a box are t0 + CODE_THREADS i
+            // Row, columns 16 col .. 16 col + 15 of its first chunk; the others' rows lie multiples of eight on, so that the swizzle is the same.  Columns below 64 and above, whose atoms have
+            // the same banks, begin with different halves.
+            const int r0 = t0 / CHUNKS, col = t0 % CHUNKS, swap = col >> 2 & 1;
+            const int at0 = (col >> 2) * ATOM_BYTES + r0 * 128 + ((2 * (col & 3) + swap ^ (r0 & 7)) << 4), at1 = at0 ^ 16;
+            static_assert(CODE_THREADS / CHUNKS % 8 == 0, "rows of a thread's chunks");
             bool ok = true;
             for (int j = team; j < 2 * n_tiles; j += 2) {
                 const int slot = j % BOXES, tile = box_of(j).x, is_v = box_of(j).y, b = tile & 1;
@@ -217,8 +218,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn8_tc_kernel(const __grid_const
                     }
 #pragma unroll
                     for (int i = 0; i < EACH / 2; i++) {
-                        const int at = t0 + CODE_THREADS * (h * EACH / 2 + i);
-                        put_codes(to, at / CHUNKS, at % CHUNKS, w[i], unit);
+                        const int rows = CODE_THREADS / CHUNKS * (h * EACH / 2 + i) * 128;
+                        const uint32_t x[4] = {swap ? w[i].z : w[i].x, swap ? w[i].w : w[i].y, swap ? w[i].x : w[i].z, swap ? w[i].y : w[i].w};
+                        put_codes(to + at0 + rows, to + at1 + rows, x, unit);
                     }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
