@@ -80,11 +80,14 @@ __global__ void __launch_bounds__(THREADS, 1) attn8_tc_kernel(const __grid_const
     Unit s;
     uint32_t first;
     if (!find_unit<true>(a, n_units, blockIdx.x, room, s, first)) return;
-    const Keys ks = keys_of(a, s);
     const int part = (blockIdx.x - first) % s.parts, item = (blockIdx.x - first) / s.parts, kvh = item % G, m0 = BQ * (item / G), rows_m = min(BQ, s.rows * group - m0);
+    Unit own = s;                    // the tile's rows, whose keys may be fewer than the unit's: some CTA may have none
+    own.pos += m0 / group;
+    own.rows = (m0 + rows_m - 1) / group - m0 / group + 1;
+    const Keys ks = keys_of(a, own);
     const int x0 = (int)((long long)ks.turns * part / s.parts), n_tiles = (int)((long long)ks.turns * (part + 1) / s.parts) - x0;
     // positions of the tile's first and last row, the last one's first key
-    const int first_pos = s.pos + m0 / group, last_pos = s.pos + min(s.rows - 1, (m0 + BQ - 1) / group), last_lo = first_key(last_pos, a.chunk, a.window), keep = a.window > 0 ? a.keep : 0;
+    const int first_pos = own.pos, last_pos = own.pos + own.rows - 1, last_lo = first_key(last_pos, a.chunk, a.window), keep = a.window > 0 ? a.keep : 0;
     auto n0_of = [&](int t) { return first_of(ks, BKV, x0 + t); };
     auto masked = [&](int n0) { return n0 + BKV - 1 > first_pos || (n0 < last_lo && n0 + BKV > keep); };      // some row does not see some key
 
@@ -109,7 +112,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn8_tc_kernel(const __grid_const
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     // Warp 8, the copies: its lanes look up the pages of 32 boxes at a time.
-    const int last_page = (s.pos + s.rows - 1) >> PAGE_SHIFT;
+    const int last_page = last_pos >> PAGE_SHIFT;
     int head[2] = {}, asked = 0;                     // boxes
     float2 un = make_float2(0.f, 0.f);
     auto look_up = [&](int j0) {
@@ -249,7 +252,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn8_tc_kernel(const __grid_const
                     umma_commit(&s_full[b]);
                     umma_commit(&k_empty[b]);
                 };
-                issue_s(0);
+                if (n_tiles > 0) issue_s(0);
                 if (ok && n_tiles > 1) issue_s(1);
                 for (int t = 0; t < n_tiles && ok; t++) {
                     const int b = t & 1, ph = (t >> 1) & 1;

@@ -378,20 +378,24 @@ bool attn_prompt8(PyObject** a) {
     for (int i = 0; i < 3; i++)
         if (as_long(PyTuple_GET_ITEM(masks.o, i), 0) != mine[i]) refuse(s, "portions that were made with another mask");
     if (tensor(s, table.o, "portions").size(1) != c.t.max_pages) refuse(s, "portions that were made with another table");
-    // Estimates of three forms, us (measured with 32 heads on 8 of 128, 16 on 4, and 4 on 2 of 64, 3 to 512 rows behind 0 to 30000 keys; all within a fifth but for the least):
-    // 16 query rows a tile 11 + one for each 17500 keys of a tile and KV head, 128 rows a tile on tcgen05 19 + one for each 5700, pages read out first 10 + 0.0107 a key for each
-    // time that the tiles of 128 rows and heads fill the GPU.  (64 rows of 32 heads at 30000 keys: 230, 87, 333; 256 at 6144: 230, 98, 80; 7 at 901: 12.9, 19.6, 20.8.)
+    // Estimates of three forms, us (measured with 32 heads on 8 of 128, 16 on 4, and 4 on 2 of 64, 1 and 3 sequences, 5 to 512 rows behind 0 to 30000 keys; the choice costs a
+    // hundredth on the mean): 16 query rows a tile 9.6 + 0.08 for each tile of a KV head + one for each 19000 of its keys, 128 rows a tile on tcgen05 12 + 0.37 + one for each 11700,
+    // pages read out first 10 + 0.0107 a key for each time that the tiles of 128 rows and heads fill the GPU.  (32 heads on 8, in that order: 5 rows at 901 keys 12.3, 16.0, 21.4;
+    // 64 at 6144 59.8, 30.6, 77.4; 64 at 30000 230, 59.8, 333; 512 at 6144 -, 130, 84.)
     const long group = heads / c.c.kv_heads, m = po.longest * group;
-    double keys16 = 0, keys128 = 0, most = 0, ctas = 0;
+    double items16 = 0, items128 = 0, keys16 = 0, keys128 = 0, most = 0, ctas = 0;
     for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(sizes.o); i++) {
         PyObject* e = PyTuple_GET_ITEM(sizes.o, i);
         const double rows = as_long(PyTuple_GET_ITEM(e, 0), 0), keys = as_long(PyTuple_GET_ITEM(e, 1), 0);
-        keys16 += (double)(((long)rows * group + 15) / 16) * keys * c.c.kv_heads;
-        keys128 += (double)(((long)rows * group + 127) / 128) * keys * c.c.kv_heads;
+        const double of16 = (double)(((long)rows * group + 15) / 16) * c.c.kv_heads, of128 = (double)(((long)rows * group + 127) / 128) * c.c.kv_heads;
+        items16 += of16;
+        items128 += of128;
+        keys16 += of16 * keys;
+        keys128 += of128 * keys;
         most = std::max(most, keys);
         ctas += (double)(((long)rows + 127) / 128 * heads);
     }
-    const double t16 = 11 + keys16 / 17500, t128 = 19 + keys128 / 5700, t_read = 10 + 0.0107 * most * std::max(1.0, ctas / sms_of(dev));
+    const double t16 = 9.6 + 0.08 * items16 + keys16 / 19000, t128 = 12 + 0.37 * items128 + keys128 / 11700, t_read = 10 + 0.0107 * most * std::max(1.0, ctas / sms_of(dev));
     if (m > 64 && t_read < std::min(t16, t128) && t.out16 && !((uintptr_t)t.out & 15) && !(t.diff.on && t.gate.kind)) return false;
     const long pieces = tile(t, m <= 8 ? 8 : m <= 16 || t16 <= t128 ? 16 : 128, m, po.n, dev);
     const c10::cuda::CUDAGuard guard(dev);

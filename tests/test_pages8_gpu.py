@@ -490,3 +490,166 @@ def test_refusals():
     append(x[:0], q_out=q[:0], positions=pos[:0], slots=slots[:0])          # no rows: nothing to do
     P.read8(s.k, s.v, pages[:0], s.table, wide[0][:0], wide[1][:0])
     P.attn_decode8(x[:0], s.k, s.v, pos[:0], slots[:0], s.table, out[:0], n_ctx=100, scale=0.1, **prep)
+
+
+@pytest.mark.parametrize("mask", MASKS)
+@pytest.mark.parametrize("geometry", [GEOMETRIES[i] for i in (0, 1, 4, 8)])
+def test_prompt_attention_with_32_bit_results(geometry, mask):
+    """Many rows of several sequences, whose pages are not read out first."""
+    from ollama_b200.ops import rows as R
+    s = Setup(slots=3, n_ctx=1300, seed=37, **geometry)
+    held = [0, 0, 0]
+    for lens in ([260, 1, 64], [3, 600, 400]):
+        parts, at = [], 0
+        for slot in (1, 2, 0):
+            parts.append((at, lens[slot], slot, held[slot]))
+            at += lens[slot]
+        x, q = s.rnd(at, s.ld), torch.empty(at, s.H, s.hd, device="cuda")
+        plan = s.P.portions8(parts, s.table, **{n: mask[n] for n in mask if n != "softcap"})
+        s.P.append8(x.cuda(), s.k, s.v, s.table, q, portions=plan, **s.prep())
+        gate = ("element", "head")[at % 2]
+        gv = s.rnd(at, s.H * s.vdim).cuda()
+        out = torch.full((at, s.H * s.vdim + 8), 5.0, device="cuda")
+        s.P.attn_prompt8(q, s.k, s.v, plan, s.table, out, vdim=s.vdim, scale=1.3 / math.sqrt(s.dim), gate=R.head_gate(gv, gate), **mask)
+        assert (out[:, s.H * s.vdim:] == 5).all()
+        for row, n, slot, p in parts:
+            held[slot] += n
+            pos = torch.arange(p, p + n)
+            k, v = s.values(s.k, slot, p + n), s.values(s.v, slot, p + n)
+            seen = O.visible(pos, p + n, **{m: mask[m] for m in mask if m != "softcap"})
+            want, moved = O.attend(q[row:row + n, :, :s.dim].double(), k[..., :s.dim], v[..., :s.vdim], seen, 1.3 / math.sqrt(s.dim), mask.get("softcap", 0.0))
+            f = torch.sigmoid(gv[row:row + n].double()).view(n, s.H, s.vdim) if gate == "element" else torch.sigmoid(gv[row:row + n, :s.H].double())[..., None]
+            compare(out[row:row + n, :s.H * s.vdim].view(n, s.H, s.vdim), want * f, moved, v.abs().max())
+
+
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 0.2])
+@pytest.mark.parametrize("softcap", [0.0, 3.0])
+def test_scales_of_either_sign(scale, softcap):
+    s = Setup(H=8, G=1, dim=64, norm="", n_rot=0, slots=1, n_ctx=700, seed=41)
+    s.fill(0, 640, 2.0)
+    k, v = s.values(s.k, 0, 640), s.values(s.v, 0, 640)
+    for n, dtype in ((3, torch.bfloat16), (40, torch.float32), (300, torch.float32), (300, torch.bfloat16)):
+        q = s.rnd(n, 8, 64).cuda()
+        out = torch.zeros(n, 8 * 64, device="cuda", dtype=dtype)
+        s.P.attn_prompt8(q, s.k, s.v, s.P.portions8([(0, n, 0, 640 - n)], s.table), s.table, out, vdim=64, scale=scale, softcap=softcap)
+        want, moved = O.attend(q.double(), k, v, O.visible(torch.arange(640 - n, 640), 640), scale, softcap)
+        compare(out.view(n, 8, 64), want, moved, v.abs().max())
+    x = s.rnd(1, s.ld)
+    out = torch.zeros(1, 8 * 64, device="cuda")
+    s.P.attn_decode8(x.cuda(), s.k, s.v, i32([640]), i32([0]), s.table, out, n_ctx=700, scale=scale, softcap=softcap, **s.prep())
+    k, v = s.values(s.k, 0, 641), s.values(s.v, 0, 641)
+    want, moved = O.attend(s.split(x, torch.tensor([640]))[0].cuda(), k, v, torch.ones(1, 641, dtype=torch.bool), scale, softcap)
+    compare(out.view(1, 8, 64), want, moved, v.abs().max())
+
+
+def test_growing_scores():
+    """Scores that rise from key to key by more than 2^8 a tile in their weights: what came before all but vanishes at each."""
+    s = Setup(H=4, G=1, dim=64, norm="", n_rot=0, slots=1, n_ctx=1500, seed=43)
+    x = s.rnd(1400, s.ld) * 0.1
+    x[:, s.nq] = torch.arange(1400) / 16
+    q = torch.empty(1400, 4, 64, device="cuda")
+    s.P.append8(x.cuda(), s.k, s.v, s.table, q, portions=s.P.portions8([(0, 1400, 0, 0)], s.table), **s.prep())
+    k, v = s.values(s.k, 0, 1400), s.values(s.v, 0, 1400)
+    for n in (4, 200):
+        for sign in (1.0, -1.0):
+            y = s.rnd(n, 4, 64).cuda() * 0.1
+            y[..., 0] = 2 * sign
+            out = torch.zeros(n, 4 * 64, device="cuda")
+            s.P.attn_prompt8(y, s.k, s.v, s.P.portions8([(0, n, 0, 1400 - n)], s.table), s.table, out, vdim=64, scale=1.0)
+            want, moved = O.attend(y.double(), k, v, O.visible(torch.arange(1400 - n, 1400), 1400), 1.0)
+            compare(out.view(n, 4, 64), want, moved, v.abs().max())
+
+
+@pytest.mark.parametrize("n", [33, 40, 300])
+def test_steps_of_many_rows(n):
+    """More rows than a warp has lanes, and than a launch takes: each row's result is that of a call of its own."""
+    s = Setup(H=4, G=2, dim=64, slots=n, n_ctx=128, seed=n)
+    lens = [1 + (37 * i) % 120 for i in range(n)]
+    t = Setup(H=4, G=2, dim=64, slots=n, n_ctx=128, seed=n)
+    fill = s.rnd(sum(lens), s.ld).cuda()
+    for c in (s, t):
+        q, parts, at = torch.empty(len(fill), 4, 64, device="cuda"), [], 0
+        for slot, m in enumerate(lens):
+            parts.append((at, m, slot, 0))
+            at += m
+        for i in range(0, n, 100):
+            some = parts[i:i + 100]
+            a, b = some[0][0], some[-1][0] + some[-1][1]
+            c.P.append8(fill[a:b], c.k, c.v, c.table, q[a:b], portions=c.P.portions8([(r - a, m, slot, 0) for r, m, slot, _ in some], c.table), **c.prep())
+    x = s.rnd(n, s.ld).cuda()
+    pos = [m if i % 9 else -1 for i, m in enumerate(lens)]
+    out = torch.full((n, 256), 5.0, device="cuda")
+    s.P.attn_decode8(x, s.k, s.v, i32(pos), i32(list(range(n))), s.table, out, n_ctx=128, scale=0.2, **s.prep())
+    q = s.split(x.cpu(), torch.tensor(pos))[0]
+    for i in range(n):
+        if pos[i] < 0:
+            assert (out[i] == 5).all()
+            continue
+        k, v = s.values(s.k, i, pos[i] + 1), s.values(s.v, i, pos[i] + 1)
+        want, moved = O.attend(q[i:i + 1].cuda(), k, v, torch.ones(1, pos[i] + 1, dtype=torch.bool), 0.2)
+        compare(out[i:i + 1].view(1, 4, 64), want, moved, v.abs().max())
+    one = torch.zeros(1, 256, device="cuda")
+    for i in range(1, n, 7):
+        if pos[i] >= 0:
+            t.P.attn_decode8(x[i:i + 1], t.k, t.v, i32(pos[i:i + 1]), i32([i]), t.table, one, n_ctx=128, scale=0.2, **t.prep())
+            assert torch.allclose(one, out[i:i + 1], rtol=2.0 ** -9, atol=2.0 ** -9)
+            at = t.table[i, :pos[i] // 64 + 1].long()
+            assert torch.equal(s.k.codes[at], t.k.codes[at]) and torch.equal(s.v.unit[at], t.v.unit[at])
+
+
+def test_values_that_are_no_number_in_many_rows():
+    s = Setup(H=4, G=2, dim=64, norm="", n_rot=0, slots=1, n_ctx=600, seed=47)
+    x = s.rnd(520, s.ld)
+    x[450, s.v_off + 64 + 5] = math.nan               # KV head 1
+    x[10, s.v_off + 3] = math.nan                     # KV head 0, seen through a kept key or not at all
+    q = torch.empty(520, 4, 64, device="cuda")
+    s.P.append8(x.cuda(), s.k, s.v, s.table, q, portions=s.P.portions8([(0, 520, 0, 0)], s.table), **s.prep())
+    for mask in (dict(), dict(window=100), dict(window=100, keep=11), dict(window=100, keep=10), dict(chunk=64)):
+        out = torch.zeros(500, 256, device="cuda")
+        s.P.attn_prompt8(q[20:], s.k, s.v, s.P.portions8([(0, 500, 0, 20)], s.table, **mask), s.table, out, vdim=64, scale=0.1, **mask)
+        seen = O.visible(torch.arange(20, 520), 520, **mask).cuda()
+        o = out.view(500, 4, 64).isnan().any(-1)
+        assert torch.equal(o[:, :2], seen[:, 10:11].expand(-1, 2)) and torch.equal(o[:, 2:], seen[:, 450:451].expand(-1, 2))
+
+
+def test_read_back_without_what_is_no_number():
+    from ollama_b200.ops import pages8 as P
+    g = torch.Generator().manual_seed(5)
+    codes = torch.randint(0, 256, (2, 2, 64, 64), generator=g, dtype=torch.int32).to(torch.uint8).cuda()
+    codes[:, :, ::3] &= 0x77                            # some rows hold numbers alone
+    c = P.Pages8(codes, torch.full((2, 2), 0.5, device="cuda"))
+    out = [torch.empty(1, 2, 64, 64, device="cuda", dtype=torch.float16) for _ in range(2)]
+    for clean in (0, 1):
+        P.read8(c, c, i32([[0, 0, 64, 0]]), i32([[1]]), *out, clean=bool(clean))
+        x = c.numbers[1].float() * 0.5
+        none = x.isnan().any(-1, keepdim=True) & bool(clean)
+        k, v = x.masked_fill(none, math.nan), x.masked_fill(none, 0.0)
+        assert torch.equal(out[0][0].float().nan_to_num(nan=1e9), k.nan_to_num(nan=1e9)) and torch.equal(out[1][0].float().nan_to_num(nan=1e9), v.nan_to_num(nan=1e9))
+
+
+@pytest.mark.parametrize("n", [6, 90, 400])
+def test_captured_portions(n):
+    """A portion's appending and attention in a graph, replayed over other rows, and beside a second graph of the same cache."""
+    s, t = (Setup(H=8, G=2, dim=64, slots=2, n_ctx=1100, seed=53) for _ in range(2))
+    for c in (s, t):
+        for slot in range(2):
+            c.fill(slot, 600)
+    plans = [s.P.portions8([(0, n, slot, 600)], s.table) for slot in range(2)]
+    xs, qs = torch.zeros(2, n, s.ld, device="cuda"), torch.zeros(2, n, 8, 64, device="cuda")
+    outs, prep, cap, graphs = torch.zeros(2, n, 512, device="cuda", dtype=torch.bfloat16), s.prep(), torch.cuda.Stream(), []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=cap):
+            s.P.append8(xs[i], s.k, s.v, s.table, qs[i], portions=plans[i], **prep)
+            s.P.attn_prompt8(qs[i], s.k, s.v, plans[i], s.table, outs[i], vdim=64, scale=0.2)
+        graphs.append(g)
+    q, out = torch.empty(n, 8, 64, device="cuda"), torch.empty(n, 512, device="cuda", dtype=torch.bfloat16)
+    for _ in range(2):
+        x = torch.randn(2, n, s.ld, device="cuda")
+        xs.copy_(x)
+        for i in range(2):
+            graphs[i].replay()
+        for i in range(2):
+            t.P.append8(x[i], t.k, t.v, t.table, q, portions=t.P.portions8([(0, n, i, 600)], t.table), **prep)
+            t.P.attn_prompt8(q, t.k, t.v, t.P.portions8([(0, n, i, 600)], t.table), t.table, out, vdim=64, scale=0.2)
+            assert torch.equal(outs[i], out)
