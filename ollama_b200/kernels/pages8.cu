@@ -4,6 +4,7 @@
 namespace {
 
 constexpr int WARPS = 8, THREADS = 32 * WARPS;
+constexpr int PAGE_WARPS = 16;               // of a CTA that appends many rows of a page
 constexpr int COLS = 4;                      // columns of a head row that a lane holds
 
 // Column i of a lane: with VEC four neighbours, so that a head row is one 16-byte load a lane, else every 32nd.
@@ -112,8 +113,9 @@ __device__ __forceinline__ uint32_t rescaled(uint32_t two, float f) {
 }
 
 // The codes of a page's head but those of rows [lo, hi), in a unit that is 1 / f of theirs.
+template <int W>
 __device__ void rescale_page(uint8_t* page, int hd, int lo, int hi, float f) {
-    for (int c = threadIdx.x; c < PAGE * hd / 16; c += THREADS) {
+    for (int c = threadIdx.x; c < PAGE * hd / 16; c += 32 * W) {
         const int r = c / (hd / 16);
         if (r >= lo && r < hi) continue;
         uint4 w = ((const uint4*)page)[c];
@@ -124,6 +126,7 @@ __device__ void rescale_page(uint8_t* page, int hd, int lo, int hi, float f) {
     }
 }
 
+template <int W>
 __device__ __forceinline__ float block_max(float v, float* red) {
     v = warp_max(v);
     __syncthreads();
@@ -131,7 +134,7 @@ __device__ __forceinline__ float block_max(float v, float* red) {
     __syncthreads();
     float m = red[0];
 #pragma unroll
-    for (int i = 1; i < WARPS; i++) m = fmaxf(m, red[i]);
+    for (int i = 1; i < W; i++) m = fmaxf(m, red[i]);
     return m;
 }
 
@@ -146,16 +149,16 @@ __device__ __forceinline__ float peer_value(const float* p, int rank) {
 
 // Rows [row, row + n) at positions [pos, pos + n), all in one page, of KV head g.  PEERS: the CTAs of the cluster have a page's KV heads, and a norm over the whole row takes each
 // head's sum from its CTA.
-template <bool VEC, bool PEERS>
+template <bool VEC, bool PEERS, int W>
 __device__ void append_to_page(const Append8Args& a, int row, int n, int slot, int pos, int g, float* cs, float* red) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int half = a.n_rot >> 1, pitch = (half + 3) & ~3, kdim = a.maps * a.dim, G = a.c.kv_heads, hd = a.c.hd;
     const int nq = a.n_heads * a.dim, nk = G * kdim, off = pos & (PAGE - 1);
     float* sn = cs + (a.positions ? 1 : PAGE) * pitch;      // as many rows as the launch has shared memory for
-    float k[PAGE / WARPS][COLS], v[PAGE / WARPS][COLS];
+    float k[PAGE / W][COLS], v[PAGE / W][COLS];
 #pragma unroll
-    for (int i = 0; i < PAGE / WARPS; i++) {
-        const int r = warp + WARPS * i;
+    for (int i = 0; i < PAGE / W; i++) {
+        const int r = warp + W * i;
         if (r < n) {
             const float* p = a.qkv + (size_t)(row + r) * a.ldq;
             load_head<VEC>(p + nq + g * kdim, kdim, lane, k[i]);
@@ -171,22 +174,23 @@ __device__ void append_to_page(const Append8Args& a, int row, int n, int slot, i
     const float old_k = a.c.ku[head], old_v = a.c.vu[head];
     __syncthreads();      // the tables may still be read for the rows before
     if (n == 1) {
-        for (int p = tid; p < half; p += THREADS) {
+        for (int p = tid; p < half; p += 32 * W) {
             float si, co;
             sincosf(rot_angle(pos, a.freqs[p]), &si, &co);
             cs[p] = co * a.mscale;
             sn[p] = si * a.mscale;
         }
     } else if (half > 0) {
-        // Row 8 i + j turns by the angle of row j and that of 8 i positions more: 16 angles a pair instead of 64 (half <= 64: four threads a pair).  The products of their cosines
+        // Row 8 i + j turns by the angle of row j and that of 8 i positions more: 16 angles a pair instead of 64 (half <= 64).  The products of their cosines
         // and sines are off by some 2^-23, the codes by up to 2^-4.
+        constexpr int PARTS = W / 2, EACH = 16 / PARTS;
         const int p = tid & 63, part = tid >> 6;
         float* step = sn + PAGE * pitch;      // [16][2][pitch]: rows 0 .. 7, then 0, 8 .. 56 positions
         if (p < half) {
             const double f = a.freqs[p];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int e = 4 * part + i;
+            for (int i = 0; i < EACH; i++) {
+                const int e = EACH * part + i;
                 float si, co;
                 sincosf(rot_angle(e < 8 ? pos + e : 8 * (e - 8), f), &si, &co);
                 step[2 * e * pitch + p] = e < 8 ? co * a.mscale : co;
@@ -195,7 +199,7 @@ __device__ void append_to_page(const Append8Args& a, int row, int n, int slot, i
         }
         __syncthreads();
         if (p < half)
-            for (int r = part; r < n; r += 4) {
+            for (int r = part; r < n; r += PARTS) {
                 const float c0 = step[2 * (r & 7) * pitch + p], s0 = step[(2 * (r & 7) + 1) * pitch + p], c1 = step[2 * (8 + (r >> 3)) * pitch + p], s1 = step[(2 * (8 + (r >> 3)) + 1) * pitch + p];
                 cs[r * pitch + p] = c0 * c1 - s0 * s1;
                 sn[r * pitch + p] = s0 * c1 + c0 * s1;
@@ -206,17 +210,17 @@ __device__ void append_to_page(const Append8Args& a, int row, int n, int slot, i
     const bool whole = PEERS && a.k_norm && !a.head_norm;
     if (whole) {
 #pragma unroll
-        for (int i = 0; i < PAGE / WARPS; i++) {
+        for (int i = 0; i < PAGE / W; i++) {
             const float sum = warp_sum(square_sum(k[i]));      // rows behind the last one hold nothing that is used
-            if (lane == 0) own[warp + WARPS * i] = sum;
+            if (lane == 0) own[warp + W * i] = sum;
         }
         cluster_sync();
     }
     const float per_column = 1.f / (float)(a.head_norm ? a.dim : nk);
     float top_k = 0.f, top_v = 0.f;
 #pragma unroll
-    for (int i = 0; i < PAGE / WARPS; i++) {
-        const int r = warp + WARPS * i;
+    for (int i = 0; i < PAGE / W; i++) {
+        const int r = warp + W * i;
         if (r < n) {
             if (a.k_norm) {
                 float s;
@@ -243,22 +247,22 @@ __device__ void append_to_page(const Append8Args& a, int row, int n, int slot, i
             }
         }
     }
-    float unit_k = unit_for(block_max(top_k, red)), unit_v = unit_for(block_max(top_v, red));
+    float unit_k = unit_for(block_max<W>(top_k, red)), unit_v = unit_for(block_max<W>(top_v, red));
     uint8_t *kp = a.c.k + head * PAGE * hd, *vp = a.c.v + head * PAGE * hd;
     if (off > 0) {        // positions before these stay: the page's unit does not shrink
         unit_k = fmaxf(unit_k, old_k);
         unit_v = fmaxf(unit_v, old_v);
     }
-    if (unit_k > old_k && n < PAGE) rescale_page(kp, hd, off, off + n, old_k / unit_k);
-    if (unit_v > old_v && n < PAGE) rescale_page(vp, hd, off, off + n, old_v / unit_v);
+    if (unit_k > old_k && n < PAGE) rescale_page<W>(kp, hd, off, off + n, old_k / unit_k);
+    if (unit_v > old_v && n < PAGE) rescale_page<W>(vp, hd, off, off + n, old_v / unit_v);
     if (tid == 0) {
         a.c.ku[head] = unit_k;
         a.c.vu[head] = unit_v;
     }
     const float ik = 1.f / unit_k, iv = 1.f / unit_v;
 #pragma unroll
-    for (int i = 0; i < PAGE / WARPS; i++) {
-        const int r = warp + WARPS * i;
+    for (int i = 0; i < PAGE / W; i++) {
+        const int r = warp + W * i;
         if (r < n) {
             store_codes<VEC>(kp + (off + r) * hd, lane, hd, k[i], ik);
             store_codes<VEC>(vp + (off + r) * hd, lane, hd, v[i], iv);
@@ -372,7 +376,7 @@ __global__ void __launch_bounds__(THREADS, 4) append8_kernel(const __grid_consta
     if (before) return;
     for (int i = u; i < (behind ? a.rows : u + 1); i++) {
         if (a.slots[i] != slot || a.positions[i] < 0) continue;
-        append_to_page<VEC, false>(a, i, 1, slot, a.positions[i], g, cs, red);
+        append_to_page<VEC, false, WARPS>(a, i, 1, slot, a.positions[i], g, cs, red);
         __syncthreads();      // what it wrote is read by the next one's rescaling
     }
 }
@@ -380,22 +384,22 @@ __global__ void __launch_bounds__(THREADS, 4) append8_kernel(const __grid_consta
 // The same for portions of prompts, in two launches, since a page's rows stay in registers between the largest magnitude and the codes, eight a warp, and would leave the queries
 // two CTAs an SM (2048 rows of 32 heads on 8: 49 us in one).  Keys and values: a KV head and a page of a portion each.
 template <bool VEC, bool PEERS>
-__global__ void __launch_bounds__(THREADS, 2) append8_pages_kernel(const __grid_constant__ Append8Args a) {
+__global__ void __launch_bounds__(32 * PAGE_WARPS, 2) append8_pages_kernel(const __grid_constant__ Append8Args a) {
     extern __shared__ __align__(16) float cs[];
-    __shared__ float red[WARPS];
+    __shared__ float red[PAGE_WARPS];
     pdl_wait();
     pdl_launch();
     const int G = a.c.kv_heads, g = blockIdx.x % G, j = blockIdx.x / G % a.per;
     const int4 s = a.segs[blockIdx.x / G / a.per];
     const int first = (s.w >> PAGE_SHIFT) + j, lo = max(s.w, first * PAGE), hi = min(s.w + s.y, (first + 1) * PAGE);
     if (s.w < 0 || s.x < 0 || s.x + s.y > a.rows || lo >= hi) return;
-    append_to_page<VEC, PEERS>(a, s.x + lo - s.w, hi - lo, s.z, lo, g, cs, red);
+    append_to_page<VEC, PEERS, PAGE_WARPS>(a, s.x + lo - s.w, hi - lo, s.z, lo, g, cs, red);
 }
 
 // Queries: a row each.  `behind`: launched behind the keys and values, which it does not read, while they are under way.  (CTAs that take several rows and have the next one's
 // values on their way: 32.8 us instead of 31.1 for 2048 rows of 32 heads on 8.)
 template <bool VEC>
-__global__ void __launch_bounds__(THREADS, 4) append8_queries_kernel(const __grid_constant__ Append8Args a, int behind) {
+__global__ void __launch_bounds__(THREADS, VEC ? 6 : 4) append8_queries_kernel(const __grid_constant__ Append8Args a, int behind) {
     extern __shared__ __align__(16) float cs[];
     __shared__ float red[WARPS];
     pdl_launch();
@@ -499,7 +503,7 @@ int append8_launch(const Append8Args& in, int pdl, cudaStream_t st) {
         cudaLaunchAttribute at[2];
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)ctas);
-        cfg.blockDim = dim3(THREADS);
+        cfg.blockDim = dim3(32 * PAGE_WARPS);
         cfg.dynamicSmemBytes = (PAGE + 16) * one;
         cfg.stream = st;
         at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
