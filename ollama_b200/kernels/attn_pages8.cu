@@ -6,8 +6,11 @@
 // the query heads of a KV head their columns, eight or sixteen of them (an item: sequence, so many rows, KV head): with the four heads of grouped-query models as the rows, three
 // quarters of every product, of its sums and of the exponentials were padding.  Codes become f16 operands in registers, exactly; the units multiply scores and sums.  An item's
 // keys, in turns of 32, are shared by as many CTAs as its part of all turns is of the CTAs that fit the GPU, so that a CTA has one item (CTAs with an equal share of all turns each
-// took 80 to 86 us where one item ended inside it and 60 to 72 elsewhere); its warps take the turns in rotation, each through a ring of its own that TMA fills, so that nothing in
+// took 80 to 86 us where one item ended inside it and 60 to 72 elsewhere; twice and three times as many CTAs an item, 88 and 96 us instead of 87); its warps take the turns in rotation, each through a ring of its own that TMA fills, so that nothing in
 // the loop waits for another warp.  A CTA leaves (largest score, sum, unnormalised result), which the merge kernel adds up.
+// In a decode step the launch runs behind the append's start: what does not depend on the appended rows (shares, places, boxes of closed pages) is under way when the append ends.
+// Measured, whole steps with append and merge in a graph, 128 columns: four sequences of 60000 keys, 32 heads on 8, 77 us, 5.1 TB/s of the 6.5 that a copy reaches (the SMs fetch
+// unevenly: CTAs end between 51 and 74 us); one of 6144 keys 13 us and 32 sequences with windows of 1024, 16 heads on 4, 20 us, of which the three launches' latencies are most.
 #include "attn_pages8.cuh"
 #include "tc_common.cuh"
 

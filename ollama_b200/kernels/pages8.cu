@@ -381,8 +381,9 @@ __global__ void __launch_bounds__(THREADS, 4) append8_kernel(const __grid_consta
     }
 }
 
-// The same for portions of prompts, in two launches, since a page's rows stay in registers between the largest magnitude and the codes, eight a warp, and would leave the queries
-// two CTAs an SM (2048 rows of 32 heads on 8: 49 us in one).  Keys and values: a KV head and a page of a portion each.
+// The same for portions of prompts, in two launches, since a page's rows stay in registers between the largest magnitude and the codes, and would leave the queries
+// two CTAs an SM (2048 rows of 32 heads on 8: 49 us in one).  Keys and values: a KV head and a page of a portion each, 16 warps (eight: 2 us more).  Together 27.5 us, 88 MB at
+// 3.2 TB/s: two waves of CTAs whose loads, norms, rotation and stores follow one another.
 template <bool VEC, bool PEERS>
 __global__ void __launch_bounds__(32 * PAGE_WARPS, 2) append8_pages_kernel(const __grid_constant__ Append8Args a) {
     extern __shared__ __align__(16) float cs[];
@@ -396,8 +397,8 @@ __global__ void __launch_bounds__(32 * PAGE_WARPS, 2) append8_pages_kernel(const
     append_to_page<VEC, PEERS, PAGE_WARPS>(a, s.x + lo - s.w, hi - lo, s.z, lo, g, cs, red);
 }
 
-// Queries: a row each.  `behind`: launched behind the keys and values, which it does not read, while they are under way.  (CTAs that take several rows and have the next one's
-// values on their way: 32.8 us instead of 31.1 for 2048 rows of 32 heads on 8.)
+// Queries: a row each.  `behind`: launched behind the keys and values, which it does not read, while they are under way.  Six CTAs an SM: 27.5 us instead of
+// 28.7 with four.  (CTAs that take several rows and have the next one's values on their way were slower, 32.8 us where these took 31.1.)
 template <bool VEC>
 __global__ void __launch_bounds__(THREADS, VEC ? 6 : 4) append8_queries_kernel(const __grid_constant__ Append8Args a, int behind) {
     extern __shared__ __align__(16) float cs[];

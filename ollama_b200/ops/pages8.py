@@ -6,8 +6,9 @@ appended to the page fits; larger magnitudes than 57344 become that.  Where an a
 row at a page's first position begins the page anew.  Rows have 64 or 128 columns; heads of fewer leave zeros behind theirs.
 
 Tables of pages are [slots, pages] int32: entry i of a slot is the page of its positions 64 i .. 64 i + 63.  Rows whose position is negative hold no token: nothing is
-appended for them and their results are left as they are.  So are rows whose slot, position or page is not there.  All calls run on the current stream of the
-tensors' device.
+appended for them and their results are left as they are.  So are rows whose slot or position the table does not have.  Where a table's entry is no page of the cache
+nothing is appended and nothing outside the cache is read; what attention makes of such positions is not defined.  A page that rows are appended to may be in one slot's
+table only, others may be in several.  All calls run on the current stream of the tensors' device.
 """
 from __future__ import annotations
 

@@ -478,7 +478,7 @@ const char attn_decode8_doc[] =
     "attn_decode8(qkv, k, v, positions, slots, table, out, *, heads, dim, vdim, q_norm, k_norm, eps, freqs, n_rot, scale, n_ctx, softcap=0.0, chunk=0, window=0, keep=0, "
     "head_norm=False, v_off=None, mscale=1.0, gate=NO_GATE, maps=1, append=True, diff=NO_DIFF, pdl=False)\n--\n\n"
     "Decode attention on raw projections, one token a sequence: what append8 does, then attention of the rows' positions over the cache, difference of maps and gate into rows of\n"
-    "`out`.  `n_ctx`: most keys that a sequence holds.";
+    "`out`.  `n_ctx`: most keys that a sequence holds, as of the 16-bit form; the work follows the positions.";
 
 PyMethodDef methods[] = {
     {"append8", (PyCFunction)(void (*)())py_append8, METH_FASTCALL | METH_KEYWORDS, append8_doc},
