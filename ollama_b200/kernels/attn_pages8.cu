@@ -456,6 +456,10 @@ __global__ void __launch_bounds__(MERGE_COLUMNS * HALVES) attn8_merge_kernel(con
 }
 
 bool bad_args(const Attn8Args& a) {
+    // counts of (turn, item) pairs and of rows times heads are 32 bits wide
+    if ((unsigned long long)min(a.positions ? a.rows : a.n_segs, MAX_UNITS) * a.tiles * a.c.kv_heads * ((unsigned long long)a.t.max_pages * PAGE / 32 + 2) >> 32 ||
+        (long long)a.rows * a.n_heads >> 31 || (long long)a.tiles * a.row_tile >> 31)
+        return true;
     return !a.q || !a.c.k || !a.c.v || !a.c.ku || !a.c.vu || a.c.n_pages < 1 || (a.c.hd != 64 && a.c.hd != 128) || a.c.kv_heads < 1 || a.n_heads < 1 || a.n_heads % a.c.kv_heads ||
            a.n_heads > 65535 || a.rows < 1 || a.rows > 65535 || a.vdim < 1 || a.vdim > a.c.hd || !a.t.table || a.t.n_slots < 1 || a.t.max_pages < 1 || a.t.max_pages > (1 << 24) ||
            (!a.positions == !a.segs) || (a.positions && !a.slots) || (a.segs && a.n_segs < 1) || a.chunk < 0 || a.window < 0 || a.keep < 0 || (a.chunk && a.window) || a.softcap < 0.f ||
@@ -511,6 +515,7 @@ static int attn8_launch(const Attn8Args& in, int pdl, cudaStream_t st) {
     const int units = in.positions ? in.rows : in.n_segs, heads = MERGE_COLUMNS / in.c.hd;
     for (int u = 0; u < units; u += MAX_UNITS) {
         Attn8Args a = in;
+        a.keep = min(a.keep, a.t.max_pages * PAGE);      // tiles of kept keys are counted in 32 bits
         const int n = units - u < MAX_UNITS ? units - u : MAX_UNITS;
         if (a.positions) {
             a.positions += u;

@@ -24,7 +24,9 @@ __device__ __forceinline__ Unit unit_at(const Attn8Args& a, int u) {
         const int4 g = a.segs[u];
         s = Unit{g.x, g.y, g.z, g.w, 0, 0};
     }
-    if ((unsigned)s.slot >= (unsigned)a.t.n_slots || s.pos < 0 || s.row < 0 || s.row + s.rows > a.rows || s.pos + s.rows > a.t.max_pages * PAGE) s.rows = 0;
+    if ((unsigned)s.slot >= (unsigned)a.t.n_slots || s.pos < 0 || s.row < 0 || s.rows < 0 || s.rows > a.rows - s.row || s.rows > a.t.max_pages * PAGE - s.pos ||
+        s.rows * (a.n_heads / a.c.kv_heads) > a.tiles * a.row_tile)
+        s.rows = 0;
     s.open = s.pos >> PAGE_SHIFT;
     return s;
 }

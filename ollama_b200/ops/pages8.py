@@ -138,7 +138,7 @@ def attn_prompt8(q, k: Pages8, v: Pages8, portions: Portions8, table, out, *, vd
     wide = torch.empty(2, m, kv_heads, PAGE, hd, device=q.device, dtype=torch.float16)
     here["read8"](k, v, pages, table, wide[0], wide[1], pdl, clean=True)
     a = AttnPrefillArgs(q.data_ptr(), wide[0].data_ptr(), wide[1].data_ptr(), out.data_ptr(), None, n, heads, kv_heads, 0, 0, 0, 0, 1, 0, scale, softcap, None, None)
-    pg = AttnPagedArgs(tiles.data_ptr(), portions.table.data_ptr(), portions.table.shape[1], chunk, vdim, out.stride(0), window, keep, gate, diff)
+    pg = AttnPagedArgs(tiles.data_ptr(), portions.table.data_ptr(), portions.table.shape[1], chunk, vdim, out.stride(0), window, min(keep, portions.table.shape[1] * PAGE), gate, diff)
     f = lib().b2_attn_prefill_paged
     f.argtypes = [P, P, I, I, I, P]
     with torch.cuda.device(q.device):

@@ -9,6 +9,7 @@
 
 #include <algorithm>
 #include <cstring>
+#include <limits>
 #include <stdexcept>
 #include <string>
 
@@ -152,6 +153,17 @@ const at::Tensor& vector(const Signature& s, PyObject* o, const char* name, at::
     if (t.dim() != 1 || t.numel() < least) refuse(s, std::string(name) + " " + told(t));
     return t;
 }
+// From a row to the next of rows that stand beside one another.
+long row_step(const Signature& s, const at::Tensor& t, const char* name) {
+    const long step = t.size(0) > 1 ? t.stride(0) : t.size(1);
+    if (step < t.size(1) || step > (1l << 31) - 1) refuse(s, std::string(name) + " " + told(t) + " with rows " + std::to_string(step) + " apart");
+    return step;
+}
+// read or written 16 bytes at a time
+const at::Tensor& wide(const Signature& s, const at::Tensor& t, const char* name) {
+    if ((uintptr_t)t.data_ptr() & 15) refuse(s, std::string(name) + " is not on a 16-byte boundary");
+    return t;
+}
 constexpr at::ScalarType F32 = at::kFloat, F64 = at::kDouble, I32 = at::kInt, F16 = at::kHalf, B16 = at::kBFloat16;
 
 struct Cache {
@@ -209,7 +221,7 @@ void fill_append(const Signature& s, Append8Args& p, const at::Tensor& qkv, cons
     const bool norm = given(a.qn);
     if (norm != given(a.kn) || (norm && (maps > 1 || !append))) refuse(s, "norms");
     p.qkv = (const float*)qkv.data_ptr();
-    p.ldq = (int)qkv.stride(0);
+    p.ldq = (int)row_step(s, qkv, "qkv");
     p.rows = (int)qkv.size(0);
     p.n_heads = heads;
     p.dim = dim;
@@ -249,7 +261,7 @@ void append8(PyObject** a) {
     Append8Args p = {};
     fill_append(s, p, qkv, c, Prep{a[A_HEADS], a[A_DIM], a[A_VDIM], a[A_QN], a[A_KN], a[A_EPS], a[A_FREQS], a[A_NROT], a[A_HEADNORM], a[A_VOFF], a[A_MSCALE], a[A_MAPS], a[A_APPEND]});
     const long n = p.rows;
-    p.q_out = (float*)shaped(s, a[A_QOUT], "q_out", F32, dev, n, p.n_heads, c.c.hd).data_ptr();
+    p.q_out = (float*)wide(s, shaped(s, a[A_QOUT], "q_out", F32, dev, n, p.n_heads, c.c.hd), "q_out").data_ptr();
     if (given(a[A_PORTIONS]) == (given(a[A_POS]) || given(a[A_SLOTS]))) refuse(s, "either positions and slots or portions");
     if (given(a[A_PORTIONS])) {
         const Portions q = portions(s, a[A_PORTIONS], n, dev);
@@ -277,8 +289,9 @@ void read8(PyObject** a) {
     const c10::Device dev = on_gpu(s, pages);
     const Cache c = cache(s, a[R_K], a[R_V], a[R_TABLE], dev);
     const long n = pages.dim() ? pages.size(0) : 0;
-    shaped(s, a[R_PAGES], "pages", I32, dev, n, 4);
-    const at::Tensor &ko = shaped(s, a[R_KOUT], "k_out", F16, dev, n, c.c.kv_heads, PAGE, c.c.hd), &vo = shaped(s, a[R_VOUT], "v_out", F16, dev, n, c.c.kv_heads, PAGE, c.c.hd);
+    wide(s, shaped(s, a[R_PAGES], "pages", I32, dev, n, 4), "pages");
+    const at::Tensor &ko = wide(s, shaped(s, a[R_KOUT], "k_out", F16, dev, n, c.c.kv_heads, PAGE, c.c.hd), "k_out"),
+                     &vo = wide(s, shaped(s, a[R_VOUT], "v_out", F16, dev, n, c.c.kv_heads, PAGE, c.c.hd), "v_out");
     if (!n) return;
     const c10::cuda::CUDAGuard guard(dev);
     launched(s, f_read(&c.c, &c.t, pages.data_ptr(), n, ko.data_ptr(), vo.data_ptr(), as_bool(a[R_CLEAN], false), as_bool(a[R_PDL], false), c10::cuda::getCurrentCUDAStream(dev.index())));
@@ -297,7 +310,7 @@ void fill_attn(const Signature& s, Attn8Args& p, long n, long heads, PyObject* o
     p.softcap = (float)as_double(m.softcap, 0.0);
     if (heads < 1 || heads % G || vdim < 1 || vdim > c.c.hd || (p.diff.on && heads / G % 2) || out.size(1) < (p.diff.on ? heads / 2 : heads) * vdim)
         refuse(s, std::to_string(heads) + " heads on " + std::to_string(G) + " of " + std::to_string(vdim) + " columns into rows of " + std::to_string(out.size(1)));
-    if (chunk < 0 || window < 0 || keep < 0 || (chunk && window) || !(p.softcap >= 0.f))
+    if (chunk < 0 || window < 0 || keep < 0 || (chunk && window) || !(p.softcap >= 0.f && p.softcap <= std::numeric_limits<float>::max()))
         refuse(s, "chunk " + std::to_string(chunk) + ", window " + std::to_string(window) + ", keep " + std::to_string(keep) + ", softcap " + std::to_string(p.softcap));
     p.rows = n;
     p.n_heads = heads;
@@ -309,7 +322,7 @@ void fill_attn(const Signature& s, Attn8Args& p, long n, long heads, PyObject* o
     p.keep = keep;
     p.scale = (float)as_double(m.scale, 0.0);
     p.out = out.data_ptr();
-    p.ldo = (int)out.stride(0);
+    p.ldo = (int)row_step(s, out, "out");
     p.out16 = out.scalar_type() == B16;
 }
 
@@ -369,7 +382,7 @@ bool attn_prompt8(PyObject** a) {
     const Cache c = cache(s, a[P_K], a[P_V], a[P_TABLE], dev);
     if (q.dim() != 3) refuse(s, "q " + told(q));
     const long n = q.size(0), heads = q.size(1), hd = c.c.hd;
-    shaped(s, a[P_Q], "q", F32, dev, n, heads, hd);
+    wide(s, shaped(s, a[P_Q], "q", F32, dev, n, heads, hd), "q");
     Attn8Args t = {};
     fill_attn(s, t, n, heads, a[P_OUT], c, dev, Mask{a[P_VDIM], a[P_SCALE], a[P_SOFTCAP], a[P_CHUNK], a[P_WINDOW], a[P_KEEP], a[P_GATE], a[P_DIFF]});
     const Portions po = portions(s, a[P_PORTIONS], n, dev);

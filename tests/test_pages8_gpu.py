@@ -653,3 +653,55 @@ def test_captured_portions(n):
             t.P.append8(x[i], t.k, t.v, t.table, q, portions=t.P.portions8([(0, n, i, 600)], t.table), **prep)
             t.P.attn_prompt8(q, t.k, t.v, t.P.portions8([(0, n, i, 600)], t.table), t.table, out, vdim=64, scale=0.2)
             assert torch.equal(outs[i], out)
+
+
+def test_masks_of_any_size():
+    """Windows, chunks and numbers of kept keys up to the largest integer are those that end with the sequence."""
+    s = Setup(H=8, G=2, dim=64, slots=1, n_ctx=700, seed=59)
+    s.fill(0, 640)
+    most = 2 ** 31 - 1
+    for n, dtype in ((1, torch.float32), (5, torch.float32), (300, torch.float32), (300, torch.bfloat16)):
+        q, got = s.rnd(n, 8, 64).cuda(), []
+        for mask in (dict(), dict(window=700), dict(window=most), dict(window=20, keep=700), dict(window=20, keep=most), dict(window=most, keep=most), dict(chunk=most)):
+            out = torch.zeros(n, 512, device="cuda", dtype=dtype)
+            s.P.attn_prompt8(q, s.k, s.v, s.P.portions8([(0, n, 0, 640 - n)], s.table, **mask), s.table, out, vdim=64, scale=0.1, **mask)
+            got.append(out)
+        assert all(torch.allclose(g.float(), got[0].float(), rtol=2.0 ** -7, atol=2.0 ** -9) for g in got)
+    x = s.rnd(1, s.ld).cuda()
+    got = []
+    for mask in (dict(), dict(window=most), dict(window=20, keep=most), dict(chunk=most)):
+        out = torch.zeros(1, 512, device="cuda")
+        s.P.attn_decode8(x, s.k, s.v, i32([640]), i32([0]), s.table, out, n_ctx=700, scale=0.1, **s.prep(), **mask)
+        got.append(out)
+    assert all(torch.allclose(g, got[0], rtol=2.0 ** -9, atol=2.0 ** -9) for g in got)
+
+
+def test_refusals_of_memory_that_does_not_fit():
+    s = Setup(H=4, G=2, dim=64)
+    P, plan, out, prep = s.P, s.P.portions8([(0, 2, 0, 0)], s.table), torch.zeros(2, 256, device="cuda"), s.prep()
+    odd = lambda *shape, dtype=torch.float32: torch.zeros(math.prod(shape) + 1, device="cuda", dtype=dtype)[1:].view(shape)  # noqa: E731
+    x = s.rnd(2, s.ld).cuda()
+    with pytest.raises(ValueError):
+        P.attn_prompt8(odd(2, 4, 64), s.k, s.v, plan, s.table, out, vdim=64, scale=0.1)
+    for kw in (dict(softcap=math.inf), dict(softcap=math.nan), dict(out=torch.zeros(1, 256, device="cuda").expand(2, 256)), dict(out=torch.zeros(600, device="cuda").as_strided((2, 256), (200, 1)))):
+        with pytest.raises(ValueError):
+            P.attn_prompt8(**{**dict(q=torch.zeros(2, 4, 64, device="cuda"), k=s.k, v=s.v, portions=plan, table=s.table, out=out, vdim=64, scale=0.1), **kw})
+    with pytest.raises(ValueError):
+        P.append8(x, s.k, s.v, s.table, odd(2, 4, 64), portions=plan, **prep)
+    with pytest.raises(ValueError):
+        P.append8(x[:1].expand(2, s.ld), s.k, s.v, s.table, torch.zeros(2, 4, 64, device="cuda"), portions=plan, **prep)
+    wide = [torch.zeros(1, 2, 64, 64, device="cuda", dtype=torch.float16) for _ in range(2)]
+    with pytest.raises(ValueError):
+        P.read8(s.k, s.v, odd(1, 4, dtype=torch.int32), s.table, *wide)
+    with pytest.raises(ValueError):
+        P.read8(s.k, s.v, i32([[0, 0, 64, 0]]), s.table, odd(1, 2, 64, 64, dtype=torch.float16), wide[1])
+    assert (out == 0).all()
+    # one row stands beside no other one: its step is not looked at
+    one = torch.zeros(1, 256, device="cuda").as_strided((1, 256), (3, 1))
+    P.attn_decode8(x[:1].as_strided((1, s.ld), (1, 1)), s.k, s.v, i32([0]), i32([0]), s.table, one, n_ctx=100, scale=0.1, **prep)
+    assert (one != 0).any()
+    # a plan that says less than its portions hold
+    import dataclasses
+    few, before = dataclasses.replace(s.P.portions8([(0, 40, 0, 0)], s.table), longest=1), torch.full((40, 256), 5.0, device="cuda")
+    P.attn_prompt8(torch.zeros(40, 4, 64, device="cuda"), s.k, s.v, few, s.table, before, vdim=64, scale=0.1)
+    assert (before == 5).all()
