@@ -8,9 +8,10 @@
 // the group's reference by a factor of 2^LAG: no group waits for the other, and nothing is read back per tile.  The groups' results meet in shared memory at the end.
 // Warps: 0-3 and 4-7 softmax (a thread a row), 8 bulk copies, 9 products and tensor memory, 12-19 codes.  Every wait is bounded; one that runs out sets KS_TIMEOUT, and all roles
 // leave their loops.
-// Measured: 64 rows of 32 heads on 8 of 128 columns behind 30000 keys, 59 us with the merge, 1.35 us a tile.  A tile moves 224 KB through the SM's shared memory (codes in and out,
-// f16 tiles in, operands out), 1800 of its 2300 cycles at 128 bytes a cycle, which bounds it now; boxes in the order K(t), V(t), six code warps, one softmax group of eight warps
-// that reads each P V back and a second look at the keys of masked tiles took 88.
+// Measured: 64 rows of 32 heads on 8 of 128 columns behind 30000 keys, 59 us with the merge, 1.4 us a tile.  A group's turn is 1.5 us of softmax (exponentials, at 16 a
+// cycle, and rounding 0.95, loads from tensor memory and maximum 0.6) and 1.1 until its next scores are there; two groups take 1.4 a tile, the tensor cores busy for 0.6 of them.
+// Leaving the expansion's stores out changed nothing.  Slower: boxes in the order K(t), V(t), six code warps and one softmax group that reads each P V back, 88; a second look at the
+// keys of masked tiles, 10 us in instruction misses; sixteen softmax warps, 60.7; a quarter of the exponentials as cubics on the FMA units, 63.7, half of them 68.
 #include "attn_pages8.cuh"
 #include "attn_tc.cuh"
 
