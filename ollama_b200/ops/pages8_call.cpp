@@ -153,6 +153,10 @@ const at::Tensor& vector(const Signature& s, PyObject* o, const char* name, at::
     if (t.dim() != 1 || t.numel() < least) refuse(s, std::string(name) + " " + told(t));
     return t;
 }
+// Rows are a dimension of the merge's grid.
+void few_rows(const Signature& s, long n) {
+    if (n > 65535) refuse(s, std::to_string(n) + " rows");
+}
 // From a row to the next of rows that stand beside one another.
 long row_step(const Signature& s, const at::Tensor& t, const char* name) {
     const long step = t.size(0) > 1 ? t.stride(0) : t.size(1);
@@ -357,6 +361,7 @@ void attn_decode8(PyObject** a) {
     Attn8Args t = {};
     fill_attn(s, t, n, heads, a[D_OUT], c, dev, Mask{a[D_VDIM], a[D_SCALE], a[D_SOFTCAP], a[D_CHUNK], a[D_WINDOW], a[D_KEEP], a[D_GATE], a[D_DIFF]});
     if (!n) return;
+    few_rows(s, n);
     const long group = heads / c.c.kv_heads, pieces = tile(t, group <= 8 ? 8 : 16, group, n, dev), nq = n * heads * hd;
     const c10::cuda::CUDAGuard guard(dev);
     const at::Tensor ws = at::empty({nq + pieces * (hd + 2)}, at::TensorOptions().dtype(F32).device(dev));      // rotated queries, partial results, their statistics
@@ -410,6 +415,7 @@ bool attn_prompt8(PyObject** a) {
     }
     const double t16 = 9.6 + 0.08 * items16 + keys16 / 19000, t128 = 12 + 0.37 * items128 + keys128 / 11700, t_read = 10 + 0.0107 * most * std::max(1.0, ctas / sms_of(dev));
     if (m > 64 && t_read < std::min(t16, t128) && t.out16 && !((uintptr_t)t.out & 15) && !(t.diff.on && t.gate.kind)) return false;
+    few_rows(s, n);
     const long pieces = tile(t, m <= 8 ? 8 : m <= 16 || t16 <= t128 ? 16 : 128, m, po.n, dev);
     const c10::cuda::CUDAGuard guard(dev);
     const at::Tensor ws = at::empty({pieces * (hd + 2)}, at::TensorOptions().dtype(F32).device(dev));

@@ -705,3 +705,14 @@ def test_refusals_of_memory_that_does_not_fit():
     few, before = dataclasses.replace(s.P.portions8([(0, 40, 0, 0)], s.table), longest=1), torch.full((40, 256), 5.0, device="cuda")
     P.attn_prompt8(torch.zeros(40, 4, 64, device="cuda"), s.k, s.v, few, s.table, before, vdim=64, scale=0.1)
     assert (before == 5).all()
+
+
+def test_refusal_of_too_many_rows():
+    s, n = Setup(H=2, G=1, dim=64, slots=1, n_ctx=65600), 65536
+    plan, out = s.P.portions8([(0, n, 0, 0)], s.table), torch.zeros(n, 128, device="cuda")
+    with pytest.raises(ValueError, match="65536 rows"):
+        s.P.attn_prompt8(torch.zeros(n, 2, 64, device="cuda"), s.k, s.v, plan, s.table, out, vdim=64, scale=0.1)
+    with pytest.raises(ValueError, match="65536 rows"):
+        s.P.attn_decode8(torch.zeros(n, s.ld, device="cuda"), s.k, s.v, torch.zeros(n, device="cuda", dtype=torch.int32), torch.zeros(n, device="cuda", dtype=torch.int32), s.table, out, n_ctx=100,
+                         scale=0.1, **s.prep())
+    assert (out == 0).all()
