@@ -456,9 +456,9 @@ __global__ void __launch_bounds__(MERGE_COLUMNS * HALVES) attn8_merge_kernel(con
 }
 
 bool bad_args(const Attn8Args& a) {
-    // counts of (turn, item) pairs and of rows times heads are 32 bits wide
-    if ((unsigned long long)min(a.positions ? a.rows : a.n_segs, MAX_UNITS) * a.tiles * a.c.kv_heads * ((unsigned long long)a.t.max_pages * PAGE / 32 + 2) >> 32 ||
-        (long long)a.rows * a.n_heads >> 31 || (long long)a.tiles * a.row_tile >> 31)
+    // counts of (turn, item) pairs, of 256 sequences' items and of rows times heads are 32 bits wide
+    if (a.items < 1 || a.items >> 23 || (unsigned long long)a.items * ((unsigned long long)a.t.max_pages * PAGE / 32 + 2) >> 32 || (long long)a.rows * a.n_heads >> 31 ||
+        (long long)a.tiles * a.row_tile >> 31)
         return true;
     return !a.q || !a.c.k || !a.c.v || !a.c.ku || !a.c.vu || a.c.n_pages < 1 || (a.c.hd != 64 && a.c.hd != 128) || a.c.kv_heads < 1 || a.n_heads < 1 || a.n_heads % a.c.kv_heads ||
            a.n_heads > 65535 || a.rows < 1 || a.rows > 65535 || a.vdim < 1 || a.vdim > a.c.hd || !a.t.table || a.t.n_slots < 1 || a.t.max_pages < 1 || a.t.max_pages > (1 << 24) ||
@@ -491,11 +491,10 @@ int launch(Attn8Args& a, int pdl, cudaStream_t st) {
     if (once.first()) cudaFuncSetAttribute(attn8_kernel<D, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL);
     void* args[] = {&mk, &mv, &a};
     // at most one CTA an item more than fit the GPU: parts are rounded down but to one
-    const int units = a.positions ? a.rows : a.n_segs;
-    return launch_rows((const void*)attn8_kernel<D, NB>, dim3(a.ctas + units * a.tiles * a.c.kv_heads), dim3(L::THREADS), L::TOTAL, args, st, pdl);
+    return launch_rows((const void*)attn8_kernel<D, NB>, dim3(a.ctas + a.items), dim3(L::THREADS), L::TOTAL, args, st, pdl);
 }
 int launch(Attn8Args& a, int pdl, cudaStream_t st) {
-    if (a.row_tile == 128) return attn8_tc_launch(a, a.ctas + (a.positions ? a.rows : a.n_segs) * a.tiles * a.c.kv_heads, pdl, st);
+    if (a.row_tile == 128) return attn8_tc_launch(a, a.ctas + a.items, pdl, st);
     if (a.c.hd == 128) return a.row_tile == 8 ? launch<128, 1>(a, pdl, st) : launch<128, 2>(a, pdl, st);
     return a.row_tile == 8 ? launch<64, 1>(a, pdl, st) : launch<64, 2>(a, pdl, st);
 }
@@ -521,6 +520,7 @@ static int attn8_launch(const Attn8Args& in, int pdl, cudaStream_t st) {
             a.positions += u;
             a.slots += u;
             a.rows = n;
+            a.items = min(a.items, n * a.tiles * a.c.kv_heads);
             a.q += (size_t)u * a.n_heads * a.c.hd;
             a.out = (char*)a.out + (size_t)u * a.ldo * (a.out16 ? 2 : 4);
             if (a.gate.kind) a.gate.g += (size_t)u * a.gate.ld;

@@ -47,6 +47,8 @@ __device__ __forceinline__ int first_of(const Keys& k, int turn, int i) { return
 
 // Items of a unit: row_tile rows of (row, head of the KV head) each, of every KV head.
 __device__ __forceinline__ int row_tiles(const Attn8Args& a, const Unit& s) { return (s.rows * (a.n_heads / a.c.kv_heads) + a.row_tile - 1) / a.row_tile; }
+// Their number, as far as there is room for them; below 2^24, so that those of MAX_UNITS units fit 32 bits.
+__device__ __forceinline__ uint32_t items_of(const Attn8Args& a, const Unit& s) { return min(row_tiles(a, s) * a.c.kv_heads, a.items + 1); }
 
 // Sum of the threads' numbers up to each and over all; at least MAX_UNITS threads, `sums` has one place a warp.
 __device__ __forceinline__ uint32_t scan(uint32_t x, uint32_t* sums, uint32_t& all) {
@@ -72,7 +74,7 @@ __device__ __forceinline__ uint32_t parts_of(const Attn8Args& a, uint32_t turns,
     return turns ? max(1u, min((uint32_t)((unsigned long long)turns * a.ctas / total), (turns * a.turn + LEAST - 1) / LEAST)) : 0;
 }
 
-// All units, and the CTAs before each one's (prefix[u]) and in all (prefix[units]).
+// All units, and the CTAs before each one's (prefix[u]) and in all (prefix[units]); none where the units have more items than there is room for.
 __device__ __forceinline__ void deal_out(const Attn8Args& a, int units, Unit* list, uint32_t* prefix, uint32_t* sums) {
     const int tid = threadIdx.x;
     Unit s;
@@ -81,7 +83,11 @@ __device__ __forceinline__ void deal_out(const Attn8Args& a, int units, Unit* li
         s = unit_at(a, tid);
         list[tid] = s;
         turns = keys_of(a, s).turns;
-        items = row_tiles(a, s) * a.c.kv_heads;
+        items = items_of(a, s);
+    }
+    if (!a.positions) {      // portions that say less than they hold
+        scan(items, sums, total);
+        if (total > (uint32_t)a.items) turns = 0;
     }
     scan(turns * items, sums, total);
     const uint32_t parts = parts_of(a, turns, total);
@@ -134,8 +140,9 @@ __device__ __forceinline__ bool find_unit(const Attn8Args& a, int units, uint32_
     if (lane < units) {
         m = unit_at(a, lane);
         turns = keys_of(a, m).turns;
-        items = row_tiles(a, m) * a.c.kv_heads;
+        items = items_of(a, m);
     }
+    if (!a.positions && __reduce_add_sync(ALL, items) > (uint32_t)a.items) return false;      // portions that say less than they hold
     const uint32_t parts = parts_of(a, turns, __reduce_add_sync(ALL, turns * items)), n = parts * items;
     uint32_t end = n;
 #pragma unroll

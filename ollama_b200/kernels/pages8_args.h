@@ -63,6 +63,7 @@ struct Attn8Args {
     float scale, softcap;
     int row_tile, turn;      // query rows (of a sequence, for the heads of a KV head) and keys that are taken together: 8 or 16 and 32, 128 and 128
     int tiles;               // most row tiles of a sequence
+    int items;               // most row tiles of a launch's sequences together, times KV heads: partial results and CTAs are counted by them, since a step has long portions beside single tokens
     int ctas;                // that fit the GPU at once
     float* part_acc;         // [items + ctas][row_tile][hd]
     float2* part_ml;         // [items + ctas][row_tile] (largest score, sum)

@@ -330,14 +330,18 @@ void fill_attn(const Signature& s, Attn8Args& p, long n, long heads, PyObject* o
     p.out16 = out.scalar_type() == B16;
 }
 
-// How many query rows (of a sequence, for the heads of a KV head) and keys are taken together; returns the rows of partial results: an item's for each sequence's row tiles and KV
-// heads, and those of as many CTAs as fit the GPU.
-long tile(Attn8Args& p, int row_tile, long most_rows, long units, c10::Device dev) {
+long tiles_of(long rows, int row_tile) { return (rows + row_tile - 1) / row_tile; }
+// How many query rows (of a sequence, for the heads of a KV head) and keys are taken together.  most_rows: of a sequence; tiles: row tiles of all sequences of a launch.  Returns the
+// rows of partial results: an item's for each row tile and KV head, and those of as many CTAs as fit the GPU.
+long tile(const Signature& s, Attn8Args& p, int row_tile, long most_rows, long tiles, c10::Device dev) {
+    const long items = tiles * p.c.kv_heads;
+    if (items >= 1l << 23) refuse(s, std::to_string(items) + " row tiles of all sequences and KV heads");
     p.row_tile = row_tile;
     p.turn = row_tile == 128 ? 128 : 32;
-    p.tiles = (int)((most_rows + row_tile - 1) / row_tile);
+    p.tiles = (int)tiles_of(most_rows, row_tile);
+    p.items = (int)items;
     p.ctas = sms_of(dev) * (row_tile == 8 ? 2 : 1);
-    return (std::min<long>(units, MAX_UNITS) * p.tiles * p.c.kv_heads + p.ctas) * row_tile;
+    return (items + p.ctas) * row_tile;
 }
 
 enum { D_QKV, D_K, D_V, D_POS, D_SLOTS, D_TABLE, D_OUT, D_HEADS, D_DIM, D_VDIM, D_QN, D_KN, D_EPS, D_FREQS, D_NROT, D_SCALE, D_NCTX, D_SOFTCAP, D_CHUNK, D_WINDOW, D_KEEP, D_HEADNORM, D_VOFF, D_MSCALE,
@@ -362,7 +366,7 @@ void attn_decode8(PyObject** a) {
     fill_attn(s, t, n, heads, a[D_OUT], c, dev, Mask{a[D_VDIM], a[D_SCALE], a[D_SOFTCAP], a[D_CHUNK], a[D_WINDOW], a[D_KEEP], a[D_GATE], a[D_DIFF]});
     if (!n) return;
     few_rows(s, n);
-    const long group = heads / c.c.kv_heads, pieces = tile(t, group <= 8 ? 8 : 16, group, n, dev), nq = n * heads * hd;
+    const long group = heads / c.c.kv_heads, row_tile = group <= 8 ? 8 : 16, pieces = tile(s, t, row_tile, group, std::min<long>(n, MAX_UNITS) * tiles_of(group, row_tile), dev), nq = n * heads * hd;
     const c10::cuda::CUDAGuard guard(dev);
     const at::Tensor ws = at::empty({nq + pieces * (hd + 2)}, at::TensorOptions().dtype(F32).device(dev));      // rotated queries, partial results, their statistics
     float* w = (float*)ws.data_ptr();
@@ -405,7 +409,7 @@ bool attn_prompt8(PyObject** a) {
     for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(sizes.o); i++) {
         PyObject* e = PyTuple_GET_ITEM(sizes.o, i);
         const double rows = as_long(PyTuple_GET_ITEM(e, 0), 0), keys = as_long(PyTuple_GET_ITEM(e, 1), 0);
-        const double of16 = (double)(((long)rows * group + 15) / 16) * c.c.kv_heads, of128 = (double)(((long)rows * group + 127) / 128) * c.c.kv_heads;
+        const double of16 = (double)tiles_of((long)rows * group, 16) * c.c.kv_heads, of128 = (double)tiles_of((long)rows * group, 128) * c.c.kv_heads;
         items16 += of16;
         items128 += of128;
         keys16 += of16 * keys;
@@ -416,7 +420,14 @@ bool attn_prompt8(PyObject** a) {
     const double t16 = 9.6 + 0.08 * items16 + keys16 / 19000, t128 = 12 + 0.37 * items128 + keys128 / 11700, t_read = 10 + 0.0107 * most * std::max(1.0, ctas / sms_of(dev));
     if (m > 64 && t_read < std::min(t16, t128) && t.out16 && !((uintptr_t)t.out & 15) && !(t.diff.on && t.gate.kind)) return false;
     few_rows(s, n);
-    const long pieces = tile(t, m <= 8 ? 8 : m <= 16 || t16 <= t128 ? 16 : 128, m, po.n, dev);
+    const int row_tile = m <= 8 ? 8 : m <= 16 || t16 <= t128 ? 16 : 128;
+    long tiles = 0, batch = 0;      // of the launch with most
+    for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(sizes.o); i++) {
+        if (i % MAX_UNITS == 0) batch = 0;
+        batch += tiles_of(as_long(PyTuple_GET_ITEM(PyTuple_GET_ITEM(sizes.o, i), 0), 0) * group, row_tile);
+        tiles = std::max(tiles, batch);
+    }
+    const long pieces = tile(s, t, row_tile, m, tiles, dev);
     const c10::cuda::CUDAGuard guard(dev);
     const at::Tensor ws = at::empty({pieces * (hd + 2)}, at::TensorOptions().dtype(F32).device(dev));
     t.q = (const float*)q.data_ptr();

@@ -1,0 +1,104 @@
+"""The 8-bit paged cache in steps whose portions differ: the memory that calls take, rows that are not there, keys of little weight, and geometries beside those of
+test_pages8_gpu.py."""
+import pytest
+import torch
+
+import pages8_oracle as O
+from test_pages8_gpu import Setup, compare, i32
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def library():
+    from ollama_b200.ops import cuda as K
+    K.need("stack")
+    yield
+    assert K.gemm_status() == 0
+
+
+def numbers(s, seed=1):
+    """Every page of the cache holds numbers, in a unit in which they are about one."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    for c in (s.k, s.v):
+        c.codes.copy_(torch.randint(0, 256, c.codes.shape, generator=g, device="cuda", dtype=torch.uint8) & 0xb7)       # up to 2^-1
+        c.unit.fill_(4.0)
+
+
+def peak(f):
+    """Bytes that a call holds at its most beyond what was held before."""
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    f()
+    torch.cuda.synchronize()
+    return torch.cuda.max_memory_allocated() - before
+
+
+def portions_of(lens, at):
+    out, row = [], 0
+    for slot, (n, p) in enumerate(zip(lens, at)):
+        out.append((row, n, slot, p))
+        row += n
+    return out
+
+
+def check_rows_of(s, q, out, row, n, slot, pos, scale):
+    """``n`` rows of a portion from its first one on, against 64 bits."""
+    k, v = s.values(s.k, slot, pos + n), s.values(s.v, slot, pos + n)
+    want, moved = O.attend(q[row:row + n].double(), k, v, O.visible(torch.arange(pos, pos + n), pos + n), scale)
+    compare(out[row:row + n].view(n, s.H, s.vdim), want, moved, v.abs().max())
+
+
+def test_memory_follows_the_rows():
+    """A long portion beside single tokens: partial results of the row tiles that there are, not of the longest portion's for each."""
+    s = Setup(H=32, G=8, dim=128, norm="", n_rot=0, slots=64, n_ctx=2900)
+    numbers(s)
+    parts = portions_of([2048] + [1] * 63, [0] + [2790 + i for i in range(63)])
+    q = torch.randn(2048 + 63, 32, 128, device="cuda")
+    out, plan = torch.zeros(len(q), 32 * 128, device="cuda"), s.P.portions8(parts, s.table)
+    # tiles of 128 rows: 64 + 63 of each of the 8 KV heads, and one a CTA that fits the GPU; 130 floats a row
+    tiles = 8 * (64 + 63) + torch.cuda.get_device_properties(0).multi_processor_count
+    assert peak(lambda: s.P.attn_prompt8(q, s.k, s.v, plan, s.table, out, vdim=128, scale=0.2)) <= tiles * 128 * 130 * 4 + (1 << 20)
+    for row, n, slot, pos in (parts[1], parts[7], parts[-1], (0, 40, 0, 0)):
+        check_rows_of(s, q, out, row, n, slot, pos, 0.2)
+    at = torch.arange(2000, 2048)
+    k, v = s.values(s.k, 0, 2048), s.values(s.v, 0, 2048)
+    want, moved = O.attend(q[at].double(), k, v, O.visible(at, 2048), 0.2)
+    compare(out[at].view(48, 32, 128), want, moved, v.abs().max())
+
+
+def test_long_tables_beside_many_portions():
+    """Counts of (keys, row tiles) that fit 32 bits, where the longest portion's tiles times all portions' do not."""
+    s = Setup(H=32, G=8, dim=128, norm="", n_rot=0, slots=256, n_ctx=128)
+    numbers(s)
+    table = torch.full((256, 20000), -1, dtype=torch.int32, device="cuda")
+    table[:, :2] = s.table
+    table[0, :32] = torch.arange(32, dtype=torch.int32)
+    s.table = table
+    parts = portions_of([2048] + [1] * 255, [0] + [i % 128 for i in range(255)])
+    q = torch.randn(2048 + 255, 32, 128, device="cuda")
+    out, plan = torch.zeros(len(q), 32 * 128, device="cuda"), s.P.portions8(parts, table)
+    s.P.attn_prompt8(q, s.k, s.v, plan, table, out, vdim=128, scale=0.2)
+    s.table = table[:, :64]
+    for row, n, slot, pos in (parts[1], parts[100], parts[-1], (0, 40, 0, 0)):
+        check_rows_of(s, q, out, row, n, slot, pos, 0.2)
+
+
+@pytest.mark.parametrize("n", [257, 300])
+def test_more_portions_than_a_launch_takes(n):
+    """The largest batch of portions is not the first."""
+    s = Setup(H=8, G=2, dim=64, norm="", n_rot=0, slots=n, n_ctx=128)
+    numbers(s)
+    lens = [1 + i % 3 for i in range(256)] + [40] * (n - 256)
+    parts = portions_of(lens, [(7 * i) % (128 - m + 1) for i, m in enumerate(lens)])
+    q = torch.randn(sum(lens), 8, 64, device="cuda")
+    for rows in (n, 200):          # tiles of 128 and 16 rows, and of 8
+        out = torch.zeros(len(q), 512, device="cuda")
+        some = parts[:rows]
+        s.P.attn_prompt8(q, s.k, s.v, s.P.portions8(some, s.table), s.table, out, vdim=64, scale=0.3)
+        for row, m, slot, pos in [*some[::17], *some[-3:]]:
+            check_rows_of(s, q, out, row, m, slot, pos, 0.3)
+        end = some[-1][0] + some[-1][1]
+        assert (out[end:] == 0).all()
