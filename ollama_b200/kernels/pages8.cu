@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(THREADS, 4) append8_kernel(const __grid_consta
         float x[HELD][COLS];
         load_heads<VEC>(a, b - kv_ctas, x);
         const int pos = a.positions[b - kv_ctas];
-        if (pos < 0) return;
+        if (!has(a.t, a.slots[b - kv_ctas], pos)) return;
         query_row<VEC>(a, b - kv_ctas, pos, x, cs, red);
         return;
     }
@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(THREADS, VEC ? 6 : 4) append8_queries_kernel(c
     int pos = -1;
     for (int i = 0; i < a.n_segs; i++) {
         const int4 s = a.segs[i];
-        if ((int)blockIdx.x >= s.x && (int)blockIdx.x < s.x + s.y) pos = s.w + blockIdx.x - s.x;
+        if ((int)blockIdx.x >= s.x && (int)blockIdx.x < s.x + s.y && has(a.t, s.z, s.w + blockIdx.x - s.x)) pos = s.w + blockIdx.x - s.x;
     }
     if (pos >= 0) query_row<VEC>(a, blockIdx.x, pos, x, cs, red);
     if (behind) pdl_wait();      // the launch does not end before the one it follows

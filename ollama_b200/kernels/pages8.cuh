@@ -38,6 +38,10 @@ __device__ __forceinline__ float unit_for(float top) {
     return pow2(min(max(e, UNIT_LOW), UNIT_HIGH));
 }
 
+// Whether the table has the position.
+__device__ __forceinline__ bool has(const PageTable& t, int slot, int pos) {
+    return (unsigned)slot < (unsigned)t.n_slots && pos >= 0 && pos >> PAGE_SHIFT < t.max_pages;
+}
 // The page of a slot's positions 64 i .. 64 i + 63; -1 for a slot, a position or a page that is not there.
 __device__ __forceinline__ int page_at(const PageTable& t, int n_pages, int slot, int i) {
     if ((unsigned)slot >= (unsigned)t.n_slots || (unsigned)i >= (unsigned)t.max_pages) return -1;

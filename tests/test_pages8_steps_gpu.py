@@ -102,3 +102,21 @@ def test_more_portions_than_a_launch_takes(n):
             check_rows_of(s, q, out, row, m, slot, pos, 0.3)
         end = some[-1][0] + some[-1][1]
         assert (out[end:] == 0).all()
+
+
+def test_queries_of_rows_that_are_not_there():
+    """Rows whose slot or position the table does not have: their queries are left as they are, as those of rows that hold no token."""
+    for append in (True, False):
+        s = Setup(H=4, G=2, dim=64, norm="", slots=3, n_ctx=130)          # three pages a slot: positions up to 191
+        slots, pos = [0, 7, -1, 3, 1, 2, 2, 1], [5, 5, 6, 0, 191, 192, 2 ** 31 - 1, -1]
+        x = s.rnd(8, s.ld)
+        q = torch.full((8, 4, 64), 9.0, device="cuda")
+        before = s.k.codes.clone()
+        s.P.append8(x.cuda(), s.k, s.v, s.table, q, positions=i32(pos), slots=i32(slots), append=append, **s.prep())
+        there = [0, 4]
+        want = s.split(x, torch.tensor(pos))[0][there]
+        assert (q[there].double().cpu() - want).abs().max() <= 2.0 ** -20 * want.abs().max()
+        assert (q[[1, 2, 3, 5, 6, 7]] == 9.0).all()
+        touched = {int(s.table[0, 0]), int(s.table[1, 2])} if append else set()
+        rest = [p for p in range(len(before)) if p not in touched]
+        assert torch.equal(s.k.codes[rest], before[rest])
