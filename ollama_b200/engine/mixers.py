@@ -13,6 +13,7 @@ from .blocks import Mat, Norm, Step, WeightSource, up
 
 
 MIN_SPLIT = 128                  # keys
+READ_OUT = 256 << 20             # bytes of an 8-bit cache's values that a prompt's attention holds in 16 bits, where one sequence's are less
 
 
 def attend8(be, m, decode: bool, qkv, kc: P8.Pages8, vc: P8.Pages8, out, hd: int, buf, diff, prep: dict, mask: dict) -> int:
@@ -22,7 +23,7 @@ def attend8(be, m, decode: bool, qkv, kc: P8.Pages8, vc: P8.Pages8, out, hd: int
         P8.attn_decode8(qkv, kc, vc, m.positions, m.slots, table, out, n_ctx=be.n_ctx, diff=diff, **prep, **mask)
         return 3
     q = buf("q", heads * hd, torch.float32).view(qkv.shape[0], heads, hd)
-    portions = m.portions(table, **{k: mask[k] for k in ("window", "keep", "chunk") if k in mask})
+    portions = m.portions(table, together=READ_OUT // (4 * P8.PAGE * kc.codes.shape[1] * hd), **{k: mask[k] for k in ("window", "keep", "chunk") if k in mask})
     P8.append8(qkv, kc, vc, table, q, portions=portions, **prep)
     P8.attn_prompt8(q, kc, vc, portions, table, out, vdim=prep["vdim"], diff=diff, **mask)
     return 4

@@ -74,11 +74,11 @@ class _Meta:
         self.tokens, self.positions, self.slots, self.offs, self.segs, self.tiles, self.half_tiles = tokens, positions, slots, offs, segs, tiles, half_tiles
         self.long, self.longest = long, longest      # by window (0: none); rows of the longest portion
 
-    def portions(self, table: torch.Tensor, **mask: int) -> P8.Portions8:
-        """The portions as attention over 8-bit caches takes them, made once for each mask."""
-        key = tuple(sorted(mask.items()))
+    def portions(self, table: torch.Tensor, **how: int) -> P8.Portions8:
+        """The portions as attention over 8-bit caches takes them, made once for each mask and size."""
+        key = tuple(sorted(how.items()))
         if key not in self._portions:
-            self._portions[key] = P8.portions8(self.parts, table, **mask)
+            self._portions[key] = P8.portions8(self.parts, table, **how)
         return self._portions[key]
 
 

@@ -24,6 +24,8 @@ from .cuda import AttnPrefillArgs, CudaKernelError, _check, lib
 from .rows import NO_DIFF, NO_GATE, AttnPagedArgs, I, P
 
 PAGE = 64
+TOGETHER = 1024                  # pages: see portions8
+
 
 @dataclass(frozen=True)
 class Pages8:
@@ -61,21 +63,25 @@ class Portions8:
     per: int                         # most pages that a portion's rows go to
     longest: int                     # most rows of one
     masks: tuple[int, int, int]      # window, keep, chunk
-    sizes: tuple                     # (rows, keys that they may see) of each
-    # for attention on values that are read out first: tiles of 128 (of 64) rows, the pages that they may see, and where each portion's pages are among those
+    sizes: tuple                     # (rows, keys that they may see, group) of each
+    # for attention on values that are read out first: tiles of 128 (of 64) rows, the pages that they may see, and where each portion's pages are among those of its group;
+    # a group is what is read out together: from which tile, half tile and page to which
+    groups: tuple
     tiles: torch.Tensor              # [tiles, 4]: first row, rows, portion, position
     half_tiles: torch.Tensor
     pages: torch.Tensor              # [pages, 4]: see read8
     table: torch.Tensor              # [n, pages of a slot]
 
 
-def portions8(parts, table: torch.Tensor, *, window: int = 0, keep: int = 0, chunk: int = 0) -> Portions8:
-    """``parts``: (first row, rows, slot, position of the first row) of each portion, rows one after the other; the masks are those of the attention."""
+def portions8(parts, table: torch.Tensor, *, window: int = 0, keep: int = 0, chunk: int = 0, together: int = TOGETHER) -> Portions8:
+    """``parts``: (first row, rows, slot, position of the first row) of each portion, rows one after the other; the masks are those of the attention.  ``together``: most pages
+    that attention which reads pages out first holds as f16 values at a time (4 * 64 bytes each for every KV head and column), or those of one slot where they are more; what takes
+    more goes in passes."""
     n_slots, max_pages = table.shape
     if window < 0 or keep < 0 or chunk < 0 or (chunk and window):
         raise ValueError(f"portions8: chunk {chunk}, window {window}, keep {keep}")
-    at, slots = 0, set()
-    tiles, halves, pages, sizes = [], [], [], []
+    at, slots, most = 0, set(), max(together, max_pages)
+    tiles, halves, pages, sizes, ends, begins = [], [], [], [], [], (0, 0, 0)
     where = np.zeros((len(parts), max_pages), np.int32)
     for i, (row, n, slot, pos) in enumerate(parts):
         if n < 1 or row != at or not 0 <= slot < n_slots or pos < 0 or pos + n > max_pages * PAGE:
@@ -89,15 +95,20 @@ def portions8(parts, table: torch.Tensor, *, window: int = 0, keep: int = 0, chu
         last = (pos + n - 1) // PAGE
         first = (pos - pos % chunk if chunk else max(0, pos - window + 1) if window else 0) // 128 * 2          # tiles of 128 keys
         seen = [*range(0, min(first, -(-keep // 128) * 2) if window else 0), *range(first, last + 1)]
-        sizes.append((n, len(seen) * PAGE))
-        where[i, seen] = np.arange(len(pages), len(pages) + len(seen))
+        if len(pages) + len(seen) - begins[2] > most:      # a group ends before this portion, whose tiles are in the lists already
+            ends.append(begins := (len(tiles) - -(-n // 128), len(halves) - -(-n // 64), len(pages)))
+        sizes.append((n, len(seen) * PAGE, len(ends)))
+        where[i, seen] = np.arange(len(pages) - begins[2], len(pages) - begins[2] + len(seen))
         pages += [(slot, b, min(PAGE, pos + n - b * PAGE), 0) for b in seen]
     if not at:
         raise ValueError("portions8: no rows")
+    ends.append((len(tiles), len(halves), len(pages)))
+    groups = tuple(zip(((0, 0, 0), *ends), ends))
     lists = [np.asarray(x, np.int32) for x in (parts, tiles, halves, pages, where)]
     flat = torch.from_numpy(np.concatenate([x.reshape(-1) for x in lists])).to(table.device)
     segs, tiles, halves, pages, where = (t.view(x.shape) for t, x in zip(flat.split([x.size for x in lists]), lists))
-    return Portions8(segs, at, max((p + n - 1) // PAGE - p // PAGE + 1 for _, n, _, p in parts), max(n for n, _ in sizes), (window, keep, chunk), tuple(sizes), tiles, halves, pages, where)
+    return Portions8(segs, at, max((p + n - 1) // PAGE - p // PAGE + 1 for _, n, _, p in parts), max(n for n, _, _ in sizes), (window, keep, chunk), tuple(sizes), groups,
+                     tiles, halves, pages, where)
 
 
 _MODULE = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_pages8.so")
@@ -129,20 +140,27 @@ def attn_prompt8(q, k: Pages8, v: Pages8, portions: Portions8, table, out, *, vd
     have to be made with this call's masks."""
     here = globals()
     call = here.get("_attn_prompt8") or __getattr__("_attn_prompt8")
-    if call(q, k, v, portions, table, out, vdim=vdim, scale=scale, softcap=softcap, chunk=chunk, window=window, keep=keep, gate=gate, diff=diff, pdl=pdl):
+    mask = dict(vdim=vdim, scale=scale, softcap=softcap, chunk=chunk, window=window, keep=keep, gate=gate, diff=diff, pdl=pdl)
+    if call(q, k, v, portions, table, out, **mask):
         return
     # many rows: the pages that they may see as f16 values, for attention on tcgen05
     n, heads, hd = q.shape
-    pages, tiles = portions.pages, portions.half_tiles if diff.on else portions.tiles
-    m, kv_heads = pages.shape[0], k.codes.shape[1]
-    wide = torch.empty(2, m, kv_heads, PAGE, hd, device=q.device, dtype=torch.float16)
-    here["read8"](k, v, pages, table, wide[0], wide[1], pdl, clean=True)
-    a = AttnPrefillArgs(q.data_ptr(), wide[0].data_ptr(), wide[1].data_ptr(), out.data_ptr(), None, n, heads, kv_heads, 0, 0, 0, 0, 1, 0, scale, softcap, None, None)
-    pg = AttnPagedArgs(tiles.data_ptr(), portions.table.data_ptr(), portions.table.shape[1], chunk, vdim, out.stride(0), window, min(keep, portions.table.shape[1] * PAGE), gate, diff)
+    kv_heads, tiles, of = k.codes.shape[1], portions.half_tiles if diff.on else portions.tiles, 1 if diff.on else 0
+    try:
+        wide = torch.empty(2, max(b[2] - a[2] for a, b in portions.groups), kv_heads, PAGE, hd, device=q.device, dtype=torch.float16)
+    except torch.OutOfMemoryError:          # the other forms take more time and little memory
+        call(q, k, v, portions, table, out, read_out=False, **mask)
+        return
     f = lib().b2_attn_prefill_paged
     f.argtypes = [P, P, I, I, I, P]
-    with torch.cuda.device(q.device):
-        _check(f(C.addressof(a), C.addressof(pg), hd, tiles.shape[0], m, torch.cuda.current_stream().cuda_stream), "attn_prompt8")
+    a = AttnPrefillArgs(q.data_ptr(), wide[0].data_ptr(), wide[1].data_ptr(), out.data_ptr(), None, n, heads, kv_heads, 0, 0, 0, 0, 1, 0, scale, softcap, None, None)
+    for begin, end in portions.groups:
+        pages, some = portions.pages[begin[2]:end[2]], tiles[begin[of]:end[of]]
+        m = pages.shape[0]
+        here["read8"](k, v, pages, table, wide[0, :m], wide[1, :m], pdl, clean=True)
+        pg = AttnPagedArgs(some.data_ptr(), portions.table.data_ptr(), portions.table.shape[1], chunk, vdim, out.stride(0), window, min(keep, portions.table.shape[1] * PAGE), gate, diff)
+        with torch.cuda.device(q.device):
+            _check(f(C.addressof(a), C.addressof(pg), hd, some.shape[0], m, torch.cuda.current_stream().cuda_stream), "attn_prompt8")
 
 
 def status() -> int:

@@ -379,10 +379,10 @@ void attn_decode8(PyObject** a) {
     launched(s, f_decode(&p, &t, as_bool(a[D_PDL], false), c10::cuda::getCurrentCUDAStream(dev.index())));
 }
 
-enum { P_Q, P_K, P_V, P_PORTIONS, P_TABLE, P_OUT, P_VDIM, P_SCALE, P_SOFTCAP, P_CHUNK, P_WINDOW, P_KEEP, P_GATE, P_DIFF, P_PDL, P_N };
-Signature prompt_sig = {"attn_prompt8", 6, P_N, {"q", "k", "v", "portions", "table", "out", "vdim", "scale", "softcap", "chunk", "window", "keep", "gate", "diff", "pdl"}};
+enum { P_Q, P_K, P_V, P_PORTIONS, P_TABLE, P_OUT, P_VDIM, P_SCALE, P_SOFTCAP, P_CHUNK, P_WINDOW, P_KEEP, P_GATE, P_DIFF, P_PDL, P_READ, P_N };
+Signature prompt_sig = {"attn_prompt8", 6, P_N, {"q", "k", "v", "portions", "table", "out", "vdim", "scale", "softcap", "chunk", "window", "keep", "gate", "diff", "pdl", "read_out"}};
 
-// False: the pages are to be read out to f16 first, nothing is launched.
+// False: the pages are to be read out to f16 first, nothing is launched.  Not with read_out=False.
 bool attn_prompt8(PyObject** a) {
     const Signature& s = prompt_sig;
     for (int i = 0; i <= P_SCALE; i++) required(s, a, i);
@@ -402,10 +402,15 @@ bool attn_prompt8(PyObject** a) {
     if (tensor(s, table.o, "portions").size(1) != c.t.max_pages) refuse(s, "portions that were made with another table");
     // Estimates of three forms, us (measured with 32 heads on 8 of 128, 16 on 4, and 4 on 2 of 64, 1 and 3 sequences, 5 to 512 rows behind 0 to 30000 keys; the choice costs a
     // hundredth on the mean): 16 query rows a tile 9.6 + 0.08 for each tile of a KV head + one for each 19000 of its keys, 128 rows a tile on tcgen05 12 + 0.37 + one for each 11700,
-    // pages read out first 10 + 0.0107 a key for each time that the tiles of 128 rows and heads fill the GPU.  (32 heads on 8, in that order: 5 rows at 901 keys 12.3, 16.0, 21.4;
+    // pages read out first 10 + 0.0107 a key for each time that the tiles of 128 rows and heads fill the GPU, for each group of portions that are read out together.  (32 heads on 8, in that order: 5 rows at 901 keys 12.3, 16.0, 21.4;
     // 64 at 6144 59.8, 30.6, 77.4; 64 at 30000 230, 59.8, 333; 512 at 6144 -, 130, 84.)
     const long group = heads / c.c.kv_heads, m = po.longest * group;
-    double items16 = 0, items128 = 0, keys16 = 0, keys128 = 0, most = 0, ctas = 0;
+    double items16 = 0, items128 = 0, keys16 = 0, keys128 = 0, most = 0, ctas = 0, t_read = 0;
+    long of = 0;
+    auto group_done = [&] {
+        t_read += 10 + 0.0107 * most * std::max(1.0, ctas / sms_of(dev));
+        most = ctas = 0;
+    };
     for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(sizes.o); i++) {
         PyObject* e = PyTuple_GET_ITEM(sizes.o, i);
         const double rows = as_long(PyTuple_GET_ITEM(e, 0), 0), keys = as_long(PyTuple_GET_ITEM(e, 1), 0);
@@ -414,11 +419,16 @@ bool attn_prompt8(PyObject** a) {
         items128 += of128;
         keys16 += of16 * keys;
         keys128 += of128 * keys;
+        if (const long g = as_long(PyTuple_GET_ITEM(e, 2), 0); g != of) {
+            group_done();
+            of = g;
+        }
         most = std::max(most, keys);
         ctas += (double)(((long)rows + 127) / 128 * heads);
     }
-    const double t16 = 9.6 + 0.08 * items16 + keys16 / 19000, t128 = 12 + 0.37 * items128 + keys128 / 11700, t_read = 10 + 0.0107 * most * std::max(1.0, ctas / sms_of(dev));
-    if (m > 64 && t_read < std::min(t16, t128) && t.out16 && !((uintptr_t)t.out & 15) && !(t.diff.on && t.gate.kind)) return false;
+    group_done();
+    const double t16 = 9.6 + 0.08 * items16 + keys16 / 19000, t128 = 12 + 0.37 * items128 + keys128 / 11700;
+    if (as_bool(a[P_READ], true) && m > 64 && t_read < std::min(t16, t128) && t.out16 && !((uintptr_t)t.out & 15) && !(t.diff.on && t.gate.kind)) return false;
     few_rows(s, n);
     const int row_tile = m <= 8 ? 8 : m <= 16 || t16 <= t128 ? 16 : 128;
     long tiles = 0, batch = 0;      // of the launch with most

@@ -128,7 +128,8 @@ def predict_memory(model: Any, num_ctx: int, num_parallel: int, free: int | None
         from ..models.stack import parse_stack
         st = parse_stack(kv[f"{arch}.stack"])
         fp8 = (envconfig.kv_cache_type() or "f16").lower() == "fp8" and (envconfig.compute_dtype() or "bfloat16") != "float32"
-        read_out = st.read_out_bytes() * num_ctx if fp8 else 0           # a prompt's attention reads a layer's rows of one sequence as f16
+        # a prompt's attention reads a layer's rows of one sequence as f16; those of several no further than engine/mixers.py allows, and none where that much is not free
+        read_out = st.read_out_bytes() * (-(-num_ctx // 64) * 64) if fp8 else 0
         return size + num_parallel * (st.kv_bytes_per_token(fp8=fp8) * num_ctx + st.state_bytes()) + read_out
     layers = _first_int(kv.get(f"{arch}.block_count"))
     heads = _first_int(kv.get(f"{arch}.attention.head_count"), 1) or 1

@@ -1,0 +1,32 @@
+"""Host side of steps whose portions differ: what is read out together."""
+import numpy as np
+import torch
+
+from ollama_b200.ops import pages8 as P
+
+
+def test_groups_of_pages():
+    """Portions in order, as many as fit, tables of pages within the group; one slot's pages always do."""
+    table = torch.zeros(5, 20, dtype=torch.int32)
+    parts = [(0, 130, 1, 700), (130, 3, 0, 0), (133, 600, 4, 600), (733, 1, 2, 1200), (734, 65, 3, 0)]
+    whole = P.portions8(parts, table)
+    assert whole.groups == (((0, 0, 0), (10, 17, 54)),) and [s[2] for s in whole.sizes] == [0] * 5
+    p = P.portions8(parts, table, together=22)
+    # pages seen: 13, 1, 19, 19, 2 -> 14 | 19 | 21
+    assert [b[2] - a[2] for a, b in p.groups] == [14, 19, 21] and [s[2] for s in p.sizes] == [0, 0, 1, 2, 2]
+    assert [(s[0], s[1]) for s in p.sizes] == [(s[0], s[1]) for s in whole.sizes]
+    assert [b[0] - a[0] for a, b in p.groups] == [3, 5, 2] and [b[1] - a[1] for a, b in p.groups] == [4, 10, 3]
+    for one, other in ((p.segs, whole.segs), (p.tiles, whole.tiles), (p.half_tiles, whole.half_tiles), (p.pages, whole.pages)):
+        assert torch.equal(one, other)
+    pages = p.pages.numpy()
+    for a, b in p.groups:
+        own = pages[a[2]:b[2]]
+        assert len(own) <= 22
+        for i in sorted(set(p.tiles[a[0]:b[0], 2].tolist())):
+            slot = parts[i][2]
+            for block in own[own[:, 0] == slot][:, 1]:
+                assert own[p.table[i, block]].tolist()[:2] == [slot, block]
+    # less than a slot's pages is not asked for
+    assert [s[2] for s in P.portions8(parts, table, together=1).sizes] == [0, 0, 1, 2, 3]
+    assert max(b[2] - a[2] for a, b in P.portions8(parts, table, together=1).groups) <= 20
+    assert np.array_equal(P.portions8(parts[:1], table, together=1).table.numpy(), P.portions8(parts[:1], table).table.numpy())

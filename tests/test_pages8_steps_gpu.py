@@ -120,3 +120,37 @@ def test_queries_of_rows_that_are_not_there():
         touched = {int(s.table[0, 0]), int(s.table[1, 2])} if append else set()
         rest = [p for p in range(len(before)) if p not in touched]
         assert torch.equal(s.k.codes[rest], before[rest])
+
+
+@pytest.mark.parametrize("diff", [False, True])
+def test_pages_are_read_out_in_passes(diff):
+    """What is held in 16 bits at a time is bounded, and the results are those of one pass."""
+    from ollama_b200.ops import rows as R
+    s = Setup(H=32, G=8, dim=64 if diff else 128, vdim=128, norm="", n_rot=0, maps=2 if diff else 1, slots=3, n_ctx=1300)
+    numbers(s)
+    parts = portions_of([600, 500, 640], [600, 700, 640])
+    q, outs = torch.randn(1740, 32, 128, device="cuda"), []
+    how = dict(diff=R.DiffHeads(0.3, 0.8, 1e-5, 1)) if diff else {}
+    for together, pages in ((1024, 58), (1, 20)):
+        out, plan = torch.zeros(1740, 16 * 128 if diff else 32 * 128, device="cuda", dtype=torch.bfloat16), s.P.portions8(parts, s.table, together=together)
+        # nothing but the pages, keys and values in 16 bits
+        assert peak(lambda: s.P.attn_prompt8(q, s.k, s.v, plan, s.table, out, vdim=128, scale=0.2, **how)) <= pages * 2 * 8 * 64 * 128 * 2 + (1 << 16)
+        outs.append(out)
+    assert torch.equal(*outs) and (outs[0] != 0).any(1).all()
+
+
+def test_prompts_without_memory_to_read_pages_out(monkeypatch):
+    """The other forms take the step where an allocation fails."""
+    s = Setup(H=8, G=2, dim=64, norm="", n_rot=0, slots=2, n_ctx=700)
+    numbers(s)
+    parts = portions_of([300, 280], [300, 0])
+    q, plan = torch.randn(580, 8, 64, device="cuda"), s.P.portions8(parts, s.table)
+    out = torch.zeros(580, 512, device="cuda", dtype=torch.bfloat16)
+
+    def full(*a, **k):
+        raise torch.OutOfMemoryError("no memory")
+    with monkeypatch.context() as m:
+        m.setattr(torch, "empty", full)
+        s.P.attn_prompt8(q, s.k, s.v, plan, s.table, out, vdim=64, scale=0.2)
+    for row, n, slot, pos in parts:
+        check_rows_of(s, q, out, row, n, slot, pos, 0.2)
