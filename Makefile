@@ -19,4 +19,4 @@ bench: build
 	$(PYTHON) bench.py
 
 clean:
-	rm -rf ollama_b200/kernels/build ollama_b200/kernels/libb200ops.so ollama_b200/native/libb200host.so ollama_b200/native/devquery ollama_b200/ops/_pages8.so
+	rm -rf ollama_b200/kernels/build ollama_b200/kernels/libb200ops.so ollama_b200/native/libb200host.so ollama_b200/native/devquery ollama_b200/ops/_pages8*.so

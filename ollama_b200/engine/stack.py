@@ -102,6 +102,8 @@ class StackBackend(StepEngine):
         self.fp8 = kv_type == "fp8" and not self.f32       # heads of up to 128 columns; other layers and 32-bit models keep theirs
         if kv_type != "f16" and not self.fp8:
             logging.getLogger("ollama_b200.engine").warning("K/V cache type %s is stored as %s (the 8-bit cache of 16-bit stack models is fp8)", kv_type, "f32" if self.f32 else "f16")
+        if self.fp8:
+            P8.load()
         self._init_steps()
         self.supports_verify = not self.cfg.recurrent
         self.max_batch = MAX_DECODE_ROWS

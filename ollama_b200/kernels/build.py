@@ -8,6 +8,8 @@ source (or a header) is newer.
 from __future__ import annotations
 
 import concurrent.futures as cf
+import glob
+import hashlib
 import os
 import shutil
 import subprocess
@@ -44,6 +46,8 @@ def build_group(group: str, verbose: bool = False, force: bool = False) -> str:
     """Compile the sources of ``group`` and link them into a library of their own; their objects are the ones a later full build uses."""
     lib = os.path.join(HERE, f"libb200{group}.so")
     _compile(sorted(GROUPS[group]), lib, verbose, force)
+    if "pages8.cu" in GROUPS[group]:
+        build_calls(verbose, force)
     return lib
 
 
@@ -63,7 +67,7 @@ def _compile(srcs: list[str], lib: str, verbose: bool, force: bool) -> None:
     for s in srcs:
         src, obj = os.path.join(HERE, s), os.path.join(objdir, s[:-3] + ".o")
         if force or _stale(obj, [src] + hdrs):
-            cmd = [nvcc, *NVCC_FLAGS, "-c", src, "-o", obj] + (["-Xptxas", "-v"] if verbose else [])
+            cmd = [nvcc, *NVCC_FLAGS, *([_layout_flag()] if s == "pages8.cu" else []), "-c", src, "-o", obj] + (["-Xptxas", "-v"] if verbose else [])
             jobs.append((s, cmd))
 
     def run(job):
@@ -110,17 +114,34 @@ def build_host(verbose: bool = False, force: bool = False) -> str | None:
     return HOSTLIB
 
 
+def _text(*path: str) -> bytes:
+    with open(os.path.join(*path), "rb") as f:
+        return f.read()
+
+
+def _layout_flag() -> str:
+    """What the kernel library and the module of calls are both compiled with: a number that follows from the argument blocks that they share."""
+    return f"-DPAGES8_LAYOUT=0x{hashlib.sha256(_text(HERE, 'pages8_args.h')).hexdigest()[:16]}ull"
+
+
+def calls_path() -> str:
+    """The module of calls for this Python and torch, of the sources as they are: one that was built for others, or from others, has another name."""
+    import torch
+    ops = os.path.join(os.path.dirname(HERE), "ops")
+    made_from = hashlib.sha256(_text(ops, "pages8_call.cpp") + _text(HERE, "pages8_args.h")).hexdigest()[:12]
+    return os.path.join(ops, f"_pages8.{sys.implementation.cache_tag}-torch{torch.__version__}.{made_from}.so")
+
+
 def build_calls(verbose: bool = False, force: bool = False) -> str:
     """The Python module of calls whose arguments are checked in C++ (ops/pages8_call.cpp); needs torch's headers, no GPU."""
-    import sysconfig
+    src, out = os.path.join(os.path.dirname(HERE), "ops", "pages8_call.cpp"), calls_path()
+    if force or not os.path.exists(out):
+        import sysconfig
 
-    from torch.utils.cpp_extension import include_paths, library_paths
-    ops = os.path.join(os.path.dirname(HERE), "ops")
-    src, out = os.path.join(ops, "pages8_call.cpp"), os.path.join(ops, "_pages8.so")
-    if force or _stale(out, [src, os.path.join(HERE, "pages8_args.h")]):
+        from torch.utils.cpp_extension import include_paths, library_paths
         cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
         part = f"{out}.{os.getpid()}"
-        cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", *(f"-I{d}" for d in (*include_paths(), os.path.join(cuda, "include"), sysconfig.get_paths()["include"])),
+        cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", _layout_flag(), *(f"-I{d}" for d in (*include_paths(), os.path.join(cuda, "include"), sysconfig.get_paths()["include"])),
                "-o", part, src, *(f"-L{d}" for d in (*library_paths(), os.path.join(cuda, "lib64"))), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-lcudart"]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if verbose or r.returncode:
@@ -128,6 +149,9 @@ def build_calls(verbose: bool = False, force: bool = False) -> str:
         if r.returncode:
             raise RuntimeError("g++ failed on pages8_call.cpp")
         os.replace(part, out)
+        for old in glob.glob(glob.escape(out.rsplit(".", 2)[0]) + ".*.so"):          # of the same Python and torch
+            if old != out:
+                os.remove(old)
     return out
 
 

@@ -522,6 +522,9 @@ int append8_launch(const Append8Args& in, int pdl, cudaStream_t st) {
     return launch_rows(vec ? (const void*)append8_queries_kernel<true> : (const void*)append8_queries_kernel<false>, dim3(a->rows), dim3(THREADS), one, args, st, pdl || behind);
 }
 
+// Which argument blocks this library takes.
+B2_API unsigned long long b2_pages8_layout() { return PAGES8_LAYOUT; }
+
 // Returns a cudaError_t value, as does the entry point below.
 B2_API int b2_append8(const Append8Args* a, int pdl, cudaStream_t st) { return a ? append8_launch(*a, pdl, st) : (int)cudaErrorInvalidValue; }
 

@@ -3,6 +3,11 @@
 #include <stdint.h>
 #include <vector_types.h>
 
+// Follows from this file (kernels/build.py): the library and the calls compare theirs before the first call.
+#ifndef PAGES8_LAYOUT
+#define PAGES8_LAYOUT 0ull
+#endif
+
 // Sigmoid gate of attention results: kind 1 one number per element, 2 one per head; before the sigmoid.
 struct HeadGate {
     const float* g;          // [rows][ld]

@@ -14,7 +14,6 @@ from __future__ import annotations
 
 import ctypes as C
 import importlib.util
-import os
 from dataclasses import dataclass
 
 import numpy as np
@@ -111,18 +110,28 @@ def portions8(parts, table: torch.Tensor, *, window: int = 0, keep: int = 0, chu
                      tiles, halves, pages, where)
 
 
-_MODULE = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_pages8.so")
+def _module():
+    """The module of the calls (pages8_call.cpp), built where there is none of these sources."""
+    from ..kernels.build import build_calls
+    spec = importlib.util.spec_from_file_location("ollama_b200.ops._pages8", build_calls())
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    return m
+
+
+def _bind(m) -> None:
+    """Hands it the kernel library's entry points."""
+    try:
+        layout = lib().b2_pages8_layout
+    except AttributeError:
+        raise RuntimeError("the kernel library is older than the calls: run python -m ollama_b200.kernels.build") from None
+    layout.restype = C.c_ulonglong
+    m.bind(*(C.cast(getattr(lib(), n), C.c_void_p).value for n in ("b2_append8", "b2_attn8", "b2_decode8", "b2_read8")), CudaKernelError, layout())
 
 
 def _calls():
-    """The module of the calls (pages8_call.cpp), built where it is missing, with the kernel library's entry points."""
-    if not os.path.exists(_MODULE):
-        from ..kernels.build import build_calls
-        build_calls()
-    spec = importlib.util.spec_from_file_location("ollama_b200.ops._pages8", _MODULE)
-    m = importlib.util.module_from_spec(spec)
-    spec.loader.exec_module(m)
-    m.bind(*(C.cast(getattr(lib(), n), C.c_void_p).value for n in ("b2_append8", "b2_attn8", "b2_decode8", "b2_read8")), CudaKernelError)
+    m = _module()
+    _bind(m)
     return m
 
 
@@ -133,6 +142,12 @@ def __getattr__(name: str):
     m = _calls()
     globals().update(append8=m.append8, read8=m.read8, attn_decode8=m.attn_decode8, _attn_prompt8=m.attn_prompt8)
     return globals()[name]
+
+
+def load() -> None:
+    """Makes the calls ready, building what is missing: before a model's first step rather than in it."""
+    if "append8" not in globals():
+        __getattr__("append8")
 
 
 def attn_prompt8(q, k: Pages8, v: Pages8, portions: Portions8, table, out, *, vdim, scale, softcap=0.0, chunk=0, window=0, keep=0, gate=NO_GATE, diff=NO_DIFF, pdl=False) -> None:

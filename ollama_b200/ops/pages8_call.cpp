@@ -488,10 +488,16 @@ PyObject* py_attn_decode8(PyObject*, PyObject* const* args, Py_ssize_t n, PyObje
 PyObject* py_attn_prompt8(PyObject*, PyObject* const* args, Py_ssize_t n, PyObject* kw) {
     return called<prompt_sig>([](PyObject** a) { return PyBool_FromLong(attn_prompt8(a)); }, args, n, kw);
 }
-// bind(append, attn, decode, read, exception): addresses of the kernel library's entry points, and what a failing launch raises
+// bind(append, attn, decode, read, exception, layout): addresses of the kernel library's entry points, what a failing launch raises, and which argument blocks the library takes
 PyObject* py_bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
-    if (n != 5) {
-        PyErr_SetString(PyExc_TypeError, "bind() takes 5 arguments");
+    if (n != 6) {
+        PyErr_SetString(PyExc_TypeError, "bind() takes 6 arguments");
+        return nullptr;
+    }
+    const unsigned long long layout = PyLong_AsUnsignedLongLong(args[5]);
+    if (layout == (unsigned long long)-1 && PyErr_Occurred()) return nullptr;
+    if (layout != PAGES8_LAYOUT) {
+        PyErr_SetString(PyExc_RuntimeError, "the kernel library was built from another pages8_args.h than the calls: run python -m ollama_b200.kernels.build");
         return nullptr;
     }
     void* f[4];

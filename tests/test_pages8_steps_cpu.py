@@ -1,5 +1,6 @@
 """Host side of steps whose portions differ: what is read out together."""
 import numpy as np
+import pytest
 import torch
 
 from ollama_b200.ops import pages8 as P
@@ -30,3 +31,40 @@ def test_groups_of_pages():
     assert [s[2] for s in P.portions8(parts, table, together=1).sizes] == [0, 0, 1, 2, 3]
     assert max(b[2] - a[2] for a, b in P.portions8(parts, table, together=1).groups) <= 20
     assert np.array_equal(P.portions8(parts[:1], table, together=1).table.numpy(), P.portions8(parts[:1], table).table.numpy())
+
+
+def test_calls_and_kernels_of_other_sources_are_refused(monkeypatch):
+    """The module is the one of these sources, this Python and this torch; it takes a kernel library with the same argument blocks alone."""
+    from ollama_b200.kernels import build as B
+    from ollama_b200.ops.cuda import lib
+    path, text = B.calls_path(), B._text
+    for name in ("pages8_args.h", "pages8_call.cpp"):
+        with monkeypatch.context() as m:
+            m.setattr(B, "_text", lambda *p: text(*p) + (b" " if p[-1] == name else b""))
+            assert B.calls_path() != path and (B._layout_flag() != f"-DPAGES8_LAYOUT=0x{_layout(lib()):016x}ull") == (name == "pages8_args.h")
+    with monkeypatch.context() as m:
+        m.setattr(torch, "__version__", "1.0")
+        assert B.calls_path() != path
+    assert B._layout_flag() == f"-DPAGES8_LAYOUT=0x{_layout(lib()):016x}ull"
+    P.load()
+    m = P._module()
+    for wrong in (0, _layout(lib()) + 1):
+        with pytest.raises(RuntimeError, match="pages8_args.h"):
+            m.bind(1, 2, 3, 4, ValueError, wrong)
+    P._bind(m)
+
+
+def _layout(library):
+    import ctypes
+    library.b2_pages8_layout.restype = ctypes.c_ulonglong
+    return library.b2_pages8_layout()
+
+
+def test_a_part_of_the_library_comes_with_its_calls(monkeypatch, tmp_path):
+    """What a first start compiles for stack models has the module of calls too."""
+    from ollama_b200.kernels import build as B
+    built = []
+    monkeypatch.setattr(B, "_compile", lambda srcs, lib, *a: built.append(lib))
+    monkeypatch.setattr(B, "build_calls", lambda *a: built.append("calls"))
+    B.build_group("stack")
+    assert built[-1] == "calls" and len(built) == 2
