@@ -745,7 +745,7 @@ template <int D, int NS>
 int launch_paged(const AttnDecodeArgs& a, const AttnRopeArgs& r, int nb, int pdl, cudaStream_t st) {
     constexpr int SMEM = (ROWS + 2 * NS * BN) * (D + PAD) * 2;
     const void* fn = (const void*)attn_decode_paged_kernel<D, NS>;
-    static PerDeviceOnce once;
+    static thread_local PerDeviceOnce once;
     if (once.first()) cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     return start(fn, SMEM, a, r, nb, -1, pdl, st);
 }
@@ -759,7 +759,7 @@ int launch_flat(const AttnDecodeArgs& a, const AttnRopeArgs& r, int nb, int pdl,
     int smem = RINGS > MERGE ? RINGS : MERGE;
     if (raw > smem) smem = raw;
     const void* fn = (const void*)attn_decode_flat_kernel<D, NS, Q8>;
-    static PerDeviceOnce once;
+    static thread_local PerDeviceOnce once;
     if (once.first()) cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (RINGS > MERGE ? RINGS : MERGE) + (ROWS + 2) * D * 4);
     // Launches of more CTAs than fit at once deal the positions out to as many as do; MHA steps that have more sequences and heads than that keep about two a sequence.
     const int per_sm = 228 * 1024 / (smem + 3 * 1024), fit = per_sm * sm_count() / a.n_kv_heads;

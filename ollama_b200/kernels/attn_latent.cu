@@ -237,7 +237,7 @@ template <int MT, int NU, int KQ>
 int launch(const LatentAttnArgs& a, int n, int pdl, cudaStream_t st) {
     const size_t smem = Lay<MT>::bytes(a.w);
     if (smem > SMEM_MAX) return (int)cudaErrorNotSupported;
-    static PerDeviceOnce once;
+    static thread_local PerDeviceOnce once;
     if (once.first()) cudaFuncSetAttribute(attn_latent_kernel<MT, NU, KQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_MAX);
     LatentAttnArgs c = a;
     void* args[] = {&c};

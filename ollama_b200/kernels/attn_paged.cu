@@ -283,7 +283,7 @@ B2_API int b2_paged_append(const PagedAppendArgs* a, int rows, int pdl, cudaStre
         return (int)cudaErrorInvalidValue;
     const size_t smem = ((size_t)a->n_heads * a->dim + (a->no_append ? 0 : (size_t)a->n_kv_heads * kdim) + a->n_rot) * 4;
     if (smem > 200 * 1024) return (int)cudaErrorNotSupported;
-    static PerDeviceOnce once;
+    static thread_local PerDeviceOnce once;
     if (once.first()) {
         cudaFuncSetAttribute(paged_append_kernel<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
         cudaFuncSetAttribute(paged_append_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);

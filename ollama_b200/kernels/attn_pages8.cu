@@ -487,7 +487,7 @@ int launch(Attn8Args& a, int pdl, cudaStream_t st) {
     CUtensorMap mk, mv;
     const size_t rows = (size_t)a.c.n_pages * a.c.kv_heads * PAGE;
     if (!code_map<D>(&mk, a.c.k, rows) || !code_map<D>(&mv, a.c.v, rows)) return (int)cudaErrorNotSupported;
-    static PerDeviceOnce once;
+    static thread_local PerDeviceOnce once;
     if (once.first()) cudaFuncSetAttribute(attn8_kernel<D, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL);
     void* args[] = {&mk, &mv, &a};
     // at most one CTA an item more than fit the GPU: parts are rounded down but to one
@@ -503,7 +503,7 @@ int launch(Attn8Args& a, int pdl, cudaStream_t st) {
 
 static int attn8_launch(const Attn8Args& in, int pdl, cudaStream_t st) {
     if (bad_args(in)) return (int)cudaErrorInvalidValue;
-    static PerDeviceOnce once;      // an SM that is set for less shared memory takes the attention kernel's CTAs only when it is empty
+    static thread_local PerDeviceOnce once;      // an SM that is set for less shared memory takes the attention kernel's CTAs only when it is empty
     if (once.first()) {
         cudaFuncSetAttribute(attn8_merge_kernel<1>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
         cudaFuncSetAttribute(attn8_merge_kernel<2>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);

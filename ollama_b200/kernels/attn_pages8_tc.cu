@@ -401,7 +401,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn8_tc_kernel(const __grid_const
 
 template <int D>
 int launch(Attn8Args& a, int grid, int pdl, cudaStream_t st) {
-    static PerDeviceOnce once;
+    static thread_local PerDeviceOnce once;
     if (once.first()) cudaFuncSetAttribute(attn8_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay<D>::TOTAL);
     void* args[] = {&a};
     return launch_rows((const void*)attn8_tc_kernel<D>, dim3(grid), dim3(THREADS), Lay<D>::TOTAL, args, st, pdl);

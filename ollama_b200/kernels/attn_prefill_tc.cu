@@ -903,7 +903,7 @@ int launch(const AttnPrefillArgs& a, int n_slots, cudaStream_t st) {
     CUtensorMap mk, mv;
     const size_t rows = (size_t)n_slots * a.Hkv * a.n_ctx;
     if (!cached_kv_map(&mk, a.k_cache, rows, D) || !cached_kv_map(&mv, a.v_cache, rows, D)) return (int)cudaErrorNotSupported;
-    static PerDeviceOnce once;
+    static thread_local PerDeviceOnce once;
     if (once.first()) cudaFuncSetAttribute(attn_prefill_tc_kernel<D, PT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay<D>::TOTAL);
     dim3 grid((a.T + BQ - 1) / BQ, a.H);
     attn_prefill_tc_kernel<D, PT><<<grid, THREADS, Lay<D>::TOTAL, st>>>(mk, mv, a);
@@ -967,7 +967,7 @@ template <int D>
 int launch2(const AttnPrefillArgs& a, int heads, size_t rows, int pdl, cudaStream_t st) {
     CUtensorMap mk, mv;
     if (!cached_kv_map(&mk, a.k_cache, rows, D) || !cached_kv_map(&mv, a.v_cache, rows, D)) return (int)cudaErrorNotSupported;
-    static PerDeviceOnce once;
+    static thread_local PerDeviceOnce once;
     if (once.first()) cudaFuncSetAttribute(attn_prefill_tc2_kernel<D, D, FLAT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay2<D, D>::TOTAL);
     dim3 grid((a.T + BQ - 1) / BQ, heads);
     AttnPrefillArgs copy = a;
@@ -993,7 +993,7 @@ int launch_paged(const AttnPrefillArgs& a, const AttnPagedArgs& pg, int n_tiles,
     CUtensorMap mk, mv;
     const size_t rows = (size_t)n_pages * a.Hkv * 64;
     if (!cached_kv_map(&mk, a.k_cache, rows, D, 64) || !cached_kv_map(&mv, a.v_cache, rows, D, 64)) return (int)cudaErrorNotSupported;
-    static PerDeviceOnce once;
+    static thread_local PerDeviceOnce once;
     if (once.first()) cudaFuncSetAttribute(attn_prefill_tc2_kernel<D, D, PAGED_CACHE, DIFF>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay2<D, D>::TOTAL);
     AttnPrefillArgs copy = a;
     const float qsign = positive_scale(copy);
@@ -1006,7 +1006,7 @@ int launch_parts(const AttnPartsArgs& p, int n_tiles, cudaStream_t st) {
     CUtensorMap mk, ms;
     if (!make_kv_map(&mk, p.kv, p.n_rows, p.H * (p.dp + p.vp), BKV) || !make_kv_map(&ms, p.rp ? p.shared : p.kv, p.n_rows, p.rp ? p.rp : p.H * (p.dp + p.vp), BKV))
         return (int)cudaErrorNotSupported;
-    static PerDeviceOnce once;
+    static thread_local PerDeviceOnce once;
     if (once.first()) cudaFuncSetAttribute(attn_prefill_tc2_kernel<D, DK, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay2<D, DK>::TOTAL);
     AttnPrefillArgs a{};
     a.H = a.Hkv = p.H;

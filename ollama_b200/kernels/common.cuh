@@ -33,7 +33,8 @@ struct WDesc {
     int out_off;         // column offset of this segment in the output row
 };
 
-// Function attributes (dynamic shared memory opt-in) are per device: first() is true once per device and call site.
+// Function attributes (dynamic shared memory opt-in) are per device: first() is true once per device, thread and call site, whose variable is thread_local.  Each thread sets them
+// before its own first launch: one that took another thread's word for it launched before the other had set them, and failed.
 struct PerDeviceOnce {
     bool done[64] = {};
     bool first() {

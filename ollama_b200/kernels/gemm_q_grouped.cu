@@ -262,7 +262,7 @@ B2_API int b2_gemm_q_grouped(const void* x, int m, const WDesc* w, int experts, 
     const int scale_pitch = ((w->k >> 5) + 3) & ~3;
     const int smem = STAGES * (A_BYTES + B_BYTES) + RING_BYTES + 128 + 128 * scale_pitch + 1024;
     if (smem > 227 * 1024) return (int)cudaErrorNotSupported;
-    static PerDeviceOnce once;
+    static thread_local PerDeviceOnce once;
     if (once.first()) cudaFuncSetAttribute(gemm_q_grouped_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
     QGroupedParams p{*w, m, tile_expert, out, ldo, bias, glu_act_id >= 0 ? 1 + glu_act_id : 0, alpha, limit, scale_pitch};
     dim3 grid((w->n + BN - 1) / BN, m / BM);

@@ -870,7 +870,7 @@ B2_API int b2_gemm_sk(const SgArgs* in, int max_ctas, int pdl, cudaStream_t st) 
     a.ring = (slots < SG_W_SLOTS ? (int)slots : SG_W_SLOTS) & ~1;
     const size_t smem = fixed + a.x_slots * chunk + a.ring * item;
     const void* fn = nt == 1 ? (const void*)gemm_sk_kernel<1> : nt == 2 ? (const void*)gemm_sk_kernel<2> : nt == 3 ? (const void*)gemm_sk_kernel<3> : (const void*)gemm_sk_kernel<4>;
-    static PerDeviceOnce once[SG_MAX_NT];
+    static thread_local PerDeviceOnce once[SG_MAX_NT];
     if (once[nt - 1].first()) {
         const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, SG_MAX_SMEM);
         if (e != cudaSuccess) return (int)e;

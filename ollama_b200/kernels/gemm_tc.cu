@@ -413,7 +413,7 @@ int launch(const void* a, const void* b, const GemmParams& p, cudaStream_t st, i
     CUtensorMap ma, mb;
     if (!make_map(&ma, a, p.m, p.k, BM, p.lda) || !make_map(&mb, b, b_rows ? b_rows : p.n, p.k, L::B_ROWS)) return (int)cudaErrorNotSupported;
     const void* fn = (const void*)gemm_bf16_tc_kernel<BN, SPLIT, TAIL, XIELU, PAIR>;
-    static PerDeviceOnce once;
+    static thread_local PerDeviceOnce once;
     if (once.first()) cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL);
     const int total = ((p.m + TM - 1) / TM) * ((p.n + BN - 1) / BN) * (SPLIT ? p.splits : 1), units = PAIR ? sm_count() / 2 : sm_count();
     cudaLaunchConfig_t cfg = {};

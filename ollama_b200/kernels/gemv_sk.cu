@@ -988,7 +988,7 @@ cudaError_t launch(const void* fn, dim3 grid, dim3 block, size_t smem, void** ar
     return cudaLaunchKernelExC(&cfg, fn, args);
 }
 
-PerDeviceOnce g_attr[16];
+thread_local PerDeviceOnce g_attr[16];
 
 }  // namespace
 

@@ -391,7 +391,7 @@ template <int R>
 int launch(const MoeFp4Args& a, int max_chunks, int pdl, cudaStream_t st) {
     const int smem = 1024 + STAGES * (A_BYTES + x_step_bytes(R) + 2 * SF_BYTES) + 128 * (a.k >> 5);
     if (smem > MAX_SMEM) return (int)cudaErrorNotSupported;
-    static PerDeviceOnce once;
+    static thread_local PerDeviceOnce once;
     if (once.first()) cudaFuncSetAttribute(moe_fp4_kernel<R>, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SMEM);
     // No more shared memory than the CTAs need (1 KB each of static and of reserved memory): the rest is the L1 that the loads under way live in.  Left to itself the SM keeps the
     // split of a kernel before it: 16 tokens behind a GEMM of 200 KB took 173 us instead of 109.

@@ -487,7 +487,7 @@ int append8_launch(const Append8Args& in, int pdl, cudaStream_t st) {
     const size_t one = 2 * sizeof(float) * (pitch ? pitch : 4);      // cosines and sines of a row
     Append8Args copy = *a;
     if (a->positions) {
-        static PerDeviceOnce once;      // an SM that is set for less shared memory takes the CTAs of the attention behind this launch only when it is empty
+        static thread_local PerDeviceOnce once;      // an SM that is set for less shared memory takes the CTAs of the attention behind this launch only when it is empty
         if (once.first()) {
             cudaFuncSetAttribute(append8_kernel<true>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
             cudaFuncSetAttribute(append8_kernel<false>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);

@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(32 * MT * Lay<MT, NP>::SP, 1) ssd_chunk_kernel
 template <int MT, int NP>
 int launch(const SsdArgs& a, int n_seg, int pdl, cudaStream_t st) {
     using L = Lay<MT, NP>;
-    static PerDeviceOnce once;
+    static thread_local PerDeviceOnce once;
     if (once.first()) cudaFuncSetAttribute(ssd_chunk_kernel<MT, NP>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL);
     SsdArgs c = a;
     void* args[] = {&c};

@@ -154,3 +154,29 @@ def test_prompts_without_memory_to_read_pages_out(monkeypatch):
         s.P.attn_prompt8(q, s.k, s.v, plan, s.table, out, vdim=64, scale=0.2)
     for row, n, slot, pos in parts:
         check_rows_of(s, q, out, row, n, slot, pos, 0.2)
+
+
+def test_calls_from_several_threads():
+    """Each on a stream and a cache of its own."""
+    import threading
+    wrong = []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                s = Setup(H=8, G=2, dim=64, slots=2, n_ctx=400, seed=i)
+                numbers(s, i)
+                q = torch.randn(300, 8, 64, device="cuda")
+                for _ in range(20):
+                    for n, dtype in ((300, torch.bfloat16), (60, torch.float32), (2, torch.float32)):
+                        out = torch.zeros(n, 512, device="cuda", dtype=dtype)
+                        s.P.attn_prompt8(q[:n], s.k, s.v, s.P.portions8([(0, n, 1, 40)], s.table), s.table, out, vdim=64, scale=0.2)
+                        check_rows_of(s, q, out, 0, n, 1, 40, 0.2)
+        except BaseException as e:
+            wrong.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong
