@@ -195,6 +195,19 @@ void launched(const Signature& s, int rc) {
     PyErr_Format(kernel_error, "%s failed with CUDA error %d", s.name, rc);
     throw Raised();
 }
+// Other threads run while memory is found and kernels are launched: either may have to wait, for blocks that are given back or for room in the launch queue.  What the call holds
+// (its arguments, which the caller holds) stays.
+struct Unlocked {
+    PyThreadState* state = PyEval_SaveThread();
+    ~Unlocked() { PyEval_RestoreThread(state); }
+};
+template <typename F>
+int unlocked(c10::Device dev, F launch) {
+    const Unlocked lock;
+    const c10::cuda::CUDAGuard guard(dev);
+    return launch(c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+}
+at::Tensor floats(c10::Device dev, long n) { return at::empty({n}, at::TensorOptions().dtype(F32).device(dev)); }
 int sms_of(c10::Device dev) {
     static int sms[64] = {};
     int& n = sms[dev.index() & 63];
@@ -277,9 +290,9 @@ void append8(PyObject** a) {
         p.slots = (const int*)shaped(s, a[A_SLOTS], "slots", I32, dev, n).data_ptr();
         p.per = 1;
     }
+    const bool pdl = as_bool(a[A_PDL], false);
     if (!n) return;
-    const c10::cuda::CUDAGuard guard(dev);
-    launched(s, f_append(&p, as_bool(a[A_PDL], false), c10::cuda::getCurrentCUDAStream(dev.index())));
+    launched(s, unlocked(dev, [&](cudaStream_t st) { return f_append(&p, pdl, st); }));
 }
 
 // ---- read8 ----------------------------------------------------------------------------------------------------------------------
@@ -296,9 +309,9 @@ void read8(PyObject** a) {
     wide(s, shaped(s, a[R_PAGES], "pages", I32, dev, n, 4), "pages");
     const at::Tensor &ko = wide(s, shaped(s, a[R_KOUT], "k_out", F16, dev, n, c.c.kv_heads, PAGE, c.c.hd), "k_out"),
                      &vo = wide(s, shaped(s, a[R_VOUT], "v_out", F16, dev, n, c.c.kv_heads, PAGE, c.c.hd), "v_out");
+    const bool clean = as_bool(a[R_CLEAN], false), pdl = as_bool(a[R_PDL], false);
     if (!n) return;
-    const c10::cuda::CUDAGuard guard(dev);
-    launched(s, f_read(&c.c, &c.t, pages.data_ptr(), n, ko.data_ptr(), vo.data_ptr(), as_bool(a[R_CLEAN], false), as_bool(a[R_PDL], false), c10::cuda::getCurrentCUDAStream(dev.index())));
+    launched(s, unlocked(dev, [&](cudaStream_t st) { return f_read(&c.c, &c.t, pages.data_ptr(), n, ko.data_ptr(), vo.data_ptr(), clean, pdl, st); }));
 }
 
 // ---- attention ------------------------------------------------------------------------------------------------------------------
@@ -367,16 +380,18 @@ void attn_decode8(PyObject** a) {
     if (!n) return;
     few_rows(s, n);
     const long group = heads / c.c.kv_heads, row_tile = group <= 8 ? 8 : 16, pieces = tile(s, t, row_tile, group, std::min<long>(n, MAX_UNITS) * tiles_of(group, row_tile), dev), nq = n * heads * hd;
-    const c10::cuda::CUDAGuard guard(dev);
-    const at::Tensor ws = at::empty({nq + pieces * (hd + 2)}, at::TensorOptions().dtype(F32).device(dev));      // rotated queries, partial results, their statistics
-    float* w = (float*)ws.data_ptr();
-    p.q_out = w;
-    t.q = w;
     t.positions = p.positions;
     t.slots = p.slots;
-    t.part_acc = w + nq;
-    t.part_ml = (float2*)(w + nq + pieces * hd);
-    launched(s, f_decode(&p, &t, as_bool(a[D_PDL], false), c10::cuda::getCurrentCUDAStream(dev.index())));
+    const bool pdl = as_bool(a[D_PDL], false);
+    launched(s, unlocked(dev, [&](cudaStream_t st) {
+        const at::Tensor ws = floats(dev, nq + pieces * (hd + 2));      // rotated queries, partial results, their statistics
+        float* w = (float*)ws.data_ptr();
+        p.q_out = w;
+        t.q = w;
+        t.part_acc = w + nq;
+        t.part_ml = (float2*)(w + nq + pieces * hd);
+        return f_decode(&p, &t, pdl, st);
+    }));
 }
 
 enum { P_Q, P_K, P_V, P_PORTIONS, P_TABLE, P_OUT, P_VDIM, P_SCALE, P_SOFTCAP, P_CHUNK, P_WINDOW, P_KEEP, P_GATE, P_DIFF, P_PDL, P_READ, P_N };
@@ -438,14 +453,16 @@ bool attn_prompt8(PyObject** a) {
         tiles = std::max(tiles, batch);
     }
     const long pieces = tile(s, t, row_tile, m, tiles, dev);
-    const c10::cuda::CUDAGuard guard(dev);
-    const at::Tensor ws = at::empty({pieces * (hd + 2)}, at::TensorOptions().dtype(F32).device(dev));
     t.q = (const float*)q.data_ptr();
     t.segs = po.segs;
     t.n_segs = po.n;
-    t.part_acc = (float*)ws.data_ptr();
-    t.part_ml = (float2*)(t.part_acc + pieces * hd);
-    launched(s, f_attn(&t, as_bool(a[P_PDL], false), c10::cuda::getCurrentCUDAStream(dev.index())));
+    const bool pdl = as_bool(a[P_PDL], false);
+    launched(s, unlocked(dev, [&](cudaStream_t st) {
+        const at::Tensor ws = floats(dev, pieces * (hd + 2));
+        t.part_acc = (float*)ws.data_ptr();
+        t.part_ml = (float2*)(t.part_acc + pieces * hd);
+        return f_attn(&t, pdl, st);
+    }));
     return true;
 }
 

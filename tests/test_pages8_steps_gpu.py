@@ -156,6 +156,43 @@ def test_prompts_without_memory_to_read_pages_out(monkeypatch):
         check_rows_of(s, q, out, row, n, slot, pos, 0.2)
 
 
+def test_other_threads_run_while_a_call_launches(tmp_path):
+    """A launch that has to wait holds up its own thread alone.  The entry points are one that sleeps, and launches nothing."""
+    import ctypes
+    import subprocess
+    import threading
+    import time
+    from ollama_b200.ops import pages8 as P
+    src = tmp_path / "wait.c"
+    src.write_text("#include <unistd.h>\nint wait_a_little(void) { usleep(300000); return 0; }\n")
+    subprocess.run(["g++", "-x", "c", "-shared", "-fPIC", "-o", str(tmp_path / "wait.so"), str(src)], check=True)
+    wait = ctypes.CDLL(str(tmp_path / "wait.so")).wait_a_little
+    s = Setup(H=4, G=2, dim=64)
+    x, q, out, prep = s.rnd(2, s.ld).cuda(), torch.empty(2, 4, 64, device="cuda"), torch.empty(2, 256, device="cuda"), s.prep()
+    plan, pages, wide = P.portions8([(0, 2, 0, 0)], s.table), i32([[0, 0, 64, 0]]), [torch.zeros(1, 2, 64, 64, device="cuda", dtype=torch.float16) for _ in range(2)]
+    P.load()
+    m, at, stop, ticks = P._module(), ctypes.cast(wait, ctypes.c_void_p).value, threading.Event(), []
+    layout = P.lib().b2_pages8_layout()
+
+    def count():
+        while not stop.wait(0.002):
+            ticks.append(time.perf_counter())
+    t = threading.Thread(target=count)
+    m.bind(at, at, at, at, ValueError, layout)
+    t.start()
+    try:
+        for call in (lambda: P.append8(x, s.k, s.v, s.table, q, portions=plan, **prep), lambda: P.read8(s.k, s.v, pages, s.table, *wide),
+                     lambda: P.attn_decode8(x, s.k, s.v, i32([0, 0]), i32([0, 1]), s.table, out, n_ctx=64, scale=0.1, **prep),
+                     lambda: P.attn_prompt8(q, s.k, s.v, plan, s.table, out, vdim=64, scale=0.1)):
+            before = len(ticks)
+            call()
+            assert len(ticks) - before > 20          # of some 150
+    finally:
+        stop.set()
+        t.join()
+        P._bind(m)
+
+
 def test_calls_from_several_threads():
     """Each on a stream and a cache of its own."""
     import threading
