@@ -100,6 +100,7 @@ class StackBackend(StepEngine):
         self.act_dtype = torch.float32 if self.f32 else torch.bfloat16
         kv_type = (getattr(opts, "kv_cache_type", None) or "f16").lower()
         self.fp8 = kv_type == "fp8" and not self.f32       # heads of up to 128 columns; other layers and 32-bit models keep theirs
+        self.pages8 = False                                # whether a layer has them so
         if kv_type != "f16" and not self.fp8:
             logging.getLogger("ollama_b200.engine").warning("K/V cache type %s is stored as %s (the 8-bit cache of 16-bit stack models is fp8)", kv_type, "f32" if self.f32 else "f16")
         if self.fp8:
@@ -293,6 +294,9 @@ class StackBackend(StepEngine):
                 self.mem.append((add(L.mixer.kv_heads, L.dk, kv_dt), add(L.mixer.kv_heads, L.dv, kv_dt)))
             else:
                 self.mem.append((self.cache.add_state(L.inner, L.mixer.state), self.cache.add_state(max(L.mixer.conv - 1, 1), L.inner)))
+        self.pages8 = any(isinstance(t, P8.Pages8) for mem in self.mem for t in mem)
+        if self.fp8 and not self.pages8:
+            logging.getLogger("ollama_b200.engine").warning("K/V cache type fp8 changes nothing: no layer of the model has attention heads of up to 128 columns")
         MB, i32 = self.max_batch, torch.int32
         b = self.buf = _Layer()
         b.rows = _Rows(MB, dev)
@@ -549,7 +553,7 @@ class StackBackend(StepEngine):
     def _forward_rows(self, segs: Sequence[tuple[int, Sequence[int], int]], x=None, embeds=None, spans=(), tap=None) -> torch.Tensor:
         """Rows of several sequences, each portion ``(slot, tokens, position of the first)``; returns the hidden rows in order."""
         dev = self.device
-        if self.fp8 and len({s for s, _, _ in segs}) < len(segs):
+        if self.pages8 and len({s for s, _, _ in segs}) < len(segs):
             raise ValueError("two portions of one slot in a step on an 8-bit cache")      # a page's unit follows from all its new rows
         self._reserve([s for s, _, _ in segs], [p0 + len(t) for _, t, p0 in segs])
         total = sum(len(t) for _, t, _ in segs)

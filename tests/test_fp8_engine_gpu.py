@@ -1,0 +1,29 @@
+"""Stack models under OLLAMA_KV_CACHE_TYPE=fp8: models that it does not reach, what a step counts, requests side by side."""
+import logging
+
+import pytest
+import torch
+
+import kavenex_models as KM
+import vazatar_models as VM
+from test_fp8_cache_gpu import engine
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("model", ["latents", "wide"])
+def test_models_without_8_bit_pages_run_as_they_did(model, tmp_path, caplog):
+    """Latent rows and wide heads stay in 16 bits: a step of two portions of one slot is taken, its results are those of the other cache type, and the log says that nothing changed."""
+    if model == "latents":
+        M, cfg = KM, KM.config([KM.layer(KM.dense()), KM.layer(), KM.layer(KM.dense(40))])
+    else:
+        M, cfg = VM, VM.config([VM.attention(heads=2, kv_heads=1, dim=160, vdim=200, size=0, rot={}, scale=0.05, ff=33)], width=37, vocab=59, loop=None)
+    path = M.write(tmp_path, cfg, M.weights(cfg, 3))
+    toks, got = M.tokens(20, cfg["vocab"], 5), []
+    for kv in ("f16", "fp8"):
+        with caplog.at_level(logging.WARNING, "ollama_b200.engine"):
+            be = engine(path, kv=kv)
+        got.append(be.step([(1, toks[:12], 0), (1, toks[12:], 12)], [range(12), range(8)]))
+        be.close()
+    assert torch.equal(*got)
+    assert [r.getMessage().split(":")[0] for r in caplog.records] == ["K/V cache type fp8 changes nothing"]
