@@ -79,7 +79,7 @@ class B200Backend(StepEngine):
         otherwise each matrix is expanded into scratch right before its GEMM).  ``prefill_gemm``: "bf16" (expand, then the
         bf16 tensor-core GEMM) or "fused" (weights expanded inside the GEMM kernel; no 16-bit copy anywhere).
         ``kv_type``: "f16" or "q8_0" (int8 values with one f16 scale per 32 dims, written by the rope kernel and expanded
-        inside the attention kernels; "q4_0" and "fp8", the 8-bit cache of stack models, are served as q8_0); default: ``opts.kv_cache_type``
+        inside the attention kernels; "q4_0" is served as q8_0); default: ``opts.kv_cache_type``
         (envconfig/config.go:183 OLLAMA_KV_CACHE_TYPE).  ``layers`` = (lo, hi): this object is one stage of a layer
         pipeline and holds blocks lo..hi-1 only; the first stage also holds the embedding, the last one the output
         norm and head, and the residual stream enters / leaves through ``buf.x`` (decode) or the ``x`` argument (prefill).
@@ -95,15 +95,15 @@ class B200Backend(StepEngine):
             raise ValueError(f"layer range {layers} outside 0..{self.cfg.n_layers}")
         self.first, self.last = self.l_lo == 0, self.l_hi == self.cfg.n_layers
         kv_type = (kv_type or getattr(opts, "kv_cache_type", None) or "f16").lower()
-        if kv_type not in ("f16", "q8_0", "q4_0", "fp8"):
-            raise ValueError(f"unknown K/V cache type {kv_type!r}")
+        if kv_type not in ("f16", "q8_0", "q4_0"):
+            raise ValueError("K/V cache type 'fp8' is for stack models: this model's caches are f16 or q8_0" if kv_type == "fp8" else f"unknown K/V cache type {kv_type!r}")
         # quantised blocks cover 32 dims; head sizes outside the flash-attention kernel read the cache through torch
         self.kv_q8 = kv_type != "f16" and self.cfg.head_dim % 32 == 0 and self.cfg.head_dim in K.ATTN_PREFILL_HEAD_DIMS
         self.kv_type = "q8_0" if self.kv_q8 else "f16"
         if kv_type != self.kv_type:       # say so: the cache costs what the stored encoding costs, not what was asked for
             import logging
             logging.getLogger("ollama_b200.engine").warning("K/V cache type %s is stored as %s (%s)", kv_type, self.kv_type,
-                                                            "the other encodings of these caches are f16 and q8_0" if self.kv_q8 else "this head size has no quantised cache")
+                                                            "there is no 4-bit cache encoding" if self.kv_q8 else "this head size has no quantised cache")
         if keep_bf16 is None:
             c = self.cfg
             est = 2 * (c.n_layers * (c.d_model * (2 * c.q_dim + 2 * c.kv_dim) + 3 * c.d_model * c.d_ff) + c.vocab_size * c.d_model)

@@ -27,3 +27,15 @@ def test_models_without_8_bit_pages_run_as_they_did(model, tmp_path, caplog):
         be.close()
     assert torch.equal(*got)
     assert [r.getMessage().split(":")[0] for r in caplog.records] == ["K/V cache type fp8 changes nothing"]
+
+
+def test_other_models_refuse_the_type(tmp_path):
+    """A model whose engine has no E4M3 cache does not get another 8-bit one in its place."""
+    from ollama_b200.engine.b200 import B200Backend
+    from ollama_b200.engine.backend import open_model
+    from ollama_b200.models.synth import write_synthetic_gguf
+    path = str(tmp_path / "m.gguf")
+    write_synthetic_gguf(path, "tiny-qwen3", "Q8_0")
+    for kv, what in (("fp8", "stack models"), ("fp9", "unknown")):
+        with pytest.raises(ValueError, match=what), open_model(path) as g:
+            B200Backend(g, "cuda", kv_type=kv)
