@@ -370,19 +370,23 @@ struct MapEntry {
     MapKey key;
     CUtensorMap map;
 };
+struct KeptMaps {
+    static constexpr int CAP = 512;               // K and V of up to 256 layers; beyond that the oldest entries are replaced
+    MapEntry* table = nullptr;
+    int used = 0, next = 0;
+};
+thread_local KeptMaps g_kept;
 bool cached_kv_map(CUtensorMap* out, const void* base, size_t rows, int d, int box_rows = BKV) {
-    constexpr int CAP = 512;                      // K and V of up to 256 layers; beyond that the oldest entries are replaced
-    static thread_local MapEntry* table = nullptr;
-    static thread_local int used = 0, next = 0;
-    if (!table) table = new MapEntry[CAP];
-    for (int i = 0; i < used; i++)
-        if (table[i].key.base == base && table[i].key.rows == rows && table[i].key.d == d && table[i].key.box_rows == box_rows) {
-            *out = table[i].map;
+    KeptMaps& k = g_kept;
+    if (!k.table) k.table = new MapEntry[KeptMaps::CAP];
+    for (int i = 0; i < k.used; i++)
+        if (k.table[i].key.base == base && k.table[i].key.rows == rows && k.table[i].key.d == d && k.table[i].key.box_rows == box_rows) {
+            *out = k.table[i].map;
             return true;
         }
     if (!make_kv_map(out, base, rows, d, box_rows)) return false;
-    const int at = used < CAP ? used++ : (next++ % CAP);
-    table[at] = MapEntry{{base, rows, d, box_rows}, *out};
+    const int at = k.used < KeptMaps::CAP ? k.used++ : (k.next++ % KeptMaps::CAP);
+    k.table[at] = MapEntry{{base, rows, d, box_rows}, *out};
     return true;
 }
 
@@ -989,10 +993,11 @@ int launch2(const AttnPrefillArgs& a, int heads, size_t rows, int pdl, cudaStrea
 }
 
 template <int D, bool DIFF>
-int launch_paged(const AttnPrefillArgs& a, const AttnPagedArgs& pg, int n_tiles, int n_pages, cudaStream_t st) {
+int launch_paged(const AttnPrefillArgs& a, const AttnPagedArgs& pg, int n_tiles, int n_pages, int passing, cudaStream_t st) {
     CUtensorMap mk, mv;
     const size_t rows = (size_t)n_pages * a.Hkv * 64;
-    if (!cached_kv_map(&mk, a.k_cache, rows, D, 64) || !cached_kv_map(&mv, a.v_cache, rows, D, 64)) return (int)cudaErrorNotSupported;
+    const auto map = passing ? make_kv_map : cached_kv_map;
+    if (!map(&mk, a.k_cache, rows, D, 64) || !map(&mv, a.v_cache, rows, D, 64)) return (int)cudaErrorNotSupported;
     static thread_local PerDeviceOnce once;
     if (once.first()) cudaFuncSetAttribute(attn_prefill_tc2_kernel<D, D, PAGED_CACHE, DIFF>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay2<D, D>::TOTAL);
     AttnPrefillArgs copy = a;
@@ -1038,8 +1043,9 @@ B2_API int b2_attn_prefill_parts(const AttnPartsArgs* p, int n_tiles, cudaStream
 }
 
 // Attention of a step's query tiles over a paged f16 cache (rows padded to head_dim 64 or 128; anything else: cudaErrorNotSupported,
-// nothing launched).  a: q [rows][H][head_dim], caches, out, H, Hkv, scale, softcap; the other fields are not used.
-B2_API int b2_attn_prefill_paged(const AttnPrefillArgs* a, const AttnPagedArgs* pg, int head_dim, int n_tiles, int n_pages, cudaStream_t st) {
+// nothing launched).  a: q [rows][H][head_dim], caches, out, H, Hkv, scale, softcap; the other fields are not used.  passing: the cache is a buffer of this call, whose address and
+// extent another call hardly has: its tensor maps are not kept, where they would take the places of layers whose caches stay.
+B2_API int b2_attn_prefill_paged(const AttnPrefillArgs* a, const AttnPagedArgs* pg, int head_dim, int n_tiles, int n_pages, int passing, cudaStream_t st) {
     if (!a || !pg || !pg->tiles || !pg->page_table || n_tiles < 1 || n_pages < 1 || pg->max_pages < 1 || a->H < 1 || a->H > 65535 || a->Hkv < 1 || a->H % a->Hkv ||
         pg->vdim < 1 || pg->vdim > head_dim || pg->ldo < (pg->diff.on ? a->H / 2 : a->H) * pg->vdim || (pg->diff.on && (a->H / a->Hkv & 1)) || pg->window < 0 || pg->keep < 0 || pg->gate.kind < 0 || pg->gate.kind > 2 ||
         (pg->gate.kind && !pg->gate.g))
@@ -1052,12 +1058,12 @@ B2_API int b2_attn_prefill_paged(const AttnPrefillArgs* a, const AttnPagedArgs* 
     c.sinks = nullptr;
     if (pg->diff.on) {
         if (pg->gate.kind) return (int)cudaErrorNotSupported;
-        if (head_dim == 128) return launch_paged<128, true>(c, *pg, n_tiles, n_pages, st);
-        if (head_dim == 64) return launch_paged<64, true>(c, *pg, n_tiles, n_pages, st);
+        if (head_dim == 128) return launch_paged<128, true>(c, *pg, n_tiles, n_pages, passing, st);
+        if (head_dim == 64) return launch_paged<64, true>(c, *pg, n_tiles, n_pages, passing, st);
         return (int)cudaErrorNotSupported;
     }
-    if (head_dim == 128) return launch_paged<128, false>(c, *pg, n_tiles, n_pages, st);
-    if (head_dim == 64) return launch_paged<64, false>(c, *pg, n_tiles, n_pages, st);
+    if (head_dim == 128) return launch_paged<128, false>(c, *pg, n_tiles, n_pages, passing, st);
+    if (head_dim == 64) return launch_paged<64, false>(c, *pg, n_tiles, n_pages, passing, st);
     return (int)cudaErrorNotSupported;
 }
 
@@ -1083,6 +1089,9 @@ B2_API int b2_attn_prefill_key_parts(const AttnPrefillArgs* a, int head_dim) {
     const int tiles = (a->T + BQ - 1) / BQ * a->H;
     return head_dim == 128 ? key_parts<128>(*a, tiles) : key_parts<64>(*a, tiles);
 }
+
+// Tensor maps that this thread keeps.
+B2_API int b2_attn_prefill_kept_maps() { return g_kept.used; }
 
 // 0: the probabilities go through shared memory; 1: they stay in TMEM; 2: the pipelined kernel (default).  Returns the previous setting.
 B2_API int b2_attn_prefill_tc_variant(int v) {

@@ -167,7 +167,7 @@ def attn_prompt8(q, k: Pages8, v: Pages8, portions: Portions8, table, out, *, vd
         call(q, k, v, portions, table, out, read_out=False, **mask)
         return
     f = lib().b2_attn_prefill_paged
-    f.argtypes = [P, P, I, I, I, P]
+    f.argtypes = [P, P, I, I, I, I, P]
     a = AttnPrefillArgs(q.data_ptr(), wide[0].data_ptr(), wide[1].data_ptr(), out.data_ptr(), None, n, heads, kv_heads, 0, 0, 0, 0, 1, 0, scale, softcap, None, None)
     for begin, end in portions.groups:
         pages, some = portions.pages[begin[2]:end[2]], tiles[begin[of]:end[of]]
@@ -175,7 +175,7 @@ def attn_prompt8(q, k: Pages8, v: Pages8, portions: Portions8, table, out, *, vd
         here["read8"](k, v, pages, table, wide[0, :m], wide[1, :m], pdl, clean=True)
         pg = AttnPagedArgs(some.data_ptr(), portions.table.data_ptr(), portions.table.shape[1], chunk, vdim, out.stride(0), window, min(keep, portions.table.shape[1] * PAGE), gate, diff)
         with torch.cuda.device(q.device):
-            _check(f(C.addressof(a), C.addressof(pg), hd, some.shape[0], m, torch.cuda.current_stream().cuda_stream), "attn_prompt8")
+            _check(f(C.addressof(a), C.addressof(pg), hd, some.shape[0], m, 1, torch.cuda.current_stream().cuda_stream), "attn_prompt8")
 
 
 def status() -> int:

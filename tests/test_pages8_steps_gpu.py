@@ -217,3 +217,17 @@ def test_calls_from_several_threads():
     for t in threads:
         t.join()
     assert not wrong, wrong
+
+
+def test_pages_that_are_read_out_keep_no_tensor_maps():
+    """The maps of caches that stay are not pushed out by buffers of single calls."""
+    from ollama_b200.ops.cuda import lib
+    s = Setup(H=8, G=2, dim=64, norm="", n_rot=0, slots=1, n_ctx=2000)
+    numbers(s)
+    q, before = torch.randn(300, 8, 64, device="cuda"), lib().b2_attn_prefill_kept_maps()
+    for pos in (0, 100, 700, 1500):
+        out, plan = torch.zeros(300, 512, device="cuda", dtype=torch.bfloat16), s.P.portions8([(0, 300, 0, pos)], s.table)
+        pages = plan.groups[0][1][2]
+        assert peak(lambda: s.P.attn_prompt8(q, s.k, s.v, plan, s.table, out, vdim=64, scale=0.2)) >= 2 * pages * 2 * 64 * 64 * 2          # read out first
+        check_rows_of(s, q, out, 0, 300, 0, pos, 0.2)
+    assert lib().b2_attn_prefill_kept_maps() == before
