@@ -23,6 +23,9 @@ using namespace tc;
 constexpr int TURN = 32;                     // keys
 constexpr int BATCH = 128;                   // turns whose places are looked up at a time
 constexpr int MERGE_COLUMNS = 256;
+// Weights count from 2^LIFT for the largest score on, so that f16 keeps those down to 2^-(24 + LIFT) of it (and 2^-25 as zero without: a book of faint keys lost its part of the sum
+// beside one that stands out).  Taken off the maximum, the one place where it is rounded; a power beyond 7 could become 2^16 there, with scores whose last digit counts 16.
+constexpr float LIFT = 7.f;
 
 __device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -256,7 +259,7 @@ __global__ void __launch_bounds__(Lay<D, NB>::THREADS, Lay<D, NB>::PER_SM)
                     for (int i = 0; i < 2; i++) {
 #pragma unroll
                         for (int d = 4; d < 32; d <<= 1) mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], d));
-                        const float m_new = fmaxf(m_run[n][i], mx[i]);
+                        const float m_new = fmaxf(m_run[n][i], mx[i] - LIFT);
                         still &= m_new == m_run[n][i];
                         corr[n][i] = ex2(m_run[n][i] - m_new);
                         m_run[n][i] = m_new;

@@ -27,6 +27,7 @@ constexpr int SOFTMAX_WARPS = 8, CODE_WARPS = 8, TEAM = CODE_WARPS / 2, FIRST_CO
 constexpr int BOXES = 3;
 constexpr uint32_t TMEM_COLS = 512;
 constexpr float LAG = 8.f;
+constexpr float LIFT = 6.f;                  // weights count from 2^LIFT for the reference on (see attn_pages8.cu), so that they end at 2^14, within f16
 
 template <int D>
 struct Lay {
@@ -334,7 +335,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn8_tc_kernel(const __grid_const
                     }
                 }
             }
-            const float2 mult2 = make_float2(mult, mult), less = make_float2(-m_ref * mult, -m_ref * mult);
+            const float2 mult2 = make_float2(mult, mult), less = make_float2(fmaf(-m_ref, mult, LIFT), fmaf(-m_ref, mult, LIFT));
             float2 ls2[2] = {};
 #pragma unroll
             for (int h = 0; h < 2; h++) {

@@ -32,6 +32,7 @@ struct AttnPagedArgs {
     int window, keep;
     HeadGate gate;
     DiffHeads diff;          // on: differential attention, H counts maps; query tiles of up to 64 rows
+    float lift;              // weights count from 2^lift for the largest score on: up to 7 keeps that many more of the faint ones that f16 would round to zero
 };
 
 // Form for keys in two parts (latent attention, latent.cu): rows of one buffer hold every head's own key part and value, rows of another the
@@ -689,7 +690,7 @@ __global__ void __launch_bounds__(THREADS2, 1) attn_prefill_tc2_kernel(const __g
             const float corr = m_new == -INFINITY ? 1.f : ex2((m_run - m_new) * mult);
             const float mref = m_new == -INFINITY ? 0.f : m_new * mult;
             m_run = m_new;
-            const float2 mult2 = make_float2(mult, mult), less = make_float2(-mref, -mref);
+            const float2 mult2 = make_float2(mult, mult), less = FORM == PAGED_CACHE ? make_float2(pg.lift - mref, pg.lift - mref) : make_float2(-mref, -mref);
             float2 ls2 = make_float2(0.f, 0.f);
             uint32_t pw[32];
 #pragma unroll

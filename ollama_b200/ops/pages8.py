@@ -24,6 +24,7 @@ from .rows import NO_DIFF, NO_GATE, AttnPagedArgs, I, P
 
 PAGE = 64
 TOGETHER = 1024                  # pages: see portions8
+LIFT = 7.0                       # weights of attention on read-out pages count from 2^7 on, as those of the other forms (attn_pages8.cu)
 
 
 @dataclass(frozen=True)
@@ -173,7 +174,7 @@ def attn_prompt8(q, k: Pages8, v: Pages8, portions: Portions8, table, out, *, vd
         pages, some = portions.pages[begin[2]:end[2]], tiles[begin[of]:end[of]]
         m = pages.shape[0]
         here["read8"](k, v, pages, table, wide[0, :m], wide[1, :m], pdl, clean=True)
-        pg = AttnPagedArgs(some.data_ptr(), portions.table.data_ptr(), portions.table.shape[1], chunk, vdim, out.stride(0), window, min(keep, portions.table.shape[1] * PAGE), gate, diff)
+        pg = AttnPagedArgs(some.data_ptr(), portions.table.data_ptr(), portions.table.shape[1], chunk, vdim, out.stride(0), window, min(keep, portions.table.shape[1] * PAGE), gate, diff, LIFT)
         with torch.cuda.device(q.device):
             _check(f(C.addressof(a), C.addressof(pg), hd, some.shape[0], m, 1, torch.cuda.current_stream().cuda_stream), "attn_prompt8")
 

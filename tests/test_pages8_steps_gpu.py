@@ -1,5 +1,7 @@
 """The 8-bit paged cache in steps whose portions differ: the memory that calls take, rows that are not there, keys of little weight, and geometries beside those of
 test_pages8_gpu.py."""
+import math
+
 import pytest
 import torch
 
@@ -231,3 +233,28 @@ def test_pages_that_are_read_out_keep_no_tensor_maps():
         assert peak(lambda: s.P.attn_prompt8(q, s.k, s.v, plan, s.table, out, vdim=64, scale=0.2)) >= 2 * pages * 2 * 64 * 64 * 2          # read out first
         check_rows_of(s, q, out, 0, 300, 0, pos, 0.2)
     assert lib().b2_attn_prefill_kept_maps() == before
+
+
+@pytest.mark.parametrize("form", ["rows", "tiles", "read out"])
+def test_faint_keys_of_long_sequences(form):
+    """Eight keys that share nearly all of the weight, one for each warp and one or more for each group, and 100000 of e^-17.5 (2^-25.2) each, whose values are what the result is.
+    Queries, keys and values are exact in 16 and in 8 bits, so that only the weights' rounding to f16 is left: of 2^-19.2 at least, whose half step is 2^-25, so 2^-5.8 of them."""
+    keys, slots, n, dtype = 100000, *{"rows": (256, 1, torch.float32), "tiles": (148, 40, torch.float32), "read out": (1, 5120, torch.bfloat16)}[form]
+    s = Setup(H=4, G=1, dim=64, norm="", n_rot=0, slots=1, n_ctx=keys)
+    at = s.table[0].long()
+    k, v = torch.zeros(len(at) * 64, 64), torch.ones(len(at) * 64, 64)
+    k[:, 0] = 0.5
+    k[:256:32, 0], v[:256:32] = 18.0, 0.0
+    for c, x in ((s.k, k), (s.v, v)):
+        c.unit.fill_(1.0)
+        c.codes.zero_()
+        c.codes[at] = x.view(len(at), 1, 64, 64).to(torch.float8_e4m3fn).view(torch.uint8).cuda()
+    table = s.table.expand(slots, -1).contiguous()          # pages that nothing is appended to may be in several slots
+    q = torch.zeros(slots * n, 4, 64, device="cuda")
+    q[..., 0] = 1.0
+    out = torch.zeros(slots * n, 256, device="cuda", dtype=dtype)
+    s.P.attn_prompt8(q, s.k, s.v, s.P.portions8(portions_of([n] * slots, [keys - n] * slots), table), table, out, vdim=64, scale=1.0)
+    faint = torch.arange(keys - n - 7, keys - 7, dtype=torch.float64, device="cuda").repeat(slots)[:, None] * math.exp(-17.5)
+    want = faint / (8 + faint)
+    off = (out.double() - want).abs() / want
+    assert off.max() <= 2.0 ** -5.8 + 2.0 ** -10 + (2.0 ** -8 if dtype == torch.bfloat16 else 0), float(off.max())
