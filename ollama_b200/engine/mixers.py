@@ -25,8 +25,8 @@ def attend8(be, m, decode: bool, qkv, kc: P8.Pages8, vc: P8.Pages8, out, hd: int
     q = buf("q", heads * hd, torch.float32).view(qkv.shape[0], heads, hd)
     portions = m.portions(table, together=READ_OUT // (4 * P8.PAGE * kc.codes.shape[1] * hd), **{k: mask[k] for k in ("window", "keep", "chunk") if k in mask})
     P8.append8(qkv, kc, vc, table, q, portions=portions, **prep)
-    P8.attn_prompt8(q, kc, vc, portions, table, out, vdim=prep["vdim"], diff=diff, **mask)
-    return 4
+    n = P8.attn_prompt8(q, kc, vc, portions, table, out, vdim=prep["vdim"], diff=diff, **mask)
+    return n + 1 + prep.get("append", True)          # queries, and keys and values, are launches of their own
 
 
 class HeadAttention:

@@ -70,6 +70,7 @@ class _Meta:
 
     def __init__(self, tokens, positions, slots, offs=None, segs=None, tiles=None, half_tiles=None, long: dict[int, LongPortions] | None = None,
                  longest: int = 1, parts: Sequence[tuple[int, int, int, int]] = ()):
+        self.copied = 0                              # bytes that portions() has brought to the device
         self.parts, self._portions = parts, {}       # (first row, rows, slot, position of the first row) of each portion
         self.tokens, self.positions, self.slots, self.offs, self.segs, self.tiles, self.half_tiles = tokens, positions, slots, offs, segs, tiles, half_tiles
         self.long, self.longest = long, longest      # by window (0: none); rows of the longest portion
@@ -79,6 +80,7 @@ class _Meta:
         key = tuple(sorted(how.items()))
         if key not in self._portions:
             self._portions[key] = P8.portions8(self.parts, table, **how)
+            self.copied += self._portions[key].nbytes
         return self._portions[key]
 
 
@@ -598,6 +600,7 @@ class StackBackend(StepEngine):
         self._n = 0
         out = self._run_rows(_Rows(at, dev), m, at, decode=False, tap=tap)
         self.kernel_launches += self._n
+        self.h2d_bytes += m.copied
         return out
 
     def _final_norm(self, x: torch.Tensor) -> torch.Tensor:

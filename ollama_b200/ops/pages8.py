@@ -72,6 +72,10 @@ class Portions8:
     pages: torch.Tensor              # [pages, 4]: see read8
     table: torch.Tensor              # [n, pages of a slot]
 
+    @property
+    def nbytes(self) -> int:
+        return sum(t.nbytes for t in (self.segs, self.tiles, self.half_tiles, self.pages, self.table))
+
 
 def portions8(parts, table: torch.Tensor, *, window: int = 0, keep: int = 0, chunk: int = 0, together: int = TOGETHER) -> Portions8:
     """``parts``: (first row, rows, slot, position of the first row) of each portion, rows one after the other; the masks are those of the attention.  ``together``: most pages
@@ -151,22 +155,21 @@ def load() -> None:
         __getattr__("append8")
 
 
-def attn_prompt8(q, k: Pages8, v: Pages8, portions: Portions8, table, out, *, vdim, scale, softcap=0.0, chunk=0, window=0, keep=0, gate=NO_GATE, diff=NO_DIFF, pdl=False) -> None:
+def attn_prompt8(q, k: Pages8, v: Pages8, portions: Portions8, table, out, *, vdim, scale, softcap=0.0, chunk=0, window=0, keep=0, gate=NO_GATE, diff=NO_DIFF, pdl=False) -> int:
     """Attention of the rows of ``portions``, whose queries ``q`` [rows, H, 64 or 128] and whose keys and values in the cache :func:`append8` has prepared.  ``portions``
-    have to be made with this call's masks."""
+    have to be made with this call's masks.  Returns the launches."""
     here = globals()
     call = here.get("_attn_prompt8") or __getattr__("_attn_prompt8")
     mask = dict(vdim=vdim, scale=scale, softcap=softcap, chunk=chunk, window=window, keep=keep, gate=gate, diff=diff, pdl=pdl)
-    if call(q, k, v, portions, table, out, **mask):
-        return
+    if n := call(q, k, v, portions, table, out, **mask):
+        return n
     # many rows: the pages that they may see as f16 values, for attention on tcgen05
     n, heads, hd = q.shape
     kv_heads, tiles, of = k.codes.shape[1], portions.half_tiles if diff.on else portions.tiles, 1 if diff.on else 0
     try:
         wide = torch.empty(2, max(b[2] - a[2] for a, b in portions.groups), kv_heads, PAGE, hd, device=q.device, dtype=torch.float16)
     except torch.OutOfMemoryError:          # the other forms take more time and little memory
-        call(q, k, v, portions, table, out, read_out=False, **mask)
-        return
+        return call(q, k, v, portions, table, out, read_out=False, **mask)
     f = lib().b2_attn_prefill_paged
     f.argtypes = [P, P, I, I, I, I, P]
     a = AttnPrefillArgs(q.data_ptr(), wide[0].data_ptr(), wide[1].data_ptr(), out.data_ptr(), None, n, heads, kv_heads, 0, 0, 0, 0, 1, 0, scale, softcap, None, None)
@@ -177,6 +180,7 @@ def attn_prompt8(q, k: Pages8, v: Pages8, portions: Portions8, table, out, *, vd
         pg = AttnPagedArgs(some.data_ptr(), portions.table.data_ptr(), portions.table.shape[1], chunk, vdim, out.stride(0), window, min(keep, portions.table.shape[1] * PAGE), gate, diff, LIFT)
         with torch.cuda.device(q.device):
             _check(f(C.addressof(a), C.addressof(pg), hd, some.shape[0], m, 1, torch.cuda.current_stream().cuda_stream), "attn_prompt8")
+    return 2 * len(portions.groups)
 
 
 def status() -> int:

@@ -397,8 +397,8 @@ void attn_decode8(PyObject** a) {
 enum { P_Q, P_K, P_V, P_PORTIONS, P_TABLE, P_OUT, P_VDIM, P_SCALE, P_SOFTCAP, P_CHUNK, P_WINDOW, P_KEEP, P_GATE, P_DIFF, P_PDL, P_READ, P_N };
 Signature prompt_sig = {"attn_prompt8", 6, P_N, {"q", "k", "v", "portions", "table", "out", "vdim", "scale", "softcap", "chunk", "window", "keep", "gate", "diff", "pdl", "read_out"}};
 
-// False: the pages are to be read out to f16 first, nothing is launched.  Not with read_out=False.
-bool attn_prompt8(PyObject** a) {
+// The launches; 0: the pages are to be read out to f16 first, nothing is launched.  Not with read_out=False.
+long attn_prompt8(PyObject** a) {
     const Signature& s = prompt_sig;
     for (int i = 0; i <= P_SCALE; i++) required(s, a, i);
     const at::Tensor& q = tensor(s, a[P_Q], "q");
@@ -443,7 +443,7 @@ bool attn_prompt8(PyObject** a) {
     }
     group_done();
     const double t16 = 9.6 + 0.08 * items16 + keys16 / 19000, t128 = 12 + 0.37 * items128 + keys128 / 11700;
-    if (as_bool(a[P_READ], true) && m > 64 && t_read < std::min(t16, t128) && t.out16 && !((uintptr_t)t.out & 15) && !(t.diff.on && t.gate.kind)) return false;
+    if (as_bool(a[P_READ], true) && m > 64 && t_read < std::min(t16, t128) && t.out16 && !((uintptr_t)t.out & 15) && !(t.diff.on && t.gate.kind)) return 0;
     few_rows(s, n);
     const int row_tile = m <= 8 ? 8 : m <= 16 || t16 <= t128 ? 16 : 128;
     long tiles = 0, batch = 0;      // of the launch with most
@@ -463,7 +463,7 @@ bool attn_prompt8(PyObject** a) {
         t.part_ml = (float2*)(t.part_acc + pieces * hd);
         return f_attn(&t, pdl, st);
     }));
-    return true;
+    return 2 * tiles_of(po.n, MAX_UNITS);
 }
 
 // ---- module ---------------------------------------------------------------------------------------------------------------------
@@ -503,7 +503,7 @@ PyObject* py_attn_decode8(PyObject*, PyObject* const* args, Py_ssize_t n, PyObje
     return called<decode_sig>([](PyObject** a) { attn_decode8(a); return none(); }, args, n, kw);
 }
 PyObject* py_attn_prompt8(PyObject*, PyObject* const* args, Py_ssize_t n, PyObject* kw) {
-    return called<prompt_sig>([](PyObject** a) { return PyBool_FromLong(attn_prompt8(a)); }, args, n, kw);
+    return called<prompt_sig>([](PyObject** a) { return PyLong_FromLong(attn_prompt8(a)); }, args, n, kw);
 }
 // bind(append, attn, decode, read, exception, layout): addresses of the kernel library's entry points, what a failing launch raises, and which argument blocks the library takes
 PyObject* py_bind(PyObject*, PyObject* const* args, Py_ssize_t n) {

@@ -39,3 +39,22 @@ def test_other_models_refuse_the_type(tmp_path):
     for kv, what in (("fp8", "stack models"), ("fp9", "unknown")):
         with pytest.raises(ValueError, match=what), open_model(path) as g:
             B200Backend(g, "cuda", kv_type=kv)
+
+
+def test_a_step_counts_what_it_copies(tmp_path):
+    """A mixed step brings its rows, its portions and, once for each mask, what the 8-bit attention has to know of them to the device."""
+    cfg = VM.config([VM.attention(), VM.attention(size=96), VM.attention()], loop=None)
+    path = VM.write(tmp_path, cfg, VM.weights(cfg, 3))
+    got = {}
+    for kv in ("f16", "fp8"):
+        be = engine(path, kv=kv)
+        be.step([(0, VM.tokens(20, cfg["vocab"], 5), 0)], [[]])
+        before = be.h2d_bytes
+        be.step([(0, VM.tokens(70, cfg["vocab"], 6), 20), (2, [3], 0)], [[], []])
+        got[kv] = be.h2d_bytes - before
+        chunks = {L.mixer.chunk for L in be.layers}
+        if kv == "fp8":
+            from ollama_b200.ops import pages8 as P
+            plans = [P.portions8([(0, 70, 0, 20), (70, 1, 2, 0)], be.cache.table, chunk=c).nbytes for c in chunks]
+        be.close()
+    assert len(plans) == 2 and got["fp8"] == got["f16"] + sum(plans)

@@ -258,3 +258,28 @@ def test_faint_keys_of_long_sequences(form):
     want = faint / (8 + faint)
     off = (out.double() - want).abs() / want
     assert off.max() <= 2.0 ** -5.8 + 2.0 ** -10 + (2.0 ** -8 if dtype == torch.bfloat16 else 0), float(off.max())
+
+
+@pytest.mark.parametrize("append", [True, False])
+def test_launches_are_counted(append):
+    """What the engine adds to its count is what a capture of the same calls holds."""
+    import ctypes
+
+    from ollama_b200.engine.mixers import attend8
+    from ollama_b200.ops import rows as O8
+    for lens, dtype, together in (([3, 2], torch.bfloat16, 1024), ([300, 260], torch.bfloat16, 1024), ([300, 260], torch.bfloat16, 1), ([2] * 300, torch.float32, 1024)):
+        s = Setup(H=8, G=2, dim=64, norm="", slots=len(lens), n_ctx=320, seed=71)
+        numbers(s)
+        x = s.rnd(sum(lens), s.ld).cuda()
+        plan, prep = s.P.portions8(portions_of(lens, [10] * len(lens)), s.table, together=together), s.prep()
+        out, q = torch.zeros(len(x), 512, device="cuda", dtype=dtype), torch.zeros(len(x), 512, device="cuda")
+        m = type("Meta", (), {"portions": lambda self, table, **how: plan})()
+        be = type("Engine", (), {"cache": type("Cache", (), {"table": s.table})()})()
+        step = lambda: attend8(be, m, False, x, s.k, s.v, out, 64, lambda *a: q, O8.NO_DIFF, dict(prep, append=append), dict(scale=0.1))  # noqa: E731
+        step()
+        g = torch.cuda.CUDAGraph(keep_graph=True)
+        with torch.cuda.graph(g):
+            n = step()
+        nodes = ctypes.c_size_t()
+        assert ctypes.CDLL("libcudart.so.12").cudaGraphGetNodes(ctypes.c_void_p(g.raw_cuda_graph()), None, ctypes.byref(nodes)) == 0
+        assert nodes.value == n
