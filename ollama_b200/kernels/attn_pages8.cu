@@ -12,7 +12,7 @@
 // Measured, whole steps with append and merge in a graph, 128 columns: four sequences of 60000 keys, 32 heads on 8, 77 us, 5.1 TB/s of the 6.5 that a copy reaches (the SMs fetch
 // unevenly: CTAs end between 51 and 74 us); one of 6144 keys 13 us and 32 sequences with windows of 1024, 16 heads on 4, 20 us, of which the three launches' latencies are most.
 #include "attn_pages8.cuh"
-#include "tc_common.cuh"
+#include "attn_tc.cuh"
 
 __device__ int g_attn8_status = 0;
 
@@ -43,16 +43,6 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ uint32_t pack_h2(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-
 // NB: blocks of eight query rows.  Of CTAs with one, two fit an SM.
 template <int D, int NB>
 struct Lay {
