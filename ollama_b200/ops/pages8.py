@@ -157,7 +157,10 @@ def load() -> None:
 
 def attn_prompt8(q, k: Pages8, v: Pages8, portions: Portions8, table, out, *, vdim, scale, softcap=0.0, chunk=0, window=0, keep=0, gate=NO_GATE, diff=NO_DIFF, pdl=False) -> int:
     """Attention of the rows of ``portions``, whose queries ``q`` [rows, H, 64 or 128] and whose keys and values in the cache :func:`append8` has prepared.  ``portions``
-    have to be made with this call's masks.  Returns the launches."""
+    have to be made with this call's masks.  Returns the launches.
+
+    Queries and weights are rounded to f16 (2^-11 each) whatever type ``out`` has, so queries beyond 65504 have no result; the scores' and weights' sums are 32-bit ones.  Soft
+    caps and gates use the fast exponential and quotient, some 2^-21.  Results of many rows, which may be of read-out pages, are within the same bounds."""
     here = globals()
     call = here.get("_attn_prompt8") or __getattr__("_attn_prompt8")
     mask = dict(vdim=vdim, scale=scale, softcap=softcap, chunk=chunk, window=window, keep=keep, gate=gate, diff=diff, pdl=pdl)

@@ -364,7 +364,7 @@ Signature decode_sig = {"attn_decode8", 7, D_N, {"qkv", "k", "v", "positions", "
 
 void attn_decode8(PyObject** a) {
     const Signature& s = decode_sig;
-    for (int i = 0; i <= D_NCTX; i++)
+    for (int i = 0; i < D_NCTX; i++)
         if (i != D_QN && i != D_KN && i != D_FREQS) required(s, a, i);
     const at::Tensor& qkv = tensor(s, a[D_QKV], "qkv");
     const c10::Device dev = on_gpu(s, qkv);
@@ -532,16 +532,19 @@ const char append8_doc[] =
     "append8(qkv, k, v, table, q_out, *, heads, dim, vdim, q_norm, k_norm, eps, freqs, n_rot, positions=None, slots=None, portions=None, head_norm=False, v_off=None, mscale=1.0, "
     "maps=1, append=True, pdl=False)\n--\n\n"
     "Norm of q and k, rotation, q to padded fp32 rows [rows, H, 64 or 128], k and v into the cache; arguments as of rows.paged_append.  Rows are one token a sequence at\n"
-    "`positions` of `slots` (of rows of one slot the later ones are appended after the earlier ones), or those of `portions`.";
+    "`positions` of `slots` (of rows of one slot the later ones are appended after the earlier ones), or those of `portions`.  Keys of portions turn by products of two angles' cosines\n"
+    "and sines, off by 2^-23 of those of a single row: a code next to a border can depend on how the tokens were cut.";
 const char read8_doc[] =
     "read8(k, v, pages, table, k_out, v_out, pdl=False, clean=False)\n--\n\n"
     "Pages as f16 values, [n, KV heads, 64, columns] each.  `pages` [n, 4] int32: slot, page of the slot, rows that are wanted (what lies behind them is written as zeros, as are\n"
     "pages that are not there), 0.  `clean`: rows of values that hold what is no number become zeros and their keys none.";
 const char attn_decode8_doc[] =
-    "attn_decode8(qkv, k, v, positions, slots, table, out, *, heads, dim, vdim, q_norm, k_norm, eps, freqs, n_rot, scale, n_ctx, softcap=0.0, chunk=0, window=0, keep=0, "
+    "attn_decode8(qkv, k, v, positions, slots, table, out, *, heads, dim, vdim, q_norm, k_norm, eps, freqs, n_rot, scale, n_ctx=0, softcap=0.0, chunk=0, window=0, keep=0, "
     "head_norm=False, v_off=None, mscale=1.0, gate=NO_GATE, maps=1, append=True, diff=NO_DIFF, pdl=False)\n--\n\n"
     "Decode attention on raw projections, one token a sequence: what append8 does, then attention of the rows' positions over the cache, difference of maps and gate into rows of\n"
-    "`out`.  `n_ctx`: most keys that a sequence holds, as of the 16-bit form; the work follows the positions.";
+    "`out`.  `n_ctx`, most keys that a sequence holds, is taken as the 16-bit form takes it and not needed: the work follows the positions.\n"
+    "Queries and weights are rounded to f16 (2^-11 each) whatever type `out` has, so queries beyond 65504 have no result; the scores' and weights' sums are 32-bit ones.  Soft caps and\n"
+    "gates use the fast exponential and quotient, some 2^-21.";
 
 PyMethodDef methods[] = {
     {"append8", (PyCFunction)(void (*)())py_append8, METH_FASTCALL | METH_KEYWORDS, append8_doc},

@@ -68,3 +68,15 @@ def test_a_part_of_the_library_comes_with_its_calls(monkeypatch, tmp_path):
     monkeypatch.setattr(B, "build_calls", lambda *a: built.append("calls"))
     B.build_group("stack")
     assert built[-1] == "calls" and len(built) == 2
+
+
+def test_calls_that_lack_an_argument():
+    """Named in the error; `n_ctx`, which nothing follows from, may be left out."""
+    k, v = P.Pages8.empty(2, 1, 64, device="cpu"), P.Pages8.empty(2, 1, 64, device="cpu")
+    x, i = torch.zeros(1, 192), torch.zeros(1, dtype=torch.int32)
+    a = dict(heads=1, dim=64, vdim=64, q_norm=None, k_norm=None, eps=1e-5, freqs=None, n_rot=0, scale=1.0)
+    with pytest.raises(ValueError, match="cpu"):
+        P.attn_decode8(x, k, v, i, i, torch.zeros(1, 2, dtype=torch.int32), torch.zeros(1, 64), **a)
+    for name in ("heads", "dim", "vdim", "eps", "n_rot", "scale"):
+        with pytest.raises(TypeError, match=name):
+            P.attn_decode8(x, k, v, i, i, torch.zeros(1, 2, dtype=torch.int32), torch.zeros(1, 64), **{n: a[n] for n in a if n != name})
