@@ -6,7 +6,8 @@ import torch
 
 import kavenex_models as KM
 import vazatar_models as VM
-from test_fp8_cache_gpu import engine
+import vazatar_oracle as VO
+from test_fp8_cache_gpu import CONFIGS, engine, rounded_caches  # noqa: F401  (a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -58,3 +59,39 @@ def test_a_step_counts_what_it_copies(tmp_path):
             plans = [P.portions8([(0, 70, 0, 20), (70, 1, 2, 0)], be.cache.table, chunk=c).nbytes for c in chunks]
         be.close()
     assert len(plans) == 2 and got["fp8"] == got["f16"] + sum(plans)
+
+
+def test_requests_side_by_side(tmp_path, rounded_caches):
+    """A request is generating while others arrive, one with most of its prompt: portions beside single tokens, a prefix copied out of a busy slot.  Every token has the largest logit
+    of the plain implementation on rounded caches, or one nearer to it than twice what rounding the products' inputs does to a logit, times three as in test_logits."""
+    from ollama_b200.engine.runner import CompletionRequest, Runner, RunnerOptions
+    from ollama_b200.engine.sampler import SamplingParams
+    cfg = CONFIGS["vazatar-heads"][1]
+    w = VM.weights(cfg, 3)
+    r = Runner(str(VM.write(tmp_path, cfg, w)), RunnerOptions(num_ctx=320, num_parallel=3, num_batch=48, device="cuda", kv_cache_type="fp8"))
+    prompt = VM.tokens(100, cfg["vocab"], 4)
+    prompts = [prompt, prompt[:80] + VM.tokens(9, cfg["vocab"], 8), VM.tokens(130, cfg["vocab"], 11)]
+
+    def request(p, n):
+        return r.submit(CompletionRequest(prompt=list(p), sampling=SamplingParams(temperature=0), num_predict=n, ignore_eos=True))
+    try:
+        assert r.backend.pages8
+        asked = [request(prompts[0], 120)]
+        got = [asked[0].out.get(timeout=60).tokens]                     # its prompt is in the cache and it is generating
+        asked += [request(p, 20) for p in prompts[1:]]
+        got += [[], []]
+        for a, tokens in zip(asked, got):
+            done = False
+            while not done:
+                c = a.out.get(timeout=60)
+                tokens += c.tokens
+                done = c.done
+        assert [len(t) for t in got] == [120, 20, 20] and r.stats["mixed_steps"] > 0 and r.stats["prefix_copies"] > 0
+    finally:
+        r.close()
+    for p, tokens in zip(prompts, got):
+        rows = list(p) + tokens[:-1]
+        want, near = VO.forward(cfg, w, rows), VO.forward(cfg, w, rows, product=VO.rounded)
+        logits = want[len(p) - 1:].cpu()
+        behind = logits.amax(-1) - logits[torch.arange(len(tokens)), torch.tensor(tokens)]
+        assert behind.max() <= 2 * 3 * (near - want).abs().max(), float(behind.max())

@@ -283,3 +283,72 @@ def test_launches_are_counted(append):
         nodes = ctypes.c_size_t()
         assert ctypes.CDLL("libcudart.so.12").cudaGraphGetNodes(ctypes.c_void_p(g.raw_cuda_graph()), None, ctypes.byref(nodes)) == 0
         assert nodes.value == n
+
+
+def test_units_at_their_borders():
+    """448 units are the most that a unit holds: the next larger number takes twice the unit, of one row and of a page's rows, keys and values."""
+    top = [448.0 * 2.0 ** e for e in (-15, -3, 0, 6, 7)]
+    above = [math.nextafter(t, math.inf) for t in top]
+    up = [torch.nextafter(torch.tensor(t), torch.tensor(math.inf)).item() for t in top]
+    assert all(u > a for u, a in zip(up, above))          # the next 32-bit number
+    want = [2.0 ** e for e in (-15, -3, 0, 6, 7)] + [2.0 ** e for e in (-14, -2, 1, 7, 7)]
+    m = [*top, *up]
+    s = Setup(H=1, G=1, dim=64, norm="", n_rot=0, slots=10, n_ctx=64)
+    x = torch.zeros(10, s.ld)
+    for i, t in enumerate(m):
+        x[i, s.nq + 3 * i], x[i, s.v_off + 5] = -t, t
+    q = torch.empty(10, 1, 64, device="cuda")
+    s.P.append8(x.cuda(), s.k, s.v, s.table, q, positions=i32([0] * 10), slots=i32(list(range(10))), **s.prep())
+    p = s.table[:, 0].long()
+    assert s.k.unit[p, 0].tolist() == want and s.v.unit[p, 0].tolist() == want
+    assert s.k.numbers[p, 0, 0].float().abs().amax(1).tolist() == [448.0] * 5 + [224.0] * 4 + [448.0]
+    t = Setup(H=1, G=1, dim=64, norm="", n_rot=0, slots=10, n_ctx=64)
+    y, q = torch.zeros(30, t.ld), torch.empty(30, 1, 64, device="cuda")
+    y[1::3] = x
+    t.P.append8(y.cuda(), t.k, t.v, t.table, q, portions=t.P.portions8([(3 * i, 3, i, 0) for i in range(10)], t.table), **t.prep())
+    p = t.table[:, 0].long()
+    assert t.k.unit[p, 0].tolist() == want and t.v.unit[p, 0].tolist() == want
+
+
+@pytest.mark.parametrize("G", [3, 5, 6, 7, 8, 9, 12])
+def test_norms_over_rows_of_any_number_of_heads(G):
+    """A page's KV heads exchange their parts of a norm where they are up to eight, and read the row where they are more."""
+    s = Setup(H=2 * G, G=G, dim=32, norm="row", slots=2, n_ctx=200, seed=G)
+    x, q = s.rnd(170, s.ld), torch.empty(170, 2 * G, 64, device="cuda")
+    parts = [(0, 130, 1, 20), (130, 40, 0, 0)]
+    s.P.append8(x.cuda(), s.k, s.v, s.table, q, portions=s.P.portions8(parts, s.table), **s.prep())
+    pos = torch.cat([torch.arange(p, p + n) for _, n, _, p in parts])
+    qx, kx, vx = s.split(x, pos)
+    assert (q[..., :32].double().cpu() - qx).abs().max() <= 2.0 ** -20 * qx.abs().max() and (q[..., 32:] == 0).all()
+    for row, n, slot, p in parts:
+        s.check_rows(s.k, 32, slot, p, kx[row:row + n])
+        s.check_rows(s.v, 32, slot, p, vx[row:row + n])
+
+
+@pytest.mark.parametrize("gate", ["element", "head"])
+def test_difference_of_maps_with_a_gate(gate):
+    from ollama_b200.ops import rows as R
+    heads, kv, dim, vdim, lam, factor, eps, scale = 8, 2, 32, 64, 0.37, 0.8, 1e-5, 0.2
+    s = Setup(H=heads, G=kv, dim=dim, vdim=vdim, norm="", maps=2, slots=1, n_ctx=500, seed=61)
+    diff, at = R.DiffHeads(lam, factor, eps, 1), 0
+    for n in (3, 60, 300, 1):
+        x, gv = s.rnd(n, s.ld), s.rnd(n, heads // 2 * vdim).cuda()
+        out = torch.zeros(n, heads // 2 * vdim, device="cuda", dtype=torch.bfloat16)
+        if n > 1:
+            q, plan = torch.empty(n, heads, s.hd, device="cuda"), s.P.portions8([(0, n, 0, at)], s.table)
+            s.P.append8(x.cuda(), s.k, s.v, s.table, q, portions=plan, **s.prep())
+            s.P.attn_prompt8(q, s.k, s.v, plan, s.table, out, vdim=vdim, scale=scale, gate=R.head_gate(gv, gate), diff=diff)
+        else:
+            s.P.attn_decode8(x.cuda(), s.k, s.v, i32([at]), i32([0]), s.table, out, n_ctx=500, scale=scale, gate=R.head_gate(gv, gate), diff=diff, **s.prep())
+        pos = torch.arange(at, at + n)
+        qx = s.split(x, pos)[0].cuda()
+        k, v = s.values(s.k, 0, at + n), s.values(s.v, 0, at + n)
+        o = [O.attend(qx[:, m::2], k[..., m * dim:(m + 1) * dim], v[..., :vdim], O.visible(pos, at + n), scale) for m in range(2)]
+        d = o[0][0] - lam * o[1][0]
+        rms = (d.square().mean(-1, keepdim=True) + eps).sqrt()
+        near = (O.tolerance(o[0][0], o[0][1], v.abs().max(), torch.float32) + lam * O.tolerance(o[1][0], o[1][1], v.abs().max(), torch.float32)).amax(-1, keepdim=True)
+        f = torch.sigmoid(gv.double()).view(n, heads // 2, vdim) if gate == "element" else torch.sigmoid(gv[:, :heads // 2].double())[..., None]
+        want = d / rms * factor * f
+        # the norm divides the difference's error and moves by as much itself; the gate's exponential and quotient are off by some 2^-21
+        assert ((out.double().view(n, heads // 2, vdim) - want).abs() <= 2 * factor * f * near / rms + want.abs() * (2.0 ** -8 + 2.0 ** -20)).all()
+        at += n
