@@ -318,5 +318,5 @@ B2_API int b2_gemv_rows(const GemvRowsArgs* a, int pdl, cudaStream_t st) {
     GemvRowsArgs copy = *a;
     void* args[] = {&copy};
     const void* fn = a->f32 ? pick_src<true>(a->src, a->nb, ks) : pick_src<false>(a->src, a->nb, ks);
-    return launch_rows(fn, dim3((unsigned)((groups + rgs - 1) / rgs)), dim3(256), 0, args, st, pdl);
+    return launch_streaming(fn, dim3((unsigned)((groups + rgs - 1) / rgs)), dim3(256), 0, args, st, pdl);
 }

@@ -329,7 +329,7 @@ B2_API int b2_moe_up_rows(const MoeUpArgs* a, int nb, int f32, int pdl, cudaStre
     const int ks = split_of(groups * nb, a->k >> 3, 1800), rgs = 8 / ks;
     MoeUpArgs c = *a;
     void* args[] = {&c};
-    return launch_rows(B2_PICK_KS(moe_up_rows_kernel, f32, ks), dim3((unsigned)((groups + rgs - 1) / rgs), nb), dim3(256), a->groups.count ? (size_t)a->n_experts * 8 : 0, args, st,
+    return launch_streaming(B2_PICK_KS(moe_up_rows_kernel, f32, ks), dim3((unsigned)((groups + rgs - 1) / rgs), nb), dim3(256), a->groups.count ? (size_t)a->n_experts * 8 : 0, args, st,
                        pdl);
 }
 
@@ -341,5 +341,5 @@ B2_API int b2_moe_down_rows(const MoeDownArgs* a, int nb, int f32, int pdl, cuda
     const int ks = split_of(groups * nb, (a->top * a->ffp + a->sfp) >> 3, 16000), rgs = 8 / ks;
     MoeDownArgs c = *a;
     void* args[] = {&c};
-    return launch_rows(B2_PICK_KS(moe_down_rows_kernel, f32, ks), dim3((unsigned)((groups + rgs - 1) / rgs), nb), dim3(256), 0, args, st, pdl);
+    return launch_streaming(B2_PICK_KS(moe_down_rows_kernel, f32, ks), dim3((unsigned)((groups + rgs - 1) / rgs), nb), dim3(256), 0, args, st, pdl);
 }

@@ -56,18 +56,27 @@ __device__ __forceinline__ int kept_tiles(int keep, int first, int tile) { retur
 __device__ __forceinline__ float sigmoid_f(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
 __device__ __forceinline__ float sigmoid_exact(float v) { return 1.f / (1.f + expf(-v)); }
 
-static inline int launch_rows(const void* fn, dim3 grid, dim3 block, size_t smem, void** args, cudaStream_t st, int pdl) {
+static inline int launch_rows(const void* fn, dim3 grid, dim3 block, size_t smem, void** args, cudaStream_t st, int pdl, int shared_percent = -1) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = pdl ? 1 : 0;
+    at[1].id = cudaLaunchAttributePreferredSharedMemoryCarveout;
+    at[1].val.sharedMemCarveout = shared_percent;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = shared_percent < 0 ? 1 : 2;
     return (int)cudaLaunchKernelExC(&cfg, fn, args);
+}
+// For kernels whose loads of weights are under way in L1, which is what an SM has beside its shared memory.  A kernel that says nothing takes the split that the one before left: behind
+// attention with 196 KB of shared memory an SM, the weights of whole models came in a sixth slower until the end of the step (steps of tirudra-2k, vazatar-1b and rinirax-1b on 8-bit
+// caches at 6000 tokens 1219, 808 and 707 us; with 4 % 1110, 748 and 695, 8 % 1111, 748 and 695, 14 % 1123, 773 and 723, 28 % 1199, 846 and 728).  4 % is what eight CTAs of 256
+// threads take for themselves; dynamic shared memory of theirs comes on top.
+static inline int launch_streaming(const void* fn, dim3 grid, dim3 block, size_t smem, void** args, cudaStream_t st, int pdl) {
+    return launch_rows(fn, grid, block, smem, args, st, pdl, (int)(4 + 800 * smem / (228 << 10)));
 }
 
 // Matrix product of a step's rows: out[m][ldo] (+)= alpha * f(a[m][lda] . b[n][ldb]^T + bias).  Served by b2_gemm_rows (bf16 operands on the
