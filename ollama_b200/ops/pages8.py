@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes as C
 import importlib.util
+import threading
 from dataclasses import dataclass
 
 import numpy as np
@@ -140,19 +141,23 @@ def _calls():
     return m
 
 
+_LOADING = threading.Lock()
+
+
+def load() -> None:
+    """Makes the calls ready, building what is missing: before a model's first step rather than in it.  Of several threads one does."""
+    with _LOADING:
+        if "append8" not in globals():
+            m = _calls()
+            globals().update(append8=m.append8, read8=m.read8, attn_decode8=m.attn_decode8, _attn_prompt8=m.attn_prompt8)
+
+
 def __getattr__(name: str):
     """The calls, when one is first asked for."""
     if name not in ("append8", "read8", "attn_decode8", "_attn_prompt8"):
         raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
-    m = _calls()
-    globals().update(append8=m.append8, read8=m.read8, attn_decode8=m.attn_decode8, _attn_prompt8=m.attn_prompt8)
+    load()
     return globals()[name]
-
-
-def load() -> None:
-    """Makes the calls ready, building what is missing: before a model's first step rather than in it."""
-    if "append8" not in globals():
-        __getattr__("append8")
 
 
 def attn_prompt8(q, k: Pages8, v: Pages8, portions: Portions8, table, out, *, vdim, scale, softcap=0.0, chunk=0, window=0, keep=0, gate=NO_GATE, diff=NO_DIFF, pdl=False) -> int:

@@ -80,3 +80,27 @@ def test_calls_that_lack_an_argument():
     for name in ("heads", "dim", "vdim", "eps", "n_rot", "scale"):
         with pytest.raises(TypeError, match=name):
             P.attn_decode8(x, k, v, i, i, torch.zeros(1, 2, dtype=torch.int32), torch.zeros(1, 64), **{n: a[n] for n in a if n != name})
+
+
+def test_threads_that_need_the_calls_at_once(monkeypatch):
+    """One of them builds and binds, the others wait for it."""
+    import threading
+    import time
+    made, calls = [], ("append8", "read8", "attn_decode8", "_attn_prompt8")
+    P.load()
+    module = P._module()
+    for name in calls:
+        monkeypatch.delitem(vars(P), name)
+
+    def slow():
+        made.append(threading.get_ident())
+        time.sleep(0.05)
+        return module
+    monkeypatch.setattr(P, "_calls", slow)
+    got = []
+    threads = [threading.Thread(target=lambda i=i: got.append(getattr(P, calls[i % 4]))) for i in range(8)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(made) == 1 and len(got) == 8
