@@ -263,10 +263,16 @@ struct Portions {                // what a Portions8 says
 };
 Portions portions(const Signature& s, PyObject* o, long rows, c10::Device dev) {
     Ref segs(o, s_segs), r(o, s_rows), per(o, s_per), longest(o, s_longest);
-    const at::Tensor& t = tensor(s, segs.o, "portions");
+    const at::Tensor& t = wide(s, piece(s, segs.o, "portions", I32, dev), "portions");
+    if (t.dim() != 2 || t.size(1) != 4) refuse(s, "portions " + told(t));
     const Portions p{(const int4*)t.data_ptr(), (int)t.size(0), (int)as_long(r.o, 0), (int)as_long(per.o, 1), (int)as_long(longest.o, 0)};
-    if (p.rows > rows || t.device() != dev) refuse(s, "portions of " + std::to_string(p.rows) + " rows on " + t.device().str() + " for " + std::to_string(rows) + " on " + dev.str());
+    if (p.rows > rows) refuse(s, "portions of " + std::to_string(p.rows) + " rows for " + std::to_string(rows));
     return p;
+}
+// A tuple of n things.
+PyObject* tuple_of(const Signature& s, PyObject* o, Py_ssize_t n, const char* what) {
+    if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != n) refuse(s, std::string("portions whose ") + what + " are not what portions8 makes");
+    return o;
 }
 
 void append8(PyObject** a) {
@@ -412,9 +418,11 @@ long attn_prompt8(PyObject** a) {
     const Portions po = portions(s, a[P_PORTIONS], n, dev);
     Ref masks(a[P_PORTIONS], s_masks), table(a[P_PORTIONS], s_table), sizes(a[P_PORTIONS], s_sizes);
     const int mine[3] = {t.window, t.keep, t.chunk};
+    tuple_of(s, masks.o, 3, "masks");
+    tuple_of(s, sizes.o, po.n, "sizes");
     for (int i = 0; i < 3; i++)
         if (as_long(PyTuple_GET_ITEM(masks.o, i), 0) != mine[i]) refuse(s, "portions that were made with another mask");
-    if (tensor(s, table.o, "portions").size(1) != c.t.max_pages) refuse(s, "portions that were made with another table");
+    if (const at::Tensor& own = tensor(s, table.o, "portions"); own.dim() != 2 || own.size(1) != c.t.max_pages) refuse(s, "portions that were made with another table");
     // Estimates of three forms, us (measured with 32 heads on 8 of 128, 16 on 4, and 4 on 2 of 64, 1 and 3 sequences, 5 to 512 rows behind 0 to 30000 keys; the choice costs a
     // hundredth on the mean): 16 query rows a tile 9.6 + 0.08 for each tile of a KV head + one for each 19000 of its keys, 128 rows a tile on tcgen05 12 + 0.37 + one for each 11700,
     // pages read out first 10 + 0.0107 a key for each time that the tiles of 128 rows and heads fill the GPU, for each group of portions that are read out together.  (32 heads on 8, in that order: 5 rows at 901 keys 12.3, 16.0, 21.4;
@@ -427,7 +435,7 @@ long attn_prompt8(PyObject** a) {
         most = ctas = 0;
     };
     for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(sizes.o); i++) {
-        PyObject* e = PyTuple_GET_ITEM(sizes.o, i);
+        PyObject* e = tuple_of(s, PyTuple_GET_ITEM(sizes.o, i), 3, "sizes");
         const double rows = as_long(PyTuple_GET_ITEM(e, 0), 0), keys = as_long(PyTuple_GET_ITEM(e, 1), 0);
         const double of16 = (double)tiles_of((long)rows * group, 16) * c.c.kv_heads, of128 = (double)tiles_of((long)rows * group, 128) * c.c.kv_heads;
         items16 += of16;

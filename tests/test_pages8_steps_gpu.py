@@ -391,3 +391,27 @@ def test_products_behind_the_attention_are_as_fast_as_elsewhere():
                 t.append(b.elapsed_time(e))
     both, attention, product = (sorted(t)[len(t) // 2] for t in times)
     assert both - attention < 1.12 * product, (both, attention, product)
+
+
+def test_portions_that_were_not_made_as_such_are_refused():
+    """What the calls take from them without looking at their rows: types, shapes, how many there are."""
+    import dataclasses
+    s = Setup(H=4, G=2, dim=64)
+    q, out = torch.zeros(5, 4, 64, device="cuda"), torch.zeros(5, 256, device="cuda")
+    x, prep = s.rnd(5, s.ld).cuda(), s.prep()
+    good = s.P.portions8([(0, 2, 0, 0), (2, 3, 1, 5)], s.table)
+    before = s.k.codes.clone()
+    segs = (good.segs.long(), good.segs[:1].expand(2, 4), good.segs.t().contiguous(), good.segs.view(-1), good.segs.float(), good.segs.cpu(), torch.zeros(9, dtype=torch.int32, device="cuda")[1:].view(2, 4))
+    for bad in (dataclasses.replace(good, segs=t) for t in segs):
+        with pytest.raises(ValueError):
+            s.P.append8(x, s.k, s.v, s.table, q, portions=bad, **prep)
+        with pytest.raises(ValueError):
+            s.P.attn_prompt8(q, s.k, s.v, bad, s.table, out, vdim=64, scale=0.1)
+    for bad in (dict(sizes=list(good.sizes)), dict(sizes=good.sizes[:1]), dict(sizes=tuple(x[:2] for x in good.sizes)), dict(sizes=tuple(list(x) for x in good.sizes)), dict(masks=[0, 0, 0]),
+                dict(masks=(0, 0)), dict(table=good.table[0]), dict(table=good.table[:, :2])):
+        with pytest.raises(ValueError):
+            s.P.attn_prompt8(q, s.k, s.v, dataclasses.replace(good, **bad), s.table, out, vdim=64, scale=0.1)
+    for bad in (None, 3, (0, 1)):
+        with pytest.raises((AttributeError, TypeError, ValueError)):
+            s.P.attn_prompt8(q, s.k, s.v, bad, s.table, out, vdim=64, scale=0.1)
+    assert torch.equal(s.k.codes, before) and (out == 0).all()
