@@ -174,15 +174,15 @@ struct Cache {
     Pages8 c;
     PageTable t;
 };
-// `codes` and `unit` of the pages are what ops/pages8.py has checked when it made them.
+// Pages as ops/pages8.py makes them; their tensors may have changed in place since.
 Cache cache(const Signature& s, PyObject* k, PyObject* v, PyObject* table, c10::Device dev) {
     Ref kc(k, s_codes), ku(k, s_unit), vc(v, s_codes), vu(v, s_unit);
-    const at::Tensor &a = tensor(s, kc.o, "k"), &b = tensor(s, vc.o, "v");
-    if (!a.sizes().equals(b.sizes()) || a.device() != dev || b.device() != dev) refuse(s, "keys " + told(a) + ", values " + told(b));
+    const at::Tensor &a = wide(s, piece(s, kc.o, "k", at::kByte, dev), "k"), &b = wide(s, piece(s, vc.o, "v", at::kByte, dev), "v");
+    if (a.dim() != 4 || a.size(2) != PAGE || (a.size(3) != 64 && a.size(3) != 128) || !a.sizes().equals(b.sizes())) refuse(s, "keys " + told(a) + ", values " + told(b));
+    const at::Tensor &ua = shaped(s, ku.o, "k's units", F32, dev, a.size(0), a.size(1)), &ub = shaped(s, vu.o, "v's units", F32, dev, a.size(0), a.size(1));
     const at::Tensor& t = piece(s, table, "table", I32, dev);
-    if (t.dim() != 2) refuse(s, "table " + told(t));
-    return Cache{Pages8{(uint8_t*)a.data_ptr(), (float*)tensor(s, ku.o, "k").data_ptr(), (uint8_t*)b.data_ptr(), (float*)tensor(s, vu.o, "v").data_ptr(), (int)a.size(0), (int)a.size(1),
-                        (int)a.size(3)},
+    if (t.dim() != 2 || !t.numel()) refuse(s, "table " + told(t));
+    return Cache{Pages8{(uint8_t*)a.data_ptr(), (float*)ua.data_ptr(), (uint8_t*)b.data_ptr(), (float*)ub.data_ptr(), (int)a.size(0), (int)a.size(1), (int)a.size(3)},
                  PageTable{(const int*)t.data_ptr(), (int)t.size(0), (int)t.size(1)}};
 }
 

@@ -415,3 +415,31 @@ def test_portions_that_were_not_made_as_such_are_refused():
         with pytest.raises((AttributeError, TypeError, ValueError)):
             s.P.attn_prompt8(q, s.k, s.v, bad, s.table, out, vdim=64, scale=0.1)
     assert torch.equal(s.k.codes, before) and (out == 0).all()
+
+
+def test_pages_that_have_changed_are_refused():
+    """Tensors of a cache that were changed in place after it was made, objects that only look like one, and codes off 16-byte boundaries."""
+    from types import SimpleNamespace
+    s = Setup(H=4, G=2, dim=64)
+    P, x, q, prep = s.P, s.rnd(1, s.ld).cuda(), torch.zeros(1, 4, 64, device="cuda"), s.prep()
+    one, zero = i32([5]), i32([0])
+
+    def calls(k, v, table=s.table):
+        yield lambda: P.append8(x, k, v, table, q, positions=one, slots=zero, **prep)
+        yield lambda: P.attn_decode8(x, k, v, one, zero, table, torch.zeros(1, 256, device="cuda"), scale=0.1, **prep)
+        yield lambda: P.attn_prompt8(q, k, v, P.portions8([(0, 1, 0, 0)], s.table), table, torch.zeros(1, 256, device="cuda"), vdim=64, scale=0.1)
+        yield lambda: P.read8(k, v, i32([[0, 0, 64, 0]]), table, *(torch.zeros(1, 2, 64, 64, device="cuda", dtype=torch.float16) for _ in range(2)))
+    n = s.k.codes.shape[0]
+    short, flat, off = P.Pages8.empty(n, 2, 64), P.Pages8.empty(n, 2, 64), torch.zeros(n * 2 * 64 * 64 + 1, device="cuda", dtype=torch.uint8)[1:].view(n, 2, 64, 64)
+    short.unit.resize_(n - 1, 2)
+    flat.codes.resize_(n, 2 * 64 * 64)
+    bad = [(short, s.v), (s.k, short), (flat, flat), (P.Pages8(off, torch.ones(n, 2, device="cuda")), s.v)]
+    bad += [(SimpleNamespace(codes=s.k.codes, unit=u), s.v) for u in (s.k.unit.double(), s.k.unit.cpu(), s.k.unit.t(), s.k.unit[:, :1])]
+    bad += [(SimpleNamespace(codes=c, unit=s.k.unit), s.v) for c in (s.k.codes.cpu(), s.k.codes.view(torch.int8), s.k.codes[:, :, :32], s.k.codes.transpose(2, 3))]
+    for k, v in bad:
+        for call in calls(k, v):
+            with pytest.raises(ValueError):
+                call()
+    for call in calls(s.k, s.v, s.table[:0]):
+        with pytest.raises(ValueError):
+            call()
