@@ -1,0 +1,485 @@
+// Attention of one token a sequence over the 4-bit cache (kv4.cuh), sm_100a.
+//
+//   out[t][h] = sum_k p_k v_k / (sum_k p_k + exp(sink)),  p_k = exp(cap(scale q . k)),  k the positions up to the token's own that its window has
+//
+// A key costs hd bytes / 2 and 1 / 16 more, a ninth of what its values weigh as fp32, so what bounds the kernel is instructions: those that turn codes into operands (nine for eight codes of a
+// key, ten for eight of a value) rather than the 32-column sums.  Hence keys and values are the row operand of m16n8k16 products and the up to eight query heads of a KV head their columns (half
+// the products of the other way round), codes become f16 numbers -8 .. 7 without their scale, and the scales, one for 32 columns, are applied to what is smaller: a key's to the fp32 sums over its
+// blocks, a value's to the weights, which are rounded to f16 with the scale in them.  Models with more than eight heads a KV head take them eight at a time.
+// Weights are exponents relative to a reference that follows the largest (score + log2 of the value's largest scale): with the scale in it, small values behind a large score keep their f16 digits.
+// The reference moves only when something exceeds it by 2^8, and weights count from 2^7 on, so a key of 2^-21 of the heaviest is an f16 number of full precision and one of 2^-31 still counts.
+// The keys of all sequences and KV heads are dealt out in runs of equal length to the CTAs that fit the GPU; four warps take 32 keys of a run in turn, through rings of their own, so that nothing
+// in the loop waits for another warp.  A second launch adds up the parts.  From raw projections the CTA turns its queries itself, and the one with the token's own position also makes its codes.
+#include "kv4.cuh"
+
+bool kv4_bad_cache(const Cache4& c);
+bool kv4_bad_rows(const Rows4& r, const Cache4& c);
+bool kv4_wide_rows(const Rows4& r);
+
+namespace {
+
+constexpr int WARPS = 4, TURN = 32, GRAIN = WARPS * TURN, HEADS = 8;
+constexpr float LIFT = 7.f, LAG = 8.f, LOG2E = 1.4426950408889634f;
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {      // of an 8 x 8 matrix of f16
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
+template <int BYTES>
+__device__ __forceinline__ void copy_few(uint32_t to, const void* from) { asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(BYTES) : "memory"); }
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float lg2(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <int D>
+struct Lay {
+    static constexpr int NB = D / 32, ROW = D / 2, SC = D / 16;               // blocks, bytes of a row's codes and scales
+    static constexpr int HALF = TURN * (ROW + SC), STAGE = 2 * HALF;          // keys (codes, scales), then values
+    static constexpr int NS = 3, RING = NS * STAGE;
+    static constexpr int LDQ = D + 8;
+    static constexpr int Q_BYTES = HEADS * LDQ * 2, RINGS = WARPS * RING, MERGE = WARPS * HEADS * (D + 4) * 4;
+    static constexpr int TOTAL = Q_BYTES + (RINGS > MERGE ? RINGS : MERGE);
+};
+
+// 16-byte piece of a row where it stands in a stage: rows that a quarter of a warp reads together (of values, every second one) are in different banks
+template <int D>
+__device__ __forceinline__ int piece_at(int row, int piece) { return row * (D / 2) + 16 * (D == 128 ? piece ^ ((row >> 1) & 3) : piece ^ ((row >> 2) & 1)); }
+
+// Which keys a CTA takes: shares of `chunk` keys, as few keys as leave at most `room` shares, sequence by sequence.
+struct Share {
+    int seq, index, count, first, end;      // count: shares of the sequence; keys first .. end - 1
+};
+__device__ __forceinline__ int keys_of(const Rows4& r, const Cache4& c, int window, int b) {
+    const int p = r.positions[b];
+    return kv4::has_row(c, p, r.slots[b]) ? p + 1 - first_key(p, 0, window) : 0;
+}
+__device__ __forceinline__ bool find_share(const Rows4& r, const Cache4& c, int window, int room, int which, int lane, Share& out) {
+    const int n = r.rows;
+    long long sum = 0;
+    for (int b = lane; b < n; b += 32) sum += keys_of(r, c, window, b);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    int chunk = (int)((sum + room - 1) / room);
+    chunk = max(GRAIN, (chunk + GRAIN - 1) / GRAIN * GRAIN);
+    // rounding up each sequence's last share needs at most one more for each: room is at least twice the rows, so this ends at twice the least chunk at the latest
+    for (;; chunk += max(GRAIN, chunk / 32 / GRAIN * GRAIN)) {
+        int shares = 0;
+        for (int b = lane; b < n; b += 32) shares += (keys_of(r, c, window, b) + chunk - 1) / chunk;
+        if ((int)__reduce_add_sync(0xffffffffu, shares) <= room) break;
+    }
+    int before = 0;
+    for (int b0 = 0; b0 < n; b0 += 32) {
+        const int b = b0 + lane, keys = b < n ? keys_of(r, c, window, b) : 0, shares = (keys + chunk - 1) / chunk;
+        int upto = shares;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, which < before + upto);
+        if (hit) {
+            const int l = __ffs(hit) - 1;
+            out.seq = b0 + l;
+            out.count = __shfl_sync(0xffffffffu, shares, l);
+            out.index = which - before - __shfl_sync(0xffffffffu, upto - shares, l);
+            const int all = __shfl_sync(0xffffffffu, keys, l), last = r.positions[out.seq] + 1;
+            out.first = last - all + out.index * chunk;
+            out.end = min(last, out.first + chunk);
+            return true;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return false;
+}
+
+template <int D>
+__global__ void __launch_bounds__(WARPS * 32, 3) attn4_kernel(const __grid_constant__ Attn4Args a, int wide) {
+    using L = Lay<D>;
+    constexpr int NB = L::NB;
+    extern __shared__ __align__(16) unsigned char smem[];
+    __half* sQ = reinterpret_cast<__half*>(smem);                 // [HEADS][LDQ]
+    unsigned char* rings = smem + L::Q_BYTES;
+    __shared__ float s_cs[D / 2], s_sn[D / 2];
+    __shared__ __align__(16) float s_row[WARPS][D];
+    __shared__ __align__(16) uint32_t s_new[2][D / 8];            // the token's own key and value
+    __shared__ __half s_newd[2][NB];
+    __shared__ float s_m[WARPS][HEADS], s_l[WARPS][HEADS];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tq = lane & 3;
+    const Rows4& r = a.r;
+    const int H = r.n_heads, G = a.c.kv_heads, group = H / G, tiles = (group + HEADS - 1) / HEADS;
+    const int kvh = blockIdx.y / tiles, tile = blockIdx.y % tiles, head0 = kvh * group + tile * HEADS, heads = min(HEADS, group - tile * HEADS);
+
+    pdl_launch();
+    pdl_wait();
+    Share sh;
+    if (!find_share(r, a.c, a.window, a.room, blockIdx.x, lane, sh)) return;
+    const int qpos = r.positions[sh.seq], slot = r.slots[sh.seq];
+    if (blockIdx.y == 0 && sh.index == 0 && tid == 0) a.shares[sh.seq] = make_int2(blockIdx.x, sh.count);
+    const size_t row0 = kv4::row_of(a.c, 0, slot, kvh);
+    const int turns = (sh.end - sh.first - TURN * warp + GRAIN - 1) / GRAIN;      // this warp has keys first + TURN (warp + 4 i) ..
+    unsigned char* ring = rings + warp * L::RING;
+    const uint32_t ring_at = smem_u32(ring);
+
+    auto request = [&](int i) {      // keys behind the share repeat its last (masked below)
+        if (i < turns) {
+            const int n0 = sh.first + TURN * (warp + WARPS * i);
+            const uint32_t to = ring_at + i % L::NS * L::STAGE;
+#pragma unroll
+            for (int v = 0; v < 2; v++) {
+                const uint8_t* from = v ? a.c.v : a.c.k;
+                const uint8_t* sc = (const uint8_t*)(v ? a.c.vs : a.c.ks);
+#pragma unroll
+                for (int p = lane; p < TURN * L::ROW / 16; p += 32) {
+                    const int row = p / (L::ROW / 16), piece = p % (L::ROW / 16);
+                    copy16(to + v * L::HALF + piece_at<D>(row, piece), from + (row0 + min(n0 + row, sh.end - 1)) * L::ROW + 16 * piece);
+                }
+                copy_few<L::SC>(to + v * L::HALF + TURN * L::ROW + lane * L::SC, sc + (row0 + min(n0 + lane, sh.end - 1)) * L::SC);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < L::NS - 1; i++) request(i);
+
+    const bool fresh = r.qkv != nullptr, owner = fresh && qpos >= sh.first && qpos < sh.end;
+    if (fresh) {
+        kv4::fill_angles(r, qpos, s_cs, s_sn, tid, WARPS * 32);
+        __syncthreads();
+        const kv4::Turn<D> turn = kv4::make_turn<D>(r, s_cs, s_sn, lane);
+        const float* src = r.qkv + (size_t)sh.seq * r.ldq;
+        // the heads of this CTA, then the key and the value
+        for (int i = warp; i < HEADS + (owner ? 2 : 0); i += WARPS) {
+            constexpr int N = D / 32;
+            float x[N];
+            const bool is_q = i < HEADS, is_k = i == HEADS;
+            if (is_q && i >= heads) {
+#pragma unroll
+                for (int j = 0; j < N; j++) x[j] = 0.f;
+            } else {
+                const float* at = src + (size_t)(is_q ? head0 + i : H + (is_k ? 0 : G) + kvh) * D;
+                if (wide) {
+                    if constexpr (N == 4) {
+                        const float4 y = __ldcg(reinterpret_cast<const float4*>(at) + lane);
+                        x[0] = y.x; x[1] = y.y; x[2] = y.z; x[3] = y.w;
+                    } else {
+                        const float2 y = __ldcg(reinterpret_cast<const float2*>(at) + lane);
+                        x[0] = y.x; x[1] = y.y;
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < N; j++) x[j] = __ldcg(at + N * lane + j);
+                }
+                kv4::prepare_head<D>(x, is_q ? r.q_norm : is_k ? r.k_norm : nullptr, r.eps, is_q || is_k, turn, s_row[warp], lane);
+            }
+            if (is_q) {
+#pragma unroll
+                for (int j = 0; j < N; j += 2) *reinterpret_cast<uint32_t*>(sQ + i * L::LDQ + N * lane + j) = pack(x[j], x[j + 1]);
+            } else {
+                const size_t row = row0 + qpos;
+                const kv4::Coded<D> y = kv4::encode<D>(x, lane);
+                const int v = is_k ? 0 : 1;
+                if (y.lead) {
+                    s_new[v][y.at] = y.word;
+                    if (tile == 0) reinterpret_cast<uint32_t*>(v ? a.c.v : a.c.k)[row * (D / 8) + y.at] = y.word;
+                }
+                if (y.first) {
+                    s_newd[v][y.block] = y.d;
+                    if (tile == 0) reinterpret_cast<__half*>(v ? a.c.vs : a.c.ks)[row * NB + y.block] = y.d;
+                }
+            }
+        }
+    } else {
+        for (int i = tid; i < HEADS * D; i += WARPS * 32) {
+            const int h = i / D, col = i % D;
+            const size_t at = ((size_t)sh.seq * H + head0 + h) * D + col;
+            sQ[h * L::LDQ + col] = h >= heads ? __half(0.f) : a.q16 ? reinterpret_cast<const __half*>(a.q)[at] : __float2half_rn(reinterpret_cast<const float*>(a.q)[at]);
+        }
+    }
+    __syncthreads();
+    // columns 32 b + 8 tq .. of head g: what lane (g, tq) of the key operand has of a row, its word of block b
+    uint32_t qf[NB][4];
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+        const uint4 y = *reinterpret_cast<const uint4*>(sQ + g * L::LDQ + 32 * b + 8 * tq);
+        qf[b][0] = y.x; qf[b][1] = y.y; qf[b][2] = y.z; qf[b][3] = y.w;
+    }
+
+    float o[NB][2][4];
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) o[b][i >> 2][i & 3] = 0.f;
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;      // of heads 2 tq, 2 tq + 1
+    const float mult = a.softcap > 0.f ? a.scale / a.softcap : a.scale * LOG2E, cap2 = a.softcap * LOG2E;
+    const int half = g & 1, sel = half ? 0x7632 : 0x5410;          // which half of a value word's codes: of two keys, side by side
+
+    for (int i = 0; i < turns; i++) {
+        request(i + L::NS - 1);                                                            // into the stage of the turn before
+        asm volatile("cp.async.wait_group %0;" ::"n"(L::NS - 1) : "memory");
+        __syncwarp();
+        unsigned char* st = ring + i % L::NS * L::STAGE;
+        const int n0 = sh.first + TURN * (warp + WARPS * i);
+        if (owner && n0 <= qpos && qpos < n0 + TURN) {      // the token's own row did not come from the cache
+            const int row = qpos - n0;
+            for (int w = lane; w < D / 4; w += 32) {
+                const int v = w / (D / 8), at = w % (D / 8);
+                *reinterpret_cast<uint32_t*>(st + v * L::HALF + piece_at<D>(row, at >> 2) + 4 * (at & 3)) = s_new[v][at];
+            }
+            if (lane < 2 * NB) reinterpret_cast<__half*>(st + lane / NB * L::HALF + TURN * L::ROW)[row * NB + lane % NB] = s_newd[lane / NB][lane % NB];
+            __syncwarp();
+        }
+        const unsigned char* vt = st + L::HALF;
+        float s[2][4];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            s[u][0] = s[u][1] = s[u][2] = s[u][3] = 0.f;
+            const int ra = 16 * u + g, rb = ra + 8;
+            uint32_t ka[NB], kb[NB];
+            float da[NB], db[NB];
+            if constexpr (D == 128) {
+                *reinterpret_cast<uint4*>(ka) = *reinterpret_cast<const uint4*>(st + piece_at<D>(ra, tq));
+                *reinterpret_cast<uint4*>(kb) = *reinterpret_cast<const uint4*>(st + piece_at<D>(rb, tq));
+            } else {
+                *reinterpret_cast<uint2*>(ka) = *reinterpret_cast<const uint2*>(st + piece_at<D>(ra, tq >> 1) + 8 * (tq & 1));
+                *reinterpret_cast<uint2*>(kb) = *reinterpret_cast<const uint2*>(st + piece_at<D>(rb, tq >> 1) + 8 * (tq & 1));
+            }
+            const __half2* sa = reinterpret_cast<const __half2*>(st + TURN * L::ROW + ra * L::SC);
+            const __half2* sb = reinterpret_cast<const __half2*>(st + TURN * L::ROW + rb * L::SC);
+#pragma unroll
+            for (int b = 0; b < NB; b += 2) {
+                const float2 x = __half22float2(sa[b / 2]), y = __half22float2(sb[b / 2]);
+                da[b] = x.x; da[b + 1] = x.y; db[b] = y.x; db[b + 1] = y.y;
+            }
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                uint32_t e[4], f[4];
+                kv4::expand(ka[b], e);
+                kv4::expand(kb[b], f);
+                float c[4] = {0.f, 0.f, 0.f, 0.f};
+                mma(c, e[0], f[0], e[1], f[1], qf[b][0], qf[b][1]);
+                mma(c, e[2], f[2], e[3], f[3], qf[b][2], qf[b][3]);
+                s[u][0] += c[0] * da[b]; s[u][1] += c[1] * da[b];
+                s[u][2] += c[2] * db[b]; s[u][3] += c[3] * db[b];
+            }
+        }
+        // s[u][0, 1]: key 16 u + g, heads 2 tq, 2 tq + 1; s[u][2, 3]: key 16 u + 8 + g.  To powers of two; the values' scales
+        float dv[4][NB], big[4];
+        float y0 = -INFINITY, y1 = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {      // key 8 k + g
+            const __half2* sc = reinterpret_cast<const __half2*>(vt + TURN * L::ROW + (8 * k + g) * L::SC);
+            float top = 5.9604644775390625e-8f;      // 2^-24: rows of zeros
+#pragma unroll
+            for (int b = 0; b < NB; b += 2) {
+                const float2 x = __half22float2(sc[b / 2]);
+                dv[k][b] = x.x;
+                dv[k][b + 1] = x.y;
+                top = fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y)));
+            }
+            big[k] = lg2(top);
+            float& v0 = s[k >> 1][2 * (k & 1)];
+            float& v1 = s[k >> 1][2 * (k & 1) + 1];
+            v0 *= mult;
+            v1 *= mult;
+            if (a.softcap > 0.f) {
+                v0 = cap2 * tanh_exp(v0);
+                v1 = cap2 * tanh_exp(v1);
+            }
+            if (n0 + 8 * k + g >= sh.end) v0 = v1 = -INFINITY;
+            y0 = fmaxf(y0, v0 + big[k]);
+            y1 = fmaxf(y1, v1 + big[k]);
+        }
+        if (__any_sync(0xffffffffu, y0 > m0 + LAG || y1 > m1 + LAG)) {
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) {
+                y0 = fmaxf(y0, __shfl_xor_sync(0xffffffffu, y0, x));
+                y1 = fmaxf(y1, __shfl_xor_sync(0xffffffffu, y1, x));
+            }
+            const float n0m = fmaxf(m0, y0), n1m = fmaxf(m1, y1);
+            const float f0 = n0m == -INFINITY ? 1.f : ex2(m0 - n0m), f1 = n1m == -INFINITY ? 1.f : ex2(m1 - n1m);
+            m0 = n0m;
+            m1 = n1m;
+            l0 *= f0;
+            l1 *= f1;
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int t = 0; t < 2; t++) {
+                    o[b][t][0] *= f0; o[b][t][1] *= f1;
+                    o[b][t][2] *= f0; o[b][t][3] *= f1;
+                }
+        }
+        const float r0 = m0 == -INFINITY ? 0.f : m0 - LIFT, r1 = m1 == -INFINITY ? 0.f : m1 - LIFT;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            float& v0 = s[k >> 1][2 * (k & 1)];
+            float& v1 = s[k >> 1][2 * (k & 1) + 1];
+            v0 = ex2(v0 - r0);
+            v1 = ex2(v1 - r1);
+            l0 += v0;
+            l1 += v1;
+        }
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            // words of block b of keys 16 u + 2 tq, + 1, + 8, + 9, of which this lane's dims are 32 b + 8 (g / 2) + 2 i + half
+            const int rr = 16 * u + 2 * tq, j = g >> 1;
+            uint32_t w[4][NB];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int row = rr + (k & 1) + 8 * (k >> 1);
+                if constexpr (D == 128) *reinterpret_cast<uint4*>(w[k]) = *reinterpret_cast<const uint4*>(vt + piece_at<D>(row, j));
+                else *reinterpret_cast<uint2*>(w[k]) = *reinterpret_cast<const uint2*>(vt + piece_at<D>(row, j >> 1) + 8 * (j & 1));
+            }
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                const uint32_t p0 = transposed(pack(s[u][0] * dv[2 * u][b], s[u][1] * dv[2 * u][b]));
+                const uint32_t p1 = transposed(pack(s[u][2] * dv[2 * u + 1][b], s[u][3] * dv[2 * u + 1][b]));
+                uint32_t e[4], f[4];
+                kv4::expand(__byte_perm(w[0][b], w[1][b], sel), e);
+                kv4::expand(__byte_perm(w[2][b], w[3][b], sel), f);
+                mma(o[b][0], e[0], e[1], f[0], f[1], p0, p1);
+                mma(o[b][1], e[2], e[3], f[2], f[3], p0, p1);
+            }
+        }
+        __syncwarp();        // every lane is done with this stage before the next turn's request overwrites it
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+
+    // the warps' parts
+#pragma unroll
+    for (int x = 4; x < 32; x <<= 1) {
+        l0 += __shfl_xor_sync(0xffffffffu, l0, x);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, x);
+    }
+    __syncthreads();         // behind it the rings are free
+    constexpr int LDO = D + 4;
+    float* s_acc = reinterpret_cast<float*>(rings);      // [WARPS][HEADS][LDO]
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                s_acc[(warp * HEADS + 2 * tq + (e & 1)) * LDO + 32 * b + 8 * (g >> 1) + 2 * (2 * t + (e >> 1)) + half] = o[b][t][e];
+    if (g == 0) {
+        s_m[warp][2 * tq] = m0; s_m[warp][2 * tq + 1] = m1;
+        s_l[warp][2 * tq] = l0; s_l[warp][2 * tq + 1] = l1;
+    }
+    __syncthreads();
+    for (int i = tid; i < heads * (D / 4); i += WARPS * 32) {
+        const int h = i / (D / 4), col = i % (D / 4) * 4;
+        const float m = fmaxf(fmaxf(s_m[0][h], s_m[1][h]), fmaxf(s_m[2][h], s_m[3][h]));
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        float l = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; w++) {
+            const float f = s_m[w][h] == -INFINITY ? 0.f : ex2(s_m[w][h] - m);
+            const float4 y = *reinterpret_cast<const float4*>(s_acc + (w * HEADS + h) * LDO + col);
+            acc.x += y.x * f; acc.y += y.y * f; acc.z += y.z * f; acc.w += y.w * f;
+            l += s_l[w][h] * f;
+        }
+        const size_t at = (size_t)blockIdx.x * H + head0 + h;
+        *reinterpret_cast<float4*>(a.part_acc + at * D + col) = acc;
+        if (col == 0) a.part_ml[at] = make_float2(m - LIFT, l);
+    }
+}
+
+// Adds up the parts of a head: grid (heads, sequences), four warps, each every fourth part, a lane D / 32 columns.
+template <int D>
+__global__ void __launch_bounds__(128) merge4_kernel(const __grid_constant__ Attn4Args a) {
+    constexpr int N = D / 32;
+    __shared__ float s_acc[4][D];
+    __shared__ float s_l[4];
+    const int h = blockIdx.x, b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, H = a.r.n_heads;
+    pdl_launch();
+    pdl_wait();
+    if (!kv4::has_row(a.c, a.r.positions[b], a.r.slots[b])) return;      // no token: the row stays as it is
+    const int2 sh = a.shares[b];
+    float m = -INFINITY;
+    for (int p = lane; p < sh.y; p += 32) m = fmaxf(m, a.part_ml[(size_t)(sh.x + p) * H + h].x);
+    m = warp_max(m);
+    const float sink = a.sinks ? a.sinks[h] * LOG2E : -INFINITY;
+    m = fmaxf(m, sink);
+    const float ref = m == -INFINITY ? 0.f : m;
+    float acc[N], l = 0.f;
+#pragma unroll
+    for (int j = 0; j < N; j++) acc[j] = 0.f;
+#pragma unroll 4
+    for (int p = warp; p < sh.y; p += 4) {
+        const size_t at = (size_t)(sh.x + p) * H + h;
+        const float2 ml = a.part_ml[at];
+        const float f = ex2(ml.x - ref);
+        if constexpr (N == 4) {
+            const float4 y = __ldcg(reinterpret_cast<const float4*>(a.part_acc + at * D) + lane);
+            acc[0] += y.x * f; acc[1] += y.y * f; acc[2] += y.z * f; acc[3] += y.w * f;
+        } else {
+            const float2 y = __ldcg(reinterpret_cast<const float2*>(a.part_acc + at * D) + lane);
+            acc[0] += y.x * f; acc[1] += y.y * f;
+        }
+        l += ml.y * f;
+    }
+#pragma unroll
+    for (int j = 0; j < N; j++) s_acc[warp][N * lane + j] = acc[j];
+    if (lane == 0) s_l[warp] = l;
+    __syncthreads();
+    const int col = threadIdx.x;
+    if (col >= D) return;
+    l = s_l[0] + s_l[1] + s_l[2] + s_l[3];
+    if (sink > -INFINITY) l += ex2(sink - ref);
+    const float y = (s_acc[0][col] + s_acc[1][col] + s_acc[2][col] + s_acc[3][col]) / l;
+    const size_t at = (size_t)b * a.ldo + (size_t)h * D + col;
+    if (a.out16) reinterpret_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(y);
+    else reinterpret_cast<float*>(a.out)[at] = y;
+}
+
+}  // namespace
+
+// CTAs of a launch for one KV head and eight of its query heads, and the parts that they leave: as many as fit the GPU, at least two a sequence.
+B2_API int b2_attn4_room(int rows, int n_heads, int kv_heads, int sms) {
+    const long group = n_heads / kv_heads, units = (long)kv_heads * ((group + HEADS - 1) / HEADS), fit = 3l * sms / units;
+    return (int)(fit > 2l * rows ? fit : 2l * rows);
+}
+
+// Two launches.  part_acc, part_ml and shares are scratch of a.room parts (b2_attn4_room) and a.r.rows sequences.
+B2_API int b2_attn4(const Attn4Args* in, int pdl, cudaStream_t st) {
+    Attn4Args a = *in;
+    if (kv4_bad_cache(a.c) || (a.r.qkv && kv4_bad_rows(a.r, a.c)) || (!a.r.qkv && !a.q) || a.r.rows < 0 || a.r.n_heads < 1 || a.r.n_heads % a.c.kv_heads) return (int)cudaErrorInvalidValue;
+    if (!a.r.rows) return 0;
+    const int group = a.r.n_heads / a.c.kv_heads, tiles = (group + HEADS - 1) / HEADS;
+    if (!a.r.positions || !a.r.slots || !a.out || !a.part_acc || !a.part_ml || !a.shares || a.window < 0 || a.room < 2 * a.r.rows || a.r.rows > 65535 || (long)a.c.kv_heads * tiles > 65535 ||
+        a.ldo < a.r.n_heads * a.c.hd)
+        return (int)cudaErrorInvalidValue;
+    int wide = kv4_wide_rows(a.r);
+    void* args[] = {&a, &wide};
+    const bool big = a.c.hd == 128;
+    const void* fn = big ? (const void*)attn4_kernel<128> : (const void*)attn4_kernel<64>;
+    const int smem = big ? Lay<128>::TOTAL : Lay<64>::TOTAL;
+    static thread_local PerDeviceOnce once;
+    if (once.first()) {
+        cudaError_t e = cudaFuncSetAttribute((const void*)attn4_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay<128>::TOTAL);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute((const void*)attn4_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay<64>::TOTAL);
+        if (e != cudaSuccess) return (int)e;
+    }
+    const int rc = launch_rows(fn, dim3(a.room, a.c.kv_heads * tiles), dim3(WARPS * 32), smem, args, st, pdl);
+    if (rc) return rc;
+    void* margs[] = {&a};
+    return launch_rows(big ? (const void*)merge4_kernel<128> : (const void*)merge4_kernel<64>, dim3(a.r.n_heads, a.r.rows), dim3(128), 0, margs, st, pdl);
+}

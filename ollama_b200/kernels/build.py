@@ -42,6 +42,10 @@ GROUPS = {"stack": ("attn_decode_mma.cu", "attn_latent.cu", "attn_paged.cu", "at
                     "gru.cu", "latent.cu", "moe.cu", "moe_rows.cu", "norm_rows.cu", "pages8.cu", "sample.cu", "ssd.cu", "ssd_chunk.cu", "ssm.cu")}
 
 
+# modules of calls (ops/<name>_call.cpp) and the kernel source that says which argument blocks (<name>_args.h) the library takes
+CALLS = {"pages8": "pages8.cu", "kv4": "kv4.cu"}
+
+
 def build_group(group: str, verbose: bool = False, force: bool = False) -> str:
     """Compile the sources of ``group`` and link them into a library of their own; their objects are the ones a later full build uses."""
     lib = os.path.join(HERE, f"libb200{group}.so")
@@ -54,7 +58,8 @@ def build_group(group: str, verbose: bool = False, force: bool = False) -> str:
 def build(verbose: bool = False, force: bool = False) -> str:
     _compile(sorted(f for f in os.listdir(HERE) if f.endswith(".cu")), LIB, verbose, force)
     build_host(verbose, force)
-    build_calls(verbose, force)
+    for what in CALLS:
+        build_calls(verbose, force, what)
     return LIB
 
 
@@ -67,7 +72,7 @@ def _compile(srcs: list[str], lib: str, verbose: bool, force: bool) -> None:
     for s in srcs:
         src, obj = os.path.join(HERE, s), os.path.join(objdir, s[:-3] + ".o")
         if force or _stale(obj, [src] + hdrs):
-            cmd = [nvcc, *NVCC_FLAGS, *([_layout_flag()] if s == "pages8.cu" else []), "-c", src, "-o", obj] + (["-Xptxas", "-v"] if verbose else [])
+            cmd = [nvcc, *NVCC_FLAGS, *(_layout_flag(n) for n, of in CALLS.items() if of == s), "-c", src, "-o", obj] + (["-Xptxas", "-v"] if verbose else [])
             jobs.append((s, cmd))
 
     def run(job):
@@ -119,35 +124,35 @@ def _text(*path: str) -> bytes:
         return f.read()
 
 
-def _layout_flag() -> str:
-    """What the kernel library and the module of calls are both compiled with: a number that follows from the argument blocks that they share."""
-    return f"-DPAGES8_LAYOUT=0x{hashlib.sha256(_text(HERE, 'pages8_args.h')).hexdigest()[:16]}ull"
+def _layout_flag(what: str = "pages8") -> str:
+    """What the kernel library and a module of calls are both compiled with: a number that follows from the argument blocks that they share."""
+    return f"-D{what.upper()}_LAYOUT=0x{hashlib.sha256(_text(HERE, f'{what}_args.h')).hexdigest()[:16]}ull"
 
 
-def calls_path() -> str:
-    """The module of calls for this Python and torch, of the sources as they are: one that was built for others, or from others, has another name."""
+def calls_path(what: str = "pages8") -> str:
+    """A module of calls for this Python and torch, of the sources as they are: one that was built for others, or from others, has another name."""
     import torch
     ops = os.path.join(os.path.dirname(HERE), "ops")
-    made_from = hashlib.sha256(_text(ops, "pages8_call.cpp") + _text(HERE, "pages8_args.h")).hexdigest()[:12]
-    return os.path.join(ops, f"_pages8.{sys.implementation.cache_tag}-torch{torch.__version__}.{made_from}.so")
+    made_from = hashlib.sha256(_text(ops, f"{what}_call.cpp") + _text(ops, "call_args.h") + _text(HERE, f"{what}_args.h")).hexdigest()[:12]
+    return os.path.join(ops, f"_{what}.{sys.implementation.cache_tag}-torch{torch.__version__}.{made_from}.so")
 
 
-def build_calls(verbose: bool = False, force: bool = False) -> str:
-    """The Python module of calls whose arguments are checked in C++ (ops/pages8_call.cpp); needs torch's headers, no GPU."""
-    src, out = os.path.join(os.path.dirname(HERE), "ops", "pages8_call.cpp"), calls_path()
+def build_calls(verbose: bool = False, force: bool = False, what: str = "pages8") -> str:
+    """A Python module of calls whose arguments are checked in C++ (ops/<what>_call.cpp); needs torch's headers, no GPU."""
+    src, out = os.path.join(os.path.dirname(HERE), "ops", f"{what}_call.cpp"), calls_path(what)
     if force or not os.path.exists(out):
         import sysconfig
 
         from torch.utils.cpp_extension import include_paths, library_paths
         cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
         part = f"{out}.{os.getpid()}"
-        cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", _layout_flag(), *(f"-I{d}" for d in (*include_paths(), os.path.join(cuda, "include"), sysconfig.get_paths()["include"])),
+        cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", _layout_flag(what), *(f"-I{d}" for d in (*include_paths(), os.path.join(cuda, "include"), sysconfig.get_paths()["include"])),
                "-o", part, src, *(f"-L{d}" for d in (*library_paths(), os.path.join(cuda, "lib64"))), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-lcudart"]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if verbose or r.returncode:
             sys.stderr.write(r.stdout + r.stderr)
         if r.returncode:
-            raise RuntimeError("g++ failed on pages8_call.cpp")
+            raise RuntimeError(f"g++ failed on {what}_call.cpp")
         os.replace(part, out)
         for old in glob.glob(glob.escape(out.rsplit(".", 2)[0]) + ".*.so"):          # of the same Python and torch
             if old != out:
