@@ -480,6 +480,6 @@ B2_API int b2_attn4(const Attn4Args* in, int pdl, cudaStream_t st) {
     }
     const int rc = launch_rows(fn, dim3(a.room, a.c.kv_heads * tiles), dim3(WARPS * 32), smem, args, st, pdl);
     if (rc) return rc;
-    void* margs[] = {&a};
-    return launch_rows(big ? (const void*)merge4_kernel<128> : (const void*)merge4_kernel<64>, dim3(a.r.n_heads, a.r.rows), dim3(128), 0, margs, st, pdl);
+    void* margs[] = {&a};      // (its CTAs may wait beside the first launch's last)
+    return launch_rows(big ? (const void*)merge4_kernel<128> : (const void*)merge4_kernel<64>, dim3(a.r.n_heads, a.r.rows), dim3(128), 0, margs, st, 1);
 }

@@ -64,17 +64,20 @@ struct Attn4Args {
     int2* shares;            // [rows] (first share, shares) of each sequence
 };
 
-// A tile of query rows of one portion (attn_packed.cu): up to 2 x floor(128 / group) tokens, for the heads of one KV head after the other.
-struct PackedTile {
+// A run of key tiles for a tile of query rows of one portion and KV head (attn_packed.cu): up to 2 x floor(128 / group) tokens.
+struct alignas(16) PackedTile {
     int row, rows;           // query rows
     int slot, pos;           // of the cache; position of the first row
     int base;                // cache row of the sequence's position 0
-    int k_lo, k_hi;          // tiles of 128 keys that this share of the tile's keys has
-    int part;                // -1: all of them; else which partial result it leaves, of a merge's
+    int k_lo, k_hi;          // tiles of 128 keys
+    int part;                // -1: all that the rows see; else which partial result it leaves
+    int kvh;
+    int pad[3];
 };
 // What a merge adds up: `parts` partial results from `first` on of `rows` query rows.
-struct PackedMerge {
-    int row, rows, first, parts;
+struct alignas(16) PackedMerge {
+    int row, rows, first, parts, kvh;
+    int pad[3];
 };
 
 struct PackedArgs {
@@ -89,7 +92,8 @@ struct PackedArgs {
     int slots, n;
     Cache4 c;
     const PackedTile* tiles;
-    int n_tiles;
+    const int* starts;       // [ctas + 1]: CTA i takes tile i, then starts[i] .. starts[i + 1] - 1
+    int ctas;
     const PackedMerge* merges;
     int n_merges, parts;
     float scale, softcap;
@@ -97,6 +101,6 @@ struct PackedArgs {
     const float* sinks;
     void* out;               // [rows][ldo], head h at column h * hd
     int ldo, out_type;       // 0 fp32, 1 f16, 2 bf16
-    float* part_acc;         // [parts][kv_heads][256][hd]
-    float2* part_ml;         // [parts][kv_heads][256]
+    float* part_acc;         // [parts][256][hd]
+    float2* part_ml;         // [parts][256]
 };

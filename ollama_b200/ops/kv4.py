@@ -14,7 +14,6 @@ import importlib.util
 import threading
 from dataclasses import dataclass
 
-import numpy as np
 import torch
 
 from .cuda import CudaKernelError, lib
@@ -74,31 +73,14 @@ def decode4(codes: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
 class Portions4:
     """Rows of several sequences in a step, for :func:`attn_prompt4` and :func:`attn_packed`: what a model makes once for a step of all its layers."""
 
-    tiles: torch.Tensor              # [n, 8] int32: first row, rows, slot, position, cache row of position 0, key tiles from .. to, partial result or -1
-    merges: torch.Tensor             # [m, 4] int32: first row, rows, first partial result, partial results
+    tiles: torch.Tensor              # [n, 12] int32: first row, rows, slot, position, cache row of position 0, key tiles from .. to, partial result or -1, KV head
+    merges: torch.Tensor             # [m, 8] int32: first row, rows, first partial result, partial results, KV head
+    starts: torch.Tensor             # [CTAs + 1] int32: CTA i takes tile i, then starts[i] .. starts[i + 1] - 1
     rows: int                        # of all portions
     parts: int                       # partial results
     window: int
     group: int                       # query heads a KV head
     cache: tuple[int, int, int, int]
-
-
-# A CTA's start and end, and the second launch where keys are shared out, in the time of a tile of 128 keys
-CTA_TILES, MERGE_TILES = 4, 3
-
-
-def _share_length(sizes: np.ndarray, kv_heads: int, sms: int) -> int:
-    """Most key tiles of a CTA: that with which the launch is estimated to end first.  A launch ends about when its CTAs' time, spread over the SMs, and half of a CTA have passed, and not before
-    its longest CTA."""
-    best, length = None, int(sizes.max())
-    for n in sorted({-(-length // k) for k in (1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128)}, reverse=True):
-        shares = -(-sizes // n)
-        most, count = int((-(-sizes // shares)).max()) + CTA_TILES, int(shares.sum()) * kv_heads
-        work = (int(sizes.sum()) * kv_heads + CTA_TILES * count) / sms
-        time = max(most, work + (most / 2 if count > sms else 0)) + (MERGE_TILES if n < length else 0)
-        if best is None or time < best:
-            best, length_best = time, n
-    return length_best
 
 
 def portions4(parts, heads: int, k, *, window: int = 0) -> Portions4:
@@ -107,37 +89,22 @@ def portions4(parts, heads: int, k, *, window: int = 0) -> Portions4:
     slots, kv_heads, n_ctx, dim = k.shape
     if heads < 1 or heads % kv_heads or heads // kv_heads > TILE or window < 0:
         raise ValueError(f"portions4: {heads} heads on {kv_heads}, window {window}")
-    group = heads // kv_heads
-    step, at, tiles = 2 * (TILE // group), 0, []
+    at, rows = 0, []
     for row, n, slot, pos, *more in parts:
         base = more[0] if more else 0
         if n < 1 or row != at or not 0 <= slot < slots or pos < 0 or base < 0 or base + pos + n > n_ctx:
             raise ValueError(f"portions4: {n} rows from {row} on at position {pos} of slot {slot}, from row {base} on, in a cache of {slots} slots of {n_ctx}")
         at += n
-        for r in range(0, n, step):
-            m, p = min(step, n - r), pos + r
-            tiles.append((row + r, m, slot, p, base, max(0, p - window + 1) // TILE if window else 0, (p + m - 1) // TILE + 1))
+        rows.append((row, n, slot, pos, base))
     if not at:
         raise ValueError("portions4: no rows")
     dev = k.codes.device if isinstance(k, Cache4) else k.device
     sms = torch.cuda.get_device_properties(dev).multi_processor_count if dev.type == "cuda" else 148
-    t = np.asarray(tiles, np.int32)
-    sizes = t[:, 6] - t[:, 5]
-    length = _share_length(sizes, kv_heads, sms)
-    out, merges, n_parts = [], [], 0
-    for tile, size in zip(tiles, sizes.tolist()):
-        shares = -(-size // length)
-        if shares == 1:
-            out.append((*tile, -1))
-            continue
-        merges.append((tile[0], tile[1], n_parts, shares))
-        for i in range(shares):
-            out.append((*tile[:5], tile[5] + size * i // shares, tile[5] + size * (i + 1) // shares, n_parts))
-            n_parts += 1
-    out.sort(key=lambda x: x[5] - x[6])          # the longest first
-    out, merges = np.asarray(out, np.int32), np.asarray(merges, np.int32).reshape(-1, 4)
-    flat = torch.from_numpy(np.concatenate([out.reshape(-1), merges.reshape(-1)])).to(dev)
-    return Portions4(flat[:out.size].view(out.shape), flat[out.size:].view(merges.shape), at, n_parts, window, group, (slots, kv_heads, n_ctx, dim))
+    here = globals()
+    *lists, n_parts = (here.get("_plan") or __getattr__("_plan"))(torch.tensor(rows, dtype=torch.int32), heads // kv_heads, kv_heads, window, sms)
+    flat = torch.cat([x.view(-1) for x in lists]).to(dev)
+    tiles, merges, starts = (t.view(x.shape) for t, x in zip(flat.split([x.numel() for x in lists]), lists))
+    return Portions4(tiles, merges, starts.view(-1), at, n_parts, window, heads // kv_heads, (slots, kv_heads, n_ctx, dim))
 
 
 CALLS = ("append4", "read4", "attn_decode4", "attn_step4", "attn_prompt4", "attn_packed")
@@ -169,12 +136,12 @@ def load() -> None:
         if CALLS[0] not in globals():
             m = _module()
             _bind(m)
-            globals().update({n: getattr(m, n) for n in CALLS})
+            globals().update({n: getattr(m, n) for n in CALLS}, _plan=m.plan)
 
 
 def __getattr__(name: str):
     """The calls, when one is first asked for."""
-    if name not in CALLS:
+    if name not in (*CALLS, "_plan"):
         raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
     load()
     return globals()[name]

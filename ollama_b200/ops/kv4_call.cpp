@@ -1,6 +1,9 @@
 // Calls of the 4-bit cache and of packed prompts from Python: the checks of their arguments, the argument blocks, workspaces, and the entry points of the kernel library.
 #include "call_args.h"
 
+#include <queue>
+#include <vector>
+
 #include "../kernels/kv4_args.h"
 
 namespace {
@@ -11,7 +14,7 @@ int (*f_read)(const Read4Args*, int, cudaStream_t);
 int (*f_attn)(const Attn4Args*, int, cudaStream_t);
 int (*f_room)(int, int, int, int);
 int (*f_packed)(const PackedArgs*, int, cudaStream_t);
-PyObject *s_codes, *s_scale, *s_tiles, *s_merges, *s_rows, *s_parts, *s_window, *s_group, *s_cache;
+PyObject *s_codes, *s_scale, *s_tiles, *s_starts, *s_merges, *s_rows, *s_parts, *s_window, *s_group, *s_cache;
 
 // A cache as ops/kv4.py makes it; its tensors may have changed in place since.
 Cache4 cache(const Signature& s, PyObject* k, PyObject* v, c10::Device dev) {
@@ -254,7 +257,7 @@ long prompt(const Signature& s, PyObject** a, bool codes) {
     p.sinks = k.sinks;
     // tiles of other heads, masks or caches would point elsewhere
     PyObject* o = a[P_PORTIONS];
-    Ref tiles(o, s_tiles), merges(o, s_merges), rows(o, s_rows), parts(o, s_parts), window(o, s_window), group(o, s_group), cached(o, s_cache);
+    Ref tiles(o, s_tiles), starts(o, s_starts), merges(o, s_merges), rows(o, s_rows), parts(o, s_parts), window(o, s_window), group(o, s_group), cached(o, s_cache);
     const long of[4] = {slots, p.kv_heads, n_ctx, p.hd};
     if (!PyTuple_Check(cached.o) || PyTuple_GET_SIZE(cached.o) != 4) refuse(s, "portions that are not what portions4 makes");
     for (int i = 0; i < 4; i++)
@@ -262,10 +265,11 @@ long prompt(const Signature& s, PyObject** a, bool codes) {
     if (as_long(window.o, 0) != p.window) refuse(s, "portions that were made with another window");
     if (as_long(group.o, 0) * p.kv_heads != heads) refuse(s, "portions that were made for " + std::to_string(as_long(group.o, 0)) + " heads a KV head");
     if (as_long(rows.o, 0) > n) refuse(s, "portions of " + std::to_string(as_long(rows.o, 0)) + " rows for " + std::to_string(n));
-    const at::Tensor &t = piece(s, tiles.o, "portions", I32, dev), &u = piece(s, merges.o, "portions", I32, dev);
-    if (t.dim() != 2 || t.size(1) * 4 != (long)sizeof(PackedTile) || u.dim() != 2 || u.size(1) * 4 != (long)sizeof(PackedMerge)) refuse(s, "portions " + told(t));
+    const at::Tensor &t = wide(s, piece(s, tiles.o, "portions", I32, dev), "portions"), &u = wide(s, piece(s, merges.o, "portions", I32, dev), "portions"), &w = piece(s, starts.o, "portions", I32, dev);
+    if (t.dim() != 2 || t.size(1) * 4 != (long)sizeof(PackedTile) || u.dim() != 2 || u.size(1) * 4 != (long)sizeof(PackedMerge) || w.dim() != 1 || w.numel() < 2) refuse(s, "portions " + told(t));
     p.tiles = (const PackedTile*)t.data_ptr();
-    p.n_tiles = (int)t.size(0);
+    p.starts = (const int*)w.data_ptr();
+    p.ctas = (int)w.numel() - 1;
     p.merges = (const PackedMerge*)u.data_ptr();
     p.n_merges = (int)u.size(0);
     p.parts = (int)as_long(parts.o, 0);
@@ -275,7 +279,7 @@ long prompt(const Signature& s, PyObject** a, bool codes) {
     p.out_type = out.scalar_type() == F32 ? 0 : out.scalar_type() == F16 ? 1 : 2;
     const bool pdl = as_bool(a[P_PDL], false);
     launched(s, unlocked(dev, [&](cudaStream_t st) {
-        const long rows256 = (long)p.parts * p.kv_heads * 256;
+        const long rows256 = (long)p.parts * 256;
         at::Tensor ws;
         if (rows256) {
             ws = floats(dev, rows256 * (p.hd + 2));
@@ -287,7 +291,100 @@ long prompt(const Signature& s, PyObject** a, bool codes) {
     return p.n_merges ? 2 : 1;
 }
 
+// ---- portions -------------------------------------------------------------------------------------------------------------------
+// What a share's start and end, and adding up partial results, cost in the time of a tile of 128 keys; fewer tiles than LEAST are not made a share of their own.
+constexpr int SHARE_TILES = 2, MERGE_TILES = 3, LEAST = 2;
+
+Signature plan_sig = {"plan", 5, 5, {"parts", "group", "kv_heads", "window", "sms"}};
+// plan(parts, group, kv_heads, window, sms): shares and merges for portions [n, 5] int32 (first row, rows, slot, position, cache row of position 0), as int32 tensors [., 12] and [., 8], where
+// each CTA's shares begin, and the number of partial results.  All tiles as they are, the longest first to the CTA that has least to do, where that ends about when equal shares would; else
+// tiles are cut where a CTA has its share.
+PyObject* plan(PyObject** a) {
+    const Signature& s = plan_sig;
+    for (int i = 0; i < 5; i++) required(s, a, i);
+    const at::Tensor& parts = piece(s, a[0], "parts", I32, c10::Device(c10::kCPU));
+    const long group = as_long(a[1], 1), heads = as_long(a[2], 1), window = as_long(a[3], 0), sms = as_long(a[4], 1);
+    if (parts.dim() != 2 || parts.size(1) != 5 || group < 1 || group > 128 || heads < 1 || sms < 1 || window < 0) refuse(s, "parts " + told(parts));
+    const int* from = (const int*)parts.data_ptr();
+    const long step = 2 * (128 / group);
+    std::vector<PackedTile> whole, out;
+    std::vector<PackedMerge> merges;
+    long work = 0;
+    for (long i = 0; i < parts.size(0); i++, from += 5)
+        for (long r = 0; r < from[1]; r += step) {
+            PackedTile t = {};
+            t.row = (int)(from[0] + r);
+            t.rows = (int)std::min<long>(step, from[1] - r);
+            t.slot = from[2];
+            t.pos = (int)(from[3] + r);
+            t.base = from[4];
+            t.k_lo = window ? std::max(0l, t.pos - window + 1) / 128 : 0;
+            t.k_hi = (t.pos + t.rows - 1) / 128 + 1;
+            t.part = -1;
+            for (t.kvh = 0; t.kvh < heads; t.kvh++) whole.push_back(t);
+            work += heads * (t.k_hi - t.k_lo);
+        }
+    std::stable_sort(whole.begin(), whole.end(), [](const PackedTile& x, const PackedTile& y) { return x.k_hi - x.k_lo > y.k_hi - y.k_lo; });
+    const long n = (long)whole.size(), share = std::max<long>((work + SHARE_TILES * (n + sms) + sms - 1) / sms, SHARE_TILES + LEAST);      // about one cut an SM
+    int n_parts = 0;
+    using Load = std::pair<long, int>;       // what a CTA has to do
+    using Least = std::priority_queue<Load, std::vector<Load>, std::greater<Load>>;
+    std::vector<std::vector<PackedTile>> of(std::min(n, sms));
+    auto all = [&] {
+        Least q;
+        for (int i = 0; i < (int)of.size(); i++) q.push({0, i});
+        return q;
+    };
+    Least q = all();
+    long last = 0;
+    for (const PackedTile& t : whole) {
+        Load x = q.top();
+        q.pop();
+        x.first += t.k_hi - t.k_lo + SHARE_TILES;
+        last = std::max(last, x.first);
+        of[x.second].push_back(t);
+        q.push(x);
+    }
+    if (last > share + MERGE_TILES) {
+        of.assign(sms, {});
+        q = all();
+        for (const PackedTile& t : whole) {
+            int lo = t.k_lo;
+            const int first = n_parts;
+            while (lo < t.k_hi) {
+                Load x = q.top();
+                q.pop();
+                const long left = t.k_hi - lo;
+                long take = std::min(left, std::max<long>(share - x.first - SHARE_TILES, LEAST));
+                if (left - take < LEAST) take = left;
+                PackedTile y = t;
+                y.k_lo = lo;
+                y.k_hi = lo += (int)take;
+                if (take < t.k_hi - t.k_lo) y.part = n_parts++;
+                of[x.second].push_back(y);
+                x.first += take + SHARE_TILES;
+                q.push(x);
+            }
+            if (n_parts > first) merges.push_back(PackedMerge{t.row, t.rows, first, n_parts - first, t.kvh, {}});
+        }
+        of.erase(std::remove_if(of.begin(), of.end(), [](const auto& x) { return x.empty(); }), of.end());
+    }
+    for (const auto& x : of) out.push_back(x[0]);
+    std::vector<int> starts(1, (int)out.size());
+    for (const auto& x : of) {
+        out.insert(out.end(), x.begin() + 1, x.end());
+        starts.push_back((int)out.size());
+    }
+    auto tensor_of = [](const void* p, size_t n, int columns) {
+        at::Tensor t = at::empty({(long)n, (long)columns}, at::TensorOptions().dtype(I32));
+        if (n) std::memcpy(t.data_ptr(), p, n * columns * 4);
+        return THPVariable_Wrap(t);
+    };
+    return Py_BuildValue("(NNNi)", tensor_of(out.data(), out.size(), 12), tensor_of(merges.data(), merges.size(), 8), tensor_of(starts.data(), starts.size(), 1), n_parts);
+}
+
 bool bound() { return f_append != nullptr; }
+bool always() { return true; }
 
 // ---- module ---------------------------------------------------------------------------------------------------------------------
 PyObject* py_append4(PyObject*, PyObject* const* args, Py_ssize_t n, PyObject* kw) {
@@ -308,6 +405,7 @@ PyObject* py_attn_prompt4(PyObject*, PyObject* const* args, Py_ssize_t n, PyObje
 PyObject* py_attn_packed(PyObject*, PyObject* const* args, Py_ssize_t n, PyObject* kw) {
     return called<packed_sig, bound>([](PyObject** a) { return PyLong_FromLong(prompt(packed_sig, a, false)); }, args, n, kw);
 }
+PyObject* py_plan(PyObject*, PyObject* const* args, Py_ssize_t n, PyObject* kw) { return called<plan_sig, always>([](PyObject** a) { return plan(a); }, args, n, kw); }
 // bind(append, read, attn, room, packed, exception, layout): addresses of the kernel library's entry points, what a failing launch raises, and which argument blocks the library takes
 PyObject* py_bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (n != 7) {
@@ -364,6 +462,7 @@ PyMethodDef methods[] = {
     {"attn_step4", (PyCFunction)(void (*)())py_attn_step4, METH_FASTCALL | METH_KEYWORDS, attn_step4_doc},
     {"attn_prompt4", (PyCFunction)(void (*)())py_attn_prompt4, METH_FASTCALL | METH_KEYWORDS, attn_prompt4_doc},
     {"attn_packed", (PyCFunction)(void (*)())py_attn_packed, METH_FASTCALL | METH_KEYWORDS, attn_packed_doc},
+    {"plan", (PyCFunction)(void (*)())py_plan, METH_FASTCALL | METH_KEYWORDS, nullptr},      // see portions4
     {"bind", (PyCFunction)(void (*)())py_bind, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
@@ -372,9 +471,9 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_kv4", nullptr, -1, methods};
 }  // namespace
 
 PyMODINIT_FUNC PyInit__kv4() {
-    for (Signature* s : {&append_sig, &read_sig, &decode_sig, &step_sig, &prompt_sig, &packed_sig}) s->intern();
-    PyObject** names[] = {&s_codes, &s_scale, &s_tiles, &s_merges, &s_rows, &s_parts, &s_window, &s_group, &s_cache};
-    const char* texts[] = {"codes", "scale", "tiles", "merges", "rows", "parts", "window", "group", "cache"};
-    for (int i = 0; i < 9; i++) *names[i] = PyUnicode_InternFromString(texts[i]);
+    for (Signature* s : {&append_sig, &read_sig, &decode_sig, &step_sig, &prompt_sig, &packed_sig, &plan_sig}) s->intern();
+    PyObject** names[] = {&s_codes, &s_scale, &s_tiles, &s_starts, &s_merges, &s_rows, &s_parts, &s_window, &s_group, &s_cache};
+    const char* texts[] = {"codes", "scale", "tiles", "starts", "merges", "rows", "parts", "window", "group", "cache"};
+    for (int i = 0; i < 10; i++) *names[i] = PyUnicode_InternFromString(texts[i]);
     return PyModule_Create(&module);
 }
