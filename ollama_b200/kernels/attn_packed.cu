@@ -3,9 +3,10 @@
 //   out[t][h] = sum_k p_k v_k / (sum_k p_k + exp(sink)),  p_k = exp(cap(scale q[t][h] . k)),  k the sequence's positions up to the token's own that its window has
 //
 // A CTA takes shares one after the other: two tiles of 128 query rows of one KV head and a run of keys; a row is a token's query head (token / group, head of the group), so all heads of a group share the keys that the CTA brings, and few
-// tokens of many heads still fill a tile.  Keys come in tiles of 128.  Roles: warps 0-3 and 4-7 the softmax of a tile each, a row a thread (no exchange between threads); warp 8 loads; warp 9
-// issues the products; warps 12-15 make operands: queries, of a 4-bit cache also keys and values, whose codes they turn into f16 rows in the swizzled layout; of 16-bit rows they look at tiles whose
-// mask is not whole (below).  Nothing waits for a share's results to be written but the next share's first P V.
+// tokens of many heads still fill a tile.  Keys come in tiles of 128.  Roles: warps 0-3 and 4-7 the softmax of a tile each, a row a thread (no exchange between threads); warp 8 loads
+// keys and values, warp 10 queries; warp 9 issues the products; warps 12-15 make operands: queries, of a 4-bit cache also keys and values, whose codes they turn into f16 rows in the swizzled layout; of 16-bit rows they look at tiles whose
+// mask is not whole (below).  The next share's first scores are computed behind the last products of this one; nothing
+// waits for a share's results to be written but the next one's first P V.
 // Tensor memory: S of both tiles (128 columns each, over whose first 64 the weights are written as 16-bit operands), O of both, accumulated there.  One tile's products run under the other's softmax, and P V
 // of keys 0 .. 63 while the weights of the others are still being made.  The weights are relative to a reference that follows a row's largest score only when that exceeds it by 2^8
 // (then the thread rescales its row of O: the product before is complete by the time a tile's scores are), and count from 2^6 on, so that f16 weights keep 20 powers of two below the largest.
@@ -25,17 +26,14 @@ using namespace tc;
 
 constexpr int BQ = 128, BKV = 128, ATOM_BYTES = 128 * 128;
 constexpr int THREADS = 512;
-// registers: 512 threads start with 128 each; two softmax warpgroups, the one that makes operands, the one that loads and multiplies
-constexpr int SOFTMAX_REGS = 184, MAKER_REGS = 104, REST_REGS = 40;
-static_assert(2 * SOFTMAX_REGS + MAKER_REGS + REST_REGS == 512, "what the block was launched with");
 constexpr float LIFT = 6.f, LAG = 8.f, LOG2E = 1.4426950408889634f;
 enum Form : int { F16 = 0, B16 = 1, CODES = 2 };
 
 template <int D>
 struct Lay {
     static constexpr int ATOMS = D / 64, TILE = ATOMS * ATOM_BYTES;
-    static constexpr int OFF_K = 2 * TILE, OFF_V = OFF_K + 2 * TILE, OFF_BAR = OFF_V + 2 * TILE;
-    static constexpr int TOTAL = OFF_BAR + 256 + 1024;
+    static constexpr int OFF_K = 2 * TILE, OFF_V = OFF_K + 2 * TILE, OFF_OUT = OFF_V + 2 * TILE;
+    static constexpr int OFF_BAR = OFF_OUT + 8 * 32 * 128, TOTAL = OFF_BAR + 256 + 1024;      // 32 rows of 128 bytes for each softmax warp's results
 };
 
 __device__ __forceinline__ uint32_t idesc(bool bf16, int n, int b_mn_major) { return idesc_f16(BQ, n, b_mn_major) | (bf16 ? (1u << 7) | (1u << 10) : 0u); }
@@ -44,20 +42,35 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, i
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
                  ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
-// 64 consecutive 32-bit columns of this thread's lane, waited for
-__device__ __forceinline__ void tmem_ld64(uint32_t at, uint32_t* v) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x64.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
-        "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
-          "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]),
-          "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31]), "=r"(v[32]), "=r"(v[33]), "=r"(v[34]), "=r"(v[35]), "=r"(v[36]), "=r"(v[37]), "=r"(v[38]), "=r"(v[39]),
-          "=r"(v[40]), "=r"(v[41]), "=r"(v[42]), "=r"(v[43]), "=r"(v[44]), "=r"(v[45]), "=r"(v[46]), "=r"(v[47]), "=r"(v[48]), "=r"(v[49]), "=r"(v[50]), "=r"(v[51]), "=r"(v[52]),
-          "=r"(v[53]), "=r"(v[54]), "=r"(v[55]), "=r"(v[56]), "=r"(v[57]), "=r"(v[58]), "=r"(v[59]), "=r"(v[60]), "=r"(v[61]), "=r"(v[62]), "=r"(v[63])
-        : "r"(at)
-        : "memory");
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                 ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z) : "memory");
+}
+// 32 consecutive 32-bit columns of this thread's lane, without waiting for them, and the wait, which hands them on: what uses them comes behind it
+__device__ __forceinline__ void tmem_ask32(uint32_t at, uint32_t (&v)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+                 : "r"(at));
+}
+__device__ __forceinline__ void tmem_have32(uint32_t (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])::"memory");
+}
+// 16 columns, not waited for
+__device__ __forceinline__ void tmem_put16(uint32_t at, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
+}
+__device__ __forceinline__ void tmem_put_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// Bounded like mbar_wait, in fewer instructions; the hint lets a thread sleep in the hardware.
+__device__ __forceinline__ bool arrived(uint64_t* bar, uint32_t parity) {
+#pragma unroll 1
+    for (int i = 0; i < 1 << 16; i++) {
+        uint32_t ok;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 20000;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+        if (ok) return true;
+    }
+    return false;
 }
 // Products and commits of a whole warp, one lane of which issues (`one`).  The warp stays together, so descriptors are in uniform registers: issued from a branch of one lane, the products of a
 // tile took 4500 cycles for what the tensor cores do in 2000.
@@ -77,11 +90,6 @@ __device__ __forceinline__ void mma_ts(uint32_t one, uint32_t d, uint32_t a, uin
 __device__ __forceinline__ void commit(uint32_t one, uint64_t* bar) {
     asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)), "r"(one) : "memory");
 }
-template <int N>
-__device__ __forceinline__ void set_registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N>
-__device__ __forceinline__ void set_registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float x, float y) {
     if (BF16) {
@@ -91,34 +99,9 @@ __device__ __forceinline__ uint32_t pack2(float x, float y) {
     return pack_h2(x, y);
 }
 
-// 32 bytes at once: rows of one thread each fill whole sectors
-__device__ __forceinline__ void store32(void* to, const uint32_t (&w)[8], bool aligned) {
-    if (aligned) {
-        asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
-    } else {
-        reinterpret_cast<uint4*>(to)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-        reinterpret_cast<uint4*>(to)[1] = make_uint4(w[4], w[5], w[6], w[7]);
-    }
-}
-// 16 values of a result row
-__device__ __forceinline__ void store16(void* out, int type, size_t at, const float* y, bool aligned) {
-    uint32_t w[8];
-    if (type == 0) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) w[i] = __float_as_uint(y[i]);
-        store32((float*)out + at, w, aligned);
-#pragma unroll
-        for (int i = 0; i < 8; i++) w[i] = __float_as_uint(y[8 + i]);
-        store32((float*)out + at + 8, w, aligned);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) w[i] = type == 1 ? pack2<false>(y[2 * i], y[2 * i + 1]) : pack2<true>(y[2 * i], y[2 * i + 1]);
-        store32((uint16_t*)out + at, w, aligned);
-    }
-}
-
 template <int D, int FORM>
-__global__ void __launch_bounds__(THREADS, 1) packed_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PackedArgs a) {
+__global__ void __launch_bounds__(THREADS, 1) packed_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_q,
+                                                                const __grid_constant__ PackedArgs a) {
     using L = Lay<D>;
     constexpr bool BF16 = FORM == B16;
     constexpr int ATOMS = L::ATOMS;
@@ -154,58 +137,52 @@ __global__ void __launch_bounds__(THREADS, 1) packed_kernel(const __grid_constan
         for (int i = 0; i < ATOMS; i++) tma_load_4d(sm + off + b * L::TILE + i * ATOM_BYTES, map, 64 * i, y, x.kvh, x.slot, &full[b]);
     };
 
-    // Query rows of a share as 16-bit operands, 16 bytes a thread at a time: copied where they are of the operands' type and taken as they are.
+    // Query rows of a share as 16-bit operands: those of the operands' type are copied, row token * group + head of a tile one after the other as a box of (64 columns, group heads, tokens) lays
+    // them (rows behind the portion's are others', whose results nothing reads); others are rounded, 16 bytes a thread at a time.
     const uint32_t per = (65536u + group - 1) / group;      // r / group = r * per >> 16 for r < 128
-    auto queries = [&](const PackedTile& u, int id, int threads) {
-        constexpr int PIECES = D / 8, BATCH = 8;
-        const int steps = (u.rows > tokens ? 2 : 1) * BQ * PIECES / threads;      // a multiple of BATCH / 2
-        const bool as_is = a.q_type == (BF16 ? 2 : 1) && a.scale >= 0.f;
-        auto place = [&](int s, const void*& from, bool& live) {      // where the sth piece goes to and comes from
-            const int idx = id + s * threads, c = idx % PIECES, r = idx / PIECES & 127, x = idx / (PIECES * BQ), of = r * per >> 16, token = x * tokens + of;
-            live = of < tokens && token < u.rows;
-            from = (const char*)a.q + ((size_t)(u.row + (live ? token : 0)) * a.ldq + (size_t)(u.kvh * group + (live ? r - of * group : 0)) * D + 8 * c) * (a.q_type ? 2 : 4);
-            return sm + x * L::TILE + (c >> 3) * ATOM_BYTES + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-        };
-        if (as_is) {
-#pragma unroll 4
-            for (int s = 0; s < steps; s++) {
-                const void* from;
-                bool live;
-                uint8_t* to = place(s, from, live);
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(live ? 16 : 0) : "memory");
-            }
-            asm volatile("cp.async.wait_all;" ::: "memory");
-        } else {
+    const bool as_is = a.q_type == (BF16 ? 2 : 1) && a.scale >= 0.f;
+    auto copy_queries = [&](const PackedTile& u) {
+        const int n_x = u.rows > tokens ? 2 : 1;
+        mbar_expect_tx(q_full, n_x * tokens * group * D * 2);
+        for (int x = 0; x < n_x; x++)
+#pragma unroll
+            for (int i = 0; i < ATOMS; i++)
+                tma_load_3d(sm + x * L::TILE + i * ATOM_BYTES, &map_q, 64 * i, u.kvh * group, u.row + x * tokens, q_full);
+    };
+    auto round_queries = [&](const PackedTile& u, int id, int threads) {
+        constexpr int PIECES = D / 8, BATCH = 4;
+        const int steps = (u.rows > tokens ? 2 : 1) * BQ * PIECES / threads;
 #pragma unroll 1
-            for (int s0 = 0; s0 < steps; s0 += BATCH / 2) {
-                uint4 w[BATCH];
+        for (int s0 = 0; s0 < steps; s0 += BATCH) {
+            uint4 w[2 * BATCH];
+            auto place = [&](int s, size_t& from) {      // where the sth piece goes to and comes from: whether there is one
+                const int idx = id + (s0 + s) * threads, c = idx % PIECES, r = idx / PIECES & 127, x = idx / (PIECES * BQ), of = r * per >> 16, token = x * tokens + of;
+                from = (size_t)(u.row + token) * a.ldq + (size_t)(u.kvh * group + r - of * group) * D + 8 * c;
+                return of < tokens && token < u.rows ? x * L::TILE + (c >> 3) * ATOM_BYTES + r * 128 + (((c & 7) ^ (r & 7)) << 4) : -1;
+            };
 #pragma unroll
-                for (int s = 0; s < BATCH / 2; s++) {
-                    const void* from;
-                    bool live;
-                    place(s0 + s, from, live);
-                    w[2 * s] = w[2 * s + 1] = make_uint4(0, 0, 0, 0);
-                    if (live) {
-                        w[2 * s] = ((const uint4*)from)[0];
-                        if (a.q_type == 0) w[2 * s + 1] = ((const uint4*)from)[1];
-                    }
+            for (int s = 0; s < BATCH; s++) {
+                size_t from;
+                if (place(s, from) < 0) continue;
+                const uint4* at = (const uint4*)((const char*)a.q + from * (a.q_type ? 2 : 4));
+                w[2 * s] = at[0];
+                if (a.q_type == 0) w[2 * s + 1] = at[1];
+            }
+#pragma unroll
+            for (int s = 0; s < BATCH; s++) {
+                size_t from;
+                const int to = place(s, from);
+                if (to < 0) continue;
+                const uint32_t z[8] = {w[2 * s].x, w[2 * s].y, w[2 * s].z, w[2 * s].w, w[2 * s + 1].x, w[2 * s + 1].y, w[2 * s + 1].z, w[2 * s + 1].w};
+                uint32_t y[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const float2 f = a.q_type == 0   ? make_float2(__uint_as_float(z[2 * j]), __uint_as_float(z[2 * j + 1]))
+                                     : a.q_type == 1 ? __half22float2(*reinterpret_cast<const __half2*>(&z[j]))
+                                                     : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&z[j]));
+                    y[j] = pack2<BF16>(f.x, f.y) ^ (a.scale < 0.f ? 0x80008000u : 0u);
                 }
-#pragma unroll
-                for (int s = 0; s < BATCH / 2; s++) {
-                    const void* from;
-                    bool live;
-                    uint8_t* to = place(s0 + s, from, live);
-                    const uint32_t z[8] = {w[2 * s].x, w[2 * s].y, w[2 * s].z, w[2 * s].w, w[2 * s + 1].x, w[2 * s + 1].y, w[2 * s + 1].z, w[2 * s + 1].w};
-                    uint32_t y[4];
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const float2 f = a.q_type == 0   ? make_float2(__uint_as_float(z[2 * j]), __uint_as_float(z[2 * j + 1]))
-                                         : a.q_type == 1 ? __half22float2(*reinterpret_cast<const __half2*>(&z[j]))
-                                                         : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&z[j]));
-                        y[j] = pack2<BF16>(f.x, f.y) ^ (a.scale < 0.f ? 0x80008000u : 0u);
-                    }
-                    *reinterpret_cast<uint4*>(to) = make_uint4(y[0], y[1], y[2], y[3]);
-                }
+                *reinterpret_cast<uint4*>(sm + to) = make_uint4(y[0], y[1], y[2], y[3]);
             }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -227,9 +204,10 @@ __global__ void __launch_bounds__(THREADS, 1) packed_kernel(const __grid_constan
             mbar_init(&o_full[b], 1);
             mbar_init(&o_empty[b], 4);
         }
-        mbar_init(q_full, 4);
+        mbar_init(q_full, as_is ? 1 : 4);
         mbar_init(q_empty, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        if (as_is) copy_queries(u0);
         if (FORM != CODES) {
             load(u0, k_full, &map_k, L::OFF_K, u0.k_lo, 0);
             load(u0, v_full, &map_v, L::OFF_V, u0.k_lo, 0);
@@ -239,7 +217,7 @@ __global__ void __launch_bounds__(THREADS, 1) packed_kernel(const __grid_constan
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    queries(u0, threadIdx.x, THREADS);
+    if (!as_is) round_queries(u0, threadIdx.x, THREADS);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -247,7 +225,6 @@ __global__ void __launch_bounds__(THREADS, 1) packed_kernel(const __grid_constan
     pdl_launch();
 
     if (wg == 2) {
-        set_registers_down<REST_REGS>();
         if (FORM != CODES && warp == 8 && lane == 0) {
             int nth = 0;
             bool ok = true;
@@ -256,23 +233,30 @@ __global__ void __launch_bounds__(THREADS, 1) packed_kernel(const __grid_constan
                 for (int t = x.k_lo; t < x.k_hi; t++, nth++) {
                     const int b = nth & 1, ph = ((nth >> 1) - 1) & 1;
                     if (nth == 0) continue;
-                    if (nth >= 2 && !mbar_wait(&k_empty[b], ph)) { ok = false; break; }
+                    if (nth >= 2 && !arrived(&k_empty[b], ph)) { ok = false; break; }
                     load(x, k_full, &map_k, L::OFF_K, t, nth);
-                    if (nth >= 2 && !mbar_wait(&v_empty[b], ph)) { ok = false; break; }
+                    if (nth >= 2 && !arrived(&v_empty[b], ph)) { ok = false; break; }
                     load(x, v_full, &map_v, L::OFF_V, t, nth);
                 }
             }
             if (!ok) atomicExch(failed, 1);
+        } else if (warp == 10 && lane == 0 && as_is) {
+            bool ok = true;
+            for (int i = 1; i < shares && ok; i++) {
+                const PackedTile u = share(i);
+                if (arrived(q_empty, (i - 1) & 1)) copy_queries(u);
+                else ok = false;
+            }
+            if (!ok) atomicExch(failed, 1);
         } else if (warp == 9) {
-            const uint32_t one = elect();
-            const uint32_t id_s = idesc(BF16, BKV, 0), id_o = idesc(BF16, D, 1);
+            // (with a warp for each tile the products of both interleave, and each chain waits for all of them: 2.3 us a tile of keys instead of 1.9)
+            const uint32_t one = elect(), id_s = idesc(BF16, BKV, 0), id_o = idesc(BF16, D, 1);
             bool ok = true;
             uint32_t looks = 0;          // bit b: parity of the tiles of stage b that were looked at
             uint32_t sp = 0, op = 0;     // bit x: parity of the scores, of the results of tile x
             int nth = 0;
             auto expect = [&](uint64_t* bar, int parity) {
-                if (!mbar_wait(bar, parity)) ok = false;
-                tc_fence_after();
+                if (!arrived(bar, parity)) ok = false;
             };
             auto wait_k = [&](int at, bool look) {
                 const int b = at & 1;
@@ -283,71 +267,77 @@ __global__ void __launch_bounds__(THREADS, 1) packed_kernel(const __grid_constan
                 }
             };
             auto scores = [&](int x, int at) {
+                const uint64_t qd = umma_desc(sm + x * L::TILE), kd = umma_desc(sm + L::OFF_K + (at & 1) * L::TILE);
 #pragma unroll
-                for (int i = 0; i < ATOMS; i++) {
-                    const uint64_t qd = umma_desc(sm + x * L::TILE + i * ATOM_BYTES), kd = umma_desc(sm + L::OFF_K + (at & 1) * L::TILE + i * ATOM_BYTES);
-#pragma unroll
-                    for (int k = 0; k < 4; k++) mma_ss(one, tmem + 128 * x, qd + 2 * k, kd + 2 * k, id_s, (i | k) != 0);
-                }
+                for (int k = 0; k < D / 16; k++) mma_ss(one, tmem + 128 * x, qd + (k >> 2) * (ATOM_BYTES / 16) + 2 * (k & 3), kd + (k >> 2) * (ATOM_BYTES / 16) + 2 * (k & 3), id_s, k != 0);
                 commit(one, &s_full[x]);
             };
             auto values = [&](int x, int at, int half, bool more) {
-                const uint8_t* vt = sm + L::OFF_V + (at & 1) * L::TILE;
+                const uint64_t vd = umma_desc_mn(sm + L::OFF_V + (at & 1) * L::TILE + half * 64 * 128, ATOM_BYTES);
 #pragma unroll
-                for (int k = 4 * half; k < 4 * half + 4; k++)
-                    mma_ts(one, tmem + 256 + 128 * x, tmem + 128 * x + 8 * k, umma_desc_mn(vt + k * 16 * 128, ATOM_BYTES), id_o, more || k != 0);
+                for (int k = 0; k < 4; k++) mma_ts(one, tmem + 256 + 128 * x, tmem + 128 * x + 32 * half + 8 * k, vd + k * (16 * 128 / 16), id_o, more || k != 0);
             };
+            auto looks_at = [&](const PackedTile& y, int t) { return FORM != CODES && masked(y, (y.k_lo + t) * BKV); };
             PackedTile next = u0;
             for (int i = 0; i < shares && ok; i++) {
                 const PackedTile u = next;
                 if (i + 1 < shares) next = share(i + 1);
                 const int n_tiles = u.k_hi - u.k_lo, n_x = u.rows > tokens ? 2 : 1;
-                auto looks_at = [&](int t) { return FORM != CODES && masked(u, (u.k_lo + t) * BKV); };
-                if (i) expect(q_full, (i - 1) & 1);      // (the first share's queries were there before)
-                if (ok) wait_k(nth, looks_at(0));
-                if (!ok) break;
-                for (int x = 0; x < n_x; x++) scores(x, nth);
-                commit(one, &k_empty[nth & 1]);
-                if (n_tiles == 1) commit(one, q_empty);
+                if (i == 0) {
+                    if (as_is) expect(q_full, 0);      // (others were there before)
+                    if (ok) wait_k(0, looks_at(u, 0));
+                    if (!ok) break;
+                    for (int x = 0; x < n_x; x++) scores(x, 0);
+                    commit(one, &k_empty[0]);
+                    if (n_tiles == 1) commit(one, q_empty);
+                }
                 for (int t = 0; t < n_tiles && ok; t++, nth++) {
-                    const bool more = t + 1 < n_tiles, look = more && looks_at(t + 1);
-                    if (more && !look) wait_k(nth + 1, false);      // (tiles that are looked at come later: their scores are not waited for ahead of this tile's values)
-                    for (int x = 0; x < n_x && ok; x++) {
-                        if (x == 0) expect(&v_full[nth & 1], (nth >> 1) & 1);
-                        if (t == 0) {      // the result before has been read: the first one finds the place empty
-                            expect(&o_empty[x], op >> x & 1 ^ 1);
-                            op ^= 1u << x;
+                    // the tile behind this one, which may be the next share's first
+                    const bool more = t + 1 < n_tiles, any = more || i + 1 < shares, look = any && (more ? looks_at(u, t + 1) : looks_at(next, 0));
+                    const int n_then = more ? n_x : any ? (next.rows > tokens ? 2 : 1) : 0;
+                    const bool late = look || !more;      // (tiles that are looked at, and queries, come late: their scores are not waited for ahead of this tile's values)
+                    if (any && !late) wait_k(nth + 1, false);
+                    for (int x = 0; x < max(n_x, n_then) && ok; x++) {
+                        if (x < n_x) {
+                            if (x == 0) expect(&v_full[nth & 1], (nth >> 1) & 1);
+                            if (t == 0) {      // the result before has been read: the first one finds the place empty
+                                expect(&o_empty[x], op >> x & 1 ^ 1);
+                                op ^= 1u << x;
+                            }
+                            expect(&p_half[x], sp >> x & 1);
+                            if (!ok) break;
+                            tc_fence_after();
+                            values(x, nth, 0, t > 0);
+                            expect(&p_ready[x], sp >> x & 1);
+                            sp ^= 1u << x;
+                            if (!ok) break;
+                            tc_fence_after();
+                            values(x, nth, 1, true);
+                            if (!more) commit(one, &o_full[x]);
                         }
-                        expect(&p_half[x], sp >> x & 1);
-                        if (!ok) break;
-                        values(x, nth, 0, t > 0);
-                        expect(&p_ready[x], sp >> x & 1);
-                        sp ^= 1u << x;
-                        if (!ok) break;
-                        values(x, nth, 1, true);
-                        if (more) {
-                            if (look && x == 0) wait_k(nth + 1, true);
+                        if (x < n_then) {
+                            if (late && x == 0) {
+                                if (!more) expect(q_full, as_is ? (i + 1) & 1 : i & 1);
+                                if (ok) wait_k(nth + 1, look);
+                            }
                             if (!ok) break;
                             scores(x, nth + 1);
-                        } else {
-                            commit(one, &o_full[x]);
                         }
                     }
                     commit(one, &v_empty[nth & 1]);
-                    if (more) commit(one, &k_empty[(nth + 1) & 1]);
-                    if (t + 2 == n_tiles) commit(one, q_empty);
+                    if (any) commit(one, &k_empty[(nth + 1) & 1]);
+                    if (any && (more ? t + 2 == n_tiles : next.k_hi - next.k_lo == 1)) commit(one, q_empty);
                 }
             }
             if (!ok && lane == 0) atomicExch(failed, 1);
         }
     } else if (wg == 3) {
-        set_registers_down<MAKER_REGS>();
         const int id = threadIdx.x & 127;
         bool ok = true;
-        auto next_queries = [&](const PackedTile& u, int i) {
-            if (i == 0) return true;
-            if (!mbar_wait(q_empty, (i - 1) & 1)) return false;
-            queries(u, id, 128);
+        auto next_queries = [&](int i) {
+            if (i == 0 || as_is) return true;
+            if (!arrived(q_empty, (i - 1) & 1)) return false;
+            round_queries(share(i), id, 128);
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full);
             return true;
@@ -361,11 +351,12 @@ __global__ void __launch_bounds__(THREADS, 1) packed_kernel(const __grid_constan
             uint4 kw[PASSES], vw[PASSES];
             uint2 kd[PASSES], vd[PASSES];
             // rows behind the portion repeat its last: their keys are masked
-            auto fetch = [&](const PackedTile& u, int t, const uint8_t* codes, const void* scales, uint4 (&w)[PASSES], uint2 (&d)[PASSES]) {
-                const size_t row0 = kv4::row_of(a.c, u.base, u.slot, u.kvh);
+            size_t row0 = kv4::row_of(a.c, u0.base, u0.slot, u0.kvh);
+            int last = u0.pos + u0.rows - 1, lo = u0.k_lo, hi = u0.k_hi;
+            auto fetch = [&](int t, const uint8_t* codes, const void* scales, uint4 (&w)[PASSES], uint2 (&d)[PASSES]) {
 #pragma unroll
                 for (int p = 0; p < PASSES; p++) {
-                    const size_t at = row0 + min(t * BKV + p * STEP + row, u.pos + u.rows - 1);
+                    const size_t at = row0 + min(t * BKV + p * STEP + row, last);
                     w[p] = ldg16(codes + at * (D / 2) + 16 * piece);
                     if (D == 128) d[p] = ldg8((const uint8_t*)scales + at * 8);
                     else d[p].x = __ldg((const uint32_t*)scales + at);
@@ -390,41 +381,45 @@ __global__ void __launch_bounds__(THREADS, 1) packed_kernel(const __grid_constan
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
             };
-            PackedTile u = u0;
-            fetch(u, u.k_lo, a.c.k, a.c.ks, kw, kd);
-            fetch(u, u.k_lo, a.c.v, a.c.vs, vw, vd);
-            for (int i = 0; i < shares && ok; i++) {
-                PackedTile next = u;
-                if (i + 1 < shares) next = share(i + 1);
-                for (int t = u.k_lo; t < u.k_hi && ok; t++, nth++) {
-                    const int b = nth & 1, ph = ((nth >> 1) - 1) & 1;
-                    const bool more = t + 1 < u.k_hi, any = more || i + 1 < shares;
-                    if (nth >= 2 && !mbar_wait(&k_empty[b], ph)) { ok = false; break; }
-                    write(sm + L::OFF_K + b * L::TILE, kw, kd);
-                    if (lane == 0) mbar_arrive(&k_full[b]);
-                    if (t == u.k_lo && !next_queries(u, i)) { ok = false; break; }
-                    if (any) fetch(more ? u : next, more ? t + 1 : next.k_lo, a.c.k, a.c.ks, kw, kd);
-                    if (nth >= 2 && !mbar_wait(&v_empty[b], ph)) { ok = false; break; }
-                    write(sm + L::OFF_V + b * L::TILE, vw, vd);
-                    if (lane == 0) mbar_arrive(&v_full[b]);
-                    if (any) fetch(more ? u : next, more ? t + 1 : next.k_lo, a.c.v, a.c.vs, vw, vd);
+            fetch(lo, a.c.k, a.c.ks, kw, kd);
+            fetch(lo, a.c.v, a.c.vs, vw, vd);
+            int i = 0, t = lo;           // share and tile
+            for (; ok; nth++) {
+                const int b = nth & 1, ph = ((nth >> 1) - 1) & 1;
+                if (nth >= 2 && !arrived(&k_empty[b], ph)) { ok = false; break; }
+                write(sm + L::OFF_K + b * L::TILE, kw, kd);
+                if (lane == 0) mbar_arrive(&k_full[b]);
+                if (t == lo && !next_queries(i)) { ok = false; break; }
+                const bool more = t + 1 < hi, any = more || i + 1 < shares;
+                t++;
+                if (!more && any) {      // on to the next share
+                    const PackedTile u = share(++i);
+                    row0 = kv4::row_of(a.c, u.base, u.slot, u.kvh);
+                    last = u.pos + u.rows - 1;
+                    t = lo = u.k_lo;
+                    hi = u.k_hi;
                 }
-                u = next;
+                if (any) fetch(t, a.c.k, a.c.ks, kw, kd);
+                if (nth >= 2 && !arrived(&v_empty[b], ph)) { ok = false; break; }
+                write(sm + L::OFF_V + b * L::TILE, vw, vd);
+                if (lane == 0) mbar_arrive(&v_full[b]);
+                if (!any) break;
+                fetch(t, a.c.v, a.c.vs, vw, vd);
             }
         } else {
             constexpr uint32_t CARRY = BF16 ? 0x00800080u : 0x04000400u;      // carries out of an exponent of ones
             for (int i = 0; i < shares && ok; i++) {
                 const PackedTile u = share(i);
-                if (!next_queries(u, i)) { ok = false; break; }
+                if (!next_queries(i)) { ok = false; break; }
                 // every tile is waited for and given back, so that no stage gets two phases ahead of these warps
                 for (int t = u.k_lo; t < u.k_hi && ok; t++, nth++) {
                     const int b = nth & 1, ph = (nth >> 1) & 1;
-                    if (!mbar_wait(&v_full[b], ph)) { ok = false; break; }
+                    if (!arrived(&v_full[b], ph)) { ok = false; break; }
                     if (!masked(u, t * BKV)) {
                         if (lane == 0) mbar_arrive(&v_empty[b]);
                         continue;
                     }
-                    if (!mbar_wait(&k_full[b], ph)) { ok = false; break; }
+                    if (!arrived(&k_full[b], ph)) { ok = false; break; }
                     uint8_t* v = sm + L::OFF_V + b * L::TILE + id * 128;
                     uint32_t odd = 0;
 #pragma unroll
@@ -448,12 +443,10 @@ __global__ void __launch_bounds__(THREADS, 1) packed_kernel(const __grid_constan
         }
         if (!ok) atomicExch(failed, 1);
     } else {
-        set_registers_up<SOFTMAX_REGS>();
         const int r = threadIdx.x & 127, of = r / group, token = wg * tokens + of;
         const uint32_t lane_base = (uint32_t)(32 * (warp & 3)) << 16, s_at = tmem + lane_base + 128 * wg, o_at = tmem + lane_base + 256 + 128 * wg;
         const float mult = a.softcap > 0.f ? 1.f : fmaxf(fabsf(a.scale) * LOG2E, 1e-37f),      // not zero: masked scores are -inf times this
                     cap2 = a.softcap * LOG2E, inv_cap = a.softcap > 0.f ? fabsf(a.scale) / a.softcap : 0.f;
-        const bool aligned = ((uintptr_t)a.out & 31) == 0 && a.ldo % (a.out_type ? 16 : 8) == 0;
         bool ok = true;
         uint32_t sp = 0, op = 0;
         for (int i = 0; i < shares && ok; i++) {
@@ -461,29 +454,56 @@ __global__ void __launch_bounds__(THREADS, 1) packed_kernel(const __grid_constan
             if (wg == 1 && u.rows <= tokens) continue;
             const bool live = of < tokens && token < u.rows;
             const int qp = min(u.pos + token, u.pos + u.rows - 1), lo = first_key(qp, 0, a.window), head = u.kvh * group + r - of * group;
+            const int q_first = __shfl_sync(0xffffffffu, qp, 0), lo_last = __shfl_sync(0xffffffffu, lo, 31);      // of the warp's rows
             float m = -INFINITY, l = 0.f;                // reference of the exponents, of two; sum
             for (int t = u.k_lo; t < u.k_hi; t++) {
-                if (!mbar_wait(&s_full[wg], sp)) { ok = false; break; }
+                if (!arrived(&s_full[wg], sp)) { ok = false; break; }
                 sp ^= 1;
                 tc_fence_after();
-                uint32_t v[BKV];
-                tmem_ld64(s_at, v);
-                tmem_ld64(s_at + 64, v + 64);
-                if (a.softcap > 0.f) {
-#pragma unroll
-                    for (int j = 0; j < BKV; j++) v[j] = __float_as_uint(cap2 * tanh_exp(__uint_as_float(v[j]) * inv_cap));
-                }
-                if (masked(u, t * BKV)) {
+                const bool edge = masked(u, t * BKV);
+                if (edge || a.softcap > 0.f) {      // scores that change before they count are written back
                     const int hi = qp - t * BKV, low = lo - t * BKV;
+#pragma unroll 1
+                    for (int c = 0; c < BKV; c += 32) {
+                        const bool all = c + 31 <= q_first - t * BKV && c >= lo_last - t * BKV;      // the warp's rows see all of these keys
+                        if (all && !(a.softcap > 0.f)) continue;
+                        uint32_t v[32];
+                        tmem_ld32(s_at + c, v);
+                        if (a.softcap > 0.f) {
 #pragma unroll
-                    for (int j = 0; j < BKV; j++)
-                        if (j > hi || j < low) v[j] = 0xff800000u;
+                            for (int j = 0; j < 32; j++) v[j] = __float_as_uint(cap2 * tanh_exp(__uint_as_float(v[j]) * inv_cap));
+                        }
+                        if (!all) {
+                            const int upto = hi - c, from = low - c;
+#pragma unroll
+                            for (int j = 0; j < 32; j++)
+                                if (j > upto) v[j] = 0xff800000u;
+                            if (from > 0) {
+#pragma unroll
+                                for (int j = 0; j < 32; j++)
+                                    if (j < from) v[j] = 0xff800000u;
+                            }
+                            __syncwarp();
+                        }
+                        tmem_st32(s_at + c, v);
+                    }
                 }
+                // Scores are read twice, 32 at a time, the next while these are worked on: with all 128 in registers, which cannot be indexed, the loop's code was longer than the
+                // instruction caches keep for warps that are out of step.  (16 at a time: 2.0 us a tile of keys instead of 1.9.)
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                uint32_t v[2][32];
+                tmem_ask32(s_at, v[0]);
+#pragma unroll 1
+                for (int c = 0; c < BKV; c += 64)
 #pragma unroll
-                for (int j = 0; j < BKV; j += 8)
+                    for (int k = 0; k < 2; k++) {
+                        tmem_have32(v[k]);
+                        tmem_ask32(s_at + ((c + 32 * k + 32) & (BKV - 1)), v[k ^ 1]);      // behind the last, the first again
 #pragma unroll
-                    for (int e = 0; e < 4; e++) mx[e] = fmaxf(fmaxf(mx[e], __uint_as_float(v[j + e])), __uint_as_float(v[j + 4 + e]));
+                        for (int j = 0; j < 32; j += 8)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) mx[e] = fmaxf(fmaxf(mx[e], __uint_as_float(v[k][j + e])), __uint_as_float(v[k][j + 4 + e]));
+                    }
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * mult;
                 if (__any_sync(0xffffffffu, top > m + LAG)) {
                     const float to = fmaxf(m, top), f = to == -INFINITY ? 1.f : ex2(m - to);
@@ -503,24 +523,31 @@ __global__ void __launch_bounds__(THREADS, 1) packed_kernel(const __grid_constan
                 const float less = LIFT - (m == -INFINITY ? 0.f : m);
                 const float2 mult2 = make_float2(mult, mult), less2 = make_float2(less, less);
                 float2 sum = make_float2(0.f, 0.f);
+                // (weights take half the columns of their scores, so none is overwritten that has not been read)
+#pragma unroll 1
+                for (int c = 0; c < BKV; c += 64) {
 #pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    uint32_t p[32];
+                    for (int k = 0; k < 2; k++) {
+                        tmem_have32(v[k]);
+                        if (k == 0 || c == 0) tmem_ask32(s_at + c + 32 * k + 32, v[k ^ 1]);
+                        uint32_t p[16];
 #pragma unroll
-                    for (int j = 0; j < 64; j += 2) {
-                        const float2 e = fma2(make_float2(__uint_as_float(v[64 * half + j]), __uint_as_float(v[64 * half + j + 1])), mult2, less2);
-                        const float2 w = make_float2(ex2(e.x), ex2(e.y));
-                        sum = add2(sum, w);
-                        p[j / 2] = pack2<BF16>(w.x, w.y);
+                        for (int j = 0; j < 32; j += 2) {
+                            const float2 e = fma2(make_float2(__uint_as_float(v[k][j]), __uint_as_float(v[k][j + 1])), mult2, less2);
+                            const float2 w = make_float2(ex2(e.x), ex2(e.y));
+                            sum = add2(sum, w);
+                            p[j / 2] = pack2<BF16>(w.x, w.y);
+                        }
+                        tmem_put16(s_at + (c + 32 * k) / 2, p);
                     }
-                    tmem_st32(s_at + 32 * half, p);
+                    tmem_put_wait();
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(half ? &p_ready[wg] : &p_half[wg]);
+                    if (lane == 0) mbar_arrive(c ? &p_ready[wg] : &p_half[wg]);
                 }
                 l += sum.x + sum.y;
             }
-            if (ok && !mbar_wait(&o_full[wg], op)) ok = false;
+            if (ok && !arrived(&o_full[wg], op)) ok = false;
             op ^= 1;
             if (!ok) break;
             tc_fence_after();
@@ -531,28 +558,52 @@ __global__ void __launch_bounds__(THREADS, 1) packed_kernel(const __grid_constan
                 inv = 1.f / l;
             }
             const size_t part = (size_t)(whole ? 0 : u.part) * (2 * BQ) + wg * BQ + r;
-            const size_t at = (size_t)(u.row + token) * a.ldo + (size_t)head * D;
             if (!whole && live) a.part_ml[part] = make_float2(m - LIFT, l);
+            // through the warp's rows of shared memory, 128 bytes of each at a time, to whole lines
+            uint8_t* mine = sm + L::OFF_OUT + warp * 32 * 128;
+            const bool wide = !whole || a.out_type == 0;
+            const uint32_t row_at = live ? (uint32_t)((whole ? ((size_t)(u.row + token) * a.ldo + (size_t)head * D) * (wide ? 4 : 2) : part * D * 4) >> 4) : 0xffffffffu;      // in 16 bytes
+            uint4* const to = reinterpret_cast<uint4*>(whole ? a.out : (void*)a.part_acc) + (lane & 7);
+            uint32_t rows_at[8];                     // of rows 4 k + lane / 8
 #pragma unroll
-            for (int c = 0; c < D; c += 64) {
-                uint32_t y[64];
-                tmem_ld64(o_at + c, y);
-                if (c + 64 == D) {       // all of it has been read
+            for (int k = 0; k < 8; k++) rows_at[k] = __shfl_sync(0xffffffffu, row_at, 4 * k + (lane >> 3));
+            auto flush = [&](int col) {      // byte col of the rows on
+                __syncwarp();
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const int row = 4 * k + (lane >> 3);
+                    const uint4 y = *reinterpret_cast<const uint4*>(mine + row * 128 + (((lane ^ row) & 7) << 4));
+                    if (rows_at[k] != 0xffffffffu) to[rows_at[k] + (col >> 4)] = y;
+                }
+                __syncwarp();
+            };
+            auto put = [&](int c, uint32_t x, uint32_t y, uint32_t z, uint32_t w) { *reinterpret_cast<uint4*>(mine + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(x, y, z, w); };
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+                uint32_t y[32];
+                tmem_ld32(o_at + c, y);
+                if (c + 32 == D) {       // all of it has been read
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&o_empty[wg]);
                 }
-                if (live) {
 #pragma unroll
-                    for (int j = 0; j < 64; j += 16) {
-                        float z[16];
+                for (int j = 0; j < 32; j++) y[j] = __float_as_uint(__uint_as_float(y[j]) * inv);
+                if (wide) {
 #pragma unroll
-                        for (int e = 0; e < 16; e++) z[e] = __uint_as_float(y[j + e]) * inv;
-                        if (whole) store16(a.out, a.out_type, at + c + j, z, aligned);
-                        else store16(a.part_acc, 0, part * D + c + j, z, true);
+                    for (int k = 0; k < 8; k++) put(k, y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]);
+                    flush(4 * c);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) {
+                        const float e0 = __uint_as_float(y[j]), e1 = __uint_as_float(y[j + 1]);
+                        y[j / 2] = a.out_type == 1 ? pack2<false>(e0, e1) : pack2<true>(e0, e1);
                     }
+                    const int to4 = c >> 3 & 4;      // the first or the second 64 bytes
+#pragma unroll
+                    for (int k = 0; k < 4; k++) put(to4 + k, y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]);
+                    if (to4) flush(2 * c - 64);
                 }
-                __syncwarp();
             }
         }
         if (!ok) atomicExch(failed, 1);
@@ -622,6 +673,19 @@ bool rows_map(CUtensorMap* map, const void* base, const PackedArgs& a, long long
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Queries [rows][heads][D] of 16-bit elements; boxes of 64 columns x the heads of a KV head x the tokens of a tile.
+bool queries_map(CUtensorMap* map, const PackedArgs& a) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    const int group = a.n_heads / a.kv_heads;
+    cuuint64_t dims[3] = {(cuuint64_t)a.hd, (cuuint64_t)a.n_heads, (cuuint64_t)a.q_rows};
+    cuuint64_t strides[2] = {(cuuint64_t)a.hd * 2, (cuuint64_t)a.ldq * 2};
+    cuuint32_t box[3] = {64u, (cuuint32_t)group, (cuuint32_t)(BQ / group)};
+    cuuint32_t ones[3] = {1, 1, 1};
+    return fn(map, a.q_type == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(a.q), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int D>
 const void* kernel_of(int form) {
     return form == F16 ? (const void*)packed_kernel<D, F16> : form == B16 ? (const void*)packed_kernel<D, B16> : (const void*)packed_kernel<D, CODES>;
@@ -634,27 +698,23 @@ B2_API int b2_attn_packed(const PackedArgs* in, int pdl, cudaStream_t st) {
     PackedArgs a = *in;
     const bool codes = a.k == nullptr;
     if (a.ctas == 0) return 0;
-    if ((a.hd != 64 && a.hd != 128) || a.kv_heads < 1 || a.kv_heads > 65535 || a.n_heads < 1 || a.n_heads % a.kv_heads || a.n_heads / a.kv_heads > BQ || !a.q || !a.out || !a.tiles || !a.starts || a.ctas < 0 || a.window < 0 ||
+    if ((a.hd != 64 && a.hd != 128) || a.kv_heads < 1 || a.kv_heads > 65535 || a.n_heads < 1 || a.n_heads % a.kv_heads || a.n_heads / a.kv_heads > BQ || !a.q || a.q_rows < 1 || !a.out || !a.tiles || !a.starts || a.ctas < 0 || a.window < 0 ||
         a.ldo < a.n_heads * a.hd || (((uintptr_t)a.q | (uintptr_t)a.out) & 15) || a.ldq % (a.q_type ? 8 : 4) || a.ldo % (a.out_type ? 8 : 4))
         return (int)cudaErrorInvalidValue;
-    if (a.n_merges && (!a.merges || !a.part_acc || !a.part_ml || a.n_merges < 0 || ((uintptr_t)a.part_acc & 31))) return (int)cudaErrorInvalidValue;
+    if (a.n_merges && (!a.merges || !a.part_acc || !a.part_ml || a.n_merges < 0 || ((uintptr_t)a.part_acc & 15))) return (int)cudaErrorInvalidValue;
     if (codes ? kv4_bad_cache(a.c) || a.c.hd != a.hd || a.c.kv_heads != a.kv_heads : !a.v || a.slots < 1 || a.n < 1) return (int)cudaErrorInvalidValue;
-    CUtensorMap mk = {}, mv = {};
+    CUtensorMap mk = {}, mv = {}, mq = {};
+    if (a.q_type && !queries_map(&mq, a)) return (int)cudaErrorInvalidValue;
     if (!codes && (!rows_map(&mk, a.k, a, a.k_slot, a.k_head, a.k_row) || !rows_map(&mv, a.v, a, a.v_slot, a.v_head, a.v_row))) return (int)cudaErrorInvalidValue;
     static thread_local PerDeviceOnce once;
     if (once.first())
         for (int form = 0; form < 3; form++) {
             cudaError_t e = cudaFuncSetAttribute(kernel_of<64>(form), cudaFuncAttributeMaxDynamicSharedMemorySize, Lay<64>::TOTAL);
             if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel_of<128>(form), cudaFuncAttributeMaxDynamicSharedMemorySize, Lay<128>::TOTAL);
-            for (const void* fn : {kernel_of<64>(form), kernel_of<128>(form)}) {      // a block launched with fewer registers would wait for more of them
-                cudaFuncAttributes at;
-                if (e == cudaSuccess) e = cudaFuncGetAttributes(&at, fn);
-                if (e == cudaSuccess && at.numRegs * 4 < 2 * SOFTMAX_REGS + MAKER_REGS + REST_REGS) e = cudaErrorLaunchOutOfResources;
-            }
             if (e != cudaSuccess) return (int)e;
         }
     const int form = codes ? CODES : a.kv_bf16 ? B16 : F16;
-    void* args[] = {&mk, &mv, &a};
+    void* args[] = {&mk, &mv, &mq, &a};
     const int rc = a.hd == 128 ? launch_rows(kernel_of<128>(form), dim3(a.ctas), dim3(THREADS), Lay<128>::TOTAL, args, st, pdl)
                                : launch_rows(kernel_of<64>(form), dim3(a.ctas), dim3(THREADS), Lay<64>::TOTAL, args, st, pdl);
     if (rc || !a.n_merges) return rc;

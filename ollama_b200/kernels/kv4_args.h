@@ -83,6 +83,7 @@ struct alignas(16) PackedMerge {
 struct PackedArgs {
     const void* q;           // [rows][n_heads][hd], ldq elements a row
     int q_type;              // 0 fp32, 1 f16, 2 bf16
+    int q_rows;
     long long ldq;
     int n_heads, kv_heads, hd;
     const void* k;           // 16-bit rows [slots][kv_heads][n][hd], elements from one to the next in ld_*; null: codes of c

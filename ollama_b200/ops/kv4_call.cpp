@@ -247,8 +247,9 @@ long prompt(const Signature& s, PyObject** a, bool codes) {
     if ((heads > 1 && q.stride(1) != p.hd) || q.stride(2) != 1 || n > (1l << 30) || heads > 65535) refuse(s, "q " + told(q));
     p.q = q.data_ptr();
     p.q_type = q.scalar_type() == F32 ? 0 : q.scalar_type() == F16 ? 1 : 2;
+    p.q_rows = (int)n;
     p.ldq = n > 1 ? q.stride(0) : heads * p.hd;
-    if (p.ldq < heads * p.hd || p.ldq * q.element_size() % 16) refuse(s, "q " + told(q) + " with rows " + std::to_string(p.ldq) + " apart");
+    if (p.ldq < heads * p.hd || p.ldq >= 1ll << 39 || p.ldq * q.element_size() % 16) refuse(s, "q " + told(q) + " with rows " + std::to_string(p.ldq) + " apart");
     p.n_heads = (int)heads;
     const Masked k = masks(s, Mask{a[P_SCALE], a[P_SOFTCAP], a[P_WINDOW], a[P_SINKS]}, heads, dev);
     p.scale = k.scale;
