@@ -26,6 +26,11 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// The same onto other accumulators than it leaves.
+__device__ __forceinline__ void mma_from(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0, float c1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+}
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {      // of an 8 x 8 matrix of f16
     uint32_t y;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -63,31 +68,40 @@ struct Lay {
 template <int D>
 __device__ __forceinline__ int piece_at(int row, int piece) { return row * (D / 2) + 16 * (D == 128 ? piece ^ ((row >> 1) & 3) : piece ^ ((row >> 2) & 1)); }
 
-// Which keys a CTA takes: shares of `chunk` keys, as few keys as leave at most `room` shares, sequence by sequence.
+// Which keys a CTA takes: each sequence's are cut into equal shares of at most `chunk` grains, as few as leave at most `room` shares.
 struct Share {
     int seq, index, count, first, end;      // count: shares of the sequence; keys first .. end - 1
 };
-__device__ __forceinline__ int keys_of(const Rows4& r, const Cache4& c, int window, int b) {
-    const int p = r.positions[b];
-    return kv4::has_row(c, p, r.slots[b]) ? p + 1 - first_key(p, 0, window) : 0;
-}
 __device__ __forceinline__ bool find_share(const Rows4& r, const Cache4& c, int window, int room, int which, int lane, Share& out) {
     const int n = r.rows;
-    long long sum = 0;
-    for (int b = lane; b < n; b += 32) sum += keys_of(r, c, window, b);
+    auto keys_at = [&](int b) {
+        if (b >= n) return 0;
+        const int p = r.positions[b];
+        return kv4::has_row(c, p, r.slots[b]) ? p + 1 - first_key(p, 0, window) : 0;
+    };
+    const int mine = keys_at(lane);          // of up to 32 sequences each lane knows its own
+    auto keys_of = [&](int b) { return b == lane ? mine : keys_at(b); };
+    auto grains = [](int keys) { return (keys + GRAIN - 1) / GRAIN; };
+    int chunk;                               // of GRAIN keys
+    if (n <= 32) {
+        chunk = (int)((__reduce_add_sync(0xffffffffu, (unsigned)grains(mine)) + room - 1) / room);
+    } else {
+        long long sum = 0;
+        for (int b = lane; b < n; b += 32) sum += grains(keys_of(b));
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    int chunk = (int)((sum + room - 1) / room);
-    chunk = max(GRAIN, (chunk + GRAIN - 1) / GRAIN * GRAIN);
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        chunk = (int)((sum + room - 1) / room);
+    }
+    chunk = max(chunk, 1);
     // rounding up each sequence's last share needs at most one more for each: room is at least twice the rows, so this ends at twice the least chunk at the latest
-    for (;; chunk += max(GRAIN, chunk / 32 / GRAIN * GRAIN)) {
+    for (;; chunk += max(1, chunk / 32)) {
         int shares = 0;
-        for (int b = lane; b < n; b += 32) shares += (keys_of(r, c, window, b) + chunk - 1) / chunk;
+        for (int b = lane; b < n; b += 32) shares += (grains(keys_of(b)) + chunk - 1) / chunk;
         if ((int)__reduce_add_sync(0xffffffffu, shares) <= room) break;
     }
     int before = 0;
     for (int b0 = 0; b0 < n; b0 += 32) {
-        const int b = b0 + lane, keys = b < n ? keys_of(r, c, window, b) : 0, shares = (keys + chunk - 1) / chunk;
+        const int keys = keys_of(b0 + lane), shares = (grains(keys) + chunk - 1) / chunk;
         int upto = shares;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -101,8 +115,8 @@ __device__ __forceinline__ bool find_share(const Rows4& r, const Cache4& c, int 
             out.count = __shfl_sync(0xffffffffu, shares, l);
             out.index = which - before - __shfl_sync(0xffffffffu, upto - shares, l);
             const int all = __shfl_sync(0xffffffffu, keys, l), last = r.positions[out.seq] + 1;
-            out.first = last - all + out.index * chunk;
-            out.end = min(last, out.first + chunk);
+            out.first = last - all + (int)((long long)grains(all) * out.index / out.count) * GRAIN;      // a sequence's shares differ by a grain
+            out.end = out.index + 1 == out.count ? last : last - all + (int)((long long)grains(all) * (out.index + 1) / out.count) * GRAIN;
             return true;
         }
         before += __shfl_sync(0xffffffffu, upto, 31);
@@ -129,6 +143,7 @@ __global__ void __launch_bounds__(WARPS * 32, 3) attn4_kernel(const __grid_const
 
     pdl_launch();
     pdl_wait();
+    const float freq = r.qkv && tid < (r.n_rot >> 1) ? r.inv_freq[tid] : 0.f;
     Share sh;
     if (!find_share(r, a.c, a.window, a.room, blockIdx.x, lane, sh)) return;
     const int qpos = r.positions[sh.seq], slot = r.slots[sh.seq];
@@ -138,21 +153,35 @@ __global__ void __launch_bounds__(WARPS * 32, 3) attn4_kernel(const __grid_const
     unsigned char* ring = rings + warp * L::RING;
     const uint32_t ring_at = smem_u32(ring);
 
+    // a lane's pieces of a turn: rows of the same place in the swizzle, so that all but the first are constant distances away
+    constexpr int PER_ROW = L::ROW / 16, STEP = 32 / PER_ROW;
+    const int my_row = lane / PER_ROW, my_piece = lane % PER_ROW;
+    const uint32_t to0 = ring_at + piece_at<D>(my_row, my_piece), sc0 = ring_at + TURN * L::ROW + lane * L::SC;
+    size_t from0 = (row0 + sh.first + TURN * warp + my_row) * L::ROW + 16 * my_piece, scale0 = (row0 + sh.first + TURN * warp + lane) * L::SC;      // of the next turn that is asked for
     auto request = [&](int i) {      // keys behind the share repeat its last (masked below)
         if (i < turns) {
             const int n0 = sh.first + TURN * (warp + WARPS * i);
-            const uint32_t to = ring_at + i % L::NS * L::STAGE;
+            const uint32_t at = i % L::NS * L::STAGE;
+            if (n0 + TURN <= sh.end) {
 #pragma unroll
-            for (int v = 0; v < 2; v++) {
-                const uint8_t* from = v ? a.c.v : a.c.k;
-                const uint8_t* sc = (const uint8_t*)(v ? a.c.vs : a.c.ks);
+                for (int v = 0; v < 2; v++) {
+                    const uint8_t* from = (v ? a.c.v : a.c.k) + from0;
 #pragma unroll
-                for (int p = lane; p < TURN * L::ROW / 16; p += 32) {
-                    const int row = p / (L::ROW / 16), piece = p % (L::ROW / 16);
-                    copy16(to + v * L::HALF + piece_at<D>(row, piece), from + (row0 + min(n0 + row, sh.end - 1)) * L::ROW + 16 * piece);
+                    for (int p = 0; p < TURN / STEP; p++) copy16(to0 + at + v * L::HALF + p * STEP * L::ROW, from + p * STEP * L::ROW);
+                    copy_few<L::SC>(sc0 + at + v * L::HALF, (const uint8_t*)(v ? a.c.vs : a.c.ks) + scale0);
                 }
-                copy_few<L::SC>(to + v * L::HALF + TURN * L::ROW + lane * L::SC, sc + (row0 + min(n0 + lane, sh.end - 1)) * L::SC);
+            } else {
+#pragma unroll 1
+                for (int v = 0; v < 2; v++) {
+                    const uint8_t* from = v ? a.c.v : a.c.k;
+#pragma unroll
+                    for (int p = 0; p < TURN / STEP; p++)
+                        copy16(to0 + at + v * L::HALF + p * STEP * L::ROW, from + (row0 + min(n0 + my_row + p * STEP, sh.end - 1)) * L::ROW + 16 * my_piece);
+                    copy_few<L::SC>(sc0 + at + v * L::HALF, (const uint8_t*)(v ? a.c.vs : a.c.ks) + (row0 + min(n0 + lane, sh.end - 1)) * L::SC);
+                }
             }
+            from0 += (size_t)GRAIN * L::ROW;
+            scale0 += (size_t)GRAIN * L::SC;
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -161,56 +190,77 @@ __global__ void __launch_bounds__(WARPS * 32, 3) attn4_kernel(const __grid_const
 
     const bool fresh = r.qkv != nullptr, owner = fresh && qpos >= sh.first && qpos < sh.end;
     if (fresh) {
-        kv4::fill_angles(r, qpos, s_cs, s_sn, tid, WARPS * 32);
+        // a warp takes two of the heads, warps 0 and 1 of the owner the key and the value: all asked for before the angles are made
+        constexpr int N = D / 32, MINE = HEADS / WARPS;
+        const float* src = r.qkv + (size_t)sh.seq * r.ldq;
+        float x[MINE + 1][N];
+#pragma unroll
+        for (int i = 0; i <= MINE; i++) {
+            const int h = warp + WARPS * i;
+            const bool there = i < MINE ? h < heads : owner && warp < 2;
+            const float* at = src + (size_t)(i < MINE ? head0 + h : H + warp * G + kvh) * D;
+#pragma unroll
+            for (int j = 0; j < N; j++) x[i][j] = 0.f;
+            if (!there) continue;
+            if (wide) {
+                if constexpr (N == 4) {
+                    const float4 y = __ldcg(reinterpret_cast<const float4*>(at) + lane);
+                    x[i][0] = y.x; x[i][1] = y.y; x[i][2] = y.z; x[i][3] = y.w;
+                } else {
+                    const float2 y = __ldcg(reinterpret_cast<const float2*>(at) + lane);
+                    x[i][0] = y.x; x[i][1] = y.y;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < N; j++) x[i][j] = __ldcg(at + N * lane + j);
+            }
+        }
+        if (tid < (r.n_rot >> 1)) kv4::make_angle(r, qpos, tid, freq, s_cs, s_sn);
         __syncthreads();
         const kv4::Turn<D> turn = kv4::make_turn<D>(r, s_cs, s_sn, lane);
-        const float* src = r.qkv + (size_t)sh.seq * r.ldq;
-        // the heads of this CTA, then the key and the value
-        for (int i = warp; i < HEADS + (owner ? 2 : 0); i += WARPS) {
-            constexpr int N = D / 32;
-            float x[N];
-            const bool is_q = i < HEADS, is_k = i == HEADS;
-            if (is_q && i >= heads) {
 #pragma unroll
-                for (int j = 0; j < N; j++) x[j] = 0.f;
-            } else {
-                const float* at = src + (size_t)(is_q ? head0 + i : H + (is_k ? 0 : G) + kvh) * D;
-                if (wide) {
-                    if constexpr (N == 4) {
-                        const float4 y = __ldcg(reinterpret_cast<const float4*>(at) + lane);
-                        x[0] = y.x; x[1] = y.y; x[2] = y.z; x[3] = y.w;
-                    } else {
-                        const float2 y = __ldcg(reinterpret_cast<const float2*>(at) + lane);
-                        x[0] = y.x; x[1] = y.y;
-                    }
-                } else {
+        for (int i = 0; i < MINE; i++) {
+            const int h = warp + WARPS * i;
+            if (h < heads) kv4::prepare_head<D>(x[i], r.q_norm, r.eps, true, turn, s_row[warp], lane);
 #pragma unroll
-                    for (int j = 0; j < N; j++) x[j] = __ldcg(at + N * lane + j);
-                }
-                kv4::prepare_head<D>(x, is_q ? r.q_norm : is_k ? r.k_norm : nullptr, r.eps, is_q || is_k, turn, s_row[warp], lane);
-            }
-            if (is_q) {
+            for (int j = 0; j < N; j += 2) *reinterpret_cast<uint32_t*>(sQ + h * L::LDQ + N * lane + j) = pack(x[i][j], x[i][j + 1]);
+        }
+        if (owner && warp < 2) {
+            if (warp == 0) kv4::prepare_head<D>(x[MINE], r.k_norm, r.eps, true, turn, s_row[warp], lane);
+            const size_t row = row0 + qpos;
+            __syncwarp();
 #pragma unroll
-                for (int j = 0; j < N; j += 2) *reinterpret_cast<uint32_t*>(sQ + i * L::LDQ + N * lane + j) = pack(x[j], x[j + 1]);
-            } else {
-                const size_t row = row0 + qpos;
-                const kv4::Coded<D> y = kv4::encode<D>(x, lane);
-                const int v = is_k ? 0 : 1;
-                if (y.lead) {
-                    s_new[v][y.at] = y.word;
-                    if (tile == 0) reinterpret_cast<uint32_t*>(v ? a.c.v : a.c.k)[row * (D / 8) + y.at] = y.word;
-                }
-                if (y.first) {
-                    s_newd[v][y.block] = y.d;
-                    if (tile == 0) reinterpret_cast<__half*>(v ? a.c.vs : a.c.ks)[row * NB + y.block] = y.d;
+            for (int j = 0; j < N; j++) s_row[warp][N * lane + j] = x[MINE][j];
+            __syncwarp();
+            const int c = lane % (D / 8), at = kv4::word_of<D>(c);      // (D / 8 lanes do what the others repeat)
+            float y[8];
+            *reinterpret_cast<float4*>(y) = *reinterpret_cast<const float4*>(s_row[warp] + 8 * c);
+            *reinterpret_cast<float4*>(y + 4) = *reinterpret_cast<const float4*>(s_row[warp] + 8 * c + 4);
+            __half d;
+            const uint32_t w = kv4::encode_word(y, d);
+            if (lane < D / 8) {
+                s_new[warp][at] = w;
+                if (tile == 0) reinterpret_cast<uint32_t*>(warp ? a.c.v : a.c.k)[row * (D / 8) + at] = w;
+                if ((c & 3) == 0) {
+                    s_newd[warp][c >> 2] = d;
+                    if (tile == 0) reinterpret_cast<__half*>(warp ? a.c.vs : a.c.ks)[row * NB + (c >> 2)] = d;
                 }
             }
         }
     } else {
-        for (int i = tid; i < HEADS * D; i += WARPS * 32) {
-            const int h = i / D, col = i % D;
+        for (int i = tid; i < HEADS * D / 8; i += WARPS * 32) {
+            const int h = i / (D / 8), col = i % (D / 8) * 8;
             const size_t at = ((size_t)sh.seq * H + head0 + h) * D + col;
-            sQ[h * L::LDQ + col] = h >= heads ? __half(0.f) : a.q16 ? reinterpret_cast<const __half*>(a.q)[at] : __float2half_rn(reinterpret_cast<const float*>(a.q)[at]);
+            uint4 y = make_uint4(0, 0, 0, 0);
+            if (h < heads) {
+                if (a.q16) {
+                    y = __ldcg(reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(a.q) + at));
+                } else {
+                    const float4 lo = __ldcg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(a.q) + at)), hi = __ldcg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(a.q) + at + 4));
+                    y = make_uint4(pack(lo.x, lo.y), pack(lo.z, lo.w), pack(hi.x, hi.y), pack(hi.z, hi.w));
+                }
+            }
+            *reinterpret_cast<uint4*>(sQ + h * L::LDQ + col) = y;
         }
     }
     __syncthreads();
@@ -221,6 +271,22 @@ __global__ void __launch_bounds__(WARPS * 32, 3) attn4_kernel(const __grid_const
         const uint4 y = *reinterpret_cast<const uint4*>(sQ + g * L::LDQ + 32 * b + 8 * tq);
         qf[b][0] = y.x; qf[b][1] = y.y; qf[b][2] = y.z; qf[b][3] = y.w;
     }
+    // Half of a key's columns come 72 too large: the products begin with what that makes for heads 2 tq and 2 tq + 1.  (Sums of 32 columns then lose some 2^-20 of their operands' size; all
+    // columns 1032 too large would cost two instructions less and 2^-16.)
+    float less[NB][2];
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 1; i < 4; i += 2) {
+            const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&qf[b][i]));
+            sum += y.x + y.y;
+        }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);      // of head g
+#pragma unroll
+        for (int e = 0; e < 2; e++) less[b][e] = -kv4::RAISED * __shfl_sync(0xffffffffu, sum, 4 * (2 * tq + e));
+    }
 
     float o[NB][2][4];
 #pragma unroll
@@ -228,7 +294,9 @@ __global__ void __launch_bounds__(WARPS * 32, 3) attn4_kernel(const __grid_const
 #pragma unroll
         for (int i = 0; i < 8; i++) o[b][i >> 2][i & 3] = 0.f;
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;      // of heads 2 tq, 2 tq + 1
-    const float mult = a.softcap > 0.f ? a.scale / a.softcap : a.scale * LOG2E, cap2 = a.softcap * LOG2E;
+    // scores times mult are exponents of two; a key that does not count has the score that makes that -inf
+    const float mult = a.softcap > 0.f ? 1.f : a.scale * LOG2E == 0.f ? 1e-37f : a.scale * LOG2E, beyond = mult > 0.f ? -INFINITY : INFINITY;
+    const float inv_cap = a.softcap > 0.f ? a.scale / a.softcap : 0.f, cap2 = a.softcap * LOG2E;
     const int half = g & 1, sel = half ? 0x7632 : 0x5410;          // which half of a value word's codes: of two keys, side by side
 
     for (int i = 0; i < turns; i++) {
@@ -271,10 +339,10 @@ __global__ void __launch_bounds__(WARPS * 32, 3) attn4_kernel(const __grid_const
 #pragma unroll
             for (int b = 0; b < NB; b++) {
                 uint32_t e[4], f[4];
-                kv4::expand(ka[b], e);
-                kv4::expand(kb[b], f);
-                float c[4] = {0.f, 0.f, 0.f, 0.f};
-                mma(c, e[0], f[0], e[1], f[1], qf[b][0], qf[b][1]);
+                kv4::expand_raised(ka[b], e);
+                kv4::expand_raised(kb[b], f);
+                float c[4];
+                mma_from(c, e[0], f[0], e[1], f[1], qf[b][0], qf[b][1], less[b][0], less[b][1]);
                 mma(c, e[2], f[2], e[3], f[3], qf[b][2], qf[b][3]);
                 s[u][0] += c[0] * da[b]; s[u][1] += c[1] * da[b];
                 s[u][2] += c[2] * db[b]; s[u][3] += c[3] * db[b];
@@ -295,17 +363,25 @@ __global__ void __launch_bounds__(WARPS * 32, 3) attn4_kernel(const __grid_const
                 top = fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y)));
             }
             big[k] = lg2(top);
-            float& v0 = s[k >> 1][2 * (k & 1)];
-            float& v1 = s[k >> 1][2 * (k & 1) + 1];
-            v0 *= mult;
-            v1 *= mult;
-            if (a.softcap > 0.f) {
-                v0 = cap2 * tanh_exp(v0);
-                v1 = cap2 * tanh_exp(v1);
-            }
-            if (n0 + 8 * k + g >= sh.end) v0 = v1 = -INFINITY;
-            y0 = fmaxf(y0, v0 + big[k]);
-            y1 = fmaxf(y1, v1 + big[k]);
+        }
+        if (a.softcap > 0.f) {      // in powers of two from here on, mult is one
+#pragma unroll
+            for (int k = 0; k < 8; k++) s[k >> 2][k & 3] = cap2 * tanh_exp(s[k >> 2][k & 3] * inv_cap);
+        }
+        if (n0 + TURN > sh.end) {
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (n0 + 8 * k + g >= sh.end) {      // (nor do its values' scales: they may be those of a row that is being written)
+                    s[k >> 1][2 * (k & 1)] = s[k >> 1][2 * (k & 1) + 1] = beyond;
+                    big[k] = 0.f;
+#pragma unroll
+                    for (int b = 0; b < NB; b++) dv[k][b] = 0.f;
+                }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            y0 = fmaxf(y0, s[k >> 1][2 * (k & 1)] * mult + big[k]);
+            y1 = fmaxf(y1, s[k >> 1][2 * (k & 1) + 1] * mult + big[k]);
         }
         if (__any_sync(0xffffffffu, y0 > m0 + LAG || y1 > m1 + LAG)) {
 #pragma unroll
@@ -313,8 +389,9 @@ __global__ void __launch_bounds__(WARPS * 32, 3) attn4_kernel(const __grid_const
                 y0 = fmaxf(y0, __shfl_xor_sync(0xffffffffu, y0, x));
                 y1 = fmaxf(y1, __shfl_xor_sync(0xffffffffu, y1, x));
             }
-            const float n0m = fmaxf(m0, y0), n1m = fmaxf(m1, y1);
-            const float f0 = n0m == -INFINITY ? 1.f : ex2(m0 - n0m), f1 = n1m == -INFINITY ? 1.f : ex2(m1 - n1m);
+            // (a head's own scores alone decide)
+            const float n0m = y0 > m0 + LAG ? y0 : m0, n1m = y1 > m1 + LAG ? y1 : m1;
+            const float f0 = n0m == m0 ? 1.f : ex2(m0 - n0m), f1 = n1m == m1 ? 1.f : ex2(m1 - n1m);
             m0 = n0m;
             m1 = n1m;
             l0 *= f0;
@@ -332,8 +409,8 @@ __global__ void __launch_bounds__(WARPS * 32, 3) attn4_kernel(const __grid_const
         for (int k = 0; k < 4; k++) {
             float& v0 = s[k >> 1][2 * (k & 1)];
             float& v1 = s[k >> 1][2 * (k & 1) + 1];
-            v0 = ex2(v0 - r0);
-            v1 = ex2(v1 - r1);
+            v0 = ex2(v0 * mult - r0);
+            v1 = ex2(v1 * mult - r1);
             l0 += v0;
             l1 += v1;
         }
@@ -402,12 +479,13 @@ __global__ void __launch_bounds__(WARPS * 32, 3) attn4_kernel(const __grid_const
     }
 }
 
-// Adds up the parts of a head: grid (heads, sequences), four warps, each every fourth part, a lane D / 32 columns.
+// Adds up the parts of a head: grid (heads, sequences), eight warps, each every eighth part, a lane D / 32 columns.
+constexpr int MERGERS = 8;
 template <int D>
-__global__ void __launch_bounds__(128) merge4_kernel(const __grid_constant__ Attn4Args a) {
+__global__ void __launch_bounds__(MERGERS * 32) merge4_kernel(const __grid_constant__ Attn4Args a) {
     constexpr int N = D / 32;
-    __shared__ float s_acc[4][D];
-    __shared__ float s_l[4];
+    __shared__ float s_acc[MERGERS][D];
+    __shared__ float s_l[MERGERS];
     const int h = blockIdx.x, b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, H = a.r.n_heads;
     pdl_launch();
     pdl_wait();
@@ -423,7 +501,7 @@ __global__ void __launch_bounds__(128) merge4_kernel(const __grid_constant__ Att
 #pragma unroll
     for (int j = 0; j < N; j++) acc[j] = 0.f;
 #pragma unroll 4
-    for (int p = warp; p < sh.y; p += 4) {
+    for (int p = warp; p < sh.y; p += MERGERS) {
         const size_t at = (size_t)(sh.x + p) * H + h;
         const float2 ml = a.part_ml[at];
         const float f = ex2(ml.x - ref);
@@ -442,9 +520,15 @@ __global__ void __launch_bounds__(128) merge4_kernel(const __grid_constant__ Att
     __syncthreads();
     const int col = threadIdx.x;
     if (col >= D) return;
-    l = s_l[0] + s_l[1] + s_l[2] + s_l[3];
+    float y = 0.f;
+    l = 0.f;
+#pragma unroll
+    for (int w = 0; w < MERGERS; w++) {
+        y += s_acc[w][col];
+        l += s_l[w];
+    }
     if (sink > -INFINITY) l += ex2(sink - ref);
-    const float y = (s_acc[0][col] + s_acc[1][col] + s_acc[2][col] + s_acc[3][col]) / l;
+    y /= l;
     const size_t at = (size_t)b * a.ldo + (size_t)h * D + col;
     if (a.out16) reinterpret_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(y);
     else reinterpret_cast<float*>(a.out)[at] = y;
@@ -481,5 +565,5 @@ B2_API int b2_attn4(const Attn4Args* in, int pdl, cudaStream_t st) {
     const int rc = launch_rows(fn, dim3(a.room, a.c.kv_heads * tiles), dim3(WARPS * 32), smem, args, st, pdl);
     if (rc) return rc;
     void* margs[] = {&a};      // (its CTAs may wait beside the first launch's last)
-    return launch_rows(big ? (const void*)merge4_kernel<128> : (const void*)merge4_kernel<64>, dim3(a.r.n_heads, a.r.rows), dim3(128), 0, margs, st, 1);
+    return launch_rows(big ? (const void*)merge4_kernel<128> : (const void*)merge4_kernel<64>, dim3(a.r.n_heads, a.r.rows), dim3(MERGERS * 32), 0, margs, st, 1);
 }

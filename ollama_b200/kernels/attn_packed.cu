@@ -505,8 +505,9 @@ __global__ void __launch_bounds__(THREADS, 1) packed_kernel(const __grid_constan
                             for (int e = 0; e < 4; e++) mx[e] = fmaxf(fmaxf(mx[e], __uint_as_float(v[k][j + e])), __uint_as_float(v[k][j + 4 + e]));
                     }
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * mult;
-                if (__any_sync(0xffffffffu, top > m + LAG)) {
-                    const float to = fmaxf(m, top), f = to == -INFINITY ? 1.f : ex2(m - to);
+                if (__any_sync(0xffffffffu, live && top > m + LAG)) {
+                    // (a row's own scores alone decide, so that it is the same whatever stands beside it)
+                    const float to = top > m + LAG ? top : m, f = to == m ? 1.f : ex2(m - to);
                     m = to;
                     l *= f;
                     if (t > u.k_lo) {

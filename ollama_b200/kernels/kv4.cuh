@@ -4,7 +4,7 @@
 // them in bits 4 i .., column 2 i + 1 in bits 16 + 4 i .., so that one mask takes two neighbours into the halves of a register.  Word j of a block of 32 columns stands before word j + 1 of any
 // (word j * (hd / 32) + b of the row is columns 32 b + 8 j ..): the lanes of a matrix product's operand, which want the same word of every block, find theirs side by side.
 // d is minus an eighth of the value of largest magnitude (of two, the negative one), rounded to f16 and at most 8188, eight times which is an f16 number; a code is the quotient rounded to the
-// nearest, ties to even.  So the largest value is held to f16's precision and the others within half a step, but for one of the other sign as large as it, which is one step smaller.  Values
+// nearest.  So the largest value is held to f16's precision and the others within half a step, but for one of the other sign as large as it, which is one step smaller.  Values
 // that are no number are held as zero.
 #pragma once
 #include "kv4_args.h"
@@ -46,31 +46,50 @@ __device__ __forceinline__ void expand(uint32_t w, uint32_t (&e)[4]) {
     e[3] = hfma2_bits(masked_or_1024<0x00f000f0u>(w8), SIXTEENTH, MINUS_72);
 }
 
+// The same but for what a product can take off at once: pairs 0 and 2 as n - 8, pairs 1 and 3 as 64 + n, seven instructions.
+constexpr float RAISED = 72.f;       // what pairs 1 and 3 are too large by
+__device__ __forceinline__ void expand_raised(uint32_t w, uint32_t (&e)[4]) {
+    constexpr uint32_t LOW = 0x64086408u;
+    const uint32_t w8 = w >> 8;
+    uint32_t e1, e3;
+    asm("lop3.b32 %0, %1, 0x00f000f0, %2, 0xEA;" : "=r"(e1) : "r"(w), "r"(0x54005400u));
+    asm("lop3.b32 %0, %1, 0x00f000f0, %2, 0xEA;" : "=r"(e3) : "r"(w8), "r"(0x54005400u));
+    e[0] = hsub2_bits(masked_or_1024<0x000f000fu>(w), LOW);
+    e[1] = e1;
+    e[2] = hsub2_bits(masked_or_1024<0x000f000fu>(w8), LOW);
+    e[3] = e3;
+}
+
 __device__ __forceinline__ bool has_row(const Cache4& c, int pos, int slot) { return (unsigned)pos < (unsigned)c.n_ctx && (unsigned)slot < (unsigned)c.slots; }
 __device__ __forceinline__ size_t row_of(const Cache4& c, int pos, int slot, int kvh) { return ((size_t)slot * c.kv_heads + kvh) * c.n_ctx + pos; }
 
 // What turns a lane's columns N lane .. N lane + N - 1 of any head of a token: x cos + y sin, y the pair's other column.
+enum Other : int { HERE, LANE, ROW };        // where that is: the lane's own neighbour, the same place of another lane, anywhere in the row
 template <int HD>
 struct Turn {
     static constexpr int N = HD / 32;
     float c[N], s[N];
-    int at[N];               // the other column, -1 of a column that is not turned
+    bool all;                // every column is turned
+    int other, from;         // from: LANE: which; ROW: how far behind the lane's columns of the first half
 };
 
 // cs, sn: cosines and sines of the token's pairs.
 template <int HD>
 __device__ __forceinline__ Turn<HD> make_turn(const Rows4& r, const float* cs, const float* sn, int lane) {
+    constexpr int N = HD / 32;
     Turn<HD> t;
+    const int half = r.n_rot >> 1, i0 = N * lane;
+    t.all = r.n_rot == HD;
+    t.other = !r.neox ? HERE : half % N == 0 ? LANE : ROW;
+    t.from = t.other == LANE ? (i0 < half ? lane + half / N : i0 < r.n_rot ? lane - half / N : lane) : half;
 #pragma unroll
-    for (int j = 0; j < Turn<HD>::N; j++) {
-        const int i = Turn<HD>::N * lane + j, half = r.n_rot >> 1;
-        t.at[j] = -1;
+    for (int j = 0; j < N; j++) {
+        const int i = i0 + j;
         t.c[j] = 1.f;
         t.s[j] = 0.f;
         if (i < r.n_rot) {
             const bool first = r.neox ? i < half : !(i & 1);
             const int p = r.neox ? (first ? i : i - half) : i >> 1;
-            t.at[j] = r.neox ? (first ? i + half : i - half) : i ^ 1;
             t.c[j] = cs[p];
             t.s[j] = first ? -sn[p] : sn[p];
         }
@@ -79,15 +98,17 @@ __device__ __forceinline__ Turn<HD> make_turn(const Rows4& r, const float* cs, c
 }
 
 // The angles are formed in double: in 32 bits a position of 100000 would leave 0.004 of a radian.
+__device__ __forceinline__ void make_angle(const Rows4& r, int pos, int p, float freq, float* cs, float* sn) {
+    float s, c;
+    sincosf(rot_angle(pos, (double)freq), &s, &c);
+    sn[p] = s * r.mscale;
+    cs[p] = c * r.mscale;
+}
 __device__ __forceinline__ void fill_angles(const Rows4& r, int pos, float* cs, float* sn, int tid, int threads) {
-    for (int p = tid; p < (r.n_rot >> 1); p += threads) {
-        float s, c;
-        sincosf(rot_angle(pos, (double)r.inv_freq[p]), &s, &c);
-        sn[p] = s * r.mscale;
-        cs[p] = c * r.mscale;
-    }
+    for (int p = tid; p < (r.n_rot >> 1); p += threads) make_angle(r, pos, p, r.inv_freq[p], cs, sn);
 }
 
+// (Roundings are spelled out, so that a row is the same whichever kernel makes it.)
 // Norm and rotation of a head by a warp: x[N] are its columns N lane ..; `row`: HD floats of the warp's own.
 template <int HD>
 __device__ __forceinline__ void prepare_head(float (&x)[HD / 32], const float* norm, float eps, bool turned, const Turn<HD>& t, float* row, int lane) {
@@ -95,65 +116,67 @@ __device__ __forceinline__ void prepare_head(float (&x)[HD / 32], const float* n
     if (norm) {
         float s = 0.f;
 #pragma unroll
-        for (int j = 0; j < N; j++) s += x[j] * x[j];
+        for (int j = 0; j < N; j++) s = __fmaf_rn(x[j], x[j], s);
         const float inv = 1.f / sqrtf(warp_sum(s) / (float)HD + eps);
 #pragma unroll
-        for (int j = 0; j < N; j++) x[j] = x[j] * inv * norm[N * lane + j];
+        for (int j = 0; j < N; j++) x[j] = __fmul_rn(__fmul_rn(x[j], inv), norm[N * lane + j]);
     }
     if (!turned) return;
-    __syncwarp();
+    float y[N];
+    if (t.other == HERE) {
 #pragma unroll
-    for (int j = 0; j < N; j++) row[N * lane + j] = x[j];
-    __syncwarp();
+        for (int j = 0; j < N; j++) y[j] = x[j ^ 1];
+    } else if (t.other == LANE) {
 #pragma unroll
-    for (int j = 0; j < N; j++)
-        if (t.at[j] >= 0) x[j] = x[j] * t.c[j] + row[t.at[j]] * t.s[j];
+        for (int j = 0; j < N; j++) y[j] = __shfl_sync(0xffffffffu, x[j], t.from);
+    } else {
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < N; j++) row[N * lane + j] = x[j];
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            const int i = N * lane + j;
+            y[j] = i < t.from ? row[i + t.from] : i < 2 * t.from ? row[i - t.from] : 0.f;
+        }
+    }
+    if (t.all) {
+#pragma unroll
+        for (int j = 0; j < N; j++) x[j] = __fmaf_rn(x[j], t.c[j], __fmul_rn(y[j], t.s[j]));
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; j++)
+            if (t.s[j] != 0.f || t.c[j] != 1.f) x[j] = __fmaf_rn(x[j], t.c[j], __fmul_rn(y[j], t.s[j]));      // columns that are not turned stay, whatever stands beside them
+    }
 }
 
-// A warp makes the codes of a row.  Lane l has columns N l ..; the lane of a word's first columns gets the word (where `lead`), that of a block's first the scale (`first`).
-template <int HD>
-struct Coded {
-    uint32_t word;
-    int at;                  // which word of the row
-    bool lead, first;
-    __half d;
-    int block;
-};
-template <int HD>
-__device__ __forceinline__ Coded<HD> encode(const float (&in)[HD / 32], int lane) {
-    constexpr int N = HD / 32, PER_BLOCK = 32 / N, PER_WORD = 8 / N;
-    float x[N], hi = -INFINITY, lo = INFINITY;
+// A lane makes a word of a row's codes from its eight columns; the four lanes of a block stand side by side, all 32 of the warp take part.  d: the block's scale.
+__device__ __forceinline__ uint32_t encode_word(const float (&in)[8], __half& scale) {
+    float x[8], hi = -INFINITY, lo = INFINITY;
 #pragma unroll
-    for (int j = 0; j < N; j++) {
+    for (int j = 0; j < 8; j++) {
         x[j] = in[j] == in[j] ? in[j] : 0.f;
         hi = fmaxf(hi, x[j]);
         lo = fminf(lo, x[j]);
     }
 #pragma unroll
-    for (int o = 1; o < PER_BLOCK; o <<= 1) {
+    for (int o = 1; o < 4; o <<= 1) {
         hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
         lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
     }
-    const float far = hi > -lo ? hi : lo;
-    Coded<HD> r;
-    r.d = __float2half_rn(fminf(fmaxf(far * -0.125f, -TOP), TOP));
-    const float d = __half2float(r.d);
-    const int i0 = (lane % PER_WORD) * N;      // first of the lane's columns in its word
+    scale = __float2half_rn(fminf(fmaxf((hi > -lo ? hi : lo) * -0.125f, -TOP), TOP));
+    const float d = __half2float(scale), inv = d != 0.f ? __frcp_rn(d) : 0.f;
     uint32_t w = 0;
 #pragma unroll
-    for (int j = 0; j < N; j++) {
-        const float q = d != 0.f ? fminf(fmaxf(rintf(x[j] / d) + 8.f, 0.f), 15.f) : 8.f;
-        const int i = i0 + j;
-        w |= (uint32_t)q << (4 * (i >> 1) + 16 * (i & 1));
+    for (int j = 0; j < 8; j++) {
+        // 1.5 * 2^23 + 8: the sum's low bits are the code.  (By the reciprocal: a quotient within 2^-23 of a border may go either way.)
+        const uint32_t q = __float_as_uint(fminf(fmaxf(x[j] * inv, -8.f), 7.f) + 12582920.f) & 15u;
+        w |= q << (4 * (j >> 1) + 16 * (j & 1));
     }
-#pragma unroll
-    for (int o = 1; o < PER_WORD; o <<= 1) w |= __shfl_xor_sync(0xffffffffu, w, o);
-    r.word = w;
-    r.block = lane / PER_BLOCK;
-    r.at = lane % PER_BLOCK / PER_WORD * (HD / 32) + r.block;
-    r.lead = lane % PER_WORD == 0;
-    r.first = lane % PER_BLOCK == 0;
-    return r;
+    return w;
 }
+// Lane or thread i of a row's HD / 8: which word of the row it makes, from columns 32 b + 8 j on.
+template <int HD>
+__device__ __forceinline__ int word_of(int i) { return (i & 3) * (HD / 32) + (i >> 2); }
 
 }  // namespace kv4

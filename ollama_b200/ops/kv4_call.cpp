@@ -38,7 +38,6 @@ void fill_rows(const Signature& s, Rows4& r, const at::Tensor& qkv, const Cache4
         refuse(s, std::to_string(heads) + " heads on " + std::to_string(c.kv_heads) + " of " + std::to_string(c.hd) + " columns in rows of " + std::to_string(qkv.size(1)));
     if (n_rot < 0 || n_rot > c.hd || n_rot % 2) refuse(s, std::to_string(n_rot) + " rotated dimensions of " + std::to_string(c.hd));
     if (n > (1l << 30)) refuse(s, std::to_string(n) + " rows");
-    if (given(a.qn) != given(a.kn)) refuse(s, "one of two norms");
     r.qkv = (const float*)qkv.data_ptr();
     r.ldq = (int)row_step(s, qkv, "qkv");
     r.rows = (int)n;
