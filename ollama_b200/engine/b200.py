@@ -29,6 +29,7 @@ from ..gguf.reader import GGUFFile
 from ..models.config import ModelConfig, config_from_gguf
 from ..models.weights import QWeight, load_tensor
 from ..ops import cuda as K
+from ..ops import kv4 as KV4
 from ..ops import reference as R
 from ..ops import sk as SK
 from ..ops.prompt import PromptPass
@@ -79,7 +80,8 @@ class B200Backend(StepEngine):
         otherwise each matrix is expanded into scratch right before its GEMM).  ``prefill_gemm``: "bf16" (expand, then the
         bf16 tensor-core GEMM) or "fused" (weights expanded inside the GEMM kernel; no 16-bit copy anywhere).
         ``kv_type``: "f16" or "q8_0" (int8 values with one f16 scale per 32 dims, written by the rope kernel and expanded
-        inside the attention kernels; "q4_0" is served as q8_0); default: ``opts.kv_cache_type``
+        inside the attention kernels; "q4_0" is served as q8_0) or "int4" (4-bit integers with one f16 scale per 32 dims, head sizes 64
+        and 128 on one GPU per model or layer range; others are served as q8_0); default: ``opts.kv_cache_type``
         (envconfig/config.go:183 OLLAMA_KV_CACHE_TYPE).  ``layers`` = (lo, hi): this object is one stage of a layer
         pipeline and holds blocks lo..hi-1 only; the first stage also holds the embedding, the last one the output
         norm and head, and the residual stream enters / leaves through ``buf.x`` (decode) or the ``x`` argument (prefill).
@@ -95,15 +97,17 @@ class B200Backend(StepEngine):
             raise ValueError(f"layer range {layers} outside 0..{self.cfg.n_layers}")
         self.first, self.last = self.l_lo == 0, self.l_hi == self.cfg.n_layers
         kv_type = (kv_type or getattr(opts, "kv_cache_type", None) or "f16").lower()
-        if kv_type not in ("f16", "q8_0", "q4_0"):
-            raise ValueError("K/V cache type 'fp8' is for stack models: this model's caches are f16 or q8_0" if kv_type == "fp8" else f"unknown K/V cache type {kv_type!r}")
+        if kv_type not in ("f16", "q8_0", "q4_0", "int4"):
+            raise ValueError("K/V cache type 'fp8' is for stack models: this model's caches are f16, q8_0 or int4" if kv_type == "fp8" else f"unknown K/V cache type {kv_type!r}")
         # quantised blocks cover 32 dims; head sizes outside the flash-attention kernel read the cache through torch
-        self.kv_q8 = kv_type != "f16" and self.cfg.head_dim % 32 == 0 and self.cfg.head_dim in K.ATTN_PREFILL_HEAD_DIMS
-        self.kv_type = "q8_0" if self.kv_q8 else "f16"
+        self.kv4 = kv_type == "int4" and type(self) is B200Backend and self.cfg.head_dim in (64, 128) and self.cfg.causal
+        self.kv_q8 = not self.kv4 and kv_type != "f16" and self.cfg.head_dim % 32 == 0 and self.cfg.head_dim in K.ATTN_PREFILL_HEAD_DIMS
+        self.kv_type = "int4" if self.kv4 else "q8_0" if self.kv_q8 else "f16"
         if kv_type != self.kv_type:       # say so: the cache costs what the stored encoding costs, not what was asked for
             import logging
             logging.getLogger("ollama_b200.engine").warning("K/V cache type %s is stored as %s (%s)", kv_type, self.kv_type,
-                                                            "there is no 4-bit cache encoding" if self.kv_q8 else "this head size has no quantised cache")
+                                                            "this head size has no quantised cache" if not self.kv_q8 else
+                                                            "int4 is the 4-bit cache" if kv_type == "q4_0" else "4-bit caches are for head sizes 64 and 128 of models on one GPU")
         if keep_bf16 is None:
             c = self.cfg
             est = 2 * (c.n_layers * (c.d_model * (2 * c.q_dim + 2 * c.kv_dim) + 3 * c.d_model * c.d_ff) + c.vocab_size * c.d_model)
@@ -277,14 +281,19 @@ class B200Backend(StepEngine):
     def alloc(self, n_slots: int, n_ctx: int) -> None:
         c, dev = self.cfg, self.device
         self.n_slots, self.n_ctx = n_slots, n_ctx
-        kv_dt = torch.int8 if self.kv_q8 else torch.float16
-        self.k_cache = [torch.zeros(n_slots, c.n_kv_heads, n_ctx, c.head_dim, device=dev, dtype=kv_dt) for _ in self.layers]
-        self.v_cache = [torch.zeros(n_slots, c.n_kv_heads, n_ctx, c.head_dim, device=dev, dtype=kv_dt) for _ in self.layers]
+        kv_dt = torch.uint8 if self.kv4 else torch.int8 if self.kv_q8 else torch.float16
+        row = c.head_dim // 2 if self.kv4 else c.head_dim
+        self.k_cache = [torch.zeros(n_slots, c.n_kv_heads, n_ctx, row, device=dev, dtype=kv_dt) for _ in self.layers]
+        self.v_cache = [torch.zeros(n_slots, c.n_kv_heads, n_ctx, row, device=dev, dtype=kv_dt) for _ in self.layers]
         self.k_scale = self.v_scale = [None] * len(self.layers)
-        if self.kv_q8:
+        if self.kv_q8 or self.kv4:
             def sc():
                 return [torch.zeros(n_slots, c.n_kv_heads, n_ctx, c.head_dim // 32, device=dev, dtype=torch.float16) for _ in self.layers]
             self.k_scale, self.v_scale = sc(), sc()
+        self.cache4 = []
+        if self.kv4:
+            KV4.load()
+            self.cache4 = [(KV4.Cache4(k, ks), KV4.Cache4(v, vs)) for k, v, ks, vs in zip(self.k_cache, self.v_cache, self.k_scale, self.v_scale)]
         MB = self.max_batch
         f32, i8, i32 = torch.float32, torch.int8, torch.int32
         qkv_dim = (c.n_heads + 2 * c.n_kv_heads) * c.head_dim
@@ -341,7 +350,7 @@ class B200Backend(StepEngine):
 
     def close(self) -> None:
         self._graphs.clear()
-        self.k_cache = self.v_cache = self.k_scale = self.v_scale = []
+        self.k_cache = self.v_cache = self.k_scale = self.v_scale = self.cache4 = []
         self.buf = self._pass = self._ws = None
 
     def check_waits(self) -> None:
@@ -536,11 +545,33 @@ class B200Backend(StepEngine):
             x16 = SK.rows16(xs, norm_w, c.norm_eps, out=buf, pdl=self.pdl)
             SK.gemm16(ws, x16, xs.shape[0], out=out[r:], mode=mode, act=c.act, alpha=c.swiglu_alpha, limit=c.swiglu_limit, pdl=self.pdl, ws=wsp)
 
+    def _rope_args(self, L) -> dict:
+        """What the calls of the 4-bit cache take of a layer's rotation and norms."""
+        c, local = self.cfg, L.swa and self.cfg.rope_base_local > 0
+        return dict(heads=c.n_heads, inv_freq=self.inv_freq_local if local else self.inv_freq, n_rot=c.rope_dim, neox=c.rope_style == "neox", mscale=1.0 if local else self.mscale,
+                    q_norm=L.q_norm, k_norm=L.k_norm, eps=c.norm_eps, pdl=self.pdl)
+
+    def _attn_args(self, L) -> dict:
+        c = self.cfg
+        return dict(scale=self.attn_scale, softcap=c.attn_softcap, window=c.sliding_window if L.swa else 0, sinks=L.sinks)
+
+    def _attn_step4(self, i: int, L, nb: int) -> None:
+        """Attention of a decode step over a 4-bit cache: raw projections in ``buf.qkv``, results in ``buf.ao``."""
+        b, (k, v) = self.buf, self.cache4[i]
+        KV4.attn_step4(b.qkv[:nb], k, v, b.positions[:nb], b.slots[:nb], b.ao[:nb], **self._rope_args(L), **self._attn_args(L))
+        self._n += 2
+
     def _decode_layer_sk(self, i: int, L, nb: int) -> None:
         """A layer on the streaming GEMV: both RMSNorms, both residual adds, the gated activation and every activation
         quantisation happen inside the four matrix kernels; attention keeps its own kernels."""
         c, b, lib, st = self.cfg, self.buf, K.lib(), K.stream
         self._sk(L.sk.qkv, b.x, b.qkv, nb, norm_w=L.attn_norm)
+        if self.kv4:
+            self._attn_step4(i, L, nb)
+            self._sk([L.sk.o], b.ao, b.x, nb, mode=SK.MODE_ACCUM)
+            self._sk([L.sk.gu], b.x, b.hf, nb, norm_w=L.ffn_norm, mode=SK.MODE_GLU)
+            self._sk([L.sk.down], b.hf, b.x, nb, mode=SK.MODE_ACCUM)
+            return
         local = L.swa and c.rope_base_local > 0
         inv_freq, mscale = (self.inv_freq_local, 1.0) if local else (self.inv_freq, self.mscale)
         ca = K.AttnCombineArgs(K.ptr(b.part_acc), K.ptr(b.part_ml), K.ptr(L.sinks), c.n_heads, self.n_splits, c.head_dim,
@@ -596,30 +627,36 @@ class B200Backend(StepEngine):
                 self._gemm_step([L.wq], [L.wqkv16], nb, b.xf, b.qkv, bias=L.bqkv)      # Q, K and V in one product
             else:
                 self._gemv([L.wq, L.wk, L.wv], nb, b.xq, b.xds, b.xf, b.qkv, b.qkv.stride(0))
-            local = L.swa and c.rope_base_local > 0
-            ra = K.RopeKvArgs(K.ptr(b.qkv), K.ptr(b.positions), K.ptr(b.slots), K.ptr(self.inv_freq_local if local else self.inv_freq),
-                              K.ptr(L.q_norm), K.ptr(L.k_norm), c.norm_eps, 1.0 if local else self.mscale, c.n_heads, c.n_kv_heads,
-                              c.head_dim, c.rope_dim, int(c.rope_style == "neox"), self.n_ctx, K.ptr(b.q), K.ptr(self.k_cache[i]),
-                              K.ptr(self.v_cache[i]), K.ptr(self.k_scale[i]), K.ptr(self.v_scale[i]))
-            K._check(lib.b2_rope_kv(C.byref(ra), nb, int(self.pdl), st()), "rope_kv")
-            aa = K.AttnDecodeArgs(K.ptr(b.q), K.ptr(self.k_cache[i]), K.ptr(self.v_cache[i]), K.ptr(b.positions), K.ptr(b.slots),
-                                  c.n_heads, c.n_kv_heads, self.n_ctx, self.n_splits, self.attn_scale, c.attn_softcap,
-                                  c.sliding_window if L.swa else 0, K.ptr(b.part_acc), K.ptr(b.part_ml), K.ptr(self.k_scale[i]),
-                                  K.ptr(self.v_scale[i]))
-            ca = K.AttnCombineArgs(K.ptr(b.part_acc), K.ptr(b.part_ml), K.ptr(L.sinks), c.n_heads, self.n_splits, c.head_dim,
-                                   K.ptr(b.ao), K.ptr(b.aq), K.ptr(b.ads))
-            if self.fuse_attn_combine:      # the last CTA of every head group merges the splits: one launch instead of two
-                K._check(lib.b2_attn_decode_fused(C.byref(aa), C.byref(ca), C.c_void_p(K.ptr(b.attn_tickets)), nb, c.head_dim, int(self.pdl), st()),
-                         "attn_decode_fused")
-                self._n += 2
+            aq, ads, ao = b.aq, b.ads, b.ao
+            if self.kv4:
+                self._attn_step4(i, L, nb)
+                self._norm_quant(b.ao, None, nb, c.q_dim, do_norm=False)
+                aq, ads, ao = b.xq, b.xds, b.xf
             else:
-                K._check(lib.b2_attn_decode(C.byref(aa), C.byref(ca), nb, c.head_dim, int(self.pdl), st()), "attn_decode")
-                self._n += 3
+                local = L.swa and c.rope_base_local > 0
+                ra = K.RopeKvArgs(K.ptr(b.qkv), K.ptr(b.positions), K.ptr(b.slots), K.ptr(self.inv_freq_local if local else self.inv_freq),
+                                  K.ptr(L.q_norm), K.ptr(L.k_norm), c.norm_eps, 1.0 if local else self.mscale, c.n_heads, c.n_kv_heads,
+                                  c.head_dim, c.rope_dim, int(c.rope_style == "neox"), self.n_ctx, K.ptr(b.q), K.ptr(self.k_cache[i]),
+                                  K.ptr(self.v_cache[i]), K.ptr(self.k_scale[i]), K.ptr(self.v_scale[i]))
+                K._check(lib.b2_rope_kv(C.byref(ra), nb, int(self.pdl), st()), "rope_kv")
+                aa = K.AttnDecodeArgs(K.ptr(b.q), K.ptr(self.k_cache[i]), K.ptr(self.v_cache[i]), K.ptr(b.positions), K.ptr(b.slots),
+                                      c.n_heads, c.n_kv_heads, self.n_ctx, self.n_splits, self.attn_scale, c.attn_softcap,
+                                      c.sliding_window if L.swa else 0, K.ptr(b.part_acc), K.ptr(b.part_ml), K.ptr(self.k_scale[i]),
+                                      K.ptr(self.v_scale[i]))
+                ca = K.AttnCombineArgs(K.ptr(b.part_acc), K.ptr(b.part_ml), K.ptr(L.sinks), c.n_heads, self.n_splits, c.head_dim,
+                                       K.ptr(b.ao), K.ptr(b.aq), K.ptr(b.ads))
+                if self.fuse_attn_combine:      # the last CTA of every head group merges the splits: one launch instead of two
+                    K._check(lib.b2_attn_decode_fused(C.byref(aa), C.byref(ca), C.c_void_p(K.ptr(b.attn_tickets)), nb, c.head_dim, int(self.pdl), st()),
+                             "attn_decode_fused")
+                    self._n += 2
+                else:
+                    K._check(lib.b2_attn_decode(C.byref(aa), C.byref(ca), nb, c.head_dim, int(self.pdl), st()), "attn_decode")
+                    self._n += 3
             if c.sandwich_norm:
-                self._gemv([L.wo], nb, b.aq, b.ads, b.ao, b.tmp, b.tmp.stride(0))
+                self._gemv([L.wo], nb, aq, ads, ao, b.tmp, b.tmp.stride(0))
                 self._norm_quant(b.tmp, L.post_attn_norm, nb, c.d_model, residual=b.x)
             else:
-                self._gemv([L.wo], nb, b.aq, b.ads, b.ao, b.x, b.x.stride(0), accumulate=True)
+                self._gemv([L.wo], nb, aq, ads, ao, b.x, b.x.stride(0), accumulate=True)
             self._norm_quant(b.x, L.ffn_norm, nb, c.d_model)
             if L.moe:
                 self._moe_decode(L, nb, act)
@@ -710,6 +747,30 @@ class B200Backend(StepEngine):
                         softcap=c.attn_softcap, sinks=L.sinks, spans=spans)
         return o.reshape(T, -1).to(torch.bfloat16)
 
+    def portions4(self, bounds, windows) -> dict:
+        """What attention of the rows ``bounds`` = [(first row, last row + 1, slot, first position)] of a step over a 4-bit cache has to know of them, for each window."""
+        return {w: KV4.portions4([(r0, r1 - r0, sl, p0) for r0, r1, sl, p0 in bounds], self.cfg.n_heads, self.cache4[0][0], window=w) for w in windows}
+
+    def _attn_rows4(self, qkv, pos, slots, i: int, L, bounds, portions: dict, spans=()) -> torch.Tensor:
+        """Attention of a prompt pass over a 4-bit cache, all its sequences in one launch: raw projections -> bf16 [T, H * hd].  Passes with ``spans`` (see _attn_prefill) take tensor operations
+        on the rows as they are held."""
+        c, (k, v) = self.cfg, self.cache4[i]
+        q = torch.empty(qkv.shape[0], c.n_heads, c.head_dim, device=qkv.device, dtype=torch.float32 if spans else torch.float16)
+        KV4.append4(qkv, k, v, pos, slots, q, **self._rope_args(L))
+        o = torch.empty(qkv.shape[0], c.q_dim, device=qkv.device, dtype=torch.bfloat16)
+        if spans:
+            for r0, r1, sl, p0 in bounds:
+                at = p0 + r1 - r0
+                kk, vv = (KV4.decode4(x.codes[sl, :, :at], x.scale[sl, :, :at]).transpose(0, 1) for x in (k, v))
+                own = [(lo, hi) for lo, hi in spans if lo < at and hi > p0]
+                o[r0:r1] = R.attention(q[r0:r1], kk, vv, torch.arange(p0, at, device=q.device), torch.arange(at, device=q.device), spans=own, causal=c.causal, **self._attn_args(L)).reshape(r1 - r0, -1)
+            return o
+        window = c.sliding_window if L.swa else 0
+        if window not in portions:
+            portions.update(self.portions4(bounds, [window]))
+        self.kernel_launches += 1 + KV4.attn_prompt4(q, k, v, portions[window], o, **self._attn_args(L), pdl=self.pdl)
+        return o
+
     @torch.no_grad()
     def _forward_rows(self, segs: Sequence[tuple[int, Sequence[int], int]], x: torch.Tensor | None = None, embeds=None, spans=()) -> torch.Tensor:
         """One pass over the rows of several chunks, each ``(slot, tokens, first position)`` of a different sequence: the
@@ -742,6 +803,7 @@ class B200Backend(StepEngine):
         if self._pass is not None and (self._pass.units if units else self._pass.wide) and not spans and mode in ("auto", "mma") and x.is_contiguous() and x.dtype == torch.float32:
             self.kernel_launches += self._pass.run(self, x, pos, slots, [(r0, r1 - r0, sl, p0) for r0, r1, sl, p0 in bounds], units, mode == "auto")
             return x
+        portions = {}          # of the step, by window
         for i, L in enumerate(self.layers):
             h = K.rmsnorm_bf16(x, L.attn_norm, c.norm_eps, pdl=self.pdl)
             qkv = torch.empty(T, (c.n_heads + 2 * c.n_kv_heads) * c.head_dim, device=dev, dtype=torch.float32)
@@ -752,15 +814,18 @@ class B200Backend(StepEngine):
                 self._mm(h, L.wq, qkv, 0)
                 self._mm(h, L.wk, qkv, c.q_dim)
                 self._mm(h, L.wv, qkv, c.q_dim + c.kv_dim)
-            local = L.swa and c.rope_base_local > 0
-            q = K.rope_kv(qkv, pos, slots, self.inv_freq_local if local else self.inv_freq, n_heads=c.n_heads, n_kv_heads=c.n_kv_heads,
-                          hd=c.head_dim, n_rot=c.rope_dim, neox=c.rope_style == "neox", mscale=1.0 if local else self.mscale,
-                          k_cache=self.k_cache[i], v_cache=self.v_cache[i], q_norm=L.q_norm, k_norm=L.k_norm, eps=c.norm_eps,
-                          k_scale=self.k_scale[i], v_scale=self.v_scale[i], pdl=self.pdl)
-            if len(bounds) == 1:
-                o = self._attn_prefill(q, i, L, bounds[0][2], bounds[0][3], bounds[0][3] + T, spans)
+            if self.kv4:
+                o = self._attn_rows4(qkv, pos, slots, i, L, bounds, portions, spans)
             else:
-                o = torch.cat([self._attn_prefill(q[r0:r1], i, L, sl, p0, p0 + r1 - r0) for r0, r1, sl, p0 in bounds])
+                local = L.swa and c.rope_base_local > 0
+                q = K.rope_kv(qkv, pos, slots, self.inv_freq_local if local else self.inv_freq, n_heads=c.n_heads, n_kv_heads=c.n_kv_heads,
+                              hd=c.head_dim, n_rot=c.rope_dim, neox=c.rope_style == "neox", mscale=1.0 if local else self.mscale,
+                              k_cache=self.k_cache[i], v_cache=self.v_cache[i], q_norm=L.q_norm, k_norm=L.k_norm, eps=c.norm_eps,
+                              k_scale=self.k_scale[i], v_scale=self.v_scale[i], pdl=self.pdl)
+                if len(bounds) == 1:
+                    o = self._attn_prefill(q, i, L, bounds[0][2], bounds[0][3], bounds[0][3] + T, spans)
+                else:
+                    o = torch.cat([self._attn_prefill(q[r0:r1], i, L, sl, p0, p0 + r1 - r0) for r0, r1, sl, p0 in bounds])
             if c.sandwich_norm:
                 x = x + R.rmsnorm(self._mm(o, L.wo), L.post_attn_norm, c.norm_eps)
             else:
@@ -805,7 +870,7 @@ class B200Backend(StepEngine):
     def shift(self, slot: int, keep: int, discard: int, n: int) -> None:
         """Context shift in place: cache rows [keep, keep + discard) of ``slot`` are dropped, the rows behind them (up to
         ``n``) move down by ``discard`` and their keys, stored rotated, are turned back by ``discard`` positions
-        (kvcache/causal.go:640-700).  int8 caches are expanded, rotated and quantised again with fresh block scales.  Runs
+        (kvcache/causal.go:640-700).  int8 and 4-bit caches are expanded, rotated and quantised again with fresh block scales.  Runs
         once per ``n_ctx / 2`` generated tokens, so it is written with tensor ops rather than a kernel of its own."""
         c = self.cfg
         src, dst = slice(keep + discard, n), slice(keep, n - discard)
@@ -813,11 +878,14 @@ class B200Backend(StepEngine):
         for i, L in enumerate(self.layers):
             inv = self.inv_freq_local if (L.swa and c.rope_base_local > 0) else self.inv_freq
             kc, vc, ks, vs = self.k_cache[i], self.v_cache[i], self.k_scale[i], self.v_scale[i]
-            k = kc[slot, :, src].float()                                   # [Hkv, S, hd]
-            if ks is not None:
+            k = KV4.decode4(kc[slot, :, src], ks[slot, :, src]) if self.kv4 else kc[slot, :, src].float()      # [Hkv, S, hd]
+            if self.kv_q8:
                 k = (k.view(*k.shape[:2], -1, 32) * ks[slot, :, src].float()[..., None]).view_as(k)
             k = R.rope(k.transpose(0, 1), back, inv[: c.rope_dim // 2], c.rope_style, 1.0).transpose(0, 1)
-            if ks is not None:
+            if self.kv4:
+                kc[slot, :, dst], ks[slot, :, dst] = KV4.encode4(k)
+                vs[slot, :, dst] = vs[slot, :, src].clone()
+            elif ks is not None:
                 blocks = k.reshape(*k.shape[:2], -1, 32)
                 d = blocks.abs().amax(-1) / 127.0
                 q = torch.where(d[..., None] > 0, blocks / d[..., None], torch.zeros_like(blocks)).round().clamp(-127, 127)

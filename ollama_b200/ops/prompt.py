@@ -6,6 +6,7 @@ import ctypes as C
 import torch
 
 from . import cuda as K
+from . import kv4 as KV4
 from . import sk as SK
 
 P, I, F = C.c_void_p, C.c_int, C.c_float
@@ -20,10 +21,18 @@ class PassSeg(C.Structure):
     _fields_ = [("row0", I), ("rows", I), ("slot", I), ("pos0", I)]
 
 
+class PassPlan4(C.Structure):
+    _fields_ = [("window", I), ("ctas", I), ("n_merges", I), ("parts", I), ("tiles", P), ("starts", P), ("merges", P)]
+
+
+class Pass4(C.Structure):
+    _fields_ = [("plan", PassPlan4 * 2), ("n", I), ("part_acc", P), ("part_ml", P)]
+
+
 class PassArgs(C.Structure):
     _fields_ = [("rows", I), ("d", I), ("n_heads", I), ("n_kv_heads", I), ("hd", I), ("n_rot", I), ("neox", I), ("n_ctx", I), ("n_slots", I), ("ff", I), ("causal", I), ("act", I),
                 ("eps", F), ("scale", F), ("softcap", F), ("alpha", F), ("limit", F), ("positions", P), ("slots", P), ("x", P), ("qkv", P), ("q", P), ("o", P), ("h", P), ("f", P),
-                ("x16", P), ("ws", P), ("ws_floats", C.c_longlong), ("status", P), ("units", I), ("tc", I), ("pdl", I), ("kv16", P), ("kv16_halves", C.c_longlong), ("launches", I)]
+                ("x16", P), ("ws", P), ("ws_floats", C.c_longlong), ("status", P), ("units", I), ("tc", I), ("pdl", I), ("kv16", P), ("kv16_halves", C.c_longlong), ("launches", I), ("kv4", P)]
 
 
 class PromptPass:
@@ -60,22 +69,29 @@ class PromptPass:
         def rows(cols, dtype=torch.float32):
             return torch.empty(n, cols, device=dev, dtype=dtype)
 
-        qkv, q, o = rows((c.n_heads + 2 * c.n_kv_heads) * c.head_dim), rows(c.q_dim), rows(c.q_dim, torch.bfloat16)
+        qkv, q, o = rows((c.n_heads + 2 * c.n_kv_heads) * c.head_dim), rows(c.q_dim, torch.float16 if be.kv4 else torch.float32), rows(c.q_dim, torch.bfloat16)
         h = None if units else rows(c.d_model, torch.bfloat16)
         f = rows(c.d_ff, torch.float32 if units else torch.bfloat16)
         x16 = torch.empty(SK.rows16_bytes(min(n, SK.ROWS16_MAX), max(c.d_model, c.q_dim, c.d_ff)), device=dev, dtype=torch.uint8) if units else None
         ws = self.ws if units else None
         size = 0 if units else max(K.gemm_bf16_scratch(n, *nk) for nk in (((c.n_heads + 2 * c.n_kv_heads) * c.head_dim, c.d_model), (c.d_model, c.q_dim), (c.d_model, c.d_ff)))
         parts = torch.empty(size, device=dev, dtype=torch.float32) if size else None
-        q8 = tc and c.head_dim in (64, 128) and be.k_scale[0] is not None and max(p0 + r for _, r, _, p0 in segs) > 64
+        q8 = tc and c.head_dim in (64, 128) and be.kv_q8 and max(p0 + r for _, r, _, p0 in segs) > 64
         kv16 = None
         if q8:
             head = max(K.attn_prefill_q8_head(p0, p0 + r, w, c.head_dim) for _, r, _, p0 in segs for w in self.windows)
             kv16 = K.attn_prefill_q8_scratch(head, c.n_kv_heads, dev)
+        kv4 = parts4 = None
+        if be.kv4:
+            plans = be.portions4([(r0, r0 + r, sl, p0) for r0, r, sl, p0 in segs], self.windows)
+            room = 256 * max(p.parts for p in plans.values())
+            parts4 = torch.empty(room * (c.head_dim + 2), device=dev, dtype=torch.float32) if room else None
+            kv4 = Pass4((PassPlan4 * 2)(*[PassPlan4(w, len(p.starts) - 1, len(p.merges), p.parts, K.ptr(p.tiles), K.ptr(p.starts), K.ptr(p.merges)) for w, p in plans.items()]), len(plans),
+                        K.ptr(parts4), K.ptr(parts4) + 4 * room * c.head_dim if room else None)
         a = PassArgs(n, c.d_model, c.n_heads, c.n_kv_heads, c.head_dim, c.rope_dim, int(c.rope_style == "neox"), be.n_ctx, be.n_slots, c.d_ff, int(c.causal), K._ACT[c.act],
                      c.norm_eps, be.attn_scale, c.attn_softcap, c.swiglu_alpha, c.swiglu_limit, K.ptr(positions), K.ptr(slots), K.ptr(x), K.ptr(qkv), K.ptr(q), K.ptr(o), K.ptr(h),
                      K.ptr(f), K.ptr(x16), *((K.ptr(ws.ws), 0, K.ptr(ws.status)) if units else (K.ptr(parts), size, None)), int(units), int(tc),
-                     int(be.pdl), K.ptr(kv16), kv16.numel() if kv16 is not None else 0, 0)
+                     int(be.pdl), K.ptr(kv16), kv16.numel() if kv16 is not None else 0, 0, C.addressof(kv4) if kv4 is not None else None)
         sg = (PassSeg * len(segs))(*[PassSeg(*s) for s in segs])
         fn = K.lib().b2_prefill_pass
         fn.argtypes = [P, I, P, P, I, P]
