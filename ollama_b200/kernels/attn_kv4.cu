@@ -479,59 +479,70 @@ __global__ void __launch_bounds__(WARPS * 32, 3) attn4_kernel(const __grid_const
     }
 }
 
-// Adds up the parts of a head: grid (heads, sequences), eight warps, each every eighth part, a lane D / 32 columns.
+// Adds up the parts of a head: WIDE warps each, which take every WIDE-th, a lane D / 32 columns; eight warps a CTA, grid (heads * WIDE / 8, sequences).  Eight warps a head where a sequence has
+// more than eight parts on the mean, else one, since CTAs then cost more than parts do.  Both launches with eight and with one: 55 parts 14.0 and 18.6 us, 4 x 14 parts of 32 heads 55.8 and
+// 57.7 us, 32 x 2 parts of 64 heads 18.7 and 14.2 us.
 constexpr int MERGERS = 8;
-template <int D>
+template <int D, int WIDE>
 __global__ void __launch_bounds__(MERGERS * 32) merge4_kernel(const __grid_constant__ Attn4Args a) {
     constexpr int N = D / 32;
     __shared__ float s_acc[MERGERS][D];
     __shared__ float s_l[MERGERS];
-    const int h = blockIdx.x, b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, H = a.r.n_heads;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, H = a.r.n_heads, h = (blockIdx.x * MERGERS + warp) / WIDE, b = blockIdx.y;
     pdl_launch();
     pdl_wait();
     if (!kv4::has_row(a.c, a.r.positions[b], a.r.slots[b])) return;      // no token: the row stays as it is
+    const bool there = h < H;
     const int2 sh = a.shares[b];
-    float m = -INFINITY;
-    for (int p = lane; p < sh.y; p += 32) m = fmaxf(m, a.part_ml[(size_t)(sh.x + p) * H + h].x);
-    m = warp_max(m);
-    const float sink = a.sinks ? a.sinks[h] * LOG2E : -INFINITY;
-    m = fmaxf(m, sink);
-    const float ref = m == -INFINITY ? 0.f : m;
-    float acc[N], l = 0.f;
+    float acc[N], l = 0.f, ref = 0.f, sink = -INFINITY;
 #pragma unroll
     for (int j = 0; j < N; j++) acc[j] = 0.f;
-#pragma unroll 4
-    for (int p = warp; p < sh.y; p += MERGERS) {
-        const size_t at = (size_t)(sh.x + p) * H + h;
-        const float2 ml = a.part_ml[at];
-        const float f = ex2(ml.x - ref);
-        if constexpr (N == 4) {
-            const float4 y = __ldcg(reinterpret_cast<const float4*>(a.part_acc + at * D) + lane);
-            acc[0] += y.x * f; acc[1] += y.y * f; acc[2] += y.z * f; acc[3] += y.w * f;
-        } else {
-            const float2 y = __ldcg(reinterpret_cast<const float2*>(a.part_acc + at * D) + lane);
-            acc[0] += y.x * f; acc[1] += y.y * f;
+    if (there) {
+        float m = -INFINITY;
+        for (int p = lane; p < sh.y; p += 32) m = fmaxf(m, a.part_ml[(size_t)(sh.x + p) * H + h].x);
+        if (a.sinks) sink = a.sinks[h] * LOG2E;
+        m = fmaxf(warp_max(m), sink);
+        ref = m == -INFINITY ? 0.f : m;
+#pragma unroll 8
+        for (int p = warp % WIDE; p < sh.y; p += WIDE) {
+            const size_t at = (size_t)(sh.x + p) * H + h;
+            const float2 ml = a.part_ml[at];
+            const float f = ex2(ml.x - ref);
+            if constexpr (N == 4) {
+                const float4 y = __ldcg(reinterpret_cast<const float4*>(a.part_acc + at * D) + lane);
+                acc[0] += y.x * f; acc[1] += y.y * f; acc[2] += y.z * f; acc[3] += y.w * f;
+            } else {
+                const float2 y = __ldcg(reinterpret_cast<const float2*>(a.part_acc + at * D) + lane);
+                acc[0] += y.x * f; acc[1] += y.y * f;
+            }
+            l += ml.y * f;
         }
-        l += ml.y * f;
     }
+    if (WIDE > 1) {
 #pragma unroll
-    for (int j = 0; j < N; j++) s_acc[warp][N * lane + j] = acc[j];
-    if (lane == 0) s_l[warp] = l;
-    __syncthreads();
-    const int col = threadIdx.x;
-    if (col >= D) return;
-    float y = 0.f;
-    l = 0.f;
+        for (int j = 0; j < N; j++) s_acc[warp][N * lane + j] = acc[j];
+        if (lane == 0) s_l[warp] = l;
+        __syncthreads();
+        if (warp % WIDE) return;
+        l = 0.f;
 #pragma unroll
-    for (int w = 0; w < MERGERS; w++) {
-        y += s_acc[w][col];
-        l += s_l[w];
+        for (int j = 0; j < N; j++) acc[j] = 0.f;
+#pragma unroll
+        for (int w = 0; w < WIDE; w++) {
+#pragma unroll
+            for (int j = 0; j < N; j++) acc[j] += s_acc[warp + w][N * lane + j];
+            l += s_l[warp + w];
+        }
     }
+    if (!there) return;
     if (sink > -INFINITY) l += ex2(sink - ref);
-    y /= l;
-    const size_t at = (size_t)b * a.ldo + (size_t)h * D + col;
-    if (a.out16) reinterpret_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(y);
-    else reinterpret_cast<float*>(a.out)[at] = y;
+    const size_t at = (size_t)b * a.ldo + (size_t)h * D + N * lane;      // (rows of results stand at any distance)
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+        const float y = acc[j] / l;
+        if (a.out16) reinterpret_cast<__nv_bfloat16*>(a.out)[at + j] = __float2bfloat16_rn(y);
+        else reinterpret_cast<float*>(a.out)[at + j] = y;
+    }
 }
 
 }  // namespace
@@ -565,5 +576,7 @@ B2_API int b2_attn4(const Attn4Args* in, int pdl, cudaStream_t st) {
     const int rc = launch_rows(fn, dim3(a.room, a.c.kv_heads * tiles), dim3(WARPS * 32), smem, args, st, pdl);
     if (rc) return rc;
     void* margs[] = {&a};      // (its CTAs may wait beside the first launch's last)
-    return launch_rows(big ? (const void*)merge4_kernel<128> : (const void*)merge4_kernel<64>, dim3(a.r.n_heads, a.r.rows), dim3(MERGERS * 32), 0, margs, st, 1);
+    const bool many = a.room / a.r.rows > MERGERS;      // shares that a sequence has on the mean
+    const void* merge = big ? (many ? (const void*)merge4_kernel<128, MERGERS> : (const void*)merge4_kernel<128, 1>) : (many ? (const void*)merge4_kernel<64, MERGERS> : (const void*)merge4_kernel<64, 1>);
+    return launch_rows(merge, dim3(many ? a.r.n_heads : (a.r.n_heads + MERGERS - 1) / MERGERS, a.r.rows), dim3(MERGERS * 32), 0, margs, st, 1);
 }
