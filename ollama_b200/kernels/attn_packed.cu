@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(THREADS, 1) packed_kernel(const __grid_constan
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wg = warp >> 2;
     pdl_wait();
     const int group = a.n_heads / a.kv_heads, tokens = BQ / group;          // tokens of a tile
-    const int behind = a.starts[blockIdx.x], shares = a.starts[blockIdx.x + 1] - behind + 1;
+    const int behind = a.starts[blockIdx.x], shares = min(max(a.starts[blockIdx.x + 1] - behind, 0), a.n_tiles) + 1;
     // whether some row does not see all of the keys from n0 on
     auto masked = [&](const PackedTile& x, int n0) { return n0 + BKV - 1 > x.pos || n0 < first_key(x.pos + x.rows - 1, 0, a.window); };
     // keys or values of 16-bit rows, the nth tile of this CTA
@@ -187,8 +187,15 @@ __global__ void __launch_bounds__(THREADS, 1) packed_kernel(const __grid_constan
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     };
-    const PackedTile u0 = a.tiles[blockIdx.x];
-    auto share = [&](int i) { return i == 0 ? u0 : a.tiles[behind + i - 1]; };
+    // Lists are on the device, so what they say is checked here: a tile that reaches beyond the queries, the cache or the partial results becomes one without rows, which writes nothing.
+    auto tile_of = [&](int at) {
+        PackedTile x = a.tiles[min(max(at, 0), a.n_tiles - 1)];
+        const bool fits = x.row >= 0 && x.rows > 0 && x.rows <= 2 * tokens && x.row <= a.q_rows - x.rows && (unsigned)x.slot < (unsigned)a.slots && (unsigned)x.kvh < (unsigned)a.kv_heads && x.base >= 0 &&
+                          x.pos >= 0 && x.base <= a.n - x.rows && x.pos <= a.n - x.rows - x.base && x.k_lo >= 0 && x.k_lo < x.k_hi && x.k_hi <= (x.pos + x.rows - 1) / BKV + 1 && x.part < a.parts;
+        return fits ? x : PackedTile{0, 0, 0, 1, 0, 0, 1, -1, 0, {}};
+    };
+    const PackedTile u0 = tile_of(blockIdx.x);
+    auto share = [&](int i) { return i == 0 ? u0 : tile_of(behind + i - 1); };
 
     if (warp == 8 && lane == 0) {        // the loading thread makes the barriers and asks for the first tiles before anything else
         *failed = 0;
@@ -625,6 +632,7 @@ __global__ void __launch_bounds__(256) packed_merge_kernel(const __grid_constant
     pdl_launch();
     pdl_wait();
     const PackedMerge u = a.merges[blockIdx.x];
+    if (u.row < 0 || u.row > a.q_rows - u.rows || (unsigned)u.kvh >= (unsigned)a.kv_heads || u.first < 0 || u.parts < 1 || u.first > a.parts - u.parts) return;      // as above
     const int group = a.n_heads / a.kv_heads, tokens = BQ / group, lane = threadIdx.x & 31, kvh = u.kvh;
     const int row = blockIdx.y * 8 + (threadIdx.x >> 5), tile = row >> 7, r = row & 127, token = tile * tokens + r / group;
     if (r / group >= tokens || token >= u.rows) return;
@@ -699,10 +707,10 @@ B2_API int b2_attn_packed(const PackedArgs* in, int pdl, cudaStream_t st) {
     PackedArgs a = *in;
     const bool codes = a.k == nullptr;
     if (a.ctas == 0) return 0;
-    if ((a.hd != 64 && a.hd != 128) || a.kv_heads < 1 || a.kv_heads > 65535 || a.n_heads < 1 || a.n_heads % a.kv_heads || a.n_heads / a.kv_heads > BQ || !a.q || a.q_rows < 1 || !a.out || !a.tiles || !a.starts || a.ctas < 0 || a.window < 0 ||
+    if ((a.hd != 64 && a.hd != 128) || a.kv_heads < 1 || a.kv_heads > 65535 || a.n_heads < 1 || a.n_heads % a.kv_heads || a.n_heads / a.kv_heads > BQ || !a.q || a.q_rows < 1 || !a.out || !a.tiles || !a.starts || a.ctas < 0 || a.n_tiles < a.ctas || a.window < 0 ||
         a.ldo < a.n_heads * a.hd || (((uintptr_t)a.q | (uintptr_t)a.out) & 15) || a.ldq % (a.q_type ? 8 : 4) || a.ldo % (a.out_type ? 8 : 4))
         return (int)cudaErrorInvalidValue;
-    if (a.n_merges && (!a.merges || !a.part_acc || !a.part_ml || a.n_merges < 0 || ((uintptr_t)a.part_acc & 15))) return (int)cudaErrorInvalidValue;
+    if (a.n_merges < 0 || a.parts < 0 || (a.n_merges && !a.merges) || (a.parts && (!a.part_acc || !a.part_ml || ((uintptr_t)a.part_acc & 15)))) return (int)cudaErrorInvalidValue;
     if (codes ? kv4_bad_cache(a.c) || a.c.hd != a.hd || a.c.kv_heads != a.kv_heads : !a.v || a.slots < 1 || a.n < 1) return (int)cudaErrorInvalidValue;
     CUtensorMap mk = {}, mv = {}, mq = {};
     if (a.q_type && !queries_map(&mq, a)) return (int)cudaErrorInvalidValue;

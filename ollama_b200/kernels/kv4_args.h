@@ -94,7 +94,7 @@ struct PackedArgs {
     Cache4 c;
     const PackedTile* tiles;
     const int* starts;       // [ctas + 1]: CTA i takes tile i, then starts[i] .. starts[i + 1] - 1
-    int ctas;
+    int ctas, n_tiles;
     const PackedMerge* merges;
     int n_merges, parts;
     float scale, softcap;

@@ -38,7 +38,7 @@ struct PassSeg {
 
 // 4-bit caches: what attention has to know of the pass's sequences, for each window that layers have (ops/kv4.py's portions), and where partial results go.
 struct PassPlan4 {
-    int window, ctas, n_merges, parts;
+    int window, ctas, n_tiles, n_merges, parts;
     const PackedTile* tiles;
     const int* starts;
     const PackedMerge* merges;
@@ -127,6 +127,7 @@ int attend4(const PassArgs& a, const PassLayer& L, int nq, int& launches, cudaSt
     t.tiles = p->tiles;
     t.starts = p->starts;
     t.ctas = p->ctas;
+    t.n_tiles = p->n_tiles;
     t.merges = p->merges;
     t.n_merges = p->n_merges;
     t.parts = p->parts;

@@ -266,17 +266,19 @@ long prompt(const Signature& s, PyObject** a, bool codes) {
     if (as_long(group.o, 0) * p.kv_heads != heads) refuse(s, "portions that were made for " + std::to_string(as_long(group.o, 0)) + " heads a KV head");
     if (as_long(rows.o, 0) > n) refuse(s, "portions of " + std::to_string(as_long(rows.o, 0)) + " rows for " + std::to_string(n));
     const at::Tensor &t = wide(s, piece(s, tiles.o, "portions", I32, dev), "portions"), &u = wide(s, piece(s, merges.o, "portions", I32, dev), "portions"), &w = piece(s, starts.o, "portions", I32, dev);
-    if (t.dim() != 2 || t.size(1) * 4 != (long)sizeof(PackedTile) || u.dim() != 2 || u.size(1) * 4 != (long)sizeof(PackedMerge) || w.dim() != 1 || w.numel() < 2) refuse(s, "portions " + told(t));
+    if (t.dim() != 2 || t.size(1) * 4 != (long)sizeof(PackedTile) || u.dim() != 2 || u.size(1) * 4 != (long)sizeof(PackedMerge) || w.dim() != 1 || w.numel() < 2 || w.numel() - 1 > t.size(0) || t.size(0) > (1l << 30) || u.size(0) > (1l << 30)) refuse(s, "portions " + told(t));
     p.tiles = (const PackedTile*)t.data_ptr();
     p.starts = (const int*)w.data_ptr();
     p.ctas = (int)w.numel() - 1;
+    p.n_tiles = (int)t.size(0);
     p.merges = (const PackedMerge*)u.data_ptr();
     p.n_merges = (int)u.size(0);
-    p.parts = (int)as_long(parts.o, 0);
+    p.parts = (int)std::max(as_long(parts.o, 0), 0l);
     const at::Tensor& out = results(s, a[P_OUT], dev, n, heads * p.hd);
     p.out = out.data_ptr();
     p.ldo = (int)aligned_step(s, out, "out");
     p.out_type = out.scalar_type() == F32 ? 0 : out.scalar_type() == F16 ? 1 : 2;
+    if (n * p.ldo * out.element_size() >= 1l << 36 || 1024l * p.parts * p.hd >= 1l << 36) refuse(s, "out " + told(out) + " with rows " + std::to_string(p.ldo) + " apart");      // in 16 bytes a 32-bit number
     const bool pdl = as_bool(a[P_PDL], false);
     launched(s, unlocked(dev, [&](cudaStream_t st) {
         const long rows256 = (long)p.parts * 256;

@@ -542,3 +542,54 @@ def test_refusals():
         kv4.attn_decode4([1], k, v, pos, slot, out, scale=1.0)
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(before, (q, out, k.codes, v.codes)))
+
+
+def test_lists_that_changed_after_they_were_made():
+    """Tiles and sums that reach beyond the queries, the cache or the partial results are left out, and the rows of the others are what they were; lists of other lengths are refused."""
+    k, v = filled(3, 2, 3000, 64)
+    q, one = torch.randn(150, 8, 64, device="cuda", generator=gen(5)).to(F16), kv4.Portions4.__match_args__
+    x = [torch.randn(3, 2, 3000, 64, device="cuda", generator=gen(6)).to(F16) for _ in range(2)]
+    p = kv4.portions4([(0, 70, 1, 0), (70, 70, 2, 2900)], 8, k)      # the second one's keys are shared out
+    assert p.parts > 1 and len(p.merges)
+    change = lambda **kw: kv4.Portions4(**({n: getattr(p, n) for n in one} | kw))
+    first = (p.tiles[:, 0] < 70).nonzero().view(-1)
+    for call, kv in ((kv4.attn_prompt4, (k, v)), (kv4.attn_packed, x)):
+        good = torch.full((150, 512), 5.0, device="cuda")
+        call(q, *kv, p, good, scale=0.1)
+        for column, worth in ((0, -1), (0, 145), (0, 2 ** 31 - 1), (1, 0), (1, -5), (1, 257), (1, 2 ** 31 - 1), (2, 3), (2, -1), (3, -1), (3, 2999), (3, 2 ** 31 - 1), (4, -1), (4, 2950), (4, 2 ** 31 - 1), (5, -1), (5, 30), (6, 0),
+                              (6, 2 ** 31 - 1), (7, p.parts), (7, 2 ** 31 - 1), (8, 2), (8, -1)):
+            tiles, out = p.tiles.clone(), torch.full((150, 512), 5.0, device="cuda")
+            tiles[first, column] = worth
+            call(q, *kv, change(tiles=tiles), out, scale=0.1)
+            assert (out[:70] == 5).all() and torch.equal(out[70:], good[70:]), (column, worth)
+        for column, worth in ((0, -1), (0, 149), (2, -1), (2, p.parts), (2, 2 ** 31 - 1), (3, 0), (3, p.parts + 1), (3, 2 ** 31 - 1), (4, 2), (4, -1)):
+            merges, out = p.merges.clone(), torch.full((150, 512), 5.0, device="cuda")
+            merges[:, column] = worth
+            call(q, *kv, change(merges=merges), out, scale=0.1)
+            split = torch.zeros(150, dtype=torch.bool, device="cuda")
+            for row, rows in p.merges[:, :2].tolist():
+                split[row:row + rows] = True
+            assert (out[split] == 5).all() and torch.equal(out[~split], good[~split]), (column, worth)
+        for starts in (p.starts - 5, p.starts + len(p.tiles), p.starts * 0 - 2 ** 31, p.starts * 0 + 2 ** 31 - 1, p.starts.flip(0)):
+            out = torch.full((150, 512), 5.0, device="cuda")
+            call(q, *kv, change(starts=starts.contiguous()), out, scale=0.1)
+            assert (out[140:] == 5).all()
+        for wrong in (dict(tiles=p.tiles[:3]), dict(tiles=p.tiles.long()), dict(tiles=p.tiles[:, :8].contiguous()), dict(starts=p.starts[:1]), dict(merges=p.merges.float())):
+            with pytest.raises(ValueError, match=call.__name__):
+                call(q, *kv, change(**wrong), good, scale=0.1)
+    torch.cuda.synchronize()
+    assert kv4.status() == 0
+
+
+def test_results_far_apart():
+    """Rows of results up to 2^36 bytes from the first, and not beyond."""
+    k, v = filled(1, 1, 40, 64)
+    q, p = torch.randn(9, 1, 64, device="cuda", generator=gen(7)), kv4.portions4([(0, 9, 0, 20)], 1, k)
+    want = torch.zeros(9, 64, device="cuda")
+    kv4.attn_prompt4(q, k, v, p, want, scale=0.2)
+    step = 2 ** 31 - 4
+    far = torch.empty(8 * step + 64, device="cuda")
+    kv4.attn_prompt4(q[:8], k, v, kv4.portions4([(0, 8, 0, 20)], 1, k), far.as_strided((8, 64), (step, 1)), scale=0.2)
+    assert torch.equal(far.as_strided((8, 64), (step, 1)), want[:8])
+    with pytest.raises(ValueError, match="apart"):
+        kv4.attn_prompt4(q, k, v, p, far.as_strided((9, 64), (step, 1)), scale=0.2)
