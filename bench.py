@@ -207,7 +207,7 @@ def main() -> None:
     ap.add_argument("--no-extras", action="store_true", help="skip the other halves of the headline workloads (4 slots, concurrency 8, 70B on one GPU)")
     ap.add_argument("--parallelism", default="tp", choices=["tp", "pp"],
                     help="N > 1: tp = tensor/expert parallel ranks (default), pp = layer pipeline driven by rank 0 (the reference's multi-GPU mode)")
-    ap.add_argument("--kv-type", default="f16", choices=["f16", "q8_0"], help="K/V cache encoding (OLLAMA_KV_CACHE_TYPE)")
+    ap.add_argument("--kv-type", default="f16", choices=["f16", "q8_0", "int4"], help="K/V cache encoding (OLLAMA_KV_CACHE_TYPE)")
     ap.add_argument("--layers", type=int, default=0, help="truncate the model to this many layers (profiling only; not a benchmark number)")
     ap.add_argument("--stack", action="store_true", help="another workload: stack models (vazatar-1b / 8b, kavenex-1b / 8b / moe, tirudra-2k / 4k, rinirax-1b / 8b / 2k) beside models of equal size, bf16, one GPU")
     args = ap.parse_args()

@@ -2,17 +2,21 @@
 //
 //   out[t][h] = sum_k p_k v_k / (sum_k p_k + exp(sink)),  p_k = exp(cap(scale q[t][h] . k)),  k the sequence's positions up to the token's own that its window has
 //
-// A CTA takes shares one after the other: two tiles of 128 query rows of one KV head and a run of keys; a row is a token's query head (token / group, head of the group), so all heads of a group share the keys that the CTA brings, and few
-// tokens of many heads still fill a tile.  Keys come in tiles of 128.  Roles: warps 0-3 and 4-7 the softmax of a tile each, a row a thread (no exchange between threads); warp 8 loads
-// keys and values, warp 10 queries; warp 9 issues the products; warps 12-15 make operands: queries, of a 4-bit cache also keys and values, whose codes they turn into f16 rows in the swizzled layout; of 16-bit rows they look at tiles whose
-// mask is not whole (below).  The next share's first scores are computed behind the last products of this one; nothing
-// waits for a share's results to be written but the next one's first P V.
+// A CTA takes shares one after the other: two tiles of 128 query rows of one KV head and a run of keys; a row is a token's query head (token / group, head of the group), so all heads of a group
+// share the keys that the CTA brings, and few tokens of many heads still fill a tile.  Keys come in tiles of 128.  Roles: warps 0-3 and 4-7 the softmax of a tile each, a row a thread (no exchange
+// between threads); warp 8 loads keys and values, warp 10 queries; warp 9 issues the products; warps 12-15 make operands: queries that are not of the operands' type, of a 4-bit cache also keys and
+// values, whose codes they turn into f16 rows in the swizzled layout; of 16-bit rows they look at tiles whose mask is not whole (below).  The next share's first scores are computed behind the last
+// products of this one; nothing waits for a share's results to be written but the next one's first P V.
 // Tensor memory: S of both tiles (128 columns each, over whose first 64 the weights are written as 16-bit operands), O of both, accumulated there.  One tile's products run under the other's softmax, and P V
 // of keys 0 .. 63 while the weights of the others are still being made.  The weights are relative to a reference that follows a row's largest score only when that exceeds it by 2^8
 // (then the thread rescales its row of O: the product before is complete by the time a tile's scores are), and count from 2^6 on, so that f16 weights keep 20 powers of two below the largest.
 // Tiles that not every row sees as a whole (the diagonal, a window's edge, the end) hold keys that must not count whatever they are, and a weight of zero times a value that is no number is
 // none either: in such tiles of 16-bit rows, values rows with such elements become zeros and their keys none, so that exactly the rows that see them have no result.  Cached codes are finite.
 // The host deals the shares out to as many CTAs as SMs (plan in ops/kv4_call.cpp); where whole tiles would leave SMs without work, keys of some are cut, and a second launch adds up the parts.
+// What bounds it: the products of a tile of keys (2 x 128 rows, 128 columns) keep the tensor cores busy for 2048 cycles and its exponentials the units that make them for as many; a tile takes some
+// 3500 in the middle of a share (1.9 us, 1.3 PFLOP/s on 148 SMs, where power allows 1.4 in a long product), since a row's scores, weights and products wait for one another and there is room for two rows
+// of tiles only.  Both pipes are busy in 50 to 54% of all cycles; a share's ends cost 4.5 us more.  Measured, 32 heads on 8 of 128: 2048 rows behind 6144 cached keys 236 us, 1.02 PFLOP/s of what the mask
+// leaves; five prompts of 4096 f16 rows 371, 0.97; 64 rows behind 30000 46.4; nine short ones 17.7.  Tried: some exponentials as polynomials (no difference), scores in halves of 64 keys (3.6 us a tile).
 #include "attn_tc.cuh"
 #include "kv4.cuh"
 

@@ -1,8 +1,9 @@
 // Rows into the 4-bit cache (kv4.cuh) and back.
 //
-// b2_append4: norm of the query and key heads, rotation, queries out, keys and values as codes.  A warp takes a head of a token at a time, 128 or 64 columns in its lanes' registers, so the norm's sum
-// and the other columns of pairs are shuffles.  Keys and values then stand in shared memory, where a thread takes eight columns and makes a word: with a head a warp (four columns a lane) the
-// extremes of a block took three rounds of shuffles and the words two, and 2048 rows of 48 heads 29 us for what takes 20 here; their bytes take 10.  What is left: three waves of CTAs, each a chain of position, angles and heads (five CTAs an SM with two heads asked for ahead; four with four 21.1, three 22.6).
+// b2_append4: norm of the query and key heads, rotation, queries out, keys and values as codes.  A warp takes a head of a token at a time, 128 or 64 columns in its lanes' registers, so the norm's
+// sum and the other columns of pairs are shuffles.  Keys and values then stand in shared memory, where a thread takes eight columns and makes a word: with a head a warp (four columns a lane) the
+// extremes of a block took three rounds of shuffles and the words two, and 2048 rows of 48 heads 29 us for what takes 20 here; their 76 MB take 12.  What is left: three waves of CTAs, each a chain
+// of position, angles and heads, that issue in 65% of their cycles (five CTAs of eight warps an SM with two heads asked for ahead; four with four 21.1, three 22.6; ten CTAs of four warps 22.1).
 // b2_read4: rows as f16 values, a lane a word of eight codes.
 #include "kv4.cuh"
 
