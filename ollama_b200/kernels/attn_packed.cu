@@ -629,17 +629,20 @@ __global__ void __launch_bounds__(THREADS, 1) packed_kernel(const __grid_constan
     if (threadIdx.x == 0 && *failed) atomicExch(&g_packed_status, KS_TIMEOUT);
 }
 
-// Adds up the parts of query tiles: grid (tiles, runs of 8 rows), a warp a row.
-template <int D>
-__global__ void __launch_bounds__(256) packed_merge_kernel(const __grid_constant__ PackedArgs a) {
+// Adds up the parts of query tiles: grid (tiles, rows * WIDE / 8), WIDE warps a row, which take every WIDE-th part.
+constexpr int MERGERS = 8;
+template <int D, int WIDE>
+__global__ void __launch_bounds__(MERGERS * 32) packed_merge_kernel(const __grid_constant__ PackedArgs a) {
     constexpr int N = D / 32;
+    __shared__ __align__(16) float s_acc[WIDE > 1 ? MERGERS : 1][D];
+    __shared__ float s_l[MERGERS];
     pdl_launch();
     pdl_wait();
     const PackedMerge u = a.merges[blockIdx.x];
     if (u.row < 0 || u.row > a.q_rows - u.rows || (unsigned)u.kvh >= (unsigned)a.kv_heads || u.first < 0 || u.parts < 1 || u.first > a.parts - u.parts) return;      // as above
-    const int group = a.n_heads / a.kv_heads, tokens = BQ / group, lane = threadIdx.x & 31, kvh = u.kvh;
-    const int row = blockIdx.y * 8 + (threadIdx.x >> 5), tile = row >> 7, r = row & 127, token = tile * tokens + r / group;
-    if (r / group >= tokens || token >= u.rows) return;
+    const int group = a.n_heads / a.kv_heads, tokens = BQ / group, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kvh = u.kvh;
+    const int row = (blockIdx.y * MERGERS + warp) / WIDE, tile = row >> 7, r = row & 127, token = tile * tokens + r / group;
+    if (r / group >= tokens || token >= u.rows) return;      // (all of a row's warps)
     const int head = kvh * group + r % group;
     const size_t step = 2 * BQ, first = (size_t)u.first * step + row;
     const float sink = a.sinks ? a.sinks[head] * LOG2E : -INFINITY;
@@ -647,11 +650,11 @@ __global__ void __launch_bounds__(256) packed_merge_kernel(const __grid_constant
     for (int p = lane; p < u.parts; p += 32) m = fmaxf(m, a.part_ml[first + p * step].x);
     m = fmaxf(warp_max(m), sink);
     const float ref = m == -INFINITY ? 0.f : m;
-    float acc[N], l = sink > -INFINITY ? ex2(sink - ref) : 0.f;
+    float acc[N], l = sink > -INFINITY && warp % WIDE == 0 ? ex2(sink - ref) : 0.f;
 #pragma unroll
     for (int j = 0; j < N; j++) acc[j] = 0.f;
 #pragma unroll 8
-    for (int p = 0; p < u.parts; p++) {
+    for (int p = warp % WIDE; p < u.parts; p += WIDE) {
         const float2 ml = a.part_ml[first + p * step];
         const float f = ex2(ml.x - ref);
         l += ml.y * f;
@@ -662,6 +665,19 @@ __global__ void __launch_bounds__(256) packed_merge_kernel(const __grid_constant
         } else {
             const float2 y = __ldcg(reinterpret_cast<const float2*>(from));
             acc[0] += y.x * f; acc[1] += y.y * f;
+        }
+    }
+    if constexpr (WIDE > 1) {
+#pragma unroll
+        for (int j = 0; j < N; j++) s_acc[warp][N * lane + j] = acc[j];
+        if (lane == 0) s_l[warp] = l;
+        __syncthreads();
+        if (warp) return;
+#pragma unroll
+        for (int w = 1; w < WIDE; w++) {
+#pragma unroll
+            for (int j = 0; j < N; j++) acc[j] += s_acc[w][N * lane + j];
+            l += s_l[w];
         }
     }
     const float inv = 1.f / l;
@@ -714,7 +730,7 @@ B2_API int b2_attn_packed(const PackedArgs* in, int pdl, cudaStream_t st) {
     if ((a.hd != 64 && a.hd != 128) || a.kv_heads < 1 || a.kv_heads > 65535 || a.n_heads < 1 || a.n_heads % a.kv_heads || a.n_heads / a.kv_heads > BQ || !a.q || a.q_rows < 1 || !a.out || !a.tiles || !a.starts || a.ctas < 0 || a.n_tiles < a.ctas || a.window < 0 ||
         a.ldo < a.n_heads * a.hd || (((uintptr_t)a.q | (uintptr_t)a.out) & 15) || a.ldq % (a.q_type ? 8 : 4) || a.ldo % (a.out_type ? 8 : 4))
         return (int)cudaErrorInvalidValue;
-    if (a.n_merges < 0 || a.parts < 0 || (a.n_merges && !a.merges) || (a.parts && (!a.part_acc || !a.part_ml || ((uintptr_t)a.part_acc & 15)))) return (int)cudaErrorInvalidValue;
+    if (a.n_merges < 0 || a.parts < 0 || (a.n_merges && (a.merge_rows < 1 || a.merge_rows > 2 * BQ)) || (a.n_merges && !a.merges) || (a.parts && (!a.part_acc || !a.part_ml || ((uintptr_t)a.part_acc & 15)))) return (int)cudaErrorInvalidValue;
     if (codes ? kv4_bad_cache(a.c) || a.c.hd != a.hd || a.c.kv_heads != a.kv_heads : !a.v || a.slots < 1 || a.n < 1) return (int)cudaErrorInvalidValue;
     CUtensorMap mk = {}, mv = {}, mq = {};
     if (a.q_type && !queries_map(&mq, a)) return (int)cudaErrorInvalidValue;
@@ -732,7 +748,11 @@ B2_API int b2_attn_packed(const PackedArgs* in, int pdl, cudaStream_t st) {
                                : launch_rows(kernel_of<64>(form), dim3(a.ctas), dim3(THREADS), Lay<64>::TOTAL, args, st, pdl);
     if (rc || !a.n_merges) return rc;
     void* margs[] = {&a};      // (its CTAs may wait beside the first launch's last)
-    return launch_rows(a.hd == 128 ? (const void*)packed_merge_kernel<128> : (const void*)packed_merge_kernel<64>, dim3(a.n_merges, 2 * BQ / 8), dim3(256), 0, margs, st, 1);
+    static_assert(MERGERS == 8, "a row's warps are one or all of a CTA's");
+    // shares that a sum has on the mean: 35 of 2 x 10 rows behind 5581 keys 22.5 us with a warp a row, 11.9 with eight; 8 of 7 rows behind 901 10.9, 10.1; 2 of 2048 rows behind 6144 234, 294
+    const bool many = a.parts / a.n_merges > 4;
+    const void* merge = a.hd == 128 ? (many ? (const void*)packed_merge_kernel<128, MERGERS> : (const void*)packed_merge_kernel<128, 1>) : (many ? (const void*)packed_merge_kernel<64, MERGERS> : (const void*)packed_merge_kernel<64, 1>);
+    return launch_rows(merge, dim3(a.n_merges, many ? a.merge_rows : (a.merge_rows + MERGERS - 1) / MERGERS), dim3(MERGERS * 32), 0, margs, st, 1);
 }
 
 // 0, or 1 once a wait has run out since the last call; synchronises.

@@ -97,6 +97,7 @@ struct PackedArgs {
     int ctas, n_tiles;
     const PackedMerge* merges;
     int n_merges, parts;
+    int merge_rows;          // rows of partial results, of the 256, that the merges' largest has
     float scale, softcap;
     int window;
     const float* sinks;

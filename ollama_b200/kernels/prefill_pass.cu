@@ -38,7 +38,7 @@ struct PassSeg {
 
 // 4-bit caches: what attention has to know of the pass's sequences, for each window that layers have (ops/kv4.py's portions), and where partial results go.
 struct PassPlan4 {
-    int window, ctas, n_tiles, n_merges, parts;
+    int window, ctas, n_tiles, n_merges, parts, merge_rows;
     const PackedTile* tiles;
     const int* starts;
     const PackedMerge* merges;
@@ -131,6 +131,7 @@ int attend4(const PassArgs& a, const PassLayer& L, int nq, int& launches, cudaSt
     t.merges = p->merges;
     t.n_merges = p->n_merges;
     t.parts = p->parts;
+    t.merge_rows = p->merge_rows;
     t.scale = a.scale;
     t.softcap = a.softcap;
     t.window = L.window;

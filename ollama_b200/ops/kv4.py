@@ -78,6 +78,7 @@ class Portions4:
     starts: torch.Tensor             # [CTAs + 1] int32: CTA i takes tile i, then starts[i] .. starts[i + 1] - 1
     rows: int                        # of all portions
     parts: int                       # partial results
+    merge_rows: int                  # rows of theirs that the largest sum has
     window: int
     group: int                       # query heads a KV head
     cache: tuple[int, int, int, int]
@@ -101,10 +102,10 @@ def portions4(parts, heads: int, k, *, window: int = 0) -> Portions4:
     dev = k.codes.device if isinstance(k, Cache4) else k.device
     sms = torch.cuda.get_device_properties(dev).multi_processor_count if dev.type == "cuda" else 148
     here = globals()
-    *lists, n_parts = (here.get("_plan") or __getattr__("_plan"))(torch.tensor(rows, dtype=torch.int32), heads // kv_heads, kv_heads, window, sms)
+    *lists, n_parts, merge_rows = (here.get("_plan") or __getattr__("_plan"))(torch.tensor(rows, dtype=torch.int32), heads // kv_heads, kv_heads, window, sms)
     flat = torch.cat([x.view(-1) for x in lists]).to(dev)
     tiles, merges, starts = (t.view(x.shape) for t, x in zip(flat.split([x.numel() for x in lists]), lists))
-    return Portions4(tiles, merges, starts.view(-1), at, n_parts, window, heads // kv_heads, (slots, kv_heads, n_ctx, dim))
+    return Portions4(tiles, merges, starts.view(-1), at, n_parts, merge_rows, window, heads // kv_heads, (slots, kv_heads, n_ctx, dim))
 
 
 CALLS = ("append4", "read4", "attn_decode4", "attn_step4", "attn_prompt4", "attn_packed")

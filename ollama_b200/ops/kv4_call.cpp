@@ -14,7 +14,7 @@ int (*f_read)(const Read4Args*, int, cudaStream_t);
 int (*f_attn)(const Attn4Args*, int, cudaStream_t);
 int (*f_room)(int, int, int, int);
 int (*f_packed)(const PackedArgs*, int, cudaStream_t);
-PyObject *s_codes, *s_scale, *s_tiles, *s_starts, *s_merges, *s_rows, *s_parts, *s_window, *s_group, *s_cache;
+PyObject *s_codes, *s_scale, *s_tiles, *s_starts, *s_merges, *s_rows, *s_parts, *s_window, *s_group, *s_cache, *s_merge_rows;
 
 // A cache as ops/kv4.py makes it; its tensors may have changed in place since.
 Cache4 cache(const Signature& s, PyObject* k, PyObject* v, c10::Device dev) {
@@ -257,7 +257,7 @@ long prompt(const Signature& s, PyObject** a, bool codes) {
     p.sinks = k.sinks;
     // tiles of other heads, masks or caches would point elsewhere
     PyObject* o = a[P_PORTIONS];
-    Ref tiles(o, s_tiles), starts(o, s_starts), merges(o, s_merges), rows(o, s_rows), parts(o, s_parts), window(o, s_window), group(o, s_group), cached(o, s_cache);
+    Ref tiles(o, s_tiles), starts(o, s_starts), merges(o, s_merges), rows(o, s_rows), parts(o, s_parts), merge_rows(o, s_merge_rows), window(o, s_window), group(o, s_group), cached(o, s_cache);
     const long of[4] = {slots, p.kv_heads, n_ctx, p.hd};
     if (!PyTuple_Check(cached.o) || PyTuple_GET_SIZE(cached.o) != 4) refuse(s, "portions that are not what portions4 makes");
     for (int i = 0; i < 4; i++)
@@ -274,6 +274,7 @@ long prompt(const Signature& s, PyObject** a, bool codes) {
     p.merges = (const PackedMerge*)u.data_ptr();
     p.n_merges = (int)u.size(0);
     p.parts = (int)std::max(as_long(parts.o, 0), 0l);
+    p.merge_rows = (int)std::min(std::max(as_long(merge_rows.o, 0), 1l), 256l);
     const at::Tensor& out = results(s, a[P_OUT], dev, n, heads * p.hd);
     p.out = out.data_ptr();
     p.ldo = (int)aligned_step(s, out, "out");
@@ -294,12 +295,13 @@ long prompt(const Signature& s, PyObject** a, bool codes) {
 }
 
 // ---- portions -------------------------------------------------------------------------------------------------------------------
-// What a share's start and end, and adding up partial results, cost in the time of a tile of 128 keys; fewer tiles than LEAST are not made a share of their own.
-constexpr int SHARE_TILES = 2, MERGE_TILES = 3, LEAST = 2;
+// What a share's start and end, and adding up partial results, cost in the time of a tile of 128 keys.  (Over 60 drawn shapes: shares at one tile a hundredth slower on the mean, adding up at three 2 % slower, 50 at
+// most, at none 2 % slower where few keys are cut, 16 % at 200 rows of 32 heads.  Shares have one tile at least; of two 7 rows behind 901 keys 12.4 for 11.0 us, of three 17.3.)
+constexpr int SHARE_TILES = 2, MERGE_TILES = 1;
 
 Signature plan_sig = {"plan", 5, 5, {"parts", "group", "kv_heads", "window", "sms"}};
 // plan(parts, group, kv_heads, window, sms): shares and merges for portions [n, 5] int32 (first row, rows, slot, position, cache row of position 0), as int32 tensors [., 12] and [., 8], where
-// each CTA's shares begin, and the number of partial results.  All tiles as they are, the longest first to the CTA that has least to do, where that ends about when equal shares would; else
+// each CTA's shares begin, the number of partial results and how many of their rows the largest sum has.  All tiles as they are, the longest first to the CTA that has least to do, where that ends about when equal shares would; else
 // tiles are cut where a CTA has its share.
 PyObject* plan(PyObject** a) {
     const Signature& s = plan_sig;
@@ -327,8 +329,8 @@ PyObject* plan(PyObject** a) {
             work += heads * (t.k_hi - t.k_lo);
         }
     std::stable_sort(whole.begin(), whole.end(), [](const PackedTile& x, const PackedTile& y) { return x.k_hi - x.k_lo > y.k_hi - y.k_lo; });
-    const long n = (long)whole.size(), share = std::max<long>((work + SHARE_TILES * (n + sms) + sms - 1) / sms, SHARE_TILES + LEAST);      // about one cut an SM
-    int n_parts = 0;
+    const long n = (long)whole.size(), share = std::max<long>((work + SHARE_TILES * (n + sms) + sms - 1) / sms, SHARE_TILES + 1);      // about one cut an SM
+    int n_parts = 0, merge_rows = 0;
     using Load = std::pair<long, int>;       // what a CTA has to do
     using Least = std::priority_queue<Load, std::vector<Load>, std::greater<Load>>;
     std::vector<std::vector<PackedTile>> of(std::min(n, sms));
@@ -357,8 +359,7 @@ PyObject* plan(PyObject** a) {
                 Load x = q.top();
                 q.pop();
                 const long left = t.k_hi - lo;
-                long take = std::min(left, std::max<long>(share - x.first - SHARE_TILES, LEAST));
-                if (left - take < LEAST) take = left;
+                const long take = std::min(left, std::max<long>(share - x.first - SHARE_TILES, 1));
                 PackedTile y = t;
                 y.k_lo = lo;
                 y.k_hi = lo += (int)take;
@@ -367,7 +368,10 @@ PyObject* plan(PyObject** a) {
                 x.first += take + SHARE_TILES;
                 q.push(x);
             }
-            if (n_parts > first) merges.push_back(PackedMerge{t.row, t.rows, first, n_parts - first, t.kvh, {}});
+            if (n_parts > first) {
+                merges.push_back(PackedMerge{t.row, t.rows, first, n_parts - first, t.kvh, {}});
+                merge_rows = std::max(merge_rows, (int)(t.rows <= step / 2 ? t.rows * group : 128 + (t.rows - step / 2) * group));
+            }
         }
         of.erase(std::remove_if(of.begin(), of.end(), [](const auto& x) { return x.empty(); }), of.end());
     }
@@ -382,7 +386,7 @@ PyObject* plan(PyObject** a) {
         if (n) std::memcpy(t.data_ptr(), p, n * columns * 4);
         return THPVariable_Wrap(t);
     };
-    return Py_BuildValue("(NNNi)", tensor_of(out.data(), out.size(), 12), tensor_of(merges.data(), merges.size(), 8), tensor_of(starts.data(), starts.size(), 1), n_parts);
+    return Py_BuildValue("(NNNii)", tensor_of(out.data(), out.size(), 12), tensor_of(merges.data(), merges.size(), 8), tensor_of(starts.data(), starts.size(), 1), n_parts, merge_rows);
 }
 
 bool bound() { return f_append != nullptr; }
@@ -474,8 +478,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_kv4", nullptr, -1, methods};
 
 PyMODINIT_FUNC PyInit__kv4() {
     for (Signature* s : {&append_sig, &read_sig, &decode_sig, &step_sig, &prompt_sig, &packed_sig, &plan_sig}) s->intern();
-    PyObject** names[] = {&s_codes, &s_scale, &s_tiles, &s_starts, &s_merges, &s_rows, &s_parts, &s_window, &s_group, &s_cache};
-    const char* texts[] = {"codes", "scale", "tiles", "starts", "merges", "rows", "parts", "window", "group", "cache"};
-    for (int i = 0; i < 10; i++) *names[i] = PyUnicode_InternFromString(texts[i]);
+    PyObject** names[] = {&s_codes, &s_scale, &s_tiles, &s_starts, &s_merges, &s_rows, &s_parts, &s_window, &s_group, &s_cache, &s_merge_rows};
+    const char* texts[] = {"codes", "scale", "tiles", "starts", "merges", "rows", "parts", "window", "group", "cache", "merge_rows"};
+    for (int i = 0; i < 11; i++) *names[i] = PyUnicode_InternFromString(texts[i]);
     return PyModule_Create(&module);
 }

@@ -22,7 +22,7 @@ class PassSeg(C.Structure):
 
 
 class PassPlan4(C.Structure):
-    _fields_ = [("window", I), ("ctas", I), ("n_tiles", I), ("n_merges", I), ("parts", I), ("tiles", P), ("starts", P), ("merges", P)]
+    _fields_ = [("window", I), ("ctas", I), ("n_tiles", I), ("n_merges", I), ("parts", I), ("merge_rows", I), ("tiles", P), ("starts", P), ("merges", P)]
 
 
 class Pass4(C.Structure):
@@ -86,7 +86,7 @@ class PromptPass:
             plans = be.portions4([(r0, r0 + r, sl, p0) for r0, r, sl, p0 in segs], self.windows)
             room = 256 * max(p.parts for p in plans.values())
             parts4 = torch.empty(room * (c.head_dim + 2), device=dev, dtype=torch.float32) if room else None
-            kv4 = Pass4((PassPlan4 * 2)(*[PassPlan4(w, len(p.starts) - 1, len(p.tiles), len(p.merges), p.parts, K.ptr(p.tiles), K.ptr(p.starts), K.ptr(p.merges)) for w, p in plans.items()]), len(plans),
+            kv4 = Pass4((PassPlan4 * 2)(*[PassPlan4(w, len(p.starts) - 1, len(p.tiles), len(p.merges), p.parts, p.merge_rows, K.ptr(p.tiles), K.ptr(p.starts), K.ptr(p.merges)) for w, p in plans.items()]), len(plans),
                         K.ptr(parts4), K.ptr(parts4) + 4 * room * c.head_dim if room else None)
         a = PassArgs(n, c.d_model, c.n_heads, c.n_kv_heads, c.head_dim, c.rope_dim, int(c.rope_style == "neox"), be.n_ctx, be.n_slots, c.d_ff, int(c.causal), K._ACT[c.act],
                      c.norm_eps, be.attn_scale, c.attn_softcap, c.swiglu_alpha, c.swiglu_limit, K.ptr(positions), K.ptr(slots), K.ptr(x), K.ptr(qkv), K.ptr(q), K.ptr(o), K.ptr(h),
