@@ -15,8 +15,9 @@
 // The host deals the shares out to as many CTAs as SMs (plan in ops/kv4_call.cpp); where whole tiles would leave SMs without work, keys of some are cut, and a second launch adds up the parts.
 // What bounds it: the products of a tile of keys (2 x 128 rows, 128 columns) keep the tensor cores busy for 2048 cycles and its exponentials the units that make them for as many; a tile takes some
 // 3500 in the middle of a share (1.9 us, 1.3 PFLOP/s on 148 SMs, where power allows 1.4 in a long product), since a row's scores, weights and products wait for one another and there is room for two rows
-// of tiles only.  Both pipes are busy in 50 to 54% of all cycles; a share's ends cost 4.5 us more.  Measured, 32 heads on 8 of 128: 2048 rows behind 6144 cached keys 236 us, 1.02 PFLOP/s of what the mask
-// leaves; five prompts of 4096 f16 rows 371, 0.97; 64 rows behind 30000 46.4; nine short ones 17.7.  Tried: some exponentials as polynomials (no difference), scores in halves of 64 keys (3.6 us a tile).
+// of tiles only.  Both pipes are busy in 50 to 54% of all cycles; a share's ends cost 4.5 us more.  Measured, 32 heads on 8 of 128: 2048 rows behind 6144 cached keys 234 us, 1.03 PFLOP/s of what the mask
+// leaves; five prompts of 4096 f16 rows 342, 1.05 (400 one after the other, under the power cap); 64 rows behind 30000 46.7; nine short ones 18.5. Of a tile's chain scores to weights are 2200 cycles and products 1100.
+// Tried: exponentials as polynomials (12 % of them 350 us for 349, 37 % 364), scores in halves of 64 keys (3.6 us a tile), weights handed over as 96 and 32 keys (no difference).
 #include "attn_tc.cuh"
 #include "kv4.cuh"
 
