@@ -143,19 +143,21 @@ def predict_memory(model: Any, num_ctx: int, num_parallel: int, free: int | None
         if hd in (64, 128):
             expanded = 2 * kvh * hd * num_ctx * 2    # a prompt's attention reads a layer's rows of one sequence as f16
     extra = sum(os.path.getsize(p) for p in list(getattr(model, "draft_paths", None) or []) if os.path.exists(p))
-    total = size + extra + expanded + int(2 * layers * kvh * hd * num_ctx * num_parallel * per_elem)
-    if kv_type == "int4" and hd in (64, 128) and not envconfig.sched_spread():
-        held = size + extra + int(2 * layers * kvh * hd * num_ctx * num_parallel * (0.5 + 2.0 / 32))
-        if not free or held <= 0.8 * free:           # models that one GPU takes; groups of them keep int8
-            total = held
+    values = 2 * layers * kvh * hd * num_ctx * num_parallel
+    total = size + extra + expanded + int(values * per_elem)
+    copy = 0
     if free:
         ff = _first_int(kv.get(f"{arch}.feed_forward_length"))
         vocab = _first_int(kv.get(f"{arch}.vocab_size")) or len(kv.get("tokenizer.ggml.tokens") or ())
         experts = _first_int(kv.get(f"{arch}.expert_count"))
         copy = 2 * (layers * (d * (2 * heads * hd + 2 * kvh * hd) + (0 if experts else 3 * d * ff)) + vocab * d)
-        if copy < 0.4 * free:
-            total += copy
-    return total
+        if copy >= 0.4 * free:
+            copy = 0
+    if kv_type == "int4" and hd in (64, 128) and not envconfig.sched_spread() and envconfig.tp_degree() < 2:
+        held = size + extra + int(values * (0.5 + 2.0 / 32))
+        if not free or held + copy <= 0.8 * free:    # models that one GPU takes (Scheduler._place); tensor-parallel ranks keep int8
+            total = held
+    return total + copy
 
 
 # prompt batch the scheduler picks when nobody set num_batch: (batch, for a total context above, share of the memory the
