@@ -116,11 +116,12 @@ def _first_int(v, default=0):
         return default
 
 
-def predict_memory(model: Any, num_ctx: int, num_parallel: int, free: int | None = None) -> int:
+def predict_memory(model: Any, num_ctx: int, num_parallel: int, free: int | None = None, gpus: int = 0) -> int:
     """Weights (+ draft model) + KV cache of the configured type for num_ctx x num_parallel tokens (llm/llama_server.go:2681-2700).
     Every layer is counted at the full context: the engine gives sliding-window layers a cache of that length too.  With
     ``free`` (bytes free on the GPU the model would go to) the 16-bit copy of the dense matrices that the engine keeps for
-    prefill is counted as well, under the engine's own rule: it is made when it takes less than 40 % of the free memory."""
+    prefill is counted as well, under the engine's own rule: it is made when it takes less than 40 % of the free memory.
+    ``gpus``: how many the node has, where that is known: one takes whatever it is given, so there an int4 cache has four bits at any size."""
     size = int(getattr(model, "size", 0) or 0)
     kv = getattr(model, "kv", lambda: {})() or {}
     arch = kv.get("general.architecture", "")
@@ -153,9 +154,10 @@ def predict_memory(model: Any, num_ctx: int, num_parallel: int, free: int | None
         copy = 2 * (layers * (d * (2 * heads * hd + 2 * kvh * hd) + (0 if experts else 3 * d * ff)) + vocab * d)
         if copy >= 0.4 * free:
             copy = 0
-    if kv_type == "int4" and hd in (64, 128) and not envconfig.sched_spread() and envconfig.tp_degree() < 2:
+    if kv_type == "int4" and hd in (64, 128):
         held = size + extra + int(values * (0.5 + 2.0 / 32))
-        if not free or held + copy <= 0.8 * free:    # models that one GPU takes (Scheduler._place); tensor-parallel ranks keep int8
+        # models that one GPU takes (Scheduler._place); tensor-parallel ranks keep int8
+        if gpus == 1 or not envconfig.sched_spread() and envconfig.tp_degree() < 2 and (not free or held + copy <= 0.8 * free):
             total = held
     return total + copy
 
@@ -422,7 +424,7 @@ class Scheduler:
         for attempt, ctx in enumerate(ladder):
             opts["num_ctx"] = ctx
             one_gpu = max((g.free_memory for g in gpus), default=0)
-            need = predict_memory(model, ctx, num_parallel, free=one_gpu or None)
+            need = predict_memory(model, ctx, num_parallel, free=one_gpu or None, gpus=len(gpus))
             copies = max(1, min(envconfig.replicas(), len(gpus))) if gpus else 1
             if gpus:
                 while need * copies > self.free_memory():

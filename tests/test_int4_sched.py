@@ -58,3 +58,21 @@ def test_forced_groups_keep_int8(model, monkeypatch, name):
     monkeypatch.setenv(name, "2" if name == "B200_TP" else "1")
     assert predict_memory(model, 4096, 2, free=180 * GB) == eight(4096, 2) + COPY
     assert predict_memory(model, 4096, 2) == eight(4096, 2)
+
+
+@pytest.mark.parametrize("name", ["", "B200_TP", "OLLAMA_SCHED_SPREAD"])
+def test_a_node_of_one_gpu_has_no_groups(model, monkeypatch, name):
+    """Its runner keeps four bits however little is left beside the cache, so an automatic context is not cut as if it were eight."""
+    if name:
+        monkeypatch.setenv(name, "2" if name == "B200_TP" else "1")
+    free, ctx, n = 180 * GB, 262144, 15
+    assert 0.8 * free < four(ctx, n) + COPY < free < eight(ctx, n) + COPY
+    assert predict_memory(model, ctx, n, free=free, gpus=1) == four(ctx, n) + COPY
+    assert predict_memory(model, ctx, n, free=free, gpus=2) == eight(ctx, n) + COPY
+    seen = []
+    s = Scheduler(new_runner_fn=lambda m, opts, parallel, use: (seen.append((opts["num_ctx"], len(use))), SimpleNamespace(close=lambda: None, ping=lambda: True))[1], get_gpus_fn=lambda: gpus(1, free))
+    monkeypatch.setenv("OLLAMA_NUM_PARALLEL", str(n))
+    model.model_path, model.name = "/blobs/a", "a"
+    s.release(s.get_runner(model, {"num_ctx": 0}, 60))
+    s.unload_all()
+    assert seen == [(ctx, 1)]
