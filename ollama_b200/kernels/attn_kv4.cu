@@ -506,7 +506,7 @@ __global__ void __launch_bounds__(MERGERS * 32) merge4_kernel(const __grid_const
         for (int p = lane; p < sh.y; p += 32) m = fmaxf(m, a.part_ml[(size_t)(sh.x + p) * H + h].x);
         if (a.sinks) sink = a.sinks[h] * LOG2E;
         m = fmaxf(warp_max(m), sink);
-        ref = m == -INFINITY ? 0.f : m;
+        ref = m == -INFINITY ? 0.f : fminf(m, 3.4e38f);      // finite: relative to it an infinite sink is infinite, and the others' weights zero
 #pragma unroll 8
         for (int p = warp % WIDE; p < sh.y; p += WIDE) {
             const size_t at = (size_t)(sh.x + p) * H + h;
@@ -539,7 +539,7 @@ __global__ void __launch_bounds__(MERGERS * 32) merge4_kernel(const __grid_const
         }
     }
     if (!there) return;
-    if (sink > -INFINITY) l += ex2(sink - ref);
+    if (a.sinks) l += ex2(sink - ref);
     const size_t at = (size_t)b * a.ldo + (size_t)h * D + N * lane;      // (rows of results stand at any distance)
 #pragma unroll
     for (int j = 0; j < N; j++) {

@@ -650,8 +650,8 @@ __global__ void __launch_bounds__(MERGERS * 32) packed_merge_kernel(const __grid
     float m = -INFINITY;
     for (int p = lane; p < u.parts; p += 32) m = fmaxf(m, a.part_ml[first + p * step].x);
     m = fmaxf(warp_max(m), sink);
-    const float ref = m == -INFINITY ? 0.f : m;
-    float acc[N], l = sink > -INFINITY && warp % WIDE == 0 ? ex2(sink - ref) : 0.f;
+    const float ref = m == -INFINITY ? 0.f : fminf(m, 3.4e38f);      // finite: relative to it an infinite sink is infinite, and the others' weights zero
+    float acc[N], l = a.sinks && warp % WIDE == 0 ? ex2(sink - ref) : 0.f;
 #pragma unroll
     for (int j = 0; j < N; j++) acc[j] = 0.f;
 #pragma unroll 8

@@ -1,0 +1,53 @@
+"""The 4-bit cache's and packed prompts' attention where keys are cut into parts: sinks that are not finite, rows alone and beside others."""
+import pytest
+import torch
+
+import kv4_oracle as O
+from ollama_b200.ops import kv4
+from test_kv4_gpu import filled, gen, ints, values
+
+pytestmark = pytest.mark.gpu
+F16 = torch.float16
+
+
+def sixteen_bit(slots, kv_heads, n_ctx, dim, seed):
+    return [torch.randn(slots, kv_heads, n_ctx, dim, device="cuda", generator=gen(seed + i)).to(F16) for i in range(2)]
+
+
+def assert_sinks(attend):
+    """``attend(sinks)`` -> results [rows, 4 heads, columns]: exp(inf) in the denominator leaves nothing, exp(-inf) adds nothing, no number none."""
+    inf = float("inf")
+    plain, got = attend(None), attend(torch.tensor([inf, -inf, float("nan"), 0.5], device="cuda"))
+    assert (got[:, 0] == 0).all() and torch.equal(got[:, 1], plain[:, 1]) and got[:, 2].isnan().all()
+    assert ((got[:, 3].abs() < plain[:, 3].abs()) | (plain[:, 3] == 0) & (got[:, 3] == 0)).all()      # (single keys have columns that are held as zeros)
+
+
+@pytest.mark.parametrize("lengths", [[1], [40], [6000], [70 + 50 * i for i in range(40)]])
+def test_infinite_sinks_of_single_tokens(lengths):
+    """One part, many of one sequence (eight warps a head add them up), few of each of many (one warp does)."""
+    n = len(lengths)
+    k, v = filled(n, 1, max(lengths), 64, n)
+    q = torch.randn(n, 4, 64, device="cuda", generator=gen(1))
+
+    def attend(sinks):
+        out = torch.full((n, 256), 7.0, device="cuda")
+        kv4.attn_decode4(q, k, v, ints(*[m - 1 for m in lengths]), ints(*range(n)), out, scale=0.1, sinks=sinks)
+        return out.view(n, 4, 64)
+    assert_sinks(attend)
+
+
+@pytest.mark.parametrize("cached", [True, False])
+@pytest.mark.parametrize("parts,cut", [([(0, 100, 0, 0)], False), ([(0, 300, 0, 0)], True), ([(0, 5, 0, 5000)], True)])
+def test_infinite_sinks_of_prompts(parts, cut, cached):
+    """A whole tile, and parts that one warp a row adds up, or eight."""
+    k, v = filled(1, 1, 5100, 64, 3) if cached else sixteen_bit(1, 1, 5100, 64, 3)
+    rows = parts[-1][0] + parts[-1][1]
+    q, p = torch.randn(rows, 4, 64, device="cuda", generator=gen(2)), kv4.portions4(parts, 4, k)
+    assert (p.parts > 0) == cut
+
+    def attend(sinks):
+        out = torch.full((rows, 256), 7.0, device="cuda")
+        (kv4.attn_prompt4 if cached else kv4.attn_packed)(q, k, v, p, out, scale=0.1, sinks=sinks)
+        return out.view(rows, 4, 64)
+    assert_sinks(attend)
+    assert kv4.status() == 0
