@@ -751,8 +751,12 @@ B2_API int b2_attn_packed(const PackedArgs* in, int pdl, cudaStream_t st) {
     void* margs[] = {&a};      // (its CTAs may wait beside the first launch's last)
     static_assert(MERGERS == 8, "a row's warps are one or all of a CTA's");
     // Eight warps a row where a sum has more than four parts on the mean (35, of 2 x 10 rows behind 5581 keys: 22.5 us with one, 11.9 with eight; 8, of 7 behind 901: 10.9, 10.1; 2, of 2048 behind 6144:
-    // 234, 294) and all rows' CTAs are on the GPU at once (19 parts of 1024 rows 35.4, 31.6; of 2048 rows 45.7, 47.1; of 4096 46.1, 52.2).
-    const bool many = a.parts / a.n_merges > 4 && (long)a.n_merges * a.merge_rows <= 8 * 148;
+    // 234, 294) and there are at most eight rows, each a CTA then, for an SM, which has room for five: beyond two rounds of CTAs these cost more than parts do (19 parts of 1024 rows 35.4 us with one
+    // warp, 31.6 with eight; of 2048 rows 45.7, 47.1; of 4096 46.1, 52.2).
+    int dev = 0, sms = 0;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    const bool many = a.parts / a.n_merges > 4 && (long)a.n_merges * a.merge_rows <= 8l * sms;
     const void* merge = a.hd == 128 ? (many ? (const void*)packed_merge_kernel<128, MERGERS> : (const void*)packed_merge_kernel<128, 1>) : (many ? (const void*)packed_merge_kernel<64, MERGERS> : (const void*)packed_merge_kernel<64, 1>);
     return launch_rows(merge, dim3(a.n_merges, many ? a.merge_rows : (a.merge_rows + MERGERS - 1) / MERGERS), dim3(MERGERS * 32), 0, margs, st, 1);
 }

@@ -51,3 +51,19 @@ def test_infinite_sinks_of_prompts(parts, cut, cached):
         return out.view(rows, 4, 64)
     assert_sinks(attend)
     assert kv4.status() == 0
+
+
+@pytest.mark.parametrize("rows", [256, 288])
+def test_both_ways_of_adding_up(rows):
+    """Sums of more than four parts, of 1024 rows (tiles of 256, four KV heads), which eight warps each add up, and of 2048, which one does."""
+    k, v = filled(1, 4, 30100, 64, 7)
+    heads = 4
+    q, pos = torch.randn(rows, heads, 64, device="cuda", generator=gen(rows)).to(F16), 30000 - rows
+    p = kv4.portions4([(0, rows, 0, pos)], heads, k)
+    assert p.parts / len(p.merges) > 4
+    out = torch.zeros(rows, heads * 64, device="cuda")
+    kv4.attn_prompt4(q, k, v, p, out, scale=0.1)
+    some = torch.arange(0, rows, 37, device="cuda")
+    want, err = O.attend(q[some], values(k, 0, pos + rows), values(v, 0, pos + rows), pos + some, scale=0.1, wide=O.HALF16)
+    O.assert_near(out[some], want, err)
+    assert kv4.status() == 0
