@@ -518,7 +518,7 @@ __global__ void __launch_bounds__(THREADS, 1) packed_kernel(const __grid_constan
                     }
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * mult;
                 if (__any_sync(0xffffffffu, live && top > m + LAG)) {
-                    // (a row's own scores alone decide, so that it is the same whatever stands beside it)
+                    // (a row's own scores alone decide: rows of a tile do not touch one another; where keys are cut, and with it a sum's order, follows from all portions of a step)
                     const float to = top > m + LAG ? top : m, f = to == m ? 1.f : ex2(m - to);
                     m = to;
                     l *= f;

@@ -86,7 +86,8 @@ class Portions4:
 
 def portions4(parts, heads: int, k, *, window: int = 0) -> Portions4:
     """``parts``: (first row, rows, slot, position of the first row) of each portion, rows one after the other, and where that is not 0 the cache row of the sequence's position 0 behind it.
-    ``heads`` query heads attend over ``k``, a :class:`Cache4` or 16-bit keys [slots, KV heads, positions, columns], with the attention's ``window``."""
+    ``heads`` query heads attend over ``k``, a :class:`Cache4` or 16-bit keys [slots, KV heads, positions, columns], with the attention's ``window``.  Where keys are cut follows from all
+    portions, so a row's result beside other portions is that of the row alone but for roundings."""
     slots, kv_heads, n_ctx, dim = k.shape
     if heads < 1 or heads % kv_heads or heads // kv_heads > TILE or window < 0:
         raise ValueError(f"portions4: {heads} heads on {kv_heads}, window {window}")

@@ -448,7 +448,8 @@ const char attn_decode4_doc[] =
     "attn_decode4(q, k, v, positions, slots, out, *, scale, softcap=0.0, window=0, sinks=None, pdl=False)\n--\n\n"
     "Attention of one token a sequence, whose queries `q` [rows, heads, columns] (fp32, rounded to f16, or f16) are rotated and whose key and value are in the cache: over the positions up to its own, the last\n"
     "`window` of them where that is not 0.  `sinks` [heads] are logits in the denominator.  `out` fp32 or bf16 [rows, heads * columns].  Rows that hold no token are left as they are.\n"
-    "Queries and weights are f16 numbers (2^-11 each) whatever type `out` has, so queries beyond 65504 have no result; sums are 32-bit ones.  Soft caps use the fast exponential and quotient, some 2^-21.";
+    "Queries and weights are f16 numbers (2^-11 each) whatever type `out` has, so queries beyond 65504 have no result; sums are 32-bit ones.  Soft caps use the fast exponential and quotient, some 2^-21.\n"
+    "Where a sequence's keys are cut follows from all sequences of the call: beside others a result is that of the sequence alone but for roundings.";
 const char attn_step4_doc[] =
     "attn_step4(qkv, k, v, positions, slots, out, *, heads, inv_freq, n_rot, scale, neox=True, mscale=1.0, q_norm=None, k_norm=None, eps=1e-6, softcap=0.0, window=0, sinks=None, pdl=False)\n--\n\n"
     "A step on raw projections, one token a sequence: what append4 does, then attn_decode4 of its queries.  The rows that hold tokens are of different slots.";

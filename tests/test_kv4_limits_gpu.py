@@ -53,6 +53,50 @@ def test_infinite_sinks_of_prompts(parts, cut, cached):
     assert kv4.status() == 0
 
 
+def assert_same_but_for_roundings(a, b, q, keys, vals, pos, scale):
+    """Two results of the same rows whose keys were cut at other places: scores are the same, weights are f16 numbers relative to other references (2^-11 each), sums have another order (2^-18 as in
+    kv4_oracle.attend), weights that are subnormals move the mean by 2^-31 of the largest value for each key, and each result is rounded to fp32.  The mean size is taken from exact scores, 5 % are for
+    theirs."""
+    size = O.attend(q.to(F16), keys, vals.abs(), pos, scale=scale)[0] * 1.05
+    off = 2 * (O.HALF16 + 2.0 ** -18) * size + 2 * keys.shape[1] * 2.0 ** -31 * vals.abs().max() + 2 * 2.0 ** -22 * size
+    assert torch.isfinite(a).all() and ((a.double() - b.double()).abs() <= off).all(), float(((a.double() - b.double()).abs() / off).max())
+
+
+def test_a_sequence_alone_and_beside_others():
+    """Where a sequence's keys are cut follows from all sequences of a call; its result does but for roundings."""
+    lengths = [5000, 300, 4100, 1, 900, 2222, 3333, 128]
+    n, scale = len(lengths), 0.1
+    k, v = filled(n, 2, 5000, 128, 4)
+    q = torch.randn(n, 8, 128, device="cuda", generator=gen(5))
+    pos, slot = ints(*[m - 1 for m in lengths]), ints(*range(n))
+    out, one = torch.zeros(n, 1024, device="cuda"), torch.zeros(n, 1024, device="cuda")
+    kv4.attn_decode4(q, k, v, pos, slot, out, scale=scale)
+    for i, m in enumerate(lengths):
+        kv4.attn_decode4(q[i:i + 1], k, v, pos[i:i + 1], slot[i:i + 1], one[i:i + 1], scale=scale)
+        assert_same_but_for_roundings(out[i:i + 1], one[i:i + 1], q[i:i + 1], values(k, i, m), values(v, i, m), torch.tensor([m - 1]), scale)
+
+
+@pytest.mark.parametrize("cached", [True, False])
+def test_a_portion_alone_and_beside_others(cached):
+    """The same of portions: alone their keys are cut at other places than beside others, or not at all."""
+    scale, heads = 0.1, 8
+    k, v = filled(3, 2, 5100, 128, 6) if cached else sixteen_bit(3, 2, 5100, 128, 6)
+    parts = [(0, 7, 1, 5000), (7, 150, 0, 4200), (157, 64, 2, 4990), (221, 1, 0, 40), (222, 300, 1, 0)]
+    q = torch.randn(522, heads, 128, device="cuda", generator=gen(6)).to(F16)
+    call, p = kv4.attn_prompt4 if cached else kv4.attn_packed, kv4.portions4(parts, heads, k)
+    out, cuts = torch.zeros(522, 1024, device="cuda"), {tuple(t[:3]) for t in p.merges[:, [0, 1, 3]].tolist()}
+    call(q, k, v, p, out, scale=scale)
+    other = 0
+    for row, n, s, pos in parts:
+        alone = kv4.portions4([(0, n, s, pos)], heads, k)
+        other += any((row + r, m, c) not in cuts for r, m, c in alone.merges[:, [0, 1, 3]].tolist())
+        one = torch.zeros(n, 1024, device="cuda")
+        call(q[row:row + n], k, v, alone, one, scale=scale)
+        keys, vals = (values(c, s, pos + n) if cached else c[s, :, :pos + n].double() for c in (k, v))
+        assert_same_but_for_roundings(out[row:row + n], one, q[row:row + n], keys, vals, torch.arange(pos, pos + n), scale)
+    assert other >= 2 and kv4.status() == 0
+
+
 @pytest.mark.parametrize("rows", [256, 288])
 def test_both_ways_of_adding_up(rows):
     """Sums of more than four parts, of 1024 rows (tiles of 256, four KV heads), which eight warps each add up, and of 2048, which one does."""
