@@ -768,7 +768,7 @@ class B200Backend(StepEngine):
         window = c.sliding_window if L.swa else 0
         if window not in portions:
             portions.update(self.portions4(bounds, [window]))
-        self.kernel_launches += 1 + KV4.attn_prompt4(q, k, v, portions[window], o, **self._attn_args(L), pdl=self.pdl)
+        self.kernel_launches += KV4.attn_prompt4(q, k, v, portions[window], o, **self._attn_args(L), pdl=self.pdl)
         return o
 
     @torch.no_grad()
@@ -831,6 +831,7 @@ class B200Backend(StepEngine):
             else:
                 self._mm(o, L.wo, x, 0, accumulate=True)                  # residual add in the GEMM epilogue
             h = K.rmsnorm_bf16(x, L.ffn_norm, c.norm_eps, pdl=self.pdl)
+            self.kernel_launches += 3                                     # the norms, and the cache's append
             if L.moe:
                 x = self._moe_prefill(h, L, x)
                 continue
@@ -839,7 +840,6 @@ class B200Backend(StepEngine):
                 x = x + R.rmsnorm(self._mm(f, L.down), L.post_ffw_norm, c.norm_eps)
             else:
                 self._mm(f, L.down, x, 0, accumulate=True)
-            self.kernel_launches += 3
         return x
 
     def _final_norm(self, x: torch.Tensor) -> torch.Tensor:
