@@ -118,6 +118,11 @@ def build_backend(model: str, ft: str, n_gpus: int, world: int, rank: int, dev: 
     return be, cfg
 
 
+def kv_cache(be) -> str:
+    """What the model's caches hold, which need not be what was asked for: tensor-parallel ranks keep int8 where one GPU has int4."""
+    return be.kv_type
+
+
 def device_epochs(be, cfg, P: int, G: int, slots: int, steps: int, warmup: int, world: int, pp: bool, dev: str, gen) -> dict:
     """``steps`` request epochs timed on the device (CUDA events, max over ranks) after ``warmup`` untimed ones."""
     import torch
@@ -275,7 +280,7 @@ def main() -> None:
     be, cfg = build_backend(model, wl["ft"], n_gpus, world, rank, dev, args.kv_type, pp, args)
     be.alloc(slots, wl["ctx"])
     torch.cuda.synchronize()
-    t_load = time.time() - t_load
+    t_load, cache = time.time() - t_load, kv_cache(be)
 
     P, G = wl["prompt"], wl["gen"]
     gen = torch.Generator().manual_seed(1234)
@@ -383,7 +388,7 @@ def main() -> None:
                       else "int8 activations x Q4_K/Q6_K weights (decode), bf16 (prefill)"), "data": "synthetic",
             "prompt_eval_tok_s": round(prefill_tok_s, 1), "ttft_ms_p50": round(ttft_p50, 3),
             "config": {"model": model, "quant": wl["ft"], "global_batch": slots, "seq_len": P + G, "prompt_tokens": P,
-                       "generated_tokens": G, "num_ctx": wl["ctx"], "slots": slots, "kv_cache": args.kv_type,
+                       "generated_tokens": G, "num_ctx": wl["ctx"], "slots": slots, "kv_cache": cache,
                        "parallelism": "single" if n_gpus == 1 else f"{args.parallelism}{n_gpus}",
                        "l2": "inputs larger than L2 (weights of several GB are re-read every token)",
                        "weights": "random-init N(0,0.02), seed 0", "graphs": not args.no_graphs, "pdl": not args.no_pdl,

@@ -1,4 +1,4 @@
-"""Models under OLLAMA_KV_CACHE_TYPE=int4: launches of passes."""
+"""Models under OLLAMA_KV_CACHE_TYPE=int4: launches of passes, what a bench line says of the cache."""
 import pytest
 import torch
 
@@ -30,3 +30,16 @@ def test_passes_count_the_same_launches(tmp_path, kv_type):
             counts.append(eng.kernel_launches - before)
         assert counts[0] == counts[1], (segs, counts)
     eng.close()
+
+
+def test_a_bench_line_says_what_the_cache_holds(tmp_path):
+    import bench
+    from ollama_b200.engine.b200 import B200Backend
+    from ollama_b200.engine.backend import open_model
+    from ollama_b200.models.synth import write_synthetic_gguf
+    for spec, ft, holds in (("tiny-gpt-oss", "MXFP4", "q8_0"), ("tiny-qwen3", "Q8_0", "int4")):
+        p = str(tmp_path / f"{spec}.gguf")
+        write_synthetic_gguf(p, spec, ft)
+        eng = B200Backend(open_model(p), "cuda", kv_type="int4")
+        assert bench.kv_cache(eng) == holds
+        eng.close()
