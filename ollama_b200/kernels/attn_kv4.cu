@@ -2,7 +2,7 @@
 //
 //   out[t][h] = sum_k p_k v_k / (sum_k p_k + exp(sink)),  p_k = exp(cap(scale q . k)),  k the positions up to the token's own that its window has
 //
-// A key's columns cost half a byte each and two bytes more for 32, a seventh of what they weigh as fp32, so what bounds the kernel is instructions: those that turn codes into operands (seven for
+// A key's columns cost half a byte each and two bytes more for 32, a seventh of what they weigh as fp32, so what the kernel spends is instructions: those that turn codes into operands (seven for
 // eight codes of a key, half of which stay 72 too large, ten for eight of two values), the scales' products, exponentials.  Hence keys and values are the row operand of m16n8k16 products and the up to eight
 // query heads of a KV head their columns (half the products of the other way round; tcgen05 would have the expanded codes written to shared memory first), codes become f16 numbers without their scale, and the
 // scales, one for 32 columns, are applied to what is smaller: a key's to the fp32 sums over its blocks, a value's to the weights, which are rounded to f16 with the scale in them.  Models with more than
@@ -11,7 +11,8 @@
 // The reference moves only when something exceeds it by 2^8, and weights count from 2^7 on, so a key of 2^-21 of the heaviest is an f16 number of full precision and one of 2^-31 still counts.
 // The keys of all sequences and KV heads are dealt out in runs of equal length to the CTAs that fit the GPU; four warps take 32 keys of a run in turn, through rings of their own, so that nothing
 // in the loop waits for another warp.  A second launch adds up the parts.  From raw projections the CTA turns its queries itself, and the one with the token's own position also makes its codes.
-// Measured, 32 heads on 8 of 128: 4 sequences, 222 MB of keys and values: 55.9 us with the sums, 4.0 TB/s, 0.60 of a copy's rate; schedulers issue in 60% of their cycles, the tensor pipe is busy in 23%.  Without the
+// Measured, 32 heads on 8 of 128: 4 sequences, 222 MB of keys and values: 55.9 us with the sums, 4.0 TB/s, 0.60 of a copy's rate; schedulers issue in 60% of their cycles, the tensor pipe is busy in 23%: chains
+// of three warps a scheduler (166 registers), and with four heads a KV head half of the products' columns and of the weights are of heads that do not exist.  Without the
 // expansion of keys it took 3.0 us less, of values 6.7, without both 8.7, without the values' products 0.8: the rest is loads, scales and exponentials.  Four CTAs an SM in place of three (fewer stages) 3.6 more.
 // A sequence of 6144 keys 14.0 us, two launches and the chain position, share, rows, part; 201 keys 9.3.
 #include "kv4.cuh"

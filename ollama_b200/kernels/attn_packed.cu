@@ -9,7 +9,8 @@
 // products of this one; nothing waits for a share's results to be written but the next one's first P V.
 // Tensor memory: S of both tiles (128 columns each, over whose first 64 the weights are written as 16-bit operands), O of both, accumulated there.  One tile's products run under the other's softmax, and P V
 // of keys 0 .. 63 while the weights of the others are still being made.  The weights are relative to a reference that follows a row's largest score only when that exceeds it by 2^8
-// (then the thread rescales its row of O: the product before is complete by the time a tile's scores are), and count from 2^6 on, so that f16 weights keep 20 powers of two below the largest.
+// (then the thread rescales its row of O: the product before is complete by the time a tile's scores are), and count from 2^6 on, so that f16 weights keep 20 powers of two below the largest (of bf16 rows
+// weights are bf16: both operands of a product have one type).
 // Tiles that not every row sees as a whole (the diagonal, a window's edge, the end) hold keys that must not count whatever they are, and a weight of zero times a value that is no number is
 // none either: in such tiles of 16-bit rows, values rows with such elements become zeros and their keys none, so that exactly the rows that see them have no result.  Cached codes are finite.
 // The host deals the shares out to as many CTAs as SMs (plan in ops/kv4_call.cpp); where whole tiles would leave SMs without work, keys of some are cut, and a second launch adds up the parts.

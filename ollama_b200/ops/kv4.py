@@ -52,7 +52,8 @@ class Cache4:
 
 
 def encode4(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    """Codes and scales of rows [..., 64 or 128] in tensor operations, on any device: what :func:`append4` makes of them."""
+    """Codes and scales of rows [..., 64 or 128] in tensor operations, on any device: what :func:`append4` makes of them, but for quotients within 2^-23 of a border between two codes, which it takes by the
+    reciprocal."""
     x = torch.nan_to_num(x.float(), nan=0.0, posinf=torch.inf, neginf=-torch.inf).unflatten(-1, (-1, BLOCK))
     hi, lo = x.amax(-1), x.amin(-1)
     d = (torch.where(hi > -lo, hi, lo) * -0.125).clamp(-TOP, TOP).to(torch.float16)
